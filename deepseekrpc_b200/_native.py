@@ -18,6 +18,17 @@ DSR_ERR_ID, DSR_ERR_NONFINITE, DSR_ERR_SCATTER, DSR_ERR_TIMEOUT = 1, 2, 3, 4
 
 _P = c_void_p  # every device pointer travels as an opaque address
 
+
+class RopeTensor(ctypes.Structure):
+    """dsr_rope_tensor: one tensor of a dsr_rope call (strides in elements)."""
+    _fields_ = [("x", c_void_p), ("out", c_void_p), ("x_token", c_int64), ("x_head", c_int64),
+                ("out_token", c_int64), ("out_head", c_int64), ("heads", ctypes.c_int32), ("width", ctypes.c_int32),
+                ("offset", ctypes.c_int32), ("interleaved", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+DSR_BF16, DSR_F32 = 0, 1
+
 # name -> (restype, argtypes); mirrors include/dsr_b200.h exactly
 SIGNATURES = {
     "dsr_abi_version": (c_int, []),
@@ -77,6 +88,10 @@ SIGNATURES = {
                                      c_size_t, _P, c_int64, _P]),
     "dsr_append_kv_index_ring": (c_int, [_P, c_int64, _P, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P,
                                          _P, _P, _P, c_int64, _P]),
+    "dsr_paged_plan": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64,
+                               _P]),
+    "dsr_rope": (c_int, [POINTER(RopeTensor), c_int64, _P, _P, c_int64, c_float, c_int, _P, c_int64, _P]),
+    "dsr_sample": (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]),
     "dsr_decode_step": (c_int, [_P, _P, c_int64, _P, _P, _P, c_int64, c_int64, _P, c_int64, _P,
                                 c_int64, c_int64, _P, _P, _P, c_float, _P, _P, _P, _P, c_size_t, _P,
                                 c_int64, _P]),

@@ -478,6 +478,124 @@ at::Tensor ds_append_kv_index_ring(at::Tensor kv_pool, at::Tensor kv_ring, at::T
   return error;
 }
 
+// ---- around the decode path.  `status`: a status word that the caller keeps (zeroed
+// once, first error wins); without it the call makes a fresh one.
+at::Tensor status_or(const c10::optional<at::Tensor>& status, const at::Tensor& anchor) {
+  if (!status) return status_like(anchor);
+  check(*status, at::kInt, anchor);
+  TORCH_CHECK(status->numel() == 1, "status must hold one int32");
+  return *status;
+}
+
+int element_type(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat, what, ": BF16 or FP32 expected");
+  return t.scalar_type() == at::kFloat ? DSR_F32 : DSR_BF16;
+}
+
+void check_vector(const at::Tensor& t, at::ScalarType dtype, int64_t n, const at::Tensor& anchor, const char* what) {
+  check(t, dtype, anchor);
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == n, what);
+}
+
+std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens, at::Tensor held,
+                                      at::Tensor block_table, at::Tensor free_ring, at::Tensor ring_state,
+                                      int64_t tokens, c10::optional<at::Tensor> status) {
+  check(lengths, at::kInt, lengths);
+  const int64_t batch = lengths.numel();
+  const char* shapes =
+      "paged_plan: lengths, new_tokens, held [batch], block_table [batch, blocks], free_ring [pool blocks] and "
+      "ring_state [4] expected";
+  check_vector(lengths, at::kInt, batch, lengths, shapes);
+  check_vector(new_tokens, at::kInt, batch, lengths, shapes);
+  check_vector(held, at::kInt, batch, lengths, shapes);
+  check(block_table, at::kInt, lengths);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == batch, shapes);
+  check_vector(free_ring, at::kInt, free_ring.numel(), lengths, shapes);
+  check_vector(ring_state, at::kInt, 4, lengths, shapes);
+  TORCH_CHECK(tokens >= 0 && tokens < (int64_t(1) << 31), "paged_plan: invalid token count");
+  const c10::cuda::CUDAGuard guard(lengths.device());
+  auto error = status_or(status, lengths);
+  auto seq = at::empty({tokens}, lengths.options()), positions = at::empty({tokens}, lengths.options());
+  auto slots = at::empty({tokens}, lengths.options()), cu = at::empty({batch + 1}, lengths.options());
+  auto visible = at::empty({batch}, lengths.options());
+  ok(dsr_paged_plan(lengths.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
+                    block_table.data_ptr<int32_t>(), block_table.size(1), free_ring.data_ptr<int32_t>(),
+                    ring_state.data_ptr<int32_t>(), free_ring.size(0), seq.data_ptr<int32_t>(),
+                    positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), tokens, cu.data_ptr<int32_t>(),
+                    visible.data_ptr<int32_t>(), error.data_ptr<int32_t>(), batch, current_stream()));
+  return {seq, positions, slots, cu, visible, error};
+}
+
+at::Tensor ds_rope(std::vector<at::Tensor> x, std::vector<at::Tensor> out, at::Tensor positions,
+                   at::Tensor frequencies, std::vector<int64_t> offsets, std::vector<bool> interleaved, double mscale,
+                   bool inverse, c10::optional<at::Tensor> status) {
+  check(positions, at::kInt, positions);
+  check(frequencies, at::kDouble, positions);
+  TORCH_CHECK(positions.dim() == 1 && frequencies.dim() == 1, "rope: positions [tokens] and frequencies [pairs] expected");
+  TORCH_CHECK(!x.empty() && x.size() <= 4 && out.size() == x.size() && offsets.size() == x.size() &&
+                  interleaved.size() == x.size(),
+              "rope: 1 to 4 tensors, each with its output, offset and layout, expected");
+  const int64_t tokens = positions.size(0);
+  const c10::cuda::CUDAGuard guard(positions.device());
+  auto error = status_or(status, positions);
+  if (tokens == 0) return error;
+  dsr_rope_tensor desc[4] = {};
+  for (size_t i = 0; i < x.size(); ++i) {
+    const at::Tensor &a = x[i], &b = out[i];
+    TORCH_CHECK(a.is_cuda() && a.device() == positions.device() && b.is_cuda() && b.device() == positions.device(),
+                "all inputs require the same CUDA device");
+    TORCH_CHECK((a.dim() == 2 || a.dim() == 3) && a.size(0) == tokens && a.sizes() == b.sizes() &&
+                    a.scalar_type() == b.scalar_type(),
+                "rope: x and out [tokens, width] or [tokens, heads, width] of one type expected");
+    TORCH_CHECK(a.numel() > 0 && (a.size(-1) == 1 || (a.stride(-1) == 1 && b.stride(-1) == 1)),
+                "rope: the columns of x and out must be contiguous");
+    const bool heads = a.dim() == 3;
+    desc[i].x = a.data_ptr();
+    desc[i].out = b.data_ptr();
+    desc[i].x_token = a.stride(0);
+    desc[i].out_token = b.stride(0);
+    desc[i].x_head = heads ? a.stride(1) : 0;
+    desc[i].out_head = heads ? b.stride(1) : 0;
+    TORCH_CHECK(a.size(-1) <= 65536 && (!heads || a.size(1) <= 65536) && offsets[i] >= 0 && offsets[i] <= a.size(-1),
+                "rope: invalid heads, width or offset");
+    desc[i].heads = heads ? int32_t(a.size(1)) : 1;
+    desc[i].width = int32_t(a.size(-1));
+    desc[i].offset = int32_t(offsets[i]);
+    desc[i].interleaved = interleaved[i];
+    desc[i].dtype = element_type(a, "rope");
+  }
+  ok(dsr_rope(desc, int64_t(x.size()), positions.data_ptr<int32_t>(), frequencies.data_ptr<double>(),
+              frequencies.size(0), static_cast<float>(mscale), inverse, error.data_ptr<int32_t>(), tokens,
+              current_stream()));
+  return error;
+}
+
+std::vector<at::Tensor> ds_sample_logits(at::Tensor logits, at::Tensor temperature, at::Tensor top_k,
+                                         at::Tensor top_p, at::Tensor min_p, at::Tensor uniform,
+                                         c10::optional<at::Tensor> status) {
+  TORCH_CHECK(logits.is_cuda(), "all inputs require the same CUDA device");
+  const int dtype = element_type(logits, "sample_logits");
+  TORCH_CHECK(logits.dim() == 2 && logits.size(0) > 0 && logits.size(1) > 0 &&
+                  (logits.size(1) == 1 || logits.stride(1) == 1),
+              "sample_logits: logits [rows, vocab] with contiguous columns expected");
+  const int64_t rows = logits.size(0);
+  const char* shapes = "sample_logits: temperature, top_k, top_p, min_p and uniform [rows] expected";
+  check_vector(temperature, at::kFloat, rows, logits, shapes);
+  check_vector(top_k, at::kInt, rows, logits, shapes);
+  check_vector(top_p, at::kFloat, rows, logits, shapes);
+  check_vector(min_p, at::kFloat, rows, logits, shapes);
+  check_vector(uniform, at::kFloat, rows, logits, shapes);
+  const c10::cuda::CUDAGuard guard(logits.device());
+  auto error = status_or(status, logits);
+  auto tokens = at::empty({rows}, logits.options().dtype(at::kInt));
+  auto chances = at::empty({rows}, logits.options().dtype(at::kFloat));
+  ok(dsr_sample(logits.data_ptr(), dtype, logits.stride(0), logits.size(1), temperature.data_ptr<float>(),
+                top_k.data_ptr<int32_t>(), top_p.data_ptr<float>(), min_p.data_ptr<float>(),
+                uniform.data_ptr<float>(), tokens.data_ptr<int32_t>(), chances.data_ptr<float>(),
+                error.data_ptr<int32_t>(), rows, current_stream()));
+  return {tokens, chances, error};
+}
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("sparse_attention", &ds_sparse_attention);
   m.def("index_scores", &ds_index_scores);
@@ -510,4 +628,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_generations"), py::arg("kv_expected"), py::arg("index_pool"), py::arg("index_ring"),
         py::arg("index_generations"), py::arg("index_expected"), py::arg("seq"), py::arg("positions"),
         py::arg("kv_values"), py::arg("index_values"));
+  m.def("paged_plan", &ds_paged_plan, py::arg("lengths"), py::arg("new_tokens"), py::arg("held"),
+        py::arg("block_table"), py::arg("free_ring"), py::arg("ring_state"), py::arg("tokens"),
+        py::arg("status") = py::none());
+  m.def("rope", &ds_rope, py::arg("x"), py::arg("out"), py::arg("positions"), py::arg("frequencies"),
+        py::arg("offsets"), py::arg("interleaved"), py::arg("mscale") = 1.0, py::arg("inverse") = false,
+        py::arg("status") = py::none());
+  m.def("sample_logits", &ds_sample_logits, py::arg("logits"), py::arg("temperature"), py::arg("top_k"),
+        py::arg("top_p"), py::arg("min_p"), py::arg("uniform"), py::arg("status") = py::none());
 }

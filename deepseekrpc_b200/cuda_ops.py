@@ -99,3 +99,38 @@ def append_kv_index(kv_pool, index_pool, generations, block_table, seq, position
     """Generation-checked append; a refused row raises ValidationError and was not written."""
     _status(extension().append_kv_index(kv_pool, index_pool, generations, block_table, seq, positions,
                                         expected, kv_values, index_values, swa))
+
+
+# -------------------------------------------------- around the decode path
+def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens: int):
+    """Blocks for every request's new tokens and the map of those tokens to pool rows.
+
+    Updates held, block_table, free_ring and ring_state in place; returns
+    (seq, positions, slots, cu_tokens, visible).  A refused batch changes nothing.
+    """
+    *value, status = extension().paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens)
+    _status(status)
+    return tuple(value)
+
+
+def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float = 1.0, inverse: bool = False,
+         out=None):
+    """Rotates 1 to 4 tensors [tokens(, heads), width] by their positions in one launch.
+
+    offsets and interleaved: first rotated column and layout of each tensor.  out:
+    where to write (the tensors themselves rotate in place); new tensors without it.
+    inverse: the transposed rotation, which is the gradient's.
+    """
+    tensors = list(tensors)
+    if out is None:
+        out = [t.clone() for t in tensors]  # padding rows keep their values
+    _status(extension().rope(tensors, list(out), positions, frequencies, list(offsets), list(interleaved),
+                             mscale=mscale, inverse=inverse))
+    return list(out)
+
+
+def sample_logits(logits, temperature, top_k, top_p, min_p, uniform):
+    """One token per row after temperature, top-k, top-p and min-p; returns (tokens, chances)."""
+    tokens, chances, status = extension().sample_logits(logits, temperature, top_k, top_p, min_p, uniform)
+    _status(status)
+    return tokens, chances

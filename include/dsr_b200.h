@@ -423,6 +423,86 @@ int dsr_pool_restore(uint16_t* data, int64_t* generations, int64_t slots, int64_
                      int32_t* err, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Around the paged decode path: block tables and slot maps, rotary positions,
+ * attention of drafted tokens, sampling.  A step with drafted tokens runs
+ * dsr_paged_plan (rows for the new tokens) -> dsr_rope (queries and keys) ->
+ * dsr_append_kv_index -> dsr_tree_mla_decode -> dsr_sample.  No reference
+ * counterpart: the reference translates slots on the host (cache_pool.py:102-113)
+ * and takes the rotations from its serving engine (vllm_attention.py:212-226).
+ * ------------------------------------------------------------------------- */
+
+/* Element types of the entry points that take more than one. */
+#define DSR_BF16 0
+#define DSR_F32 1
+
+/* Gives every request of a paged batch the pool blocks that its length needs and
+ * maps its new tokens to pool rows.  lengths i32[batch] tokens already cached,
+ * new_tokens i32[batch] tokens to come (both >= 0, together at most
+ * table_stride*64); held i32[batch] blocks mapped in block_table
+ * i32[batch,table_stride] (entries at or past held are unmapped, -1 by custom).
+ * need = ceil((lengths+new_tokens)/64) blocks: missing ones are taken from the
+ * head of the ring of free blocks, surplus ones (a finished request: both counts
+ * 0) are given back behind its tail and their entries set to -1, both in request
+ * order, then block order; held becomes need.  free_ring i32[pool_blocks] with
+ * ring_state i32[4] = {head, count, 0, 0}: the free blocks are entries head ..
+ * head+count-1 modulo pool_blocks.  Blocks given back in a call are free from the
+ * next call on.  All four are updated in place.
+ * Outputs: seq, positions, slots i32[tokens] of the new tokens, request by
+ * request (slots = block*64 + position%64), -1 behind the last; cu_tokens
+ * i32[batch+1] their exclusive sums; visible i32[batch] = lengths + new_tokens.
+ * Refused with status 1, the four tables unchanged, no token mapped (-1, sums 0)
+ * and visible = lengths: counts out of range, more new tokens than `tokens`, too
+ * few free blocks, a ring state out of range.  A block id outside the pool met on
+ * the way gives status 1 and -1 in its place.  batch <= 16384.  Calls that share
+ * a ring must not overlap on the GPU. */
+int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* held,
+                   int32_t* block_table, int64_t table_stride, int32_t* free_ring,
+                   int32_t* ring_state, int64_t pool_blocks, int32_t* seq, int32_t* positions,
+                   int32_t* slots, int64_t tokens, int32_t* cu_tokens, int32_t* visible,
+                   int32_t* err, int64_t batch, void* stream);
+
+/* One tensor of dsr_rope: x and out [tokens, heads, width] of type dtype with unit
+ * column stride and token and head strides in elements (any sign; rows of one
+ * tensor must not overlap).  out == x rotates in place (equal strides), otherwise
+ * x and out must not overlap. */
+typedef struct {
+  const void* x;
+  void* out;
+  int64_t x_token, x_head, out_token, out_head;
+  int32_t heads, width, offset, interleaved, dtype, reserved;
+} dsr_rope_tensor;
+
+/* Rotary positions of 1..4 tensors in one launch (`tensors` is read by the call).
+ * The columns [offset, offset + 2 pairs) of every head are rotated by the angles
+ * positions[token] * frequencies[i] (f64[pairs], 64-bit angles):
+ *   y_a = mscale (x_a cos - x_b sin),  y_b = mscale (x_b cos + x_a sin),
+ * (a, b) = offset + (2i, 2i+1) when interleaved, offset + (i, i + pairs) when not;
+ * the other columns are copied.  inverse: the rotation by the negated angles,
+ * which is also the gradient (same mscale).  positions i32[tokens]; -1 marks a
+ * padding row, left as it is; anything below gives status 1 and is left too.
+ * pairs <= 256. */
+int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int32_t* positions,
+             const double* frequencies, int64_t pairs, float mscale, int inverse, int32_t* err,
+             int64_t tokens, void* stream);
+
+/* One token per row of logits [rows, vocab] (dtype, row_stride elements apart, 0:
+ * all rows the same):
+ * with w_i = exp((x_i - max)/temperature) and the order (value descending, index
+ * ascending), keeps the first top_k entries (0: all), of those the shortest prefix
+ * whose mass reaches top_p times theirs (>= 1 entry; 1: all), of those the ones
+ * with w_i >= min_p; tokens i32[rows] = the first kept index in vocabulary order
+ * whose cumulative weight exceeds uniform times the kept weight, chances f32[rows]
+ * its share of the kept weight.  temperature 0: the arg max (lowest index), chance
+ * 1.  Settings per row: temperature >= 0, top_k >= 0, top_p, min_p in [0, 1],
+ * uniform in [0, 1); others give status 1.  -inf logits are never drawn; a row of
+ * them alone gives token -1 and chance 0; NaN or +inf gives status 2; a row with
+ * a status has token -1.  vocab <= 262144. */
+int dsr_sample(const void* logits, int dtype, int64_t row_stride, int64_t vocab,
+               const float* temperature, const int32_t* top_k, const float* top_p,
+               const float* min_p, const float* uniform, int32_t* tokens, float* chances,
+               int32_t* err, int64_t rows, void* stream);
+
+/* ---------------------------------------------------------------------------
  * NVLink peer exchange for the sequence-sharded step (one process per GPU).
  * Replaces the collective library's all_gather at the two exchange points of a
  * decode step (torch.distributed.all_gather_into_tensor in the reference-style
