@@ -91,6 +91,9 @@ SIGNATURES = {
     "dsr_paged_plan": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64,
                                _P]),
     "dsr_rope": (c_int, [POINTER(RopeTensor), c_int64, _P, _P, c_int64, c_float, c_int, _P, c_int64, _P]),
+    "dsr_tree_mla_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
+    "dsr_tree_mla_decode": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, c_float, _P, c_int,
+                                    _P, _P, c_size_t, _P, c_int64, c_int64, c_int64, _P]),
     "dsr_sample": (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]),
     "dsr_decode_step": (c_int, [_P, _P, c_int64, _P, _P, _P, c_int64, c_int64, _P, c_int64, _P,
                                 c_int64, c_int64, _P, _P, _P, c_float, _P, _P, _P, _P, c_size_t, _P,

@@ -27,7 +27,7 @@ EXT_NAME = "deepseekrpc_cuda"
 
 CUDA_SOURCES = ["legacy_ops.cu", "topk.cu", "topk_noalloc.cu", "indexer_decode.cu", "indexer_prefill.cu",
                 "candidates.cu", "mla_decode.cu", "append.cu", "decode_step.cu", "p2p.cu", "pool.cu", "plan.cu", "rope.cu",
-                "sample.cu"]
+                "sample.cu", "tree_mla.cu"]
 HOST_SOURCES = ["host_common.cpp"]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -570,6 +570,54 @@ at::Tensor ds_rope(std::vector<at::Tensor> x, std::vector<at::Tensor> out, at::T
   return error;
 }
 
+std::vector<at::Tensor> ds_tree_mla_decode(at::Tensor q, at::Tensor kv_pool, at::Tensor block_table,
+                                           at::Tensor context, at::Tensor cu_nodes, at::Tensor tree_mask,
+                                           int64_t max_nodes, double scale, c10::optional<at::Tensor> sink,
+                                           bool return_lse, c10::optional<at::Tensor> out,
+                                           c10::optional<at::Tensor> status) {
+  const int dtype = element_type(q, "tree_mla_decode");
+  check(q, q.scalar_type(), q);
+  check_cache(kv_pool, q);
+  check(block_table, at::kInt, q);
+  TORCH_CHECK(q.dim() == 3 && q.size(0) > 0 && q.size(2) == DSR_KV_DIM,
+              "tree_mla_decode: q [nodes, heads, 576] expected");
+  const int64_t nodes = q.size(0), heads = q.size(1), batch = context.numel();
+  const char* shapes =
+      "tree_mla_decode: context [batch], cu_nodes [batch + 1], tree_mask [nodes], block_table [batch, blocks], "
+      "kv_pool [blocks*64, 576] and sink [heads] expected";
+  check_vector(context, at::kInt, batch, q, shapes);
+  check_vector(cu_nodes, at::kInt, batch + 1, q, shapes);
+  check_vector(tree_mask, at::kLong, nodes, q, shapes);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == batch && kv_pool.dim() == 2 &&
+                  kv_pool.size(1) == DSR_KV_DIM && kv_pool.size(0) % DSR_BLOCK_TOKENS == 0,
+              shapes);
+  if (sink) check_vector(*sink, at::kFloat, heads, q, shapes);
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto error = status_or(status, q);
+  at::Tensor result;
+  if (out) {
+    result = *out;
+    element_type(result, "tree_mla_decode");
+    check(result, result.scalar_type(), q);
+    TORCH_CHECK(result.dim() == 3 && result.size(0) == nodes && result.size(1) == heads &&
+                    result.size(2) == DSR_V_DIM,
+                "tree_mla_decode: out [nodes, heads, 512] expected");
+  } else {
+    result = at::empty({nodes, heads, DSR_V_DIM}, q.options());
+  }
+  at::Tensor lse = return_lse ? at::empty({nodes, heads}, q.options().dtype(at::kFloat)) : at::Tensor();
+  const size_t ws_bytes = dsr_tree_mla_workspace_bytes(batch, heads, max_nodes);
+  auto ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  ok(dsr_tree_mla_decode(q.data_ptr(), dtype, bf16(kv_pool), kv_pool.size(0) / DSR_BLOCK_TOKENS,
+                         block_table.data_ptr<int32_t>(), block_table.size(1), context.data_ptr<int32_t>(),
+                         cu_nodes.data_ptr<int32_t>(), tree_mask.data_ptr<int64_t>(), max_nodes,
+                         sink ? sink->data_ptr<float>() : nullptr, static_cast<float>(scale), result.data_ptr(),
+                         element_type(result, "tree_mla_decode"), return_lse ? lse.data_ptr<float>() : nullptr,
+                         ws.data_ptr(), ws_bytes, error.data_ptr<int32_t>(), batch, nodes, heads, current_stream()));
+  if (return_lse) return {result, error, lse};
+  return {result, error};
+}
+
 std::vector<at::Tensor> ds_sample_logits(at::Tensor logits, at::Tensor temperature, at::Tensor top_k,
                                          at::Tensor top_p, at::Tensor min_p, at::Tensor uniform,
                                          c10::optional<at::Tensor> status) {
@@ -633,6 +681,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("status") = py::none());
   m.def("rope", &ds_rope, py::arg("x"), py::arg("out"), py::arg("positions"), py::arg("frequencies"),
         py::arg("offsets"), py::arg("interleaved"), py::arg("mscale") = 1.0, py::arg("inverse") = false,
+        py::arg("status") = py::none());
+  m.def("tree_mla_decode", &ds_tree_mla_decode, py::arg("q"), py::arg("kv_pool"), py::arg("block_table"),
+        py::arg("context"), py::arg("cu_nodes"), py::arg("tree_mask"), py::arg("max_nodes"), py::arg("scale"),
+        py::arg("sink") = py::none(), py::arg("return_lse") = false, py::arg("out") = py::none(),
         py::arg("status") = py::none());
   m.def("sample_logits", &ds_sample_logits, py::arg("logits"), py::arg("temperature"), py::arg("top_k"),
         py::arg("top_p"), py::arg("min_p"), py::arg("uniform"), py::arg("status") = py::none());

@@ -1,0 +1,868 @@
+// MLA attention of drafted tokens over a paged BF16 cache (sm_100a): every node of
+// a request's draft tree attends over all cached rows of the request and over the
+// drafted rows that its mask names (its branch).
+//
+//   out[n,h] = sum_j seen(n,j) e^{s_j} v_j / (e^{sink_h} + sum_j seen(n,j) e^{s_j}),
+//   s_j = scale q[n,h].k_j,  v_j = the leading 512 columns of the 576-wide row k_j,
+//   seen(n,j) = j < context, or bit (j - context) of node n's mask.
+//
+// The (node, head) pairs of a request are its query rows, N of which (16, 32 or 64)
+// form a group.  A work unit is one group x one 128-key tile, as two products:
+//   S^T[key, row] = K[key, :576] Q[row, :576]   (M = 128 keys, N rows)
+//   O^T[dim, row] += V[key, dim] P[row, key]    (M = 128 dims x 4, N rows)
+// so that the key tile, once in shared memory, is the A operand of both (K-major,
+// then MN-major) and O^T of 64 rows takes half of the tensor memory.  The units
+// of all requests, in the order (request, group, tile), are cut into equal runs,
+// one per CTA, whatever the lengths; a group that spans CTAs leaves partials (m, l,
+// unnormalised O in FP32) that tree_combine_kernel joins.
+//
+//   warps 0..3  query -> shared memory, softmax over the tile's keys (running
+//               maximum; O is rescaled only when a maximum grows by more than 2^8),
+//               output
+//   warp 4      TMEM and the MMAs
+//   warp 5      key tiles by TMA: column blocks 0..7 (the value columns) through a
+//               ring of block pairs that the O MMA frees pair by pair, block 8 (the
+//               rotary columns) in a buffer that P^T takes over once S^T is done
+#include <math_constants.h>
+
+#include "common.cuh"
+#include "host_common.h"
+
+namespace dsr {
+namespace {
+
+constexpr int kTreeThreads = 192;
+constexpr int kTreeKeys = 128;
+constexpr int kTreeD = DSR_KV_DIM, kTreeDv = DSR_V_DIM;
+constexpr int kTreeMaxNodes = 64;
+constexpr float kTreeLog2e = 1.4426950408889634f;
+constexpr float kTreeSlack = 8.f;  // log2 units a row's maximum may lag behind
+
+template <int N>
+struct TreeLayout {
+  static constexpr int kPairs = N == 64 ? 4 : 5;        // ring of 32 KB block pairs
+  static constexpr int kRingOff = 0;
+  static constexpr int kROff = kPairs * 32768;          // rotary block, then P^T
+  static constexpr int kQOff = kROff + 16384;           // 9 x N x 128 B
+  static constexpr int kBarOff = kQOff + 9 * N * 128;
+  static constexpr int kBars = 2 * kPairs + 6;
+  static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N] seen-masks of the rows
+  static constexpr int kRedOff = kMaskOff + N * 8;      // f32[4][N] per-warp maxima, then sums
+  static constexpr int kStatOff = kRedOff + 4 * N * 4;  // f32[N] factors / reciprocals
+  static constexpr int kMiscOff = kStatOff + N * 4;
+  static constexpr int kBytes = kMiscOff + 64;
+  static constexpr int kAlloc = kBytes + 1024;
+  static constexpr uint32_t kTmemCols = N == 64 ? 512 : (N == 32 ? 256 : 128);  // >= 5 N
+  static_assert(2 * N * 128 <= 16384, "P^T fits the rotary block's buffer");
+  static_assert(kAlloc <= 232448, "shared memory of one CTA");
+};
+
+struct TreeArgs {
+  const void* q;
+  bool q_wide, out_wide;  // fp32 (else bf16)
+  const int32_t* table;
+  int64_t stride, pool_rows;
+  const int32_t* context;
+  const int32_t* cu_nodes;
+  const int64_t* masks;
+  const float* sink;  // nullable
+  float scale_log2;
+  void* out;
+  float* lse;  // nullable
+  int32_t* err;
+  int64_t* unit_start;  // [batch + 1]
+  float* part_o;        // [2 * CTAs][N][512]
+  float* part_m;        // [2 * CTAs][N]
+  float* part_l;
+  int64_t nodes;
+  int batch, heads, max_nodes, ctas;
+};
+
+// ---- the work of request b
+struct TreeSeq {
+  int32_t node0, nodes, context, tiles, groups;
+  bool ok;
+};
+template <int N>
+__device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
+  const int32_t n0 = a.cu_nodes[b], n1 = a.cu_nodes[b + 1], ctx = a.context[b];
+  TreeSeq s{n0, 0, ctx, 0, 0, true};
+  if (n0 < 0 || n1 < n0 || n1 > a.nodes || n1 - n0 > a.max_nodes || ctx < 0 ||
+      int64_t(ctx) + (n1 - n0) > a.stride * DSR_BLOCK_TOKENS) {
+    s.ok = false;
+    s.node0 = s.context = 0;
+    return s;
+  }
+  s.nodes = n1 - n0;
+  s.tiles = int32_t((int64_t(ctx) + s.nodes + kTreeKeys - 1) / kTreeKeys);
+  s.groups = (s.nodes * a.heads + N - 1) / N;
+  if (s.nodes == 0) s.tiles = 0;
+  return s;
+}
+
+// ---- a CTA's run of units, walked segment by segment (one group's consecutive tiles)
+template <int N>
+struct TreeWalk {
+  const TreeArgs& a;
+  int64_t u, end, base;  // base: first unit of request b
+  int b, group, tile0, count;
+  TreeSeq s;
+  __device__ __forceinline__ TreeWalk(const TreeArgs& args, int64_t first, int64_t last, int b0, int64_t base0)
+      : a(args), u(first), end(last), base(base0), b(b0), group(0), tile0(0), count(0) {
+    if (u < end) s = tree_seq<N>(a, b);
+  }
+  __device__ __forceinline__ bool next() {
+    u += count;
+    if (u >= end) return false;
+    int64_t units = int64_t(s.groups) * s.tiles;
+    while (u >= base + units) {
+      base += units;
+      s = tree_seq<N>(a, ++b);
+      units = int64_t(s.groups) * s.tiles;
+    }
+    const int64_t at = u - base;
+    group = int(at / s.tiles);
+    tile0 = int(at - int64_t(group) * s.tiles);
+    const int64_t left = end - u;
+    count = int(left < s.tiles - tile0 ? left : s.tiles - tile0);
+    return true;
+  }
+};
+
+__device__ __forceinline__ int64_t run_start(int64_t units, int c, int ctas) { return units * c / ctas; }
+// The CTA whose run holds unit u.
+__device__ __forceinline__ int run_of(int64_t units, int64_t u, int ctas) { return int(((u + 1) * ctas - 1) / units); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// 16 TMEM lanes x 8 C columns: thread i holds lanes i/4 and i/4 + 8 (of the 16),
+// columns 8c + 2(i%4) and the next: r[4c + 2h + e] is lane i/4 + 8h, column + e.
+template <int C>
+__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t (&r)[4 * C]) {
+  static_assert(C == 2 || C == 4 || C == 8, "");
+  if constexpr (C == 2) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+  } else if constexpr (C == 4) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr));
+  }
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Four 8x8 b16 matrices (row i/4, columns 2(i%4).. in thread i's register) stored
+// transposed: thread i gives the address of row i%8 of the transposed matrix i/8.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(r0), "r"(r1),
+               "r"(r2), "r"(r3)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// All 128 softmax threads: the barrier, and whether every one of them is fine.
+__device__ __forceinline__ bool softmax_sync(bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(ok))
+      : "memory");
+  return r != 0;
+}
+
+// A row's total with its head's sink (in units of 2^top), and the logarithm of its sum.
+__device__ __forceinline__ float tree_total(const TreeArgs& a, int head, float top, float sum, float& total) {
+  total = sum;
+  if (a.sink == nullptr) return top == -CUDART_INF_F ? top : (top + log2f(sum)) / kTreeLog2e;
+  float sink = a.sink[head];
+  if (!isfinite(sink)) {
+    flag(a.err, DSR_ERR_NONFINITE);
+    sink = 0.f;
+  }
+  if (top == -CUDART_INF_F) return sink;
+  const float over = sink * kTreeLog2e - top;  // the sink's weight, log2
+  total = sum + ex2(over);
+  return over > 100.f ? sink : (top + log2f(total)) / kTreeLog2e;
+}
+
+// Value column d = this thread's of 16 consecutive rows (of which `rows` exist);
+// returns whether one is not finite.
+__device__ __forceinline__ bool tree_store16(const TreeArgs& a, int64_t row, int rows, int d, int lane,
+                                             const float (&x)[16]) {
+  bool bad = false;
+  if (a.out_wide) {
+    float* dst = static_cast<float*>(a.out) + row * kTreeDv + d;
+#pragma unroll
+    for (int y = 0; y < 16; ++y)
+      if (y < rows) {
+        dst[int64_t(y) * kTreeDv] = x[y];
+        bad |= !isfinite(x[y]);
+      }
+  } else {
+    // lanes 2i and 2i + 1 swap halves of two rows: each stores two columns of one
+    const int odd = lane & 1;
+    uint16_t* dst = static_cast<uint16_t*>(a.out) + (row + odd) * kTreeDv + (d - odd);
+#pragma unroll
+    for (int y = 0; y < 16; y += 2) {
+      const float mine = odd ? x[y + 1] : x[y], other = __shfl_xor_sync(~0u, odd ? x[y] : x[y + 1], 1);
+      if (y + odd < rows) {
+        *reinterpret_cast<uint32_t*>(dst + int64_t(y) * kTreeDv) = odd ? bf16x2(other, mine) : bf16x2(mine, other);
+        bad |= !isfinite(mine) || !isfinite(other);
+      }
+    }
+  }
+  return bad;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kTreeThreads, 1)
+    tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeArgs a) {
+  using L = TreeLayout<N>;
+  constexpr int C = N / 8;  // 8-row column chunks of S^T
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  uint64_t* full = bars;                    // [kPairs] block pair loaded (TMA bytes + 1)
+  uint64_t* empty = bars + L::kPairs;       // [kPairs] block pair read by the O MMA (commit)
+  uint64_t* bar_r = bars + 2 * L::kPairs;   // rotary block loaded
+  uint64_t* bar_s = bar_r + 1;              // S^T complete (commit)
+  uint64_t* bar_p = bar_r + 2;              // P^T written (128 arrivals)
+  uint64_t* bar_o = bar_r + 3;              // the tile's O MMAs complete (commit)
+  uint64_t* bar_q = bar_r + 4;              // query in place (128 arrivals)
+  uint64_t* bar_free = bar_r + 5;           // O^T read by the epilogue (128 arrivals)
+  uint64_t* masks = reinterpret_cast<uint64_t*>(smem + L::kMaskOff);
+  float* red = reinterpret_cast<float*>(smem + L::kRedOff);
+  float* stat = reinterpret_cast<float*>(smem + L::kStatOff);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  int* first_b = reinterpret_cast<int*>(smem + L::kMiscOff + 8);
+  int* loaded = reinterpret_cast<int*>(smem + L::kMiscOff + 12);    // block pairs requested, for an abort
+  int* loaded_r = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // rotary blocks
+  int64_t* first_base = reinterpret_cast<int64_t*>(smem + L::kMiscOff + 24);
+  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);  // [6], before the ring is used
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  if (tid == 0) {
+    tma_prefetch_desc(&kv_map);
+    for (int i = 0; i < L::kPairs; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
+    mbar_init(bar_r, 1);
+    mbar_init(bar_s, 1);
+    mbar_init(bar_p, 128);
+    mbar_init(bar_o, 1);
+    mbar_init(bar_q, 128);
+    mbar_init(bar_free, 128);
+    *abort = 0;
+    *loaded = *loaded_r = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(tmem_slot, L::kTmemCols);
+    tmem_relinquish();
+  }
+
+  // ---- units before each thread's run of requests, and in all
+  const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
+  const int r0 = min(tid * per, a.batch), r1 = min(r0 + per, a.batch);
+  int64_t own = 0;
+  for (int b = r0; b < r1; ++b) {
+    const TreeSeq s = tree_seq<N>(a, b);
+    if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
+    own += int64_t(s.groups) * s.tiles;
+  }
+  int64_t run = own;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(~0u, run, d);
+    if (lane >= d) run += up;
+  }
+  if (lane == 31) warp_units[warp] = run;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  int64_t before = run - own, units = 0;
+  for (int w = 0; w < kTreeThreads / 32; ++w) {
+    if (w < warp) before += warp_units[w];
+    units += warp_units[w];
+  }
+  const int ctas = int(units < a.ctas ? units : a.ctas);
+  int64_t w0 = 0, w1 = 0;
+  if (int(blockIdx.x) < ctas) {
+    w0 = run_start(units, blockIdx.x, ctas);
+    w1 = run_start(units, blockIdx.x + 1, ctas);
+    if (w0 >= before && w0 < before + own) {
+      int64_t base = before;
+      int b = r0;
+      for (;; ++b) {
+        const TreeSeq s = tree_seq<N>(a, b);
+        const int64_t n = int64_t(s.groups) * s.tiles;
+        if (w0 < base + n) break;
+        base += n;
+      }
+      *first_b = b;
+      *first_base = base;
+    }
+  }
+  if (blockIdx.x == 0) {
+    for (int b = r0; b < r1; ++b) {
+      const TreeSeq s = tree_seq<N>(a, b);
+      a.unit_start[b] = before;
+      before += int64_t(s.groups) * s.tiles;
+    }
+    if (tid == 0) a.unit_start[a.batch] = units;
+  }
+  __syncthreads();
+  const uint32_t tmem_o = *tmem_slot, tmem_s = tmem_o + 4 * N;
+  TreeWalk<N> walk(a, w0, w1, w0 < w1 ? *first_b : 0, w0 < w1 ? *first_base : 0);
+  pdl_launch_dependents();
+
+  if (warp < 4) {
+    // ------------------------------------------------------------ softmax
+    const int quad = lane >> 2, pairc = 2 * (lane & 3);  // key of a fragment, first of its two rows
+    int n = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const TreeSeq s = walk.s;
+      const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
+      const int64_t qrow = int64_t(s.node0) * a.heads + row0;
+      // ---- query rows -> bf16, K-major, 128-byte swizzle
+      constexpr int kVec = N * (kTreeD / 8), kBatch = 6;
+      for (int i0 = tid; i0 < kVec; i0 += 128 * kBatch) {
+        uint4 v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + 128 * j, r = i / (kTreeD / 8);
+          v[j] = make_uint4(0, 0, 0, 0);
+          if (i < kVec && r < rows) {
+            const int64_t at = (qrow + r) * kTreeD + (i - r * (kTreeD / 8)) * 8;
+            if (a.q_wide) {
+              const float4 lo = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
+              const float4 hi = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at) + 1);
+              v[j] = make_uint4(bf16x2(lo.x, lo.y), bf16x2(lo.z, lo.w), bf16x2(hi.x, hi.y), bf16x2(hi.z, hi.w));
+            } else {
+              v[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at));
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          const int i = i0 + 128 * j, r = i / (kTreeD / 8), d = (i - r * (kTreeD / 8)) * 8;
+          if (i < kVec)
+            *reinterpret_cast<uint4*>(smem + L::kQOff + (d >> 6) * (N * 128) + sw128_offset(r, d & 63)) = v[j];
+        }
+      }
+      if (tid < N) masks[tid] = tid < rows ? uint64_t(a.masks[s.node0 + (row0 + tid) / a.heads]) : 0ull;
+      fence_proxy_async_smem();
+      mbar_arrive(bar_q);
+
+      float m[C][2], l[C][2];
+#pragma unroll
+      for (int c = 0; c < C; ++c) m[c][0] = m[c][1] = -CUDART_INF_F, l[c][0] = l[c][1] = 0.f;
+      for (int i = 0; i < walk.count; ++i, ++n) {
+        const int32_t p0 = (walk.tile0 + i) * kTreeKeys;
+        ok = mbar_wait(bar_s, n & 1, abort, a.err);
+        // ---- scores of keys 32 warp + quad + 8j, rows 8c + pairc + e
+        float v[C][4][2];
+        if (ok) {
+          tc_fence_after();
+          uint32_t t0[4 * C], t1[4 * C];
+          const uint32_t at = tmem_s + (uint32_t(warp * 32) << 16);
+          tmem_ld_16x256<C>(at, t0);
+          tmem_ld_16x256<C>(at + (16u << 16), t1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              v[c][0][e] = __uint_as_float(t0[4 * c + e]);
+              v[c][1][e] = __uint_as_float(t0[4 * c + 2 + e]);
+              v[c][2][e] = __uint_as_float(t1[4 * c + e]);
+              v[c][3][e] = __uint_as_float(t1[4 * c + 2 + e]);
+            }
+          if (s.context - p0 < kTreeKeys) {  // drafted rows, or past the end
+            const int32_t drafted = p0 - s.context;
+            uint64_t any = 0;
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint64_t word = masks[8 * c + pairc + e];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const int32_t d = drafted + warp * 32 + quad + 8 * j;
+                  if (d >= 0 && (d >= s.nodes || !(word >> d & 1))) v[c][j][e] = -CUDART_INF_F;
+                }
+              }
+            // a row that no node of the group sees may hold anything: it is cleared,
+            // since 0 x NaN would reach the output
+            for (int r = 0; r < N; ++r) any |= masks[r];
+            const int32_t d = drafted + tid;
+            if (d >= 0 && (d >= s.nodes || !(any >> d & 1))) {
+#pragma unroll 1
+              for (int c = 0; c < 8; ++c) {
+                const int slot = (4 * n + (c >> 1)) % L::kPairs;
+                uint4* dst = reinterpret_cast<uint4*>(smem + L::kRingOff + slot * 32768 + (c & 1) * 16384 + tid * 128);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
+              }
+            }
+          }
+          // ---- maximum of each row over this warp's keys
+#pragma unroll
+          for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float x = fmaxf(fmaxf(v[c][0][e], v[c][1][e]), fmaxf(v[c][2][e], v[c][3][e]));
+              x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
+              x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
+              x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
+              if (quad == 0) red[warp * N + 8 * c + pairc + e] = x;
+            }
+        }
+        ok = softmax_sync(ok);
+        if (!ok) break;
+        // ---- running maximum: every thread follows its rows, all alike
+        bool grows = false;
+        float f[C][2];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float2 x = *reinterpret_cast<const float2*>(red + 8 * c + pairc);
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            const float2 y = *reinterpret_cast<const float2*>(red + w * N + 8 * c + pairc);
+            x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
+          }
+          const float t[2] = {x.x * a.scale_log2, x.y * a.scale_log2};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            f[c][e] = 1.f;
+            if (t[e] > m[c][e] + kTreeSlack || (m[c][e] == -CUDART_INF_F && t[e] > -CUDART_INF_F)) {
+              f[c][e] = ex2(m[c][e] - t[e]);  // 0 when the row had seen nothing
+              l[c][e] *= f[c][e];
+              m[c][e] = t[e];
+              grows = true;
+            }
+          }
+        }
+        if (i > 0 && __any_sync(~0u, grows)) {  // a warp holds every row: all warps decide alike
+          if (warp == 0 && quad == 0) {
+#pragma unroll
+            for (int c = 0; c < C; ++c) stat[8 * c + pairc] = f[c][0], stat[8 * c + pairc + 1] = f[c][1];
+          }
+          softmax_sync(true);
+#pragma unroll 1
+          for (int col = 0; col < 4 * N; col += 16) {
+            uint32_t o[16];
+            const uint32_t at = tmem_o + col + (uint32_t(warp * 32) << 16);
+            tmem_ld16(at, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * stat[(col & (N - 1)) + x]);
+            tmem_st16(at, o);
+          }
+          tmem_wait_st();
+        }
+        // ---- weights, their sums, P^T
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          uint32_t packed[4];
+          const float b0 = m[c][0] == -CUDART_INF_F ? 0.f : m[c][0], b1 = m[c][1] == -CUDART_INF_F ? 0.f : m[c][1];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float x = ex2(fmaf(v[c][j][0], a.scale_log2, -b0)), y = ex2(fmaf(v[c][j][1], a.scale_log2, -b1));
+            l[c][0] += x;
+            l[c][1] += y;
+            packed[j] = bf16x2(x, y);
+          }
+          const int r = 8 * c + (lane & 7), key = warp * 32 + 8 * (lane >> 3);
+          stmatrix_x4_trans(sbase + L::kROff + (key >> 6) * (N * 128) + sw128_offset(r, key & 63), packed[0], packed[1],
+                            packed[2], packed[3]);
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(bar_p);
+      }
+      if (!ok) break;
+
+      // ---- output of the segment: sums over the keys' threads, then O^T.  The last O
+      // MMA follows every thread's last use of red and stat
+      ok = mbar_wait(bar_o, (n - 1) & 1, abort, a.err);
+      const bool whole = walk.count == s.tiles;
+      const int slot = 2 * int(blockIdx.x) + (walk.tile0 > 0 ? 0 : 1);
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = l[c][e];
+          x += __shfl_xor_sync(~0u, x, 4);
+          x += __shfl_xor_sync(~0u, x, 8);
+          x += __shfl_xor_sync(~0u, x, 16);
+          if (quad == 0) {
+            red[warp * N + 8 * c + pairc + e] = x;
+            if (warp == 0) stat[8 * c + pairc + e] = m[c][e];
+          }
+        }
+      ok = softmax_sync(ok);
+      if (!ok) break;
+      if (tid < N) {
+        const float sum = (red[tid] + red[N + tid]) + (red[2 * N + tid] + red[3 * N + tid]), top = stat[tid];
+        if (tid < rows && !(sum < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
+        if (whole) {
+          float total;
+          const float lse = tree_total(a, (row0 + tid) % a.heads, top, sum, total);
+          stat[tid] = total > 0.f ? 1.f / total : 0.f;
+          if (a.lse != nullptr && tid < rows) a.lse[qrow + tid] = lse;
+        } else {
+          a.part_m[int64_t(slot) * N + tid] = top;
+          a.part_l[int64_t(slot) * N + tid] = sum;
+          stat[tid] = 1.f;
+        }
+      }
+      softmax_sync(true);
+      tc_fence_after();
+      bool bad = false;
+#pragma unroll 1
+      for (int col = 0; col < 4 * N; col += 16) {
+        uint32_t o[16];
+        tmem_ld16(tmem_o + col + (uint32_t(warp * 32) << 16), o);
+        tmem_wait_ld();
+        const int d = (col / N) * 128 + tid, r = col & (N - 1);
+        float x[16];
+#pragma unroll
+        for (int y = 0; y < 16; ++y) x[y] = __uint_as_float(o[y]) * stat[r + y];
+        if (!whole) {
+          float* dst = a.part_o + (int64_t(slot) * N + r) * kTreeDv + d;
+#pragma unroll
+          for (int y = 0; y < 16; ++y)
+            if (r + y < rows) dst[y * kTreeDv] = x[y];
+        } else {
+          bad |= tree_store16(a, qrow + r, rows - r, d, lane, x);
+        }
+      }
+      if (bad) flag(a.err, DSR_ERR_NONFINITE);
+      tc_fence_before();
+      mbar_arrive(bar_free);
+    }
+  } else if (warp == 4 && lane == 0) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, N, false, false);
+    constexpr uint32_t idesc_o = umma_idesc_bf16(128, N, true, false);
+    int n = 0, segment = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      ok = mbar_wait(bar_q, segment & 1, abort, a.err);
+      for (int i = 0; i < walk.count && ok; ++i, ++n) {
+        // S^T: column blocks 0..7 pair by pair, then the rotary block
+#pragma unroll 1
+        for (int c = 0; c < 5 && ok; ++c) {
+          const int k = 4 * n + c;
+          ok = c < 4 ? mbar_wait(full + k % L::kPairs, (k / L::kPairs) & 1, abort, a.err)
+                     : mbar_wait(bar_r, n & 1, abort, a.err);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t key = sbase + (c < 4 ? L::kRingOff + (k % L::kPairs) * 32768 : L::kROff);
+          const int steps = c < 4 ? 8 : 4;
+#pragma unroll 4
+          for (int x = 0; x < steps; ++x) {
+            const uint64_t ad = umma_desc_sw128(key + (x >> 2) * 16384 + (x & 3) * 32, 16, 1024);
+            const uint64_t bd =
+                umma_desc_sw128(sbase + L::kQOff + (2 * c + (x >> 2)) * (N * 128) + (x & 3) * 32, 16, 1024);
+            umma_bf16(tmem_s, ad, bd, idesc_s, (c | x) != 0 ? 1u : 0u);
+          }
+        }
+        if (!ok) break;
+        umma_commit(bar_s);
+        ok = mbar_wait(bar_p, n & 1, abort, a.err);
+        // the previous segment's O^T has been read
+        if (ok && i == 0 && segment > 0) ok = mbar_wait(bar_free, (segment - 1) & 1, abort, a.err);
+        if (!ok) break;
+        tc_fence_after();
+        // O^T, 128 value columns after another, so that their block pair is free early
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const int pair = (4 * n + c) % L::kPairs;
+#pragma unroll
+          for (int ks = 0; ks < kTreeKeys / 16; ++ks) {
+            const uint64_t ad = umma_desc_sw128(sbase + L::kRingOff + pair * 32768 + ks * 2048, 16384, 1024);
+            const uint64_t bd =
+                umma_desc_sw128(sbase + L::kROff + (ks >> 2) * (N * 128) + (ks & 3) * 32, 16, 1024);
+            umma_bf16(tmem_o + c * N, ad, bd, idesc_o, (i > 0 || ks > 0) ? 1u : 0u);
+          }
+          umma_commit(empty + pair);
+        }
+        umma_commit(bar_o);
+      }
+      ++segment;
+    }
+    // the last MMAs retire before TMEM is released (commits cover all before them)
+    if (n > 0) mbar_drain(bar_o, (n - 1) & 1);
+  } else if (warp == 5 && lane == 0) {
+    // ------------------------------------------------------------ key tiles
+    int n = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const TreeSeq s = walk.s;
+      const int32_t* table = a.table + int64_t(walk.b) * a.stride;
+      const int32_t blocks = int32_t((int64_t(s.context) + s.nodes + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS);
+      auto row_of = [&](int32_t j) -> int32_t {  // first pool row of block j; past the pool: reads zeros
+        if (j >= blocks) return int32_t(a.pool_rows);
+        const int64_t blk = table[j];
+        if (blk < 0 || blk * DSR_BLOCK_TOKENS >= a.pool_rows) {
+          flag(a.err, DSR_ERR_ID);
+          return int32_t(a.pool_rows);
+        }
+        return int32_t(blk * DSR_BLOCK_TOKENS);
+      };
+      int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
+      for (int i = 0; i < walk.count && ok; ++i, ++n) {
+        const int32_t x0 = y0, x1 = y1;
+        if (i + 1 < walk.count) y0 = row_of(2 * (walk.tile0 + i) + 2), y1 = row_of(2 * (walk.tile0 + i) + 3);
+#pragma unroll 1
+        for (int c = 0; c < 4; ++c) {
+          const int k = 4 * n + c, pair = k % L::kPairs;
+          ok = mbar_wait(empty + pair, ((k / L::kPairs) & 1) ^ 1, abort, a.err);
+          if (!ok) break;
+          mbar_arrive_expect_tx(full + pair, 32768);
+          const uint32_t dst = sbase + L::kRingOff + pair * 32768;
+          for (int h = 0; h < 2; ++h) {
+            tma_load_2d(dst + h * 16384, &kv_map, full + pair, (2 * c + h) * 64, x0);
+            tma_load_2d(dst + h * 16384 + 8192, &kv_map, full + pair, (2 * c + h) * 64, x1);
+          }
+          *loaded = k + 1;
+        }
+        // P^T of the tile before sits in the rotary buffer until its O MMAs are done
+        if (ok && n > 0) ok = mbar_wait(bar_o, (n - 1) & 1, abort, a.err);
+        if (!ok) break;
+        mbar_arrive_expect_tx(bar_r, 16384);
+        tma_load_2d(sbase + L::kROff, &kv_map, bar_r, 512, x0);
+        tma_load_2d(sbase + L::kROff + 8192, &kv_map, bar_r, 512, x1);
+        *loaded_r = n + 1;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort && tid == 0) {
+    // a wait gave up: let the copies in flight land before exit
+    for (int k = max(0, *loaded - L::kPairs); k < *loaded; ++k) mbar_drain(full + k % L::kPairs, (k / L::kPairs) & 1);
+    if (*loaded_r > 0) mbar_drain(bar_r, (*loaded_r - 1) & 1);
+  }
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem_o, L::kTmemCols);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Joins the partials of a group that spans CTAs: one CTA per query row, thread t
+// four value columns.  out = sum_p 2^(m_p - M) O_p / (2^(sink - M) + sum_p 2^(m_p - M) l_p).
+// ---------------------------------------------------------------------------
+constexpr int kTreeMaxCtas = 256;  // partials of one row at most
+
+template <int N>
+__global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
+  __shared__ float weight[kTreeMaxCtas];
+  __shared__ float inverse;
+  const int64_t row = blockIdx.x;
+  const int32_t node = int32_t(row / a.heads);
+  const int tid = threadIdx.x;
+  // the request of the node: the largest b with cu_nodes[b] <= node
+  int lo = 0, hi = a.batch;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_nodes[mid] <= node) lo = mid;
+    else hi = mid;
+  }
+  const TreeSeq s = tree_seq<N>(a, lo);
+  if (node < s.node0 || node >= s.node0 + s.nodes) return;
+  pdl_wait();
+  const int64_t units = a.unit_start[a.batch];
+  const int in = int(row - int64_t(s.node0) * a.heads), group = in / N, r = in % N;
+  const int64_t u0 = a.unit_start[lo] + int64_t(group) * s.tiles;
+  const int ctas = int(units < a.ctas ? units : a.ctas);
+  const int c0 = run_of(units, u0, ctas), c1 = run_of(units, u0 + s.tiles - 1, ctas);
+  if (c0 == c1) return;  // whole in one CTA, written there
+  const int parts = c1 - c0 + 1;
+  auto slot = [&](int p) { return int64_t(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * N + r; };
+  if (tid < 32) {
+    float top = -CUDART_INF_F, sum = 0.f;
+    for (int p = tid; p < parts; p += 32) top = fmaxf(top, a.part_m[slot(p)]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    const float base = top == -CUDART_INF_F ? 0.f : top;
+    for (int p = tid; p < parts; p += 32) {
+      const float w = ex2(a.part_m[slot(p)] - base);
+      weight[p] = w;
+      sum += w * a.part_l[slot(p)];
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+    if (tid == 0) {
+      float total;
+      const float lse = tree_total(a, int(row % a.heads), top, sum, total);
+      inverse = total > 0.f ? 1.f / total : 0.f;
+      if (a.lse != nullptr) a.lse[row] = lse;
+    }
+  }
+  __syncthreads();
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (p0 + j < parts) v[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(p0 + j) * kTreeDv) + tid);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (p0 + j < parts) {
+        const float w = weight[p0 + j];
+        acc.x = fmaf(w, v[j].x, acc.x), acc.y = fmaf(w, v[j].y, acc.y);
+        acc.z = fmaf(w, v[j].z, acc.z), acc.w = fmaf(w, v[j].w, acc.w);
+      }
+  }
+  const float f = inverse;
+  acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+  if (!(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w))) flag(a.err, DSR_ERR_NONFINITE);
+  if (a.out_wide)
+    reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * kTreeDv)[tid] = acc;
+  else
+    reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * kTreeDv)[tid] =
+        make_uint2(bf16x2(acc.x, acc.y), bf16x2(acc.z, acc.w));
+}
+
+// Rows per group: all of a request's rows in one group when that fits, since a
+// group reads every key tile once.
+int tree_rows(int64_t heads, int64_t max_nodes) {
+  const int64_t rows = heads * max_nodes;
+  return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+}
+
+size_t tree_start_bytes(int64_t batch) { return (size_t(batch + 1) * 8 + 255) / 256 * 256; }
+
+template <int N>
+int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStream_t stream) {
+  using L = TreeLayout<N>;
+  int rc = set_max_smem(tree_mla_kernel<N>, L::kAlloc, "tree_mla_decode");
+  if (rc != DSR_OK) return rc;
+  CUtensorMap map;  // one page by 64 columns
+  rc = encode_tmap_bf16_2d(&map, kv_pool, kTreeD, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
+  if (rc != DSR_OK) return rc;
+  a.unit_start = static_cast<int64_t*>(workspace);
+  a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_start_bytes(a.batch));
+  a.part_m = a.part_o + size_t(2) * a.ctas * N * kTreeDv;
+  a.part_l = a.part_m + size_t(2) * a.ctas * N;
+  tree_mla_kernel<N><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, a);
+  rc = launch_status("tree_mla_decode launch");
+  if (rc != DSR_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.nodes * a.heads), 1, 1);
+  cfg.blockDim = dim3(128, 1, 1);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_combine_kernel<N>, a);
+  if (e != cudaSuccess) return fail(DSR_ECUDA, "tree_mla_decode combine launch: %s", cudaGetErrorString(e));
+  return DSR_OK;
+}
+
+}  // namespace
+}  // namespace dsr
+
+extern "C" size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes) {
+  using namespace dsr;
+  if (batch <= 0 || heads <= 0 || max_nodes <= 0) return 0;
+  const size_t rows = size_t(2) * sm_count() * tree_rows(heads, max_nodes);
+  return tree_start_bytes(batch) + rows * (kTreeDv + 2) * 4;
+}
+
+extern "C" int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
+                                   const int32_t* block_table, int64_t table_stride, const int32_t* context,
+                                   const int32_t* cu_nodes, const int64_t* tree_mask, int64_t max_nodes,
+                                   const float* sink, float scale, void* out, int out_dtype, float* lse,
+                                   void* workspace, size_t workspace_bytes, int32_t* err, int64_t batch,
+                                   int64_t nodes, int64_t heads, void* stream) {
+  using namespace dsr;
+  clear_error();
+  PoolAddr pa;
+  const int rc = paged_addr(&pa, block_table, table_stride, pool_blocks, "tree_mla_decode");
+  if (rc != DSR_OK) return rc;
+  DSR_REQUIRE(q && kv_pool && context && cu_nodes && tree_mask && out && workspace && err,
+              "tree_mla_decode: null pointer");
+  DSR_REQUIRE((q_dtype == DSR_BF16 || q_dtype == DSR_F32) && (out_dtype == DSR_BF16 || out_dtype == DSR_F32),
+              "tree_mla_decode: unknown element type");
+  DSR_REQUIRE(heads == 16 || heads == 32 || heads == 64 || heads == 128,
+              "tree_mla_decode: heads %lld not in {16,32,64,128}", (long long)heads);
+  DSR_REQUIRE(max_nodes > 0 && max_nodes <= kTreeMaxNodes, "tree_mla_decode: max nodes %lld outside [1, %d]",
+              (long long)max_nodes, kTreeMaxNodes);
+  DSR_REQUIRE(batch > 0 && batch <= 65535, "tree_mla_decode: batch %lld outside [1, 65535]", (long long)batch);
+  DSR_REQUIRE(nodes > 0 && nodes <= int64_t(65535) * kTreeMaxNodes, "tree_mla_decode: nodes %lld outside [1, %d]",
+              (long long)nodes, 65535 * kTreeMaxNodes);
+  DSR_REQUIRE(isfinite(scale) && scale > 0.f, "invalid attention scale");
+  DSR_REQUIRE(aligned16(q) && aligned16(kv_pool) && aligned16(out),
+              "tree_mla_decode: q, kv_pool and out must be 16-byte aligned");
+  DSR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0, "tree_mla_decode: workspace must be 256-byte aligned");
+  const size_t need = dsr_tree_mla_workspace_bytes(batch, heads, max_nodes);
+  DSR_REQUIRE(workspace_bytes >= need, "tree_mla_decode: workspace %zu < %zu bytes", workspace_bytes, need);
+  TreeArgs a = {};
+  a.q = q;
+  a.q_wide = q_dtype == DSR_F32;
+  a.out_wide = out_dtype == DSR_F32;
+  a.table = block_table;
+  a.stride = table_stride;
+  a.pool_rows = pa.rows;
+  a.context = context;
+  a.cu_nodes = cu_nodes;
+  a.masks = tree_mask;
+  a.sink = sink;
+  a.scale_log2 = scale * kTreeLog2e;
+  a.out = out;
+  a.lse = lse;
+  a.err = err;
+  a.nodes = nodes;
+  a.batch = int(batch);
+  a.heads = int(heads);
+  a.max_nodes = int(max_nodes);
+  a.ctas = sm_count() < kTreeMaxCtas ? sm_count() : kTreeMaxCtas;
+  switch (tree_rows(heads, max_nodes)) {
+    case 16:
+      return launch_tree<16>(a, kv_pool, workspace, as_stream(stream));
+    case 32:
+      return launch_tree<32>(a, kv_pool, workspace, as_stream(stream));
+    default:
+      return launch_tree<64>(a, kv_pool, workspace, as_stream(stream));
+  }
+}

@@ -129,6 +129,17 @@ def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float
     return list(out)
 
 
+def tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes: int, *, scale: float,
+                    sink=None, out=None, return_lse: bool = False):
+    """Attention of drafted tokens over their request's cached rows and their own branch."""
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValidationError("invalid attention scale")
+    result = extension().tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes, scale,
+                                         sink=sink, return_lse=return_lse, out=out)
+    _status(result[1])
+    return (result[0], result[2]) if return_lse else result[0]
+
+
 def sample_logits(logits, temperature, top_k, top_p, min_p, uniform):
     """One token per row after temperature, top-k, top-p and min-p; returns (tokens, chances)."""
     tokens, chances, status = extension().sample_logits(logits, temperature, top_k, top_p, min_p, uniform)

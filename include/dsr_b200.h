@@ -485,6 +485,34 @@ int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int32_t* posit
              const double* frequencies, int64_t pairs, float mscale, int inverse, int32_t* err,
              int64_t tokens, void* stream);
 
+/* MLA attention of drafted tokens: node n of request b, i.e. query row n of
+ * q [nodes, heads, 576] (q_dtype) with cu_nodes[b] <= n < cu_nodes[b+1], attends
+ * over the request's positions 0 .. context[b]-1 and over the drafted positions
+ * context[b] + j whose bit j is set in tree_mask[n] (i64, one word a node; a node's
+ * own bit is not implied).  The drafted rows are in the cache already, node j of
+ * the request at position context[b] + j (dsr_append_kv_index).  kv_pool and
+ * block_table as in dsr_sparse_mla_decode; cu_nodes i32[batch+1]; heads in
+ * {16,32,64,128}; at most max_nodes <= 64 nodes a request.
+ *   out [nodes, heads, 512] (out_dtype) = sum_j e^{s_j} v_j / (e^{sink_h} + sum_j e^{s_j})
+ * over what the node sees, s_j = scale q.k_j, v_j the first 512 columns; without
+ * sink (NULL) that term is absent.  A row that sees nothing gives zeros.  lse
+ * f32[nodes,heads] (nullable): the logarithm of the denominator (-inf for zero).
+ * q is contracted as BF16 and the weights e^s are rounded to BF16 before the value
+ * product; sums and statistics are FP32.  Output rows at or past cu_nodes[batch]
+ * are not written.  Status 1: a context or node range that is negative, larger
+ * than max_nodes, `nodes` or the table (that request's rows are not written), or a
+ * block id outside the pool (its keys count as zeros); status 2: a NaN or infinite
+ * score, sink or output.  Cached rows that no node sees may hold anything.
+ * Scratch: dsr_tree_mla_workspace_bytes() on the current device, 256-byte
+ * aligned, need not be cleared; calls sharing it must not overlap. */
+size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes);
+int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
+                        const int32_t* block_table, int64_t table_stride, const int32_t* context,
+                        const int32_t* cu_nodes, const int64_t* tree_mask, int64_t max_nodes,
+                        const float* sink, float scale, void* out, int out_dtype, float* lse,
+                        void* workspace, size_t workspace_bytes, int32_t* err, int64_t batch,
+                        int64_t nodes, int64_t heads, void* stream);
+
 /* One token per row of logits [rows, vocab] (dtype, row_stride elements apart, 0:
  * all rows the same):
  * with w_i = exp((x_i - max)/temperature) and the order (value descending, index
