@@ -16,11 +16,13 @@
 // one per CTA, whatever the lengths; a group that spans CTAs leaves partials (m, l,
 // unnormalised O in FP32) that tree_combine_kernel joins.
 //
-//   warps 0..3  query -> shared memory, softmax over the tile's keys (running
+//   warps 0..7  query -> shared memory, softmax over the tile's keys (running
 //               maximum; O is rescaled only when a maximum grows by more than 2^8),
-//               output
-//   warp 4      TMEM and the MMAs
-//   warp 5      key tiles by TMA: column blocks 0..7 (the value columns) through a
+//               output.  Warps 0..3 have the first half of the group's rows, warps
+//               4..7 the second; warp w and w + 4 hold the tensor memory's lanes
+//               (keys, value columns) 32 w and up
+//   warp 8      TMEM and the MMAs
+//   warp 9      key tiles by TMA: column blocks 0..7 (the value columns) through a
 //               ring of block pairs that the O MMA frees pair by pair, block 8 (the
 //               rotary columns) in a buffer that P^T takes over once S^T is done
 #include <math_constants.h>
@@ -31,7 +33,8 @@
 namespace dsr {
 namespace {
 
-constexpr int kTreeThreads = 192;
+constexpr int kTreeSoftmax = 256;  // warps 0..7
+constexpr int kTreeThreads = kTreeSoftmax + 64;
 constexpr int kTreeKeys = 128;
 constexpr int kTreeD = DSR_KV_DIM, kTreeDv = DSR_V_DIM;
 constexpr int kTreeMaxNodes = 64;
@@ -133,6 +136,38 @@ __device__ __forceinline__ int64_t run_start(int64_t units, int c, int ctas) { r
 // The CTA whose run holds unit u.
 __device__ __forceinline__ int run_of(int64_t units, int64_t u, int ctas) { return int(((u + 1) * ctas - 1) / units); }
 
+// mbar_wait whose polls sleep in the barrier unit until the phase completes (or a few
+// microseconds pass): the ten warps that wait here would otherwise poll shared memory
+// all the time, whose bandwidth the MMAs of 64 columns need to the last byte.
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t start = global_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (global_ns() - start > kWaitNs) {
+      *abort = 1;
+      flag(err, DSR_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -143,36 +178,50 @@ __device__ __forceinline__ float ex2(float x) {
 // columns 8c + 2(i%4) and the next: r[4c + 2h + e] is lane i/4 + 8h, column + e.
 template <int C>
 __device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, uint32_t (&r)[4 * C]) {
-  static_assert(C == 2 || C == 4 || C == 8, "");
-  if constexpr (C == 2) {
+  static_assert(C == 1 || C == 2 || C == 4, "");
+  if constexpr (C == 1) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(taddr));
+  } else if constexpr (C == 2) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                  : "r"(taddr));
-  } else if constexpr (C == 4) {
+  } else {
     asm volatile(
         "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
           "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
-  } else {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x8.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr));
   }
 }
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
-          taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
+// 32 lanes x W columns, thread i lane i
+template <int W>
+__device__ __forceinline__ void tmem_ld_lanes(uint32_t taddr, uint32_t (&r)[W]) {
+  static_assert(W == 8 || W == 16, "");
+  if constexpr (W == 16) {
+    tmem_ld16(taddr, r);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
+  }
+}
+template <int W>
+__device__ __forceinline__ void tmem_st_lanes(uint32_t taddr, const uint32_t (&r)[W]) {
+  static_assert(W == 8 || W == 16, "");
+  if constexpr (W == 16) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+  } else {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+                 "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+  }
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -190,14 +239,14 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
   return r;
 }
 
-// All 128 softmax threads: the barrier, and whether every one of them is fine.
-__device__ __forceinline__ bool softmax_sync(bool ok) {
+// The 128 softmax threads of one half: a barrier, and whether every one is fine.
+__device__ __forceinline__ bool softmax_sync(int half, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "barrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
-      : "r"(uint32_t(ok))
+      : "r"(uint32_t(ok)), "r"(1 + half)
       : "memory");
   return r != 0;
 }
@@ -217,15 +266,16 @@ __device__ __forceinline__ float tree_total(const TreeArgs& a, int head, float t
   return over > 100.f ? sink : (top + log2f(total)) / kTreeLog2e;
 }
 
-// Value column d = this thread's of 16 consecutive rows (of which `rows` exist);
+// Value column d = this thread's of W consecutive rows (of which `rows` exist);
 // returns whether one is not finite.
-__device__ __forceinline__ bool tree_store16(const TreeArgs& a, int64_t row, int rows, int d, int lane,
-                                             const float (&x)[16]) {
+template <int W>
+__device__ __forceinline__ bool tree_store(const TreeArgs& a, int64_t row, int rows, int d, int lane,
+                                           const float (&x)[W]) {
   bool bad = false;
   if (a.out_wide) {
     float* dst = static_cast<float*>(a.out) + row * kTreeDv + d;
 #pragma unroll
-    for (int y = 0; y < 16; ++y)
+    for (int y = 0; y < W; ++y)
       if (y < rows) {
         dst[int64_t(y) * kTreeDv] = x[y];
         bad |= !isfinite(x[y]);
@@ -235,7 +285,7 @@ __device__ __forceinline__ bool tree_store16(const TreeArgs& a, int64_t row, int
     const int odd = lane & 1;
     uint16_t* dst = static_cast<uint16_t*>(a.out) + (row + odd) * kTreeDv + (d - odd);
 #pragma unroll
-    for (int y = 0; y < 16; y += 2) {
+    for (int y = 0; y < W; y += 2) {
       const float mine = odd ? x[y + 1] : x[y], other = __shfl_xor_sync(~0u, odd ? x[y] : x[y + 1], 1);
       if (y + odd < rows) {
         *reinterpret_cast<uint32_t*>(dst + int64_t(y) * kTreeDv) = odd ? bf16x2(other, mine) : bf16x2(mine, other);
@@ -250,7 +300,8 @@ template <int N>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeArgs a) {
   using L = TreeLayout<N>;
-  constexpr int C = N / 8;  // 8-row column chunks of S^T
+  constexpr int kHalf = N / 2, C = kHalf / 8;  // rows of a half of the softmax warps, in chunks of 8
+  constexpr int W = kHalf < 16 ? kHalf : 16;   // rows taken from O^T at a time
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
   const uint32_t sbase = smem_u32(smem);
@@ -259,10 +310,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   uint64_t* empty = bars + L::kPairs;       // [kPairs] block pair read by the O MMA (commit)
   uint64_t* bar_r = bars + 2 * L::kPairs;   // rotary block loaded
   uint64_t* bar_s = bar_r + 1;              // S^T complete (commit)
-  uint64_t* bar_p = bar_r + 2;              // P^T written (128 arrivals)
+  uint64_t* bar_p = bar_r + 2;              // P^T written (kTreeSoftmax arrivals)
   uint64_t* bar_o = bar_r + 3;              // the tile's O MMAs complete (commit)
-  uint64_t* bar_q = bar_r + 4;              // query in place (128 arrivals)
-  uint64_t* bar_free = bar_r + 5;           // O^T read by the epilogue (128 arrivals)
+  uint64_t* bar_q = bar_r + 4;              // query in place (kTreeSoftmax arrivals)
+  uint64_t* bar_free = bar_r + 5;           // O^T read by the epilogue (kTreeSoftmax arrivals)
   uint64_t* masks = reinterpret_cast<uint64_t*>(smem + L::kMaskOff);
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   float* stat = reinterpret_cast<float*>(smem + L::kStatOff);
@@ -272,7 +323,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   int* loaded = reinterpret_cast<int*>(smem + L::kMiscOff + 12);    // block pairs requested, for an abort
   int* loaded_r = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // rotary blocks
   int64_t* first_base = reinterpret_cast<int64_t*>(smem + L::kMiscOff + 24);
-  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);  // [6], before the ring is used
+  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);  // [10], before the ring is used
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -280,15 +331,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     for (int i = 0; i < L::kPairs; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(bar_r, 1);
     mbar_init(bar_s, 1);
-    mbar_init(bar_p, 128);
+    mbar_init(bar_p, kTreeSoftmax);
     mbar_init(bar_o, 1);
-    mbar_init(bar_q, 128);
-    mbar_init(bar_free, 128);
+    mbar_init(bar_q, kTreeSoftmax);
+    mbar_init(bar_free, kTreeSoftmax);
     *abort = 0;
     *loaded = *loaded_r = 0;
     fence_barrier_init();
   }
-  if (warp == 4) {
+  if (warp == 8) {
     tmem_alloc(tmem_slot, L::kTmemCols);
     tmem_relinquish();
   }
@@ -348,9 +399,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   TreeWalk<N> walk(a, w0, w1, w0 < w1 ? *first_b : 0, w0 < w1 ? *first_base : 0);
   pdl_launch_dependents();
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    const int quad = lane >> 2, pairc = 2 * (lane & 3);  // key of a fragment, first of its two rows
+    const int half = warp >> 2, row_h = half * kHalf, t = tid & 127;  // t: key, or value column
+    const uint32_t lanes = uint32_t(warp & 3) * 32 << 16;             // this warp's TMEM lanes
+    const int quad = lane >> 2, mine = row_h + 2 * (lane & 3);        // key of a fragment, first of its two rows
     int n = 0;
     bool ok = true;
     while (ok && walk.next()) {
@@ -358,12 +411,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
       const int64_t qrow = int64_t(s.node0) * a.heads + row0;
       // ---- query rows -> bf16, K-major, 128-byte swizzle
-      constexpr int kVec = N * (kTreeD / 8), kBatch = 6;
-      for (int i0 = tid; i0 < kVec; i0 += 128 * kBatch) {
+      constexpr int kVec = N * (kTreeD / 8), kBatch = kVec / kTreeSoftmax < 9 ? 5 : 9;
+      for (int i0 = tid; i0 < kVec; i0 += kTreeSoftmax * kBatch) {
         uint4 v[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + 128 * j, r = i / (kTreeD / 8);
+          const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8);
           v[j] = make_uint4(0, 0, 0, 0);
           if (i < kVec && r < rows) {
             const int64_t at = (qrow + r) * kTreeD + (i - r * (kTreeD / 8)) * 8;
@@ -378,7 +431,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + 128 * j, r = i / (kTreeD / 8), d = (i - r * (kTreeD / 8)) * 8;
+          const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8), d = (i - r * (kTreeD / 8)) * 8;
           if (i < kVec)
             *reinterpret_cast<uint4*>(smem + L::kQOff + (d >> 6) * (N * 128) + sw128_offset(r, d & 63)) = v[j];
         }
@@ -387,20 +440,21 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       fence_proxy_async_smem();
       mbar_arrive(bar_q);
 
+      // a maximum follows when a score passes it by more than the slack (or is the first)
+      auto limit = [](float m) { return m + kTreeSlack; };
       float m[C][2], l[C][2];
 #pragma unroll
       for (int c = 0; c < C; ++c) m[c][0] = m[c][1] = -CUDART_INF_F, l[c][0] = l[c][1] = 0.f;
       for (int i = 0; i < walk.count; ++i, ++n) {
         const int32_t p0 = (walk.tile0 + i) * kTreeKeys;
-        ok = mbar_wait(bar_s, n & 1, abort, a.err);
-        // ---- scores of keys 32 warp + quad + 8j, rows 8c + pairc + e
+        ok = tree_wait(bar_s, n & 1, abort, a.err);
+        // ---- scores of keys 32 (warp % 4) + quad + 8j, rows row_h + 8c + 2 (lane % 4) + e
         float v[C][4][2];
         if (ok) {
           tc_fence_after();
           uint32_t t0[4 * C], t1[4 * C];
-          const uint32_t at = tmem_s + (uint32_t(warp * 32) << 16);
-          tmem_ld_16x256<C>(at, t0);
-          tmem_ld_16x256<C>(at + (16u << 16), t1);
+          tmem_ld_16x256<C>(tmem_s + row_h + lanes, t0);
+          tmem_ld_16x256<C>(tmem_s + row_h + lanes + (16u << 16), t1);
           tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < C; ++c)
@@ -413,27 +467,27 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
           if (s.context - p0 < kTreeKeys) {  // drafted rows, or past the end
             const int32_t drafted = p0 - s.context;
-            uint64_t any = 0;
 #pragma unroll
             for (int c = 0; c < C; ++c)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const uint64_t word = masks[8 * c + pairc + e];
+                const uint64_t word = masks[8 * c + mine + e];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                  const int32_t d = drafted + warp * 32 + quad + 8 * j;
+                  const int32_t d = drafted + (warp & 3) * 32 + quad + 8 * j;
                   if (d >= 0 && (d >= s.nodes || !(word >> d & 1))) v[c][j][e] = -CUDART_INF_F;
                 }
               }
             // a row that no node of the group sees may hold anything: it is cleared,
             // since 0 x NaN would reach the output
+            uint64_t any = 0;
             for (int r = 0; r < N; ++r) any |= masks[r];
-            const int32_t d = drafted + tid;
+            const int32_t d = drafted + t;
             if (d >= 0 && (d >= s.nodes || !(any >> d & 1))) {
 #pragma unroll 1
-              for (int c = 0; c < 8; ++c) {
-                const int slot = (4 * n + (c >> 1)) % L::kPairs;
-                uint4* dst = reinterpret_cast<uint4*>(smem + L::kRingOff + slot * 32768 + (c & 1) * 16384 + tid * 128);
+              for (int c = 4 * half; c < 4 * half + 4; ++c) {
+                const int pair = (4 * n + (c >> 1)) % L::kPairs;
+                uint4* dst = reinterpret_cast<uint4*>(smem + L::kRingOff + pair * 32768 + (c & 1) * 16384 + t * 128);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
               }
@@ -441,58 +495,62 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           }
           // ---- maximum of each row over this warp's keys
 #pragma unroll
+          for (int c = 0; c < C; ++c) {
+            float x[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              x[e] = fmaxf(fmaxf(v[c][0][e], v[c][1][e]), fmaxf(v[c][2][e], v[c][3][e]));
+              x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 4));
+              x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 8));
+              x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 16));
+            }
+            if (quad == 0) *reinterpret_cast<float2*>(red + (warp & 3) * N + 8 * c + mine) = make_float2(x[0], x[1]);
+          }
+        }
+        ok = softmax_sync(half, ok);
+        if (!ok) break;
+        // ---- running maximum: every thread follows its rows, all alike
+        float top[C][2];
+        bool grows = false;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float2 x = *reinterpret_cast<const float2*>(red + 8 * c + mine);
+#pragma unroll
+          for (int w = 1; w < 4; ++w) {
+            const float2 y = *reinterpret_cast<const float2*>(red + w * N + 8 * c + mine);
+            x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
+          }
+          top[c][0] = x.x * a.scale_log2, top[c][1] = x.y * a.scale_log2;
+          grows |= top[c][0] > limit(m[c][0]) || top[c][1] > limit(m[c][1]);
+        }
+        if (__any_sync(~0u, grows)) {  // a warp holds every row of its half: its four warps decide alike
+#pragma unroll
           for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float x = fmaxf(fmaxf(v[c][0][e], v[c][1][e]), fmaxf(v[c][2][e], v[c][3][e]));
-              x = fmaxf(x, __shfl_xor_sync(~0u, x, 4));
-              x = fmaxf(x, __shfl_xor_sync(~0u, x, 8));
-              x = fmaxf(x, __shfl_xor_sync(~0u, x, 16));
-              if (quad == 0) red[warp * N + 8 * c + pairc + e] = x;
+              float f = 1.f;
+              if (top[c][e] > limit(m[c][e])) {
+                f = ex2(m[c][e] - top[c][e]);  // 0 when the row had seen nothing
+                l[c][e] *= f;
+                m[c][e] = top[c][e];
+              }
+              if (quad == 0 && (warp & 3) == 0) stat[8 * c + mine + e] = f;
             }
-        }
-        ok = softmax_sync(ok);
-        if (!ok) break;
-        // ---- running maximum: every thread follows its rows, all alike
-        bool grows = false;
-        float f[C][2];
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float2 x = *reinterpret_cast<const float2*>(red + 8 * c + pairc);
-#pragma unroll
-          for (int w = 1; w < 4; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(red + w * N + 8 * c + pairc);
-            x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
-          }
-          const float t[2] = {x.x * a.scale_log2, x.y * a.scale_log2};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            f[c][e] = 1.f;
-            if (t[e] > m[c][e] + kTreeSlack || (m[c][e] == -CUDART_INF_F && t[e] > -CUDART_INF_F)) {
-              f[c][e] = ex2(m[c][e] - t[e]);  // 0 when the row had seen nothing
-              l[c][e] *= f[c][e];
-              m[c][e] = t[e];
-              grows = true;
-            }
-          }
-        }
-        if (i > 0 && __any_sync(~0u, grows)) {  // a warp holds every row: all warps decide alike
-          if (warp == 0 && quad == 0) {
-#pragma unroll
-            for (int c = 0; c < C; ++c) stat[8 * c + pairc] = f[c][0], stat[8 * c + pairc + 1] = f[c][1];
-          }
-          softmax_sync(true);
+          if (i > 0) {
+            softmax_sync(half, true);
 #pragma unroll 1
-          for (int col = 0; col < 4 * N; col += 16) {
-            uint32_t o[16];
-            const uint32_t at = tmem_o + col + (uint32_t(warp * 32) << 16);
-            tmem_ld16(at, o);
-            tmem_wait_ld();
+            for (int r = 0; r < 4 * kHalf; r += W) {
+              uint32_t o[W];
+              const int col = (r / kHalf) * N + row_h + r % kHalf;
+              tmem_ld_lanes<W>(tmem_o + col + lanes, o);
+              tmem_wait_ld();
 #pragma unroll
-            for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * stat[(col & (N - 1)) + x]);
-            tmem_st16(at, o);
+              for (int x = 0; x < W; ++x)
+                o[x] = __float_as_uint(__uint_as_float(o[x]) * stat[row_h + r % kHalf + x]);
+              tmem_st_lanes<W>(tmem_o + col + lanes, o);
+            }
+            tmem_wait_st();
           }
-          tmem_wait_st();
         }
         // ---- weights, their sums, P^T
 #pragma unroll
@@ -506,7 +564,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             l[c][1] += y;
             packed[j] = bf16x2(x, y);
           }
-          const int r = 8 * c + (lane & 7), key = warp * 32 + 8 * (lane >> 3);
+          const int r = row_h + 8 * c + (lane & 7), key = (warp & 3) * 32 + 8 * (lane >> 3);
           stmatrix_x4_trans(sbase + L::kROff + (key >> 6) * (N * 128) + sw128_offset(r, key & 63), packed[0], packed[1],
                             packed[2], packed[3]);
         }
@@ -518,7 +576,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 
       // ---- output of the segment: sums over the keys' threads, then O^T.  The last O
       // MMA follows every thread's last use of red and stat
-      ok = mbar_wait(bar_o, (n - 1) & 1, abort, a.err);
+      ok = tree_wait(bar_o, (n - 1) & 1, abort, a.err);
       const bool whole = walk.count == s.tiles;
       const int slot = 2 * int(blockIdx.x) + (walk.tile0 > 0 ? 0 : 1);
 #pragma unroll
@@ -530,105 +588,134 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           x += __shfl_xor_sync(~0u, x, 8);
           x += __shfl_xor_sync(~0u, x, 16);
           if (quad == 0) {
-            red[warp * N + 8 * c + pairc + e] = x;
-            if (warp == 0) stat[8 * c + pairc + e] = m[c][e];
+            red[(warp & 3) * N + 8 * c + mine + e] = x;
+            if ((warp & 3) == 0) stat[8 * c + mine + e] = m[c][e];
           }
         }
-      ok = softmax_sync(ok);
+      ok = softmax_sync(half, ok);
       if (!ok) break;
-      if (tid < N) {
-        const float sum = (red[tid] + red[N + tid]) + (red[2 * N + tid] + red[3 * N + tid]), top = stat[tid];
-        if (tid < rows && !(sum < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
+      if (t < kHalf) {
+        const int r = row_h + t;
+        const float sum = (red[r] + red[N + r]) + (red[2 * N + r] + red[3 * N + r]), top = stat[r];
+        if (r < rows && !(sum < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
         if (whole) {
           float total;
-          const float lse = tree_total(a, (row0 + tid) % a.heads, top, sum, total);
-          stat[tid] = total > 0.f ? 1.f / total : 0.f;
-          if (a.lse != nullptr && tid < rows) a.lse[qrow + tid] = lse;
+          const float lse = tree_total(a, (row0 + r) % a.heads, top, sum, total);
+          stat[r] = total > 0.f ? 1.f / total : 0.f;
+          if (a.lse != nullptr && r < rows) a.lse[qrow + r] = lse;
         } else {
-          a.part_m[int64_t(slot) * N + tid] = top;
-          a.part_l[int64_t(slot) * N + tid] = sum;
-          stat[tid] = 1.f;
+          a.part_m[int64_t(slot) * N + r] = top;
+          a.part_l[int64_t(slot) * N + r] = sum;
+          stat[r] = 1.f;
         }
       }
-      softmax_sync(true);
+      softmax_sync(half, true);
       tc_fence_after();
       bool bad = false;
 #pragma unroll 1
-      for (int col = 0; col < 4 * N; col += 16) {
-        uint32_t o[16];
-        tmem_ld16(tmem_o + col + (uint32_t(warp * 32) << 16), o);
+      for (int x0 = 0; x0 < 4 * kHalf; x0 += W) {
+        uint32_t o[W];
+        const int r = row_h + x0 % kHalf, d = (x0 / kHalf) * 128 + t;
+        tmem_ld_lanes<W>(tmem_o + (x0 / kHalf) * N + r + lanes, o);
         tmem_wait_ld();
-        const int d = (col / N) * 128 + tid, r = col & (N - 1);
-        float x[16];
+        float x[W];
 #pragma unroll
-        for (int y = 0; y < 16; ++y) x[y] = __uint_as_float(o[y]) * stat[r + y];
+        for (int y = 0; y < W; ++y) x[y] = __uint_as_float(o[y]) * stat[r + y];
         if (!whole) {
           float* dst = a.part_o + (int64_t(slot) * N + r) * kTreeDv + d;
 #pragma unroll
-          for (int y = 0; y < 16; ++y)
+          for (int y = 0; y < W; ++y)
             if (r + y < rows) dst[y * kTreeDv] = x[y];
         } else {
-          bad |= tree_store16(a, qrow + r, rows - r, d, lane, x);
+          bad |= tree_store<W>(a, qrow + r, rows - r, d, lane, x);
         }
       }
       if (bad) flag(a.err, DSR_ERR_NONFINITE);
       tc_fence_before();
       mbar_arrive(bar_free);
     }
-  } else if (warp == 4 && lane == 0) {
+  } else if (warp == 8) {
     // ------------------------------------------------------------ MMA issuer
+    // The whole warp runs the loop and one lane issues, on values that are the same in
+    // all lanes: descriptors then stay in uniform registers.  Issued from a one-lane
+    // branch each MMA waited some 80 to 120 cycles for its operands to get there
+    // (measured; the MMA itself takes 48).
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, N, false, false);
     constexpr uint32_t idesc_o = umma_idesc_bf16(128, N, true, false);
-    int n = 0, segment = 0;
+    const uint32_t sb = __shfl_sync(~0u, sbase, 0);
+    const uint32_t ts = __shfl_sync(~0u, tmem_s, 0), to = __shfl_sync(~0u, tmem_o, 0);
+    const bool leader = elect_one();
+    const uint64_t desc_s = umma_desc_sw128(sb, 16, 1024), desc_q = umma_desc_sw128(sb + L::kQOff, 16, 1024);
+    const uint64_t desc_v = umma_desc_sw128(sb + L::kRingOff, 16384, 1024);
+    const uint64_t desc_p = umma_desc_sw128(sb + L::kROff, 16, 1024);
+    int n = 0, segment = 0, pair = 0;  // pair: ring position of the tile's first block pair
+    uint32_t lap = 0;                  // the ring's phase there
     bool ok = true;
-    while (ok && walk.next()) {
-      ok = mbar_wait(bar_q, segment & 1, abort, a.err);
-      for (int i = 0; i < walk.count && ok; ++i, ++n) {
-        // S^T: column blocks 0..7 pair by pair, then the rotary block
-#pragma unroll 1
-        for (int c = 0; c < 5 && ok; ++c) {
-          const int k = 4 * n + c;
-          ok = c < 4 ? mbar_wait(full + k % L::kPairs, (k / L::kPairs) & 1, abort, a.err)
-                     : mbar_wait(bar_r, n & 1, abort, a.err);
-          if (!ok) break;
-          tc_fence_after();
-          const uint32_t key = sbase + (c < 4 ? L::kRingOff + (k % L::kPairs) * 32768 : L::kROff);
-          const int steps = c < 4 ? 8 : 4;
-#pragma unroll 4
-          for (int x = 0; x < steps; ++x) {
-            const uint64_t ad = umma_desc_sw128(key + (x >> 2) * 16384 + (x & 3) * 32, 16, 1024);
-            const uint64_t bd =
-                umma_desc_sw128(sbase + L::kQOff + (2 * c + (x >> 2)) * (N * 128) + (x & 3) * 32, 16, 1024);
-            umma_bf16(tmem_s, ad, bd, idesc_s, (c | x) != 0 ? 1u : 0u);
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tree_wait(bar, parity, abort, a.err)); };
+    while (ok) {
+      const bool more = walk.next();
+      if (!__shfl_sync(~0u, int(more), 0)) break;
+      const int count = __shfl_sync(~0u, walk.count, 0);
+      ok = wait(bar_q, segment & 1);
+      for (int i = 0; i < count && ok; ++i, ++n) {
+        // S^T: column blocks 0..7 pair by pair, then the rotary block.  A step of 16
+        // columns moves both operands by 32 bytes, a block by its size: constants added
+        // to a descriptor's address field (units of 16 bytes)
+        int at = pair;
+        uint32_t phase = lap;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          ok = ok && wait(full + at, phase);
+          if (ok) {
+            tc_fence_after();
+            const uint64_t ad = desc_s + (L::kRingOff + at * 32768) / 16, bd = desc_q + 2 * c * (N * 128 / 16);
+            if (leader) {
+#pragma unroll
+              for (int x = 0; x < 8; ++x)
+                umma_bf16(ts, ad + (x >> 2) * 1024 + 2 * (x & 3), bd + (x >> 2) * (N * 128 / 16) + 2 * (x & 3), idesc_s,
+                          (c | x) != 0 ? 1u : 0u);
+            }
           }
+          if (++at == L::kPairs) at = 0, phase ^= 1;
         }
+        ok = ok && wait(bar_r, n & 1);
         if (!ok) break;
-        umma_commit(bar_s);
-        ok = mbar_wait(bar_p, n & 1, abort, a.err);
+        tc_fence_after();
+        if (leader) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            umma_bf16(ts, desc_s + L::kROff / 16 + 2 * x, desc_q + 8 * (N * 128 / 16) + 2 * x, idesc_s, 1u);
+          umma_commit(bar_s);
+        }
+        ok = wait(bar_p, n & 1);
         // the previous segment's O^T has been read
-        if (ok && i == 0 && segment > 0) ok = mbar_wait(bar_free, (segment - 1) & 1, abort, a.err);
+        if (ok && i == 0 && segment > 0) ok = wait(bar_free, (segment - 1) & 1);
         if (!ok) break;
         tc_fence_after();
         // O^T, 128 value columns after another, so that their block pair is free early
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          const int pair = (4 * n + c) % L::kPairs;
+        at = pair;
+        const uint32_t accumulate = i > 0;
 #pragma unroll
-          for (int ks = 0; ks < kTreeKeys / 16; ++ks) {
-            const uint64_t ad = umma_desc_sw128(sbase + L::kRingOff + pair * 32768 + ks * 2048, 16384, 1024);
-            const uint64_t bd =
-                umma_desc_sw128(sbase + L::kROff + (ks >> 2) * (N * 128) + (ks & 3) * 32, 16, 1024);
-            umma_bf16(tmem_o + c * N, ad, bd, idesc_o, (i > 0 || ks > 0) ? 1u : 0u);
+        for (int c = 0; c < 4; ++c) {
+          const uint64_t ad = desc_v + at * (32768 / 16);
+          if (leader) {
+#pragma unroll
+            for (int ks = 0; ks < kTreeKeys / 16; ++ks)
+              umma_bf16(to + c * N, ad + ks * (2048 / 16), desc_p + (ks >> 2) * (N * 128 / 16) + 2 * (ks & 3), idesc_o,
+                        ks > 0 ? 1u : accumulate);
+            umma_commit(empty + at);
           }
-          umma_commit(empty + pair);
+          if (++at == L::kPairs) at = 0;
         }
-        umma_commit(bar_o);
+        if (leader) umma_commit(bar_o);
+        lap = pair + 4 >= L::kPairs ? lap ^ 1 : lap;
+        pair = at;
       }
       ++segment;
     }
     // the last MMAs retire before TMEM is released (commits cover all before them)
     if (n > 0) mbar_drain(bar_o, (n - 1) & 1);
-  } else if (warp == 5 && lane == 0) {
+  } else if (warp == 9 && lane == 0) {
     // ------------------------------------------------------------ key tiles
     int n = 0;
     bool ok = true;
@@ -652,7 +739,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           const int k = 4 * n + c, pair = k % L::kPairs;
-          ok = mbar_wait(empty + pair, ((k / L::kPairs) & 1) ^ 1, abort, a.err);
+          ok = tree_wait(empty + pair, ((k / L::kPairs) & 1) ^ 1, abort, a.err);
           if (!ok) break;
           mbar_arrive_expect_tx(full + pair, 32768);
           const uint32_t dst = sbase + L::kRingOff + pair * 32768;
@@ -663,7 +750,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           *loaded = k + 1;
         }
         // P^T of the tile before sits in the rotary buffer until its O MMAs are done
-        if (ok && n > 0) ok = mbar_wait(bar_o, (n - 1) & 1, abort, a.err);
+        if (ok && n > 0) ok = tree_wait(bar_o, (n - 1) & 1, abort, a.err);
         if (!ok) break;
         mbar_arrive_expect_tx(bar_r, 16384);
         tma_load_2d(sbase + L::kROff, &kv_map, bar_r, 512, x0);
@@ -679,7 +766,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     for (int k = max(0, *loaded - L::kPairs); k < *loaded; ++k) mbar_drain(full + k % L::kPairs, (k / L::kPairs) & 1);
     if (*loaded_r > 0) mbar_drain(bar_r, (*loaded_r - 1) & 1);
   }
-  if (warp == 4) {
+  if (warp == 8) {
     tc_fence_after();
     tmem_dealloc(tmem_o, L::kTmemCols);
   }
