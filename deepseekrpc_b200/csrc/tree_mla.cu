@@ -493,49 +493,74 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
               }
             }
           }
-          // ---- maximum of each row over this warp's keys
+        }
+        // ---- weights against the running maxima as they stand, their sums, P^T
+        float sum[C][2];
+        bool fits = ok && i > 0;
+        auto weigh = [&] {
+#pragma unroll
+          for (int c = 0; c < C; ++c) {
+            uint32_t packed[4];
+            const float b0 = m[c][0] == -CUDART_INF_F ? 0.f : m[c][0], b1 = m[c][1] == -CUDART_INF_F ? 0.f : m[c][1];
+            sum[c][0] = sum[c][1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = ex2(fmaf(v[c][j][0], a.scale_log2, -b0)), y = ex2(fmaf(v[c][j][1], a.scale_log2, -b1));
+              sum[c][0] += x;
+              sum[c][1] += y;
+              packed[j] = bf16x2(x, y);
+            }
+            const int r = row_h + 8 * c + (lane & 7), key = (warp & 3) * 32 + 8 * (lane >> 3);
+            stmatrix_x4_trans(sbase + L::kROff + (key >> 6) * (N * 128) + sw128_offset(r, key & 63), packed[0],
+                              packed[1], packed[2], packed[3]);
+          }
+        };
+        auto top_of = [&](int c, int e) {
+          return fmaxf(fmaxf(v[c][0][e], v[c][1][e]), fmaxf(v[c][2][e], v[c][3][e])) * a.scale_log2;
+        };
+        if (fits) {
+#pragma unroll
+          for (int c = 0; c < C; ++c) fits = fits && !(top_of(c, 0) > limit(m[c][0])) && !(top_of(c, 1) > limit(m[c][1]));
+          weigh();
+        }
+        // most tiles end here: no maximum has to follow, no row needs the others' maxima
+        if (!softmax_sync(half, fits)) {
+          ok = softmax_sync(half, ok);
+          if (!ok) break;
+          // ---- the maximum of each row over the tile's keys; a thread follows its rows, all alike
 #pragma unroll
           for (int c = 0; c < C; ++c) {
             float x[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              x[e] = fmaxf(fmaxf(v[c][0][e], v[c][1][e]), fmaxf(v[c][2][e], v[c][3][e]));
+              x[e] = top_of(c, e);
               x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 4));
               x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 8));
               x[e] = fmaxf(x[e], __shfl_xor_sync(~0u, x[e], 16));
             }
             if (quad == 0) *reinterpret_cast<float2*>(red + (warp & 3) * N + 8 * c + mine) = make_float2(x[0], x[1]);
           }
-        }
-        ok = softmax_sync(half, ok);
-        if (!ok) break;
-        // ---- running maximum: every thread follows its rows, all alike
-        float top[C][2];
-        bool grows = false;
+          softmax_sync(half, true);
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float2 x = *reinterpret_cast<const float2*>(red + 8 * c + mine);
+          for (int c = 0; c < C; ++c) {
+            float2 x = *reinterpret_cast<const float2*>(red + 8 * c + mine);
 #pragma unroll
-          for (int w = 1; w < 4; ++w) {
-            const float2 y = *reinterpret_cast<const float2*>(red + w * N + 8 * c + mine);
-            x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
-          }
-          top[c][0] = x.x * a.scale_log2, top[c][1] = x.y * a.scale_log2;
-          grows |= top[c][0] > limit(m[c][0]) || top[c][1] > limit(m[c][1]);
-        }
-        if (__any_sync(~0u, grows)) {  // a warp holds every row of its half: its four warps decide alike
-#pragma unroll
-          for (int c = 0; c < C; ++c)
+            for (int w = 1; w < 4; ++w) {
+              const float2 y = *reinterpret_cast<const float2*>(red + w * N + 8 * c + mine);
+              x.x = fmaxf(x.x, y.x), x.y = fmaxf(x.y, y.y);
+            }
+            const float top[2] = {x.x, x.y};
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               float f = 1.f;
-              if (top[c][e] > limit(m[c][e])) {
-                f = ex2(m[c][e] - top[c][e]);  // 0 when the row had seen nothing
+              if (top[e] > limit(m[c][e])) {
+                f = ex2(m[c][e] - top[e]);  // 0 when the row had seen nothing
                 l[c][e] *= f;
-                m[c][e] = top[c][e];
+                m[c][e] = top[e];
               }
               if (quad == 0 && (warp & 3) == 0) stat[8 * c + mine + e] = f;
             }
+          }
           if (i > 0) {
             softmax_sync(half, true);
 #pragma unroll 1
@@ -551,23 +576,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
             tmem_wait_st();
           }
+          weigh();
         }
-        // ---- weights, their sums, P^T
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          uint32_t packed[4];
-          const float b0 = m[c][0] == -CUDART_INF_F ? 0.f : m[c][0], b1 = m[c][1] == -CUDART_INF_F ? 0.f : m[c][1];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float x = ex2(fmaf(v[c][j][0], a.scale_log2, -b0)), y = ex2(fmaf(v[c][j][1], a.scale_log2, -b1));
-            l[c][0] += x;
-            l[c][1] += y;
-            packed[j] = bf16x2(x, y);
-          }
-          const int r = row_h + 8 * c + (lane & 7), key = (warp & 3) * 32 + 8 * (lane >> 3);
-          stmatrix_x4_trans(sbase + L::kROff + (key >> 6) * (N * 128) + sw128_offset(r, key & 63), packed[0], packed[1],
-                            packed[2], packed[3]);
-        }
+        for (int c = 0; c < C; ++c) l[c][0] += sum[c][0], l[c][1] += sum[c][1];
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(bar_p);
