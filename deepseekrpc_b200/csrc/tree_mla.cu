@@ -11,10 +11,16 @@
 //   S^T[key, row] = K[key, :576] Q[row, :576]   (M = 128 keys, N rows)
 //   O^T[dim, row] += V[key, dim] P[row, key]    (M = 128 dims x 4, N rows)
 // so that the key tile, once in shared memory, is the A operand of both (K-major,
-// then MN-major) and O^T of 64 rows takes half of the tensor memory.  The units
-// of all requests, in the order (request, group, tile), are cut into equal runs,
-// one per CTA, whatever the lengths; a group that spans CTAs leaves partials (m, l,
-// unnormalised O in FP32) that tree_combine_kernel joins.
+// then MN-major) and O^T of 64 rows takes half of the tensor memory.
+//
+// A job is one group over a segment of consecutive tiles.  Every CTA finds the same
+// segment length (tree_plan) from the lengths on the device; a request's tiles are
+// cut into equal segments, and job j, in the order (request, segment, group), goes to
+// CTA j modulo the grid: the groups of a segment then run side by side and share its
+// rows in L2.  (Runs of units in the order request, group, tile balance better, but
+// read the rows once per group: 1213 us against 1010 us for 32 requests of 3 to 6
+// groups.)  A group of several segments leaves partials (m, l, unnormalised O in
+// FP32) that tree_combine_kernel joins.
 //
 //   warps 0..7  query -> shared memory, softmax over the tile's keys (running
 //               maximum; O is rescaled only when a maximum grows by more than 2^8),
@@ -52,7 +58,8 @@ struct TreeLayout {
   static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N] seen-masks of the rows
   static constexpr int kRedOff = kMaskOff + N * 8;      // f32[4][N] per-warp maxima, then sums
   static constexpr int kStatOff = kRedOff + 4 * N * 4;  // f32[N] factors / reciprocals
-  static constexpr int kMiscOff = kStatOff + N * 4;
+  static constexpr int kChunkOff = kStatOff + N * 4;    // i32[2][kTreeThreads]
+  static constexpr int kMiscOff = kChunkOff + 2 * kTreeThreads * 4;
   static constexpr int kBytes = kMiscOff + 64;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr uint32_t kTmemCols = N == 64 ? 512 : (N == 32 ? 256 : 128);  // >= 5 N
@@ -73,9 +80,9 @@ struct TreeArgs {
   void* out;
   float* lse;  // nullable
   int32_t* err;
-  int64_t* unit_start;  // [batch + 1]
-  float* part_o;        // [2 * CTAs][N][512]
-  float* part_m;        // [2 * CTAs][N]
+  int32_t* slot_start;  // [batch + 1] first partial slot of each request; the segment length
+  float* part_o;        // [slots][N][512]
+  float* part_m;        // [slots][N]
   float* part_l;
   int64_t nodes;
   int batch, heads, max_nodes, ctas;
@@ -103,38 +110,82 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeArgs& a, int b) {
   return s;
 }
 
-// ---- a CTA's run of units, walked segment by segment (one group's consecutive tiles)
+__device__ __forceinline__ int32_t tree_segments(const TreeSeq& s, int32_t length) {
+  return (s.tiles + length - 1) / length;
+}
+
+// ---- the jobs of a call
+constexpr int kTreeSearchBatch = 2048;  // larger batches take the even share (the search reads every request)
+constexpr int kTreeSlotsPerCta = 4;  // partial slots, per CTA of the grid
+// A job's cost beside its tiles, in tiles: query load, first copies, output.
+constexpr float kTreeJobCost = 2.f;
+
+// A segment length for `waves` jobs per CTA at most: starts at the even share and
+// grows until the jobs (requests' tiles rounded up to whole segments) and the partial
+// slots fit.  One warp; estimates the time in tiles (infinite when none was found).
+template <int N>
+__device__ __forceinline__ float tree_length(const TreeArgs& a, int64_t units, int waves, int lane, int32_t& length) {
+  const int64_t room = int64_t(waves) * a.ctas;
+  float len = fmaxf(ceilf(float(units) / float(room)), 1.f);
+  for (int tries = 0; tries < 8; ++tries) {
+    length = int32_t(len);
+    int64_t jobs = 0, slots = 0;
+    for (int b = lane; b < a.batch; b += 32) {
+      const TreeSeq s = tree_seq<N>(a, b);
+      const int64_t n = int64_t(s.groups) * tree_segments(s, length);
+      jobs += n;
+      if (s.tiles > length) slots += n;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+      jobs += __shfl_xor_sync(~0u, jobs, o);
+      slots += __shfl_xor_sync(~0u, slots, o);
+    }
+    if (jobs <= room && slots <= int64_t(kTreeSlotsPerCta) * a.ctas) {
+      // full waves of equal jobs, or list scheduling's mean plus half a job
+      const float mean = float(units) / float(a.ctas);
+      return fminf(float(waves) * len, mean + 0.5f * len) + float(waves) * kTreeJobCost;
+    }
+    len += fmaxf(floorf(len * (1.f - float(room) / float(jobs))), 1.f);
+  }
+  return CUDART_INF_F;
+}
+
+// ---- a CTA's jobs, one after another
 template <int N>
 struct TreeWalk {
   const TreeArgs& a;
-  int64_t u, end, base;  // base: first unit of request b
-  int b, group, tile0, count;
+  const int32_t *chunk_jobs, *chunk_slots;  // [kTreeThreads] before each chunk of `per` requests
+  int32_t length, jobs, job;
+  int per, b, group, tile0, count, slot;    // slot < 0: the group's only segment
   TreeSeq s;
-  __device__ __forceinline__ TreeWalk(const TreeArgs& args, int64_t first, int64_t last, int b0, int64_t base0)
-      : a(args), u(first), end(last), base(base0), b(b0), group(0), tile0(0), count(0) {
-    if (u < end) s = tree_seq<N>(a, b);
-  }
   __device__ __forceinline__ bool next() {
-    u += count;
-    if (u >= end) return false;
-    int64_t units = int64_t(s.groups) * s.tiles;
-    while (u >= base + units) {
-      base += units;
-      s = tree_seq<N>(a, ++b);
-      units = int64_t(s.groups) * s.tiles;
+    if (job >= jobs) return false;
+    int lo = 0, hi = kTreeThreads;  // the last chunk that starts at or before the job
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (chunk_jobs[mid] <= job) lo = mid;
+      else hi = mid;
     }
-    const int64_t at = u - base;
-    group = int(at / s.tiles);
-    tile0 = int(at - int64_t(group) * s.tiles);
-    const int64_t left = end - u;
-    count = int(left < s.tiles - tile0 ? left : s.tiles - tile0);
+    int32_t base = chunk_jobs[lo], slots = chunk_slots[lo], segments;
+    for (b = lo * per;; ++b) {
+      s = tree_seq<N>(a, b);
+      segments = tree_segments(s, length);
+      const int32_t n = s.groups * segments;
+      if (job < base + n) break;
+      base += n;
+      if (segments > 1) slots += n;
+    }
+    const int32_t at = job - base, segment = at / s.groups;
+    group = at - segment * s.groups;
+    const int32_t whole = s.tiles / segments, longer = s.tiles - whole * segments;
+    tile0 = segment * whole + min(segment, longer);
+    count = whole + (segment < longer);
+    slot = segments > 1 ? slots + at : -1;
+    job += gridDim.x;
     return true;
   }
 };
-
-__device__ __forceinline__ int64_t run_start(int64_t units, int c, int ctas) { return units * c / ctas; }
-// The CTA whose run holds unit u.
-__device__ __forceinline__ int run_of(int64_t units, int64_t u, int ctas) { return int(((u + 1) * ctas - 1) / units); }
 
 // mbar_wait whose polls sleep in the barrier unit until the phase completes (or a few
 // microseconds pass): the ten warps that wait here would otherwise poll shared memory
@@ -319,11 +370,15 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   float* stat = reinterpret_cast<float*>(smem + L::kStatOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
-  int* first_b = reinterpret_cast<int*>(smem + L::kMiscOff + 8);
-  int* loaded = reinterpret_cast<int*>(smem + L::kMiscOff + 12);    // block pairs requested, for an abort
-  int* loaded_r = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // rotary blocks
-  int64_t* first_base = reinterpret_cast<int64_t*>(smem + L::kMiscOff + 24);
-  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);  // [10], before the ring is used
+  int* loaded = reinterpret_cast<int*>(smem + L::kMiscOff + 8);     // block pairs requested, for an abort
+  int* loaded_r = reinterpret_cast<int*>(smem + L::kMiscOff + 12);  // rotary blocks
+  int32_t* chunk_jobs = reinterpret_cast<int32_t*>(smem + L::kChunkOff);
+  int32_t* chunk_slots = chunk_jobs + kTreeThreads;
+  // before the ring is used: [10] sums of the warps (units, groups), [4] estimates and lengths
+  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);
+  int64_t* warp_groups = warp_units + kTreeThreads / 32;
+  float* estimate = reinterpret_cast<float*>(warp_groups + kTreeThreads / 32);
+  int32_t* estimated = reinterpret_cast<int32_t*>(estimate + 4);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   if (tid == 0) {
@@ -344,59 +399,77 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     tmem_relinquish();
   }
 
-  // ---- units before each thread's run of requests, and in all
+  // ---- the work of all requests, each thread a chunk of consecutive ones
   const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
   const int r0 = min(tid * per, a.batch), r1 = min(r0 + per, a.batch);
-  int64_t own = 0;
+  int64_t units = 0, groups = 0;
   for (int b = r0; b < r1; ++b) {
     const TreeSeq s = tree_seq<N>(a, b);
     if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
-    own += int64_t(s.groups) * s.tiles;
+    units += int64_t(s.groups) * s.tiles;
+    groups += s.groups;
   }
-  int64_t run = own;
+  auto block_sums = [&](int64_t x, int64_t y) {  // inclusive over the warp; the warps' sums in shared memory
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int64_t up = __shfl_up_sync(~0u, run, d);
-    if (lane >= d) run += up;
-  }
-  if (lane == 31) warp_units[warp] = run;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t u = __shfl_up_sync(~0u, x, d), v = __shfl_up_sync(~0u, y, d);
+      if (lane >= d) x += u, y += v;
+    }
+    if (lane == 31) warp_units[warp] = x, warp_groups[warp] = y;
+    return make_longlong2(x, y);
+  };
+  block_sums(units, groups);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  int64_t before = run - own, units = 0;
-  for (int w = 0; w < kTreeThreads / 32; ++w) {
-    if (w < warp) before += warp_units[w];
-    units += warp_units[w];
-  }
-  const int ctas = int(units < a.ctas ? units : a.ctas);
-  int64_t w0 = 0, w1 = 0;
-  if (int(blockIdx.x) < ctas) {
-    w0 = run_start(units, blockIdx.x, ctas);
-    w1 = run_start(units, blockIdx.x + 1, ctas);
-    if (w0 >= before && w0 < before + own) {
-      int64_t base = before;
-      int b = r0;
-      for (;; ++b) {
-        const TreeSeq s = tree_seq<N>(a, b);
-        const int64_t n = int64_t(s.groups) * s.tiles;
-        if (w0 < base + n) break;
-        base += n;
-      }
-      *first_b = b;
-      *first_base = base;
+  units = groups = 0;
+  for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
+  // ---- the segment length: the best of four wave counts
+  int32_t length = 0;
+  if (a.batch <= kTreeSearchBatch) {
+    if (warp < 4) {
+      const int waves = (int(groups) + a.ctas - 1) / a.ctas + warp;
+      int32_t len = 1;
+      const float e = units > 0 ? tree_length<N>(a, units, waves, lane, len) : CUDART_INF_F;
+      if (lane == 0) estimate[warp] = e, estimated[warp] = len;
     }
+    __syncthreads();
+    float best = CUDART_INF_F;
+    for (int w = 0; w < 4; ++w)
+      if (estimate[w] < best) best = estimate[w], length = estimated[w];
   }
+  // or the even share of two jobs per CTA, whose partials always fit: a cut request's
+  // groups have at most 2 U / length of them
+  if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
+  __syncthreads();
+  // ---- jobs and partial slots before each chunk
+  int64_t jobs = 0, slots = 0;
+  for (int b = r0; b < r1; ++b) {
+    const TreeSeq s = tree_seq<N>(a, b);
+    const int64_t n = int64_t(s.groups) * tree_segments(s, length);
+    jobs += n;
+    if (s.tiles > length) slots += n;
+  }
+  const longlong2 upto = block_sums(jobs, slots);
+  __syncthreads();
+  int64_t jobs_before = upto.x - jobs, slots_before = upto.y - slots, all_jobs = 0;
+  for (int w = 0; w < kTreeThreads / 32; ++w) {
+    if (w < warp) jobs_before += warp_units[w], slots_before += warp_groups[w];
+    all_jobs += warp_units[w];
+  }
+  chunk_jobs[tid] = int32_t(jobs_before);
+  chunk_slots[tid] = int32_t(slots_before);
   if (blockIdx.x == 0) {
     for (int b = r0; b < r1; ++b) {
       const TreeSeq s = tree_seq<N>(a, b);
-      a.unit_start[b] = before;
-      before += int64_t(s.groups) * s.tiles;
+      a.slot_start[b] = int32_t(slots_before);
+      if (s.tiles > length) slots_before += int64_t(s.groups) * tree_segments(s, length);
     }
-    if (tid == 0) a.unit_start[a.batch] = units;
+    if (tid == 0) a.slot_start[a.batch] = length;
   }
   __syncthreads();
   const uint32_t tmem_o = *tmem_slot, tmem_s = tmem_o + 4 * N;
-  TreeWalk<N> walk(a, w0, w1, w0 < w1 ? *first_b : 0, w0 < w1 ? *first_base : 0);
+  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, length, int32_t(all_jobs), int32_t(blockIdx.x), per};
   pdl_launch_dependents();
 
   if (warp < 8) {
@@ -589,8 +662,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       // ---- output of the segment: sums over the keys' threads, then O^T.  The last O
       // MMA follows every thread's last use of red and stat
       ok = tree_wait(bar_o, (n - 1) & 1, abort, a.err);
-      const bool whole = walk.count == s.tiles;
-      const int slot = 2 * int(blockIdx.x) + (walk.tile0 > 0 ? 0 : 1);
+      const int slot = walk.slot;
+      const bool whole = slot < 0;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -788,11 +861,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 // Joins the partials of a group that spans CTAs: one CTA per query row, thread t
 // four value columns.  out = sum_p 2^(m_p - M) O_p / (2^(sink - M) + sum_p 2^(m_p - M) l_p).
 // ---------------------------------------------------------------------------
-constexpr int kTreeMaxCtas = 256;  // partials of one row at most
+constexpr int kTreeMaxCtas = 256;
+constexpr int kTreeMaxParts = kTreeSlotsPerCta * kTreeMaxCtas;  // of one row
 
 template <int N>
 __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
-  __shared__ float weight[kTreeMaxCtas];
+  __shared__ float weight[kTreeMaxParts];
   __shared__ float inverse;
   const int64_t row = blockIdx.x;
   const int32_t node = int32_t(row / a.heads);
@@ -807,14 +881,11 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   const TreeSeq s = tree_seq<N>(a, lo);
   if (node < s.node0 || node >= s.node0 + s.nodes) return;
   pdl_wait();
-  const int64_t units = a.unit_start[a.batch];
+  const int parts = tree_segments(s, a.slot_start[a.batch]);
+  if (parts <= 1) return;  // written by its job
   const int in = int(row - int64_t(s.node0) * a.heads), group = in / N, r = in % N;
-  const int64_t u0 = a.unit_start[lo] + int64_t(group) * s.tiles;
-  const int ctas = int(units < a.ctas ? units : a.ctas);
-  const int c0 = run_of(units, u0, ctas), c1 = run_of(units, u0 + s.tiles - 1, ctas);
-  if (c0 == c1) return;  // whole in one CTA, written there
-  const int parts = c1 - c0 + 1;
-  auto slot = [&](int p) { return int64_t(p == 0 ? 2 * c0 + 1 : 2 * (c0 + p)) * N + r; };
+  const int64_t first = a.slot_start[lo] + group;
+  auto slot = [&](int p) { return (first + int64_t(p) * s.groups) * N + r; };
   if (tid < 32) {
     float top = -CUDART_INF_F, sum = 0.f;
     for (int p = tid; p < parts; p += 32) top = fmaxf(top, a.part_m[slot(p)]);
@@ -867,7 +938,9 @@ int tree_rows(int64_t heads, int64_t max_nodes) {
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
-size_t tree_start_bytes(int64_t batch) { return (size_t(batch + 1) * 8 + 255) / 256 * 256; }
+int tree_ctas() { return sm_count() < kTreeMaxCtas ? sm_count() : kTreeMaxCtas; }
+
+size_t tree_start_bytes(int64_t batch) { return (size_t(batch + 1) * 4 + 255) / 256 * 256; }
 
 template <int N>
 int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStream_t stream) {
@@ -877,10 +950,10 @@ int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStrea
   CUtensorMap map;  // one page by 64 columns
   rc = encode_tmap_bf16_2d(&map, kv_pool, kTreeD, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
   if (rc != DSR_OK) return rc;
-  a.unit_start = static_cast<int64_t*>(workspace);
+  a.slot_start = static_cast<int32_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_start_bytes(a.batch));
-  a.part_m = a.part_o + size_t(2) * a.ctas * N * kTreeDv;
-  a.part_l = a.part_m + size_t(2) * a.ctas * N;
+  a.part_m = a.part_o + size_t(kTreeSlotsPerCta) * a.ctas * N * kTreeDv;
+  a.part_l = a.part_m + size_t(kTreeSlotsPerCta) * a.ctas * N;
   tree_mla_kernel<N><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, a);
   rc = launch_status("tree_mla_decode launch");
   if (rc != DSR_OK) return rc;
@@ -904,7 +977,7 @@ int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStrea
 extern "C" size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes) {
   using namespace dsr;
   if (batch <= 0 || heads <= 0 || max_nodes <= 0) return 0;
-  const size_t rows = size_t(2) * sm_count() * tree_rows(heads, max_nodes);
+  const size_t rows = size_t(kTreeSlotsPerCta) * tree_ctas() * tree_rows(heads, max_nodes);
   return tree_start_bytes(batch) + rows * (kTreeDv + 2) * 4;
 }
 
@@ -955,7 +1028,7 @@ extern "C" int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* k
   a.batch = int(batch);
   a.heads = int(heads);
   a.max_nodes = int(max_nodes);
-  a.ctas = sm_count() < kTreeMaxCtas ? sm_count() : kTreeMaxCtas;
+  a.ctas = tree_ctas();
   switch (tree_rows(heads, max_nodes)) {
     case 16:
       return launch_tree<16>(a, kv_pool, workspace, as_stream(stream));
