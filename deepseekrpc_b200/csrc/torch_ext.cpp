@@ -6,6 +6,7 @@
 // New entry points expose the paged decode path.  Outputs are allocated with
 // the caching allocator on the input's device; work runs on the current stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -492,6 +493,11 @@ int element_type(const at::Tensor& t, const char* what) {
   return t.scalar_type() == at::kFloat ? DSR_F32 : DSR_BF16;
 }
 
+// An uninitialised tensor without the dispatcher's round trip (a small call is made of these).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& anchor) {
+  return at::detail::empty_cuda(sizes, dtype, anchor.device(), c10::nullopt);
+}
+
 void check_vector(const at::Tensor& t, at::ScalarType dtype, int64_t n, const at::Tensor& anchor, const char* what) {
   check(t, dtype, anchor);
   TORCH_CHECK(t.dim() == 1 && t.size(0) == n, what);
@@ -515,9 +521,9 @@ std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens,
   TORCH_CHECK(tokens >= 0 && tokens < (int64_t(1) << 31), "paged_plan: invalid token count");
   const c10::cuda::CUDAGuard guard(lengths.device());
   auto error = status_or(status, lengths);
-  auto seq = at::empty({tokens}, lengths.options()), positions = at::empty({tokens}, lengths.options());
-  auto slots = at::empty({tokens}, lengths.options()), cu = at::empty({batch + 1}, lengths.options());
-  auto visible = at::empty({batch}, lengths.options());
+  auto seq = fresh({tokens}, at::kInt, lengths), positions = fresh({tokens}, at::kInt, lengths);
+  auto slots = fresh({tokens}, at::kInt, lengths), cu = fresh({batch + 1}, at::kInt, lengths);
+  auto visible = fresh({batch}, at::kInt, lengths);
   ok(dsr_paged_plan(lengths.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
                     block_table.data_ptr<int32_t>(), block_table.size(1), free_ring.data_ptr<int32_t>(),
                     ring_state.data_ptr<int32_t>(), free_ring.size(0), seq.data_ptr<int32_t>(),
@@ -603,11 +609,11 @@ std::vector<at::Tensor> ds_tree_mla_decode(at::Tensor q, at::Tensor kv_pool, at:
                     result.size(2) == DSR_V_DIM,
                 "tree_mla_decode: out [nodes, heads, 512] expected");
   } else {
-    result = at::empty({nodes, heads, DSR_V_DIM}, q.options());
+    result = fresh({nodes, heads, DSR_V_DIM}, q.scalar_type(), q);
   }
-  at::Tensor lse = return_lse ? at::empty({nodes, heads}, q.options().dtype(at::kFloat)) : at::Tensor();
+  at::Tensor lse = return_lse ? fresh({nodes, heads}, at::kFloat, q) : at::Tensor();
   const size_t ws_bytes = dsr_tree_mla_workspace_bytes(batch, heads, max_nodes);
-  auto ws = at::empty({int64_t(ws_bytes)}, q.options().dtype(at::kByte));
+  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, q);
   ok(dsr_tree_mla_decode(q.data_ptr(), dtype, bf16(kv_pool), kv_pool.size(0) / DSR_BLOCK_TOKENS,
                          block_table.data_ptr<int32_t>(), block_table.size(1), context.data_ptr<int32_t>(),
                          cu_nodes.data_ptr<int32_t>(), tree_mask.data_ptr<int64_t>(), max_nodes,
@@ -635,8 +641,7 @@ std::vector<at::Tensor> ds_sample_logits(at::Tensor logits, at::Tensor temperatu
   check_vector(uniform, at::kFloat, rows, logits, shapes);
   const c10::cuda::CUDAGuard guard(logits.device());
   auto error = status_or(status, logits);
-  auto tokens = at::empty({rows}, logits.options().dtype(at::kInt));
-  auto chances = at::empty({rows}, logits.options().dtype(at::kFloat));
+  auto tokens = fresh({rows}, at::kInt, logits), chances = fresh({rows}, at::kFloat, logits);
   ok(dsr_sample(logits.data_ptr(), dtype, logits.stride(0), logits.size(1), temperature.data_ptr<float>(),
                 top_k.data_ptr<int32_t>(), top_p.data_ptr<float>(), min_p.data_ptr<float>(),
                 uniform.data_ptr<float>(), tokens.data_ptr<int32_t>(), chances.data_ptr<float>(),

@@ -81,7 +81,7 @@ struct TreeArgs {
   float* lse;  // nullable
   int32_t* err;
   int32_t* slot_start;  // [batch + 1] first partial slot of each request; the segment length
-  float* part_o;        // [slots][N][512]
+  float* part_o;        // [slots][N / 4][512][4]: value columns of four rows side by side
   float* part_m;        // [slots][N]
   float* part_l;
   int64_t nodes;
@@ -151,16 +151,39 @@ __device__ __forceinline__ float tree_length(const TreeArgs& a, int64_t units, i
   return CUDART_INF_F;
 }
 
-// ---- a CTA's jobs, one after another
+// ---- a CTA's jobs, one after another (every warp walks them for itself)
 template <int N>
 struct TreeWalk {
   const TreeArgs& a;
   const int32_t *chunk_jobs, *chunk_slots;  // [kTreeThreads] before each chunk of `per` requests
   int32_t length, jobs, job;
-  int per, b, group, tile0, count, slot;    // slot < 0: the group's only segment
+  int per;
+  // up to 32 requests: lane b keeps request b, and the jobs and slots before it
+  TreeSeq own;
+  int32_t own_jobs, own_slots;
+  int b, group, tile0, count, slot;  // slot < 0: the group's only segment
   TreeSeq s;
+  __device__ __forceinline__ void at_job(int32_t at, int32_t segments, int32_t slots) {
+    const int32_t segment = at / s.groups;
+    group = at - segment * s.groups;
+    const int32_t whole = s.tiles / segments, longer = s.tiles - whole * segments;
+    tile0 = segment * whole + min(segment, longer);
+    count = whole + (segment < longer);
+    slot = segments > 1 ? slots + at : -1;
+    job += gridDim.x;
+  }
   __device__ __forceinline__ bool next() {
     if (job >= jobs) return false;
+    if (a.batch <= 32) {
+      b = 31 - __clz(__ballot_sync(~0u, own_jobs <= job));  // the last request that starts at or before the job
+      s.node0 = __shfl_sync(~0u, own.node0, b);
+      s.nodes = __shfl_sync(~0u, own.nodes, b);
+      s.context = __shfl_sync(~0u, own.context, b);
+      s.tiles = __shfl_sync(~0u, own.tiles, b);
+      s.groups = __shfl_sync(~0u, own.groups, b);
+      at_job(job - __shfl_sync(~0u, own_jobs, b), tree_segments(s, length), __shfl_sync(~0u, own_slots, b));
+      return true;
+    }
     int lo = 0, hi = kTreeThreads;  // the last chunk that starts at or before the job
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -176,13 +199,7 @@ struct TreeWalk {
       base += n;
       if (segments > 1) slots += n;
     }
-    const int32_t at = job - base, segment = at / s.groups;
-    group = at - segment * s.groups;
-    const int32_t whole = s.tiles / segments, longer = s.tiles - whole * segments;
-    tile0 = segment * whole + min(segment, longer);
-    count = whole + (segment < longer);
-    slot = segments > 1 ? slots + at : -1;
-    job += gridDim.x;
+    at_job(job - base, segments, slots);
     return true;
   }
 };
@@ -399,38 +416,39 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     tmem_relinquish();
   }
 
-  // ---- the work of all requests, each thread a chunk of consecutive ones
-  const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;
-  const int r0 = min(tid * per, a.batch), r1 = min(r0 + per, a.batch);
-  int64_t units = 0, groups = 0;
+  // ---- the work of all requests
+  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, 1, 0, int32_t(blockIdx.x), 1, TreeSeq{}, 0, 0};
+  const bool small = a.batch <= 32;
+  const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;  // else: requests of a thread's chunk
+  const int r0 = small ? lane : min(tid * per, a.batch), r1 = small ? min(lane + 1, a.batch) : min(r0 + per, a.batch);
+  walk.per = per;
+  int64_t units = 0;
+  int32_t groups = 0;
   for (int b = r0; b < r1; ++b) {
     const TreeSeq s = tree_seq<N>(a, b);
     if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
     units += int64_t(s.groups) * s.tiles;
     groups += s.groups;
+    walk.own = s;
   }
-  auto block_sums = [&](int64_t x, int64_t y) {  // inclusive over the warp; the warps' sums in shared memory
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int64_t u = __shfl_up_sync(~0u, x, d), v = __shfl_up_sync(~0u, y, d);
-      if (lane >= d) x += u, y += v;
-    }
-    if (lane == 31) warp_units[warp] = x, warp_groups[warp] = y;
-    return make_longlong2(x, y);
-  };
-  block_sums(units, groups);
+  // sums over the warp: low and high parts of the units by themselves
+  units = (int64_t(__reduce_add_sync(~0u, uint32_t(units >> 24))) << 24) +
+          __reduce_add_sync(~0u, uint32_t(units) & 0xffffffu);
+  groups = __reduce_add_sync(~0u, groups);
   tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  units = groups = 0;
-  for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
-  // ---- the segment length: the best of four wave counts
-  int32_t length = 0;
-  if (a.batch <= kTreeSearchBatch) {
+  if (!small) {
+    if (lane == 0) warp_units[warp] = units, warp_groups[warp] = groups;
+    __syncthreads();
+    units = groups = 0;
+    for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
+  }
+  // ---- the segment length: one tile when that fills no more than the grid, else the
+  // best of four wave counts
+  int32_t length = units <= a.ctas ? 1 : 0;
+  if (length == 0 && a.batch <= kTreeSearchBatch) {
     if (warp < 4) {
-      const int waves = (int(groups) + a.ctas - 1) / a.ctas + warp;
       int32_t len = 1;
-      const float e = units > 0 ? tree_length<N>(a, units, waves, lane, len) : CUDART_INF_F;
+      const float e = tree_length<N>(a, units, (groups + a.ctas - 1) / a.ctas + warp, lane, len);
       if (lane == 0) estimate[warp] = e, estimated[warp] = len;
     }
     __syncthreads();
@@ -441,35 +459,49 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   // or the even share of two jobs per CTA, whose partials always fit: a cut request's
   // groups have at most 2 U / length of them
   if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
-  __syncthreads();
-  // ---- jobs and partial slots before each chunk
-  int64_t jobs = 0, slots = 0;
+  // ---- jobs and partial slots before each lane's request, or each thread's chunk
+  int32_t jobs = 0, slots = 0;
   for (int b = r0; b < r1; ++b) {
-    const TreeSeq s = tree_seq<N>(a, b);
-    const int64_t n = int64_t(s.groups) * tree_segments(s, length);
+    const TreeSeq s = small ? walk.own : tree_seq<N>(a, b);
+    const int32_t n = s.groups * tree_segments(s, length);
     jobs += n;
     if (s.tiles > length) slots += n;
   }
-  const longlong2 upto = block_sums(jobs, slots);
-  __syncthreads();
-  int64_t jobs_before = upto.x - jobs, slots_before = upto.y - slots, all_jobs = 0;
-  for (int w = 0; w < kTreeThreads / 32; ++w) {
-    if (w < warp) jobs_before += warp_units[w], slots_before += warp_groups[w];
-    all_jobs += warp_units[w];
+  int32_t jobs_upto = jobs, slots_upto = slots;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
+    if (lane >= d) jobs_upto += u, slots_upto += v;
   }
-  chunk_jobs[tid] = int32_t(jobs_before);
-  chunk_slots[tid] = int32_t(slots_before);
-  if (blockIdx.x == 0) {
+  walk.length = length;
+  walk.own_jobs = jobs_upto - jobs;
+  walk.own_slots = slots_upto - slots;
+  if (small) {
+    walk.jobs = __shfl_sync(~0u, jobs_upto, 31);
+    if (lane >= a.batch) walk.own_jobs = INT32_MAX;
+  } else {
+    __syncthreads();  // the sums above have been read
+    if (lane == 31) warp_units[warp] = jobs_upto, warp_groups[warp] = slots_upto;
+    __syncthreads();
+    for (int w = 0; w < kTreeThreads / 32; ++w) {
+      if (w < warp) walk.own_jobs += int32_t(warp_units[w]), walk.own_slots += int32_t(warp_groups[w]);
+      walk.jobs += int32_t(warp_units[w]);
+    }
+    chunk_jobs[tid] = walk.own_jobs;
+    chunk_slots[tid] = walk.own_slots;
+  }
+  if (blockIdx.x == 0 && (!small || warp == 0)) {
+    int32_t before = walk.own_slots;
     for (int b = r0; b < r1; ++b) {
-      const TreeSeq s = tree_seq<N>(a, b);
-      a.slot_start[b] = int32_t(slots_before);
-      if (s.tiles > length) slots_before += int64_t(s.groups) * tree_segments(s, length);
+      const TreeSeq s = small ? walk.own : tree_seq<N>(a, b);
+      a.slot_start[b] = before;
+      if (s.tiles > length) before += s.groups * tree_segments(s, length);
     }
     if (tid == 0) a.slot_start[a.batch] = length;
   }
   __syncthreads();
+  tc_fence_after();
   const uint32_t tmem_o = *tmem_slot, tmem_s = tmem_o + 4 * N;
-  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, length, int32_t(all_jobs), int32_t(blockIdx.x), per};
   pdl_launch_dependents();
 
   if (warp < 8) {
@@ -707,10 +739,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
         for (int y = 0; y < W; ++y) x[y] = __uint_as_float(o[y]) * stat[r + y];
         if (!whole) {
-          float* dst = a.part_o + (int64_t(slot) * N + r) * kTreeDv + d;
+          float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * N + r) * kTreeDv) + d;
 #pragma unroll
-          for (int y = 0; y < W; ++y)
-            if (r + y < rows) dst[y * kTreeDv] = x[y];
+          for (int y = 0; y < W; y += 4)
+            if (r + y < rows) dst[y / 4 * kTreeDv] = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
         } else {
           bad |= tree_store<W>(a, qrow + r, rows - r, d, lane, x);
         }
@@ -738,8 +770,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tree_wait(bar, parity, abort, a.err)); };
     while (ok) {
-      const bool more = walk.next();
-      if (!__shfl_sync(~0u, int(more), 0)) break;
+      if (!walk.next()) break;  // alike in all lanes
       const int count = __shfl_sync(~0u, walk.count, 0);
       ok = wait(bar_q, segment & 1);
       for (int i = 0; i < count && ok; ++i, ++n) {
@@ -800,7 +831,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     }
     // the last MMAs retire before TMEM is released (commits cover all before them)
     if (n > 0) mbar_drain(bar_o, (n - 1) & 1);
-  } else if (warp == 9 && lane == 0) {
+  } else if (warp == 9) {
     // ------------------------------------------------------------ key tiles
     int n = 0;
     bool ok = true;
@@ -809,7 +840,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const int32_t* table = a.table + int64_t(walk.b) * a.stride;
       const int32_t blocks = int32_t((int64_t(s.context) + s.nodes + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS);
       auto row_of = [&](int32_t j) -> int32_t {  // first pool row of block j; past the pool: reads zeros
-        if (j >= blocks) return int32_t(a.pool_rows);
+        if (j >= blocks || lane != 0) return int32_t(a.pool_rows);
         const int64_t blk = table[j];
         if (blk < 0 || blk * DSR_BLOCK_TOKENS >= a.pool_rows) {
           flag(a.err, DSR_ERR_ID);
@@ -818,7 +849,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         return int32_t(blk * DSR_BLOCK_TOKENS);
       };
       int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
-      for (int i = 0; i < walk.count && ok; ++i, ++n) {
+      for (int i = 0; lane == 0 && i < walk.count && ok; ++i, ++n) {
         const int32_t x0 = y0, x1 = y1;
         if (i + 1 < walk.count) y0 = row_of(2 * (walk.tile0 + i) + 2), y1 = row_of(2 * (walk.tile0 + i) + 3);
 #pragma unroll 1
@@ -842,6 +873,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         tma_load_2d(sbase + L::kROff + 8192, &kv_map, bar_r, 512, x1);
         *loaded_r = n + 1;
       }
+      ok = __shfl_sync(~0u, int(ok), 0) != 0;
     }
   }
   tc_fence_before();
@@ -858,19 +890,24 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 }
 
 // ---------------------------------------------------------------------------
-// Joins the partials of a group that spans CTAs: one CTA per query row, thread t
-// four value columns.  out = sum_p 2^(m_p - M) O_p / (2^(sink - M) + sum_p 2^(m_p - M) l_p).
+// Joins the partials of a group of several segments: one CTA per four query rows
+// (of one node, since heads come in sixteens) and 128 value columns, a thread one
+// column of all four.
+//   out = sum_p 2^(m_p - M) O_p / (2^(sink - M) + sum_p 2^(m_p - M) l_p)
+// The statistics and a thread's first values are requested together, so that few
+// parts take one memory round trip.
 // ---------------------------------------------------------------------------
 constexpr int kTreeMaxCtas = 256;
 constexpr int kTreeMaxParts = kTreeSlotsPerCta * kTreeMaxCtas;  // of one row
+constexpr int kJoinThreads = 128, kJoinBatch = 8;  // kJoinBatch: parts requested together
 
 template <int N>
-__global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
-  __shared__ float weight[kTreeMaxParts];
-  __shared__ float inverse;
-  const int64_t row = blockIdx.x;
+__global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
+  __shared__ float weight[4][kTreeMaxParts];
+  __shared__ float inverse[4];
+  const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, d = blockIdx.y * kJoinThreads + tid;
   // the request of the node: the largest b with cu_nodes[b] <= node
   int lo = 0, hi = a.batch;
   while (hi - lo > 1) {
@@ -881,54 +918,60 @@ __global__ void __launch_bounds__(128) tree_combine_kernel(const __grid_constant
   const TreeSeq s = tree_seq<N>(a, lo);
   if (node < s.node0 || node >= s.node0 + s.nodes) return;
   pdl_wait();
-  const int parts = tree_segments(s, a.slot_start[a.batch]);
+  const int parts = tree_segments(s, __ldcg(a.slot_start + a.batch));
   if (parts <= 1) return;  // written by its job
   const int in = int(row - int64_t(s.node0) * a.heads), group = in / N, r = in % N;
-  const int64_t first = a.slot_start[lo] + group;
+  const int64_t first = int64_t(__ldcg(a.slot_start + lo)) + group;
   auto slot = [&](int p) { return (first + int64_t(p) * s.groups) * N + r; };
-  if (tid < 32) {
-    float top = -CUDART_INF_F, sum = 0.f;
-    for (int p = tid; p < parts; p += 32) top = fmaxf(top, a.part_m[slot(p)]);
+  float4 v[kJoinBatch];
+  auto request = [&](int p0) {
+#pragma unroll
+    for (int j = 0; j < kJoinBatch; ++j)
+      if (p0 + j < parts) v[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(p0 + j) * kTreeDv) + d);
+  };
+  request(0);
+  {
+    const int w = tid >> 5, lane = tid & 31;  // one warp per row
+    const float m0 = lane < parts ? __ldcg(a.part_m + slot(lane) + w) : -CUDART_INF_F;
+    const float l0 = lane < parts ? __ldcg(a.part_l + slot(lane) + w) : 0.f;
+    float top = m0, sum = 0.f;
+    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, __ldcg(a.part_m + slot(p) + w));
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
     const float base = top == -CUDART_INF_F ? 0.f : top;
-    for (int p = tid; p < parts; p += 32) {
-      const float w = ex2(a.part_m[slot(p)] - base);
-      weight[p] = w;
-      sum += w * a.part_l[slot(p)];
+    for (int p = lane; p < parts; p += 32) {
+      const float e = ex2((p < 32 ? m0 : __ldcg(a.part_m + slot(p) + w)) - base);
+      weight[w][p] = e;
+      sum += e * (p < 32 ? l0 : __ldcg(a.part_l + slot(p) + w));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (tid == 0) {
+    if (lane == 0) {
       float total;
-      const float lse = tree_total(a, int(row % a.heads), top, sum, total);
-      inverse = total > 0.f ? 1.f / total : 0.f;
-      if (a.lse != nullptr) a.lse[row] = lse;
+      const float lse = tree_total(a, int((row + w) % a.heads), top, sum, total);
+      inverse[w] = total > 0.f ? 1.f / total : 0.f;
+      if (a.lse != nullptr && blockIdx.y == 0) a.lse[row + w] = lse;
     }
   }
   __syncthreads();
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += 8) {
-    float4 v[8];
+  for (int p0 = 0; p0 < parts; p0 += kJoinBatch) {
+    if (p0 > 0) request(p0);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (p0 + j < parts) v[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + slot(p0 + j) * kTreeDv) + tid);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
+    for (int j = 0; j < kJoinBatch; ++j)
       if (p0 + j < parts) {
-        const float w = weight[p0 + j];
-        acc.x = fmaf(w, v[j].x, acc.x), acc.y = fmaf(w, v[j].y, acc.y);
-        acc.z = fmaf(w, v[j].z, acc.z), acc.w = fmaf(w, v[j].w, acc.w);
+        acc.x = fmaf(weight[0][p0 + j], v[j].x, acc.x), acc.y = fmaf(weight[1][p0 + j], v[j].y, acc.y);
+        acc.z = fmaf(weight[2][p0 + j], v[j].z, acc.z), acc.w = fmaf(weight[3][p0 + j], v[j].w, acc.w);
       }
   }
-  const float f = inverse;
-  acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
-  if (!(isfinite(acc.x) && isfinite(acc.y) && isfinite(acc.z) && isfinite(acc.w))) flag(a.err, DSR_ERR_NONFINITE);
-  if (a.out_wide)
-    reinterpret_cast<float4*>(static_cast<float*>(a.out) + row * kTreeDv)[tid] = acc;
-  else
-    reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + row * kTreeDv)[tid] =
-        make_uint2(bf16x2(acc.x, acc.y), bf16x2(acc.z, acc.w));
+  const float out[4] = {acc.x * inverse[0], acc.y * inverse[1], acc.z * inverse[2], acc.w * inverse[3]};
+#pragma unroll
+  for (int y = 0; y < 4; ++y) {
+    if (!isfinite(out[y])) flag(a.err, DSR_ERR_NONFINITE);
+    const int64_t at = (row + y) * kTreeDv + d;
+    if (a.out_wide) static_cast<float*>(a.out)[at] = out[y];
+    else static_cast<uint16_t*>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16_rn(out[y]));
+  }
 }
 
 // Rows per group: all of a request's rows in one group when that fits, since a
@@ -958,8 +1001,8 @@ int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStrea
   rc = launch_status("tree_mla_decode launch");
   if (rc != DSR_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.nodes * a.heads), 1, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  cfg.gridDim = dim3(unsigned(a.nodes * a.heads / 4), kTreeDv / kJoinThreads, 1);
+  cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
