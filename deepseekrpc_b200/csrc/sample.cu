@@ -12,13 +12,19 @@
 // borders between tokens by up to a few percent of a token).
 //
 // A cluster of 1 to 8 CTAs takes a row and holds it in shared memory, so that it is
-// read from memory once.  Prefixes are found from a histogram of counts over 2048 equal
-// steps of the value below the maximum: it says exactly which step holds rank k, and,
-// since the weights of a step are known to within its width, between which two steps
-// the mass p lies (where those hold too many entries, their exact masses say which).
-// Only the entries there are ranked, in the first CTA, on the unique 64-bit rank
-// (order-preserving value, inverted index) with exact weights.  Where the steps hold too many entries (equal logits, masks), the prefix comes from a
-// radix descent over the ranks instead, 11 bits a level.
+// read from memory once.  Prefixes are found from a histogram over 2048 equal steps of
+// the value below the maximum, of which each CTA sums up its share for the cluster:
+//   up to 100 by rank   the histogram is that of the threads' maxima, 512 a CTA, instead
+//                       of all entries: at least k entries lie in the steps down to the
+//                       one that holds the k-th maximum, and hardly any more
+//   by rank             the counts say which step holds entry k
+//   by mass             the weights of a step are known to within its width, which says
+//                       between which two steps p lies; their exact masses say in which
+// Entries in question go to a list in the first CTA, which ranks them on the unique
+// 64-bit rank (order-preserving value, inverted index) with exact weights: by comparing
+// all with all where there are few, after a finer histogram where there are more.  Where
+// a list overflows (equal logits, masks), the prefix comes from a radix descent over the
+// ranks, 11 bits a level.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -38,7 +44,8 @@ constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 2048, kSamplePer = kSampleBins / kSampleThreads;
 constexpr int kSampleMaxCluster = 8;
-constexpr int kSampleList = 2048;  // entries ranked by the sort
+constexpr int kSampleList = 1984;  // entries of a list
+constexpr int kSampleFew = 128;    // entries compared with one another
 constexpr int kSampleMaxVocab = 1 << 18;
 constexpr int kWeightBits = 44;  // 2^18 weights of at most 2^44 fit 62 bits
 constexpr double kLog2eD = 1.4426950408889634074;
@@ -101,12 +108,17 @@ struct alignas(16) SampleSmem {
   unsigned long long part[kSampleWarps], part2[kSampleWarps];
   float2 bounds[kSampleWarps];
   // written by every CTA of the cluster for all
+  unsigned long long counts[2][kSampleMaxCluster];  // of a scan, and of the one before
+  float2 masses[kSampleMaxCluster];
+  int2 steps[kSampleMaxCluster];
+  unsigned long long before[kSampleMaxCluster], through[kSampleMaxCluster];
   unsigned long long best[kSampleMaxCluster], sums[kSampleMaxCluster], above[kSampleMaxCluster],
       kept[kSampleMaxCluster];
   float low[kSampleMaxCluster];
   int bad[kSampleMaxCluster];
-  // written by the first CTA for all
-  unsigned long long cut;
+  // written by one CTA for all
+  unsigned long long cut, step_before;
+  int step_bin, step_in;
   // this CTA's own
   unsigned long long found_before, found_through;
   int found_bin, found_last, listed;
@@ -150,56 +162,21 @@ __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
   return v;
 }
 
-// Bitonic sort of list[0, n), n <= kSampleThreads * Q, in descending (or ascending)
-// order; thread t holds the entries t, t + kSampleThreads, ..: exchanges over less than
-// a warp go by shuffles, over a warp or more through the list itself.
-template <int Q, bool Descending>
+// Bitonic sort of list[0, n) in descending order; list has room for the next power of two.
 __device__ __forceinline__ void block_sort(unsigned long long* list, int n) {
-  const int tid = threadIdx.x;
-  unsigned long long v[Q];
-  __syncthreads();
-#pragma unroll
-  for (int q = 0; q < Q; ++q) {
-    const int e = q * kSampleThreads + tid;
-    v[q] = e < n ? list[e] : (Descending ? 0 : ~0ull);
-  }
-  for (int size = 2; size < 2 * n; size <<= 1)
+  int all = 2;
+  while (all < n) all <<= 1;
+  for (int i = n + threadIdx.x; i < all; i += kSampleThreads) list[i] = 0;
+  for (int size = 2; size <= all; size <<= 1)
     for (int gap = size >> 1; gap > 0; gap >>= 1) {
-      unsigned long long other[Q];
-      if (gap >= kSampleThreads) {
-#pragma unroll
-        for (int q = 0; q < Q; ++q) {
-          other[q] = v[q ^ 1];
-          if (Q > 2 && gap == 2 * kSampleThreads) other[q] = v[(q ^ 2) % Q];
-        }
-      } else if (gap >= 32) {
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) list[q * kSampleThreads + tid] = v[q];
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < Q; ++q) other[q] = list[(q * kSampleThreads + tid) ^ gap];
-      } else {
-#pragma unroll
-        for (int q = 0; q < Q; ++q) other[q] = __shfl_xor_sync(~0u, v[q], gap);
-      }
-#pragma unroll
-      for (int q = 0; q < Q; ++q) {
-        const int e = q * kSampleThreads + tid;
-        const bool ascends = ((e & size) == 0) != Descending, smaller = ((e & gap) == 0) == ascends;
-        if (smaller == (other[q] < v[q])) v[q] = other[q];
+      __syncthreads();
+      for (int i = threadIdx.x; i < all / 2; i += kSampleThreads) {
+        const int lo = (i & ~(gap - 1)) * 2 + (i & (gap - 1)), hi = lo + gap;
+        const unsigned long long x = list[lo], y = list[hi];
+        if (((lo & size) == 0) == (x < y)) list[lo] = y, list[hi] = x;
       }
     }
   __syncthreads();
-#pragma unroll
-  for (int q = 0; q < Q; ++q) list[q * kSampleThreads + tid] = v[q];
-  __syncthreads();
-}
-template <bool Descending>
-__device__ __forceinline__ void block_sort_any(unsigned long long* list, int n) {
-  static_assert(kSampleList == 4 * kSampleThreads, "");
-  if (n <= kSampleThreads) block_sort<1, Descending>(list, n);
-  else block_sort<4, Descending>(list, n);
 }
 
 template <bool W>
@@ -343,24 +320,62 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     atomicAdd(&s.wide[1][b], uint32_t(w >> 15) & 0x7fffu);
     atomicAdd(&s.wide[2][b], uint32_t(w >> 30));
   };
-  // Adds the cluster's sums of four consecutive words, shifted.
-  static_assert(kSamplePer == 4, "a thread's steps are one 16-byte piece");
-  auto cluster_words = [&](const uint32_t* words, unsigned long long (&sum)[kSamplePer], int bits) {
-    const uint32_t* mine = words + tid * kSamplePer;
-    constexpr int kTogether = 4;
+  // This CTA's share of the steps: `share` of them from first_step on, thread t those from
+  // first_step + t * per on (threads with t * per >= share: none).
+  static_assert(kSamplePer == 4, "a thread's piece is 16 bytes");
+  const int share = kSampleBins / ctas, first_step = rank * share;
+  const int per = share > kSampleThreads ? share / kSampleThreads : 1, my_step = first_step + tid * per;
+  const bool mine_any = tid * per < share;
+  // Adds the cluster's sums of this thread's steps, shifted: every thread fetches 16 bytes
+  // of one CTA's words.  After a cluster barrier; `words` must not change until the next.
+  auto gather_words = [&](const uint32_t* words, unsigned long long (&sum)[kSamplePer], int bits) {
+    const int pieces = share / 4, c = tid / pieces, q = tid % pieces;
+    uint4* stage = reinterpret_cast<uint4*>(s.list);  // 8 KB
+    __syncthreads();
+    stage[tid] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(words + first_step + 4 * q, c));
+    __syncthreads();
+    const uint32_t* staged = reinterpret_cast<const uint32_t*>(s.list);
+    if (mine_any) {
 #pragma unroll
-    for (int c0 = 0; c0 < kSampleMaxCluster; c0 += kTogether) {
-      uint4 h[kTogether];
-#pragma unroll
-      for (int c = 0; c < kTogether; ++c)
-        h[c] = c0 + c < ctas ? *reinterpret_cast<const uint4*>(cluster.map_shared_rank(mine, c0 + c))
-                             : make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int c = 0; c < kTogether; ++c) {
-        sum[0] += static_cast<unsigned long long>(h[c].x) << bits, sum[1] += static_cast<unsigned long long>(h[c].y) << bits;
-        sum[2] += static_cast<unsigned long long>(h[c].z) << bits, sum[3] += static_cast<unsigned long long>(h[c].w) << bits;
-      }
+      for (int j = 0; j < kSamplePer; ++j)
+        if (j < per)
+          for (int o = 0; o < ctas; ++o)
+            sum[j] += static_cast<unsigned long long>(staged[o * share + tid * per + j]) << bits;
     }
+    __syncthreads();
+  };
+  // Sums of this CTA's share before this thread's steps become sums over the cluster's
+  // steps; `total`: over all.
+  int scans = 0;
+  auto cluster_scan = [&](const unsigned long long (&v)[kSamplePer], unsigned long long& total) {
+    unsigned long long sum;
+    unsigned long long at = block_scan(s, (v[0] + v[1]) + (v[2] + v[3]), sum);
+    scans ^= 1;
+    if (tid < ctas) cluster.map_shared_rank(&s, tid)->counts[scans][rank] = sum;
+    cluster.sync();
+    total = 0;
+    for (int c = 0; c < ctas; ++c) {
+      if (c < rank) at += s.counts[scans][c];
+      total += s.counts[scans][c];
+    }
+    return at;
+  };
+  // The step in which the sums reach target, what lies before it and in it: the thread
+  // that has it tells everybody.  A barrier of the cluster.
+  auto find_step = [&](unsigned long long at, const unsigned long long (&v)[kSamplePer], unsigned long long target,
+                       const unsigned long long (&in)[kSamplePer]) {
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+      if (at < target && at + v[j] >= target)
+        for (int c = 0; c < ctas; ++c) {
+          SampleSmem* other = cluster.map_shared_rank(&s, c);
+          other->step_bin = my_step + j;
+          other->step_before = at;
+          other->step_in = int(in[j]);
+        }
+      at += v[j];
+    }
+    cluster.sync();
   };
 
   // The rank of the last entry of the shortest prefix, among ranks >= cut, whose count
@@ -378,21 +393,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       });
       cluster.sync();
       unsigned long long digit[kSamplePer] = {0, 0, 0, 0}, total;
-      cluster_words(s.wide[0], digit, 0);
-      if (mass) cluster_words(s.wide[1], digit, 15), cluster_words(s.wide[2], digit, 30);
-      const unsigned long long own = (digit[0] + digit[1]) + (digit[2] + digit[3]);
-      unsigned long long at = before + block_scan(s, own, total);
-#pragma unroll
-      for (int j = 0; j < kSamplePer; ++j) {
-        if (at < target && at + digit[j] >= target) {
-          s.found_bin = kSampleBins - 1 - (tid * kSamplePer + j);
-          s.found_before = at;
-        }
-        at += digit[j];
-      }
-      cluster.sync();  // before the sums are cleared again
-      known = (known << 11) | unsigned(s.found_bin);
-      before = s.found_before;
+      gather_words(s.wide[0], digit, 0);
+      if (mass) gather_words(s.wide[1], digit, 15), gather_words(s.wide[2], digit, 30);
+      const unsigned long long at = before + cluster_scan(digit, total);
+      find_step(at, digit, target, digit);
+      known = (known << 11) | unsigned(kSampleBins - 1 - s.step_bin);
+      before = s.step_before;
       __syncthreads();
     }
     return known;
@@ -433,111 +439,123 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     a.chances[row] = float(double(w) / double(all));
   };
   auto border_of = [&](unsigned long long all) { return (unsigned long long)(double(u) * double(all)); };
-  // The first CTA, with every entry that may be kept in its list: the rest of the
-  // filters and the draw.  `limit` entries by rank; `mass`: what p refers to, or 0 for theirs.
+  // The first CTA, with every entry that may be kept (at most kSampleFew) in its list: the
+  // rest of the filters and the draw.  `limit` entries by rank; `mass`: what p refers to, or 0 for theirs.
   auto finish = [&](int n, int limit, unsigned long long mass) {
-    constexpr int kFew = 128, kShare = kSampleThreads / kFew;
-    if (n <= kFew) {
-      // four threads per entry compare it with all: how many and how much lie above it
-      const int e = tid / kShare, part = tid % kShare;
-      __syncthreads();
-      const unsigned long long r = e < n ? s.list[e] : 0;
-      const unsigned long long w = e < n ? weight(rank_value(r)) : 0;
-      unsigned long long* weights = s.list + kFew;
-      if (part == 0) weights[e] = w;
-      __syncthreads();
-      int ahead = 0;
-      unsigned long long above = 0;
-      for (int j = part; j < n; j += kShare) {
-        const bool more = s.list[j] > r;
-        ahead += more;
-        above += more ? weights[j] : 0;
-      }
-#pragma unroll
-      for (int o = 1; o < kShare; o <<= 1) {
-        ahead += __shfl_xor_sync(~0u, ahead, o);
-        above += __shfl_xor_sync(~0u, above, o);
-      }
-      const bool in = e < n && ahead < limit;
-      unsigned long long all;
-      block_scan(s, in && part == 0 ? w : 0, all);  // also: the weights have been read
-      const unsigned long long target = by_mass ? mass_target(mass == 0 ? all : mass) : ~0ull;
-      const unsigned long long stays = in && above < target && enough(rank_value(r)) ? w : 0;
-      if (part == 0) weights[e] = stays;
-      __syncthreads();
-      unsigned long long before = 0;
-      all = 0;
-      for (int j = part; j < n; j += kShare) {
-        const unsigned long long v = weights[j];
-        all += v;
-        before += uint32_t(s.list[j]) > uint32_t(r) ? v : 0;  // a lower index
-      }
-#pragma unroll
-      for (int o = 1; o < kShare; o <<= 1) {
-        all += __shfl_xor_sync(~0u, all, o);
-        before += __shfl_xor_sync(~0u, before, o);
-      }
-      const unsigned long long border = border_of(all);
-      if (part == 0 && before <= border && before + stays > border) draw(int(0xffffffffu - uint32_t(r)), stays, all);
-      return;
+    constexpr int kShare = kSampleThreads / kSampleFew;
+    // four threads per entry compare it with all: how many and how much lie above it
+    const int e = tid / kShare, part = tid % kShare;
+    __syncthreads();
+    const unsigned long long r = e < n ? s.list[e] : 0;
+    const unsigned long long w = e < n ? weight(rank_value(r)) : 0;
+    unsigned long long* weights = s.list + kSampleFew;
+    if (part == 0) weights[e] = w;
+    __syncthreads();
+    int ahead = 0;
+    unsigned long long above = 0;
+    for (int j = part; j < n; j += kShare) {
+      const bool more = s.list[j] > r;
+      ahead += more;
+      above += more ? weights[j] : 0;
     }
-    block_sort_any<true>(s.list, n);
-    n = min(n, limit);
-    unsigned long long w[kSamplePer], own = 0, all;
-    static_assert(kSampleList == kSamplePer * kSampleThreads, "");
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-      const int i = tid * kSamplePer + j;
-      w[j] = weight(i < n ? rank_value(s.list[i]) : nothing);
-      own += w[j];
+    for (int o = 1; o < kShare; o <<= 1) {
+      ahead += __shfl_xor_sync(~0u, ahead, o);
+      above += __shfl_xor_sync(~0u, above, o);
     }
-    unsigned long long run = block_scan(s, own, all);
+    const bool in = e < n && ahead < limit;
+    unsigned long long all;
+    block_scan(s, in && part == 0 ? w : 0, all);  // also: the weights have been read
     const unsigned long long target = by_mass ? mass_target(mass == 0 ? all : mass) : ~0ull;
-    // kept: what is above has not reached the target, and the weight is large enough
-    int mine = 0;
-    unsigned long long stays[kSamplePer];
-#pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-      const int i = tid * kSamplePer + j;
-      stays[j] = 0;
-      if (i < n && run < target && w[j] > 0) {
-        const unsigned long long r = s.list[i];
-        if (enough(rank_value(r))) {
-          stays[j] = (static_cast<unsigned long long>(0xffffffffu - uint32_t(r)) << (kWeightBits + 1)) | w[j];
-          ++mine;
-        }
-      }
-      run += w[j];
+    const unsigned long long stays = in && above < target && enough(rank_value(r)) ? w : 0;
+    if (part == 0) weights[e] = stays;
+    __syncthreads();
+    unsigned long long before = 0;
+    all = 0;
+    for (int j = part; j < n; j += kShare) {
+      const unsigned long long v = weights[j];
+      all += v;
+      before += uint32_t(s.list[j]) > uint32_t(r) ? v : 0;  // a lower index
     }
-    unsigned long long m;
-    int to = int(block_scan(s, unsigned(mine), m));  // also: the list has been read
 #pragma unroll
-    for (int j = 0; j < kSamplePer; ++j)
-      if (stays[j] != 0) s.list[to++] = stays[j];
-    block_sort_any<false>(s.list, int(m));  // vocabulary order
-    constexpr unsigned long long kMask = (1ull << (kWeightBits + 1)) - 1;
-    own = 0;
-#pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-      const int i = tid * kSamplePer + j;
-      w[j] = i < int(m) ? s.list[i] & kMask : 0;
-      own += w[j];
+    for (int o = 1; o < kShare; o <<= 1) {
+      all += __shfl_xor_sync(~0u, all, o);
+      before += __shfl_xor_sync(~0u, before, o);
     }
-    run = block_scan(s, own, all);
     const unsigned long long border = border_of(all);
-#pragma unroll
-    for (int j = 0; j < kSamplePer; ++j) {
-      if (run <= border && run + w[j] > border) draw(int(s.list[tid * kSamplePer + j] >> (kWeightBits + 1)), w[j], all);
-      run += w[j];
-    }
+    if (part == 0 && before <= border && before + stays > border) draw(int(0xffffffffu - uint32_t(r)), stays, all);
   };
-  // Every CTA: after the first one has read their lists they may leave; it draws.
+  // Every CTA, after a barrier behind its list: once the first one has read the lists they
+  // may leave; it draws.  False (alike in all) when there are too many entries.
   auto finish_alone = [&](int limit, unsigned long long mass) {
-    cluster.sync();
     const int n = bring();
+    if (n > kSampleFew) return false;
     auto read = cluster.barrier_arrive();
     if (rank == 0) finish(n, limit, mass);
     cluster.barrier_wait(std::move(read));
+    return true;
+  };
+  // The first CTA, with n entries of step `bin` in its list: the rank of the one at which
+  // their count, or mass, reaches target.  A finer histogram of the step, then the entries
+  // of one of its parts.
+  auto rank_listed = [&](int n, bool mass, unsigned long long target, auto&& part_of) {
+    for (int b = tid; b < kSampleBins; b += kSampleThreads) s.hist[b] = 0;
+    if (mass)
+      for (int b = tid; b < kSampleBins; b += kSampleThreads) s.wide[0][b] = s.wide[1][b] = s.wide[2][b] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const float f = rank_value(s.list[i]);
+      const int b = part_of(f);
+      atomicAdd(&s.hist[b], 1u);
+      if (mass) add_wide(b, weight(f));
+    }
+    __syncthreads();
+    unsigned long long v[kSamplePer], own = 0, all;
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+      const int b = tid * kSamplePer + j;
+      v[j] = !mass ? s.hist[b]
+                   : s.wide[0][b] + (static_cast<unsigned long long>(s.wide[1][b]) << 15) +
+                         (static_cast<unsigned long long>(s.wide[2][b]) << 30);
+      own += v[j];
+    }
+    unsigned long long at = block_scan(s, own, all);
+#pragma unroll
+    for (int j = 0; j < kSamplePer; ++j) {
+      if (at < target && at + v[j] >= target) s.found_bin = tid * kSamplePer + j, s.found_before = at;
+      at += v[j];
+    }
+    if (tid == 0) s.found_last = 0;
+    __syncthreads();
+    const int part = s.found_bin;
+    const unsigned long long before = s.found_before;
+    unsigned long long* some = reinterpret_cast<unsigned long long*>(s.wide);  // 24 KB: every entry fits
+    for (int i = tid; i < n; i += kSampleThreads) {
+      const unsigned long long r = s.list[i];
+      if (part_of(rank_value(r)) == part) some[atomicAdd(&s.found_last, 1)] = r;
+    }
+    __syncthreads();
+    const int m = s.found_last;
+    if (m > 1) block_sort(some, m);
+    // entry by entry from the top (a part holds one entry as a rule; many when they are equal)
+    unsigned long long cut = some[0];
+    if (!mass) {
+      cut = some[target - before - 1];
+    } else if (m > 1) {
+      const int each_has = (m + kSampleThreads - 1) / kSampleThreads, i0 = min(tid * each_has, m),
+                i1 = min(i0 + each_has, m);
+      own = 0;
+      for (int i = i0; i < i1; ++i) own += weight(rank_value(some[i]));
+      unsigned long long run = before + block_scan(s, own, all);
+      for (int i = i0; i < i1; ++i) {
+        const unsigned long long w = weight(rank_value(some[i]));
+        if (run < target && run + w >= target) s.found_through = some[i];
+        run += w;
+      }
+      __syncthreads();
+      cut = s.found_through;
+    }
+    if (tid < ctas) cluster.map_shared_rank(&s, tid)->cut = cut;
   };
 
   // ---- filters: the prefix of ranks >= cut
@@ -548,55 +566,67 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const float step = reach / float(kSampleBins);  // inverse of per_step
     // one value only, or a temperature whose steps are no normal numbers: all in step 0
     const bool binned = per_step > 0.f && per_step < CUDART_INF_F && heat > 1e-30f;
-    auto bin_of = [&](float f) {
-      return binned ? int(fminf((top - f) * per_step, float(kSampleBins - 1))) : 0;
+    // where f lies among the steps; its step; whether that is at most b, or below it
+    auto place_of = [&](float f) { return binned ? (top - f) * per_step : 0.f; };
+    auto bin_of = [&](float f) { return int(fminf(place_of(f), float(kSampleBins - 1))); };
+    auto bound_after = [&](int b) { return b < kSampleBins - 1 ? float(b + 1) : CUDART_INF_F; };  // place < it: step <= b
+    auto part_of = [&](int bin) {  // of step `bin`, in kSampleBins parts
+      return [=](float f) {
+        return int(fminf(fmaxf((place_of(f) - float(bin)) * float(kSampleBins), 0.f), float(kSampleBins - 1)));
+      };
     };
+    unsigned long long count[kSamplePer] = {0, 0, 0, 0}, total;
+
+    if (by_rank && k <= 100) {
+      // the steps of the threads' maxima
+      if (most != nothing) atomicAdd(&s.hist[bin_of(most)], 1u);
+      cluster.sync();
+      gather_words(s.hist, count, 0);
+      const unsigned long long at = cluster_scan(count, total);
+      if (unsigned(k) <= total) {
+        find_step(at, count, unsigned(k), count);
+        const float bound = bound_after(s.step_bin);
+        each([&](float f, int i) {
+          if (place_of(f) < bound && f != nothing) keep(f, i);
+        });
+        cluster.sync();
+        if (finish_alone(k, 0)) return;
+      }
+      // too many of them: the ordinary way, from the start
+      cluster.sync();
+      if (tid == 0) s.listed = 0;
+      for (int b = tid; b < kSampleBins; b += kSampleThreads) s.hist[b] = 0;
+#pragma unroll
+      for (int j = 0; j < kSamplePer; ++j) count[j] = 0;
+      __syncthreads();
+    }
     // the last step holds all that is far below (a mask's low value): counted by thread
     uint32_t tail = 0;
     each([&](float f, int) {
-      const int b = bin_of(f);
+      const float at = place_of(f);
       const bool counts = f != nothing;  // -inf is never drawn, and all that lies off the row
-      if (b == kSampleBins - 1 || !binned) tail += counts;
-      else if (counts) atomicAdd(&s.hist[b], 1u);
+      if (at >= float(kSampleBins - 1) || !binned) tail += counts;
+      else if (counts) atomicAdd(&s.hist[int(at)], 1u);
     });
     tail = __reduce_add_sync(~0u, tail);
     if (lane == 0 && tail > 0) atomicAdd(&s.hist[binned ? kSampleBins - 1 : 0], tail);
     cluster.sync();
-    // thread t: the counts of steps kSamplePer t .., over all CTAs
-    unsigned long long count[kSamplePer] = {0, 0, 0, 0}, total;
-    cluster_words(s.hist, count, 0);
-    const unsigned long long own = (count[0] + count[1]) + (count[2] + count[3]);
-    unsigned long long at = block_scan(s, own, total);
+    gather_words(s.hist, count, 0);
+    const unsigned long long at = cluster_scan(count, total);
 
     if (by_rank && unsigned(k) < total) {
-#pragma unroll
-      for (int j = 0; j < kSamplePer; ++j) {
-        if (at < unsigned(k) && at + count[j] >= unsigned(k)) {
-          s.found_bin = tid * kSamplePer + j;
-          s.found_before = at;
-          s.found_last = int(count[j]);
-        }
-        at += count[j];
-      }
+      find_step(at, count, unsigned(k), count);
+      const int bin = s.step_bin, before = int(s.step_before), in = s.step_in;
       __syncthreads();
-      const int bin = s.found_bin, before = int(s.found_before), in = s.found_last;
-      if (before + in <= kSampleList) {  // every kept entry fits the list
-        each([&](float f, int i) {
-          if (bin_of(f) <= bin && f != nothing) keep(f, i);
-        });
-        finish_alone(k, 0);
-        return;
-      }
       if (in <= kSampleList) {
+        const float from = float(bin), bound = bound_after(bin);
         each([&](float f, int i) {
-          if (bin_of(f) == bin && f != nothing) keep(f, i);
+          const float at = place_of(f);
+          if (at >= from && at < bound && f != nothing) keep(f, i);
         });
         cluster.sync();
         const int n = bring();
-        if (rank == 0) {
-          block_sort_any<true>(s.list, n);
-          if (tid < ctas) cluster.map_shared_rank(&s, tid)->cut = s.list[k - before - 1];
-        }
+        if (rank == 0) rank_listed(n, false, unsigned(k - before), part_of(bin));
         cluster.sync();
         cut = s.cut;
         if (tid == 0) s.listed = 0;
@@ -607,8 +637,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       // the counts of the prefix, for the mass below
 #pragma unroll
       for (int j = 0; j < kSamplePer; ++j) {
-        const int b = tid * kSamplePer + j;
-        if (b == bin) count[j] = unsigned(k - before);
+        const int b = my_step + j;
+        if (b == bin && count[j] > 0) count[j] = unsigned(k - before);  // 0: not this thread's
         else if (b > bin) count[j] = 0;
       }
     }
@@ -618,10 +648,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       float lo[kSamplePer], hi[kSamplePer], lo_own = 0.f, hi_own = 0.f;
 #pragma unroll
       for (int j = 0; j < kSamplePer; ++j) {
-        const int b = tid * kSamplePer + j;
+        const int b = my_step + j;
         // a hundredth of a step covers the rounding of the step's number
-        hi_own += float(count[j]) * expf(-fmaxf(float(b) - 0.01f, 0.f) * fall) * 1.0001f;
-        if (b < kSampleBins - 1) lo_own += float(count[j]) * expf(-(float(b) + 1.01f) * fall) * 0.9999f;
+        if (count[j] > 0) {
+          hi_own += float(count[j]) * expf(-fmaxf(float(b) - 0.01f, 0.f) * fall) * 1.0001f;
+          if (b < kSampleBins - 1) lo_own += float(count[j]) * expf(-(float(b) + 1.01f) * fall) * 0.9999f;
+        }
         lo[j] = lo_own, hi[j] = hi_own;
       }
       float lo_run = lo_own, hi_run = hi_own;
@@ -630,9 +662,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const float l = __shfl_up_sync(~0u, lo_run, d), h = __shfl_up_sync(~0u, hi_run, d);
         if (lane >= d) lo_run += l, hi_run += h;
       }
-      __syncthreads();
       if (lane == 31) s.bounds[warp] = make_float2(lo_run, hi_run);
-      if (tid == 0) s.found_bin = kSampleBins, s.found_last = kSampleBins - 1;
       __syncthreads();
       float lo_at = lo_run - lo_own, hi_at = hi_run - hi_own, lo_all = 0.f, hi_all = 0.f;
 #pragma unroll
@@ -641,35 +671,59 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         if (w < warp) lo_at += v.x, hi_at += v.y;
         lo_all += v.x, hi_all += v.y;
       }
+      if (tid < ctas) cluster.map_shared_rank(&s, tid)->masses[rank] = make_float2(lo_all, hi_all);
+      unsigned long long upto = cluster_scan(count, total);  // its barrier covers the masses
+      lo_all = hi_all = 0.f;
+      for (int c = 0; c < ctas; ++c) {
+        const float2 v = s.masses[c];
+        if (c < rank) lo_at += v.x, hi_at += v.y;
+        lo_all += v.x, hi_all += v.y;
+      }
       // the cut lies past every step whose upper bound is below p times the total's
       // lower one, and no later than the first whose lower bound reaches p times the
       // total's upper one (the sums' own rounding: below 10^-4)
       const float below = p * lo_all * 0.999f, reached = p * hi_all * 1.001f;
-      int first_bin = kSampleBins, last_bin = kSampleBins;
-#pragma unroll
-      for (int j = kSamplePer - 1; j >= 0; --j) {
-        const int b = tid * kSamplePer + j;
-        if (hi_at + hi[j] >= below) first_bin = b;
-        if (lo_at + lo[j] >= reached) last_bin = b;
-      }
-      first_bin = __reduce_min_sync(~0u, first_bin), last_bin = __reduce_min_sync(~0u, last_bin);
-      if (lane == 0) atomicMin(&s.found_bin, first_bin), atomicMin(&s.found_last, last_bin);
+      if (tid == 0) s.found_bin = s.found_last = kSampleBins, s.found_before = s.found_through = total;
       __syncthreads();
-      const int from = binned ? s.found_bin : 0, to = binned ? s.found_last : kSampleBins - 1;
-      // counts before the one and through the other
-      unsigned long long total2;
-      unsigned long long upto = block_scan(s, (count[0] + count[1]) + (count[2] + count[3]), total2);
+      if (mine_any) {
+        int first_bin = kSampleBins, last_bin = kSampleBins;
 #pragma unroll
-      for (int j = 0; j < kSamplePer; ++j) {
-        const int b = tid * kSamplePer + j;
-        if (b == from) s.found_before = upto;
-        upto += count[j];
-        if (b == to) s.found_through = upto;
+        for (int j = kSamplePer - 1; j >= 0; --j) {
+          if (j < per && hi_at + hi[j] >= below) first_bin = my_step + j;
+          if (j < per && lo_at + lo[j] >= reached) last_bin = my_step + j;
+        }
+        if (first_bin < kSampleBins) atomicMin(&s.found_bin, first_bin);
+        if (last_bin < kSampleBins) atomicMin(&s.found_last, last_bin);
       }
       __syncthreads();
-      const unsigned long long before = s.found_before, through = s.found_through;
-      const bool whole = cut == 0 && through <= kSampleList, some = whole || through - before <= kSampleList;
-      const int list_from = whole ? 0 : from;
+      if (mine_any) {
+#pragma unroll
+        for (int j = 0; j < kSamplePer; ++j)
+          if (j < per) {
+            if (my_step + j == s.found_bin) s.found_before = upto;
+            upto += count[j];
+            if (my_step + j == s.found_last) s.found_through = upto;
+          }
+      }
+      __syncthreads();
+      if (tid < ctas) {
+        SampleSmem* other = cluster.map_shared_rank(&s, tid);
+        other->steps[rank] = make_int2(s.found_bin, s.found_last);
+        other->before[rank] = s.found_before;
+        other->through[rank] = s.found_through;
+      }
+      cluster.sync();
+      // the first step of each kind that a CTA has found; without one, or without steps, all
+      int from = 0, to = kSampleBins - 1;
+      unsigned long long before = 0, through = total;
+      if (binned) {
+        for (int c = ctas - 1; c >= 0; --c) {
+          if (s.steps[c].x < kSampleBins) from = s.steps[c].x, before = s.before[c];
+          if (s.steps[c].y < kSampleBins) to = s.steps[c].y, through = s.through[c];
+        }
+      }
+      const bool whole = cut == 0 && through <= kSampleFew, some = whole || through - before <= kSampleList;
+      const float begin = whole ? 0.f : float(from), middle = float(from), bound = bound_after(to);
       // one pass: the exact mass of the prefix and of its part before step `from`, and the
       // entries of the steps between, where they fit the list, else the steps' exact masses
       if (!some) clear_wide();
@@ -684,11 +738,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
           const bool in = f[j] > cut_at || (f[j] == cut_at && rank_of(f[j], i + j) >= cut);
           w[j] = in ? w[j] : 0;
           z += w[j];
-          const int b = bin_of(f[j]);
-          over += b < from ? w[j] : 0;
-          if (in && b >= list_from && b <= to && f[j] != nothing) {
+          const float at = place_of(f[j]);
+          over += at < middle ? w[j] : 0;
+          if (in && at >= begin && at < bound && f[j] != nothing) {
             if (some) keep(f[j], i + j);
-            else add_wide(b, w[j]);
+            else add_wide(bin_of(f[j]), w[j]);
           }
         }
       });
@@ -705,58 +759,38 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       cluster.sync();
       z = over = 0;
       for (int c = 0; c < ctas; ++c) z += s.sums[c], over += s.above[c];
-      if (whole) {
-        finish_alone(kSampleList, z);
-        return;
-      }
+      if (whole && finish_alone(kSampleFew, z)) return;
       const unsigned long long target = mass_target(z);
+      // the step that the target lies in, and its entries
       bool fits = some;
+      int bin = from;
+      auto parts = [&](float f) {  // of the listed entries' steps
+        return fits && some ? int(fminf(fmaxf((place_of(f) - float(from)) / float(to - from + 1) * float(kSampleBins), 0.f),
+                                        float(kSampleBins - 1)))
+                            : part_of(bin)(f);
+      };
       if (!some) {
-        // the step that the target lies in; its entries
         unsigned long long mass[kSamplePer] = {0, 0, 0, 0};
-        cluster_words(s.wide[0], mass, 0);
-        cluster_words(s.wide[1], mass, 15);
-        cluster_words(s.wide[2], mass, 30);
-        unsigned long long run = over + block_scan(s, (mass[0] + mass[1]) + (mass[2] + mass[3]), total2);
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j) {
-          if (run < target && run + mass[j] >= target) {
-            s.found_bin = tid * kSamplePer + j;
-            s.found_before = run;
-            s.found_last = int(count[j]);
-          }
-          run += mass[j];
-        }
-        __syncthreads();
-        const int bin = s.found_bin;
-        fits = s.found_last <= kSampleList;
-        over = s.found_before;
-        if (fits) each([&](float f, int i) {
-            if (bin_of(f) == bin && f != nothing && rank_of(f, i) >= cut) keep(f, i);
+        gather_words(s.wide[0], mass, 0);
+        gather_words(s.wide[1], mass, 15);
+        gather_words(s.wide[2], mass, 30);
+        const unsigned long long run = over + cluster_scan(mass, total);
+        find_step(run, mass, target, count);
+        bin = s.step_bin;
+        fits = s.step_in <= kSampleList;
+        over = s.step_before;
+        if (fits) {
+          const float low_end = float(bin), high_end = bound_after(bin);
+          each([&](float f, int i) {
+            const float at = place_of(f);
+            if (at >= low_end && at < high_end && f != nothing && rank_of(f, i) >= cut) keep(f, i);
           });
+        }
         cluster.sync();
       }
       if (fits) {
         const int n = bring();
-        if (rank == 0) {
-          block_sort_any<true>(s.list, n);
-          unsigned long long w[kSamplePer], own = 0, all;
-#pragma unroll
-          for (int j = 0; j < kSamplePer; ++j) {
-            const int i = tid * kSamplePer + j;
-            w[j] = weight(i < n ? rank_value(s.list[i]) : nothing);
-            own += w[j];
-          }
-          unsigned long long run = over + block_scan(s, own, all);
-#pragma unroll
-          for (int j = 0; j < kSamplePer; ++j) {
-            if (run < target && run + w[j] >= target) {
-              const unsigned long long r = s.list[tid * kSamplePer + j];
-              for (int c = 0; c < ctas; ++c) cluster.map_shared_rank(&s, c)->cut = r;
-            }
-            run += w[j];
-          }
-        }
+        if (rank == 0) rank_listed(n, true, target - over, parts);
         cluster.sync();
         cut = s.cut;
       } else {
@@ -846,6 +880,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     }
   }
 }
+
+static_assert(sizeof(SampleSmem) <= 50160, "two CTAs with 65,552 bytes of a row each share an SM");
 
 template <bool W>
 int launch_sample(SampleArgs& a, int64_t rows, cudaStream_t stream) {
