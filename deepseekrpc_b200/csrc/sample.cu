@@ -29,6 +29,7 @@
 #include <math_constants.h>
 
 #include <cfloat>
+#include <climits>
 #include <type_traits>
 #include <utility>
 
@@ -71,8 +72,8 @@ struct SampleArgs {
 struct Weight {
   const double* table;  // [16] 2^(j/16)
   double high, scale;   // scale: 16 log2(e) / heat
-  float floor;          // below: no weight (2^-60 of the largest, or -inf)
-  // The weight in the fixed point's steps, plus the bits of 2^(52 - kWeightBits).
+  float floor;          // below: no weight (less than 2^-60 of the largest, or -inf)
+  // The weight plus 2^(52 - kWeightBits), whose lowest bit is a step of the fixed point.
   __device__ __forceinline__ double shifted(float x) const {
     const double t = (double(fmaxf(x, floor)) - high) * scale;
     constexpr double kRound = 6755399441055744.0, c = 0.043321698784996582;  // 1.5 * 2^52; ln(2) / 16
@@ -87,11 +88,12 @@ struct Weight {
     return fma(p, __hiloint2double(__double2hiint(e) + (m >> 4) * (1 << 20), __double2loint(e)), kMagic);
   }
   static constexpr double kMagic = double(1ull << (52 - kWeightBits));
-  // what a weight is in steps of 2^-44, rounded
+  // What a weight is in steps of 2^-44, rounded.  At the floor that is zero by itself, but
+  // in a row whose finite values end there (a maximum near the lowest number).
   __device__ __forceinline__ unsigned long long operator()(float x) const {
-    const double w = shifted(x);
-    const unsigned long long bits = (unsigned long long)__double_as_longlong(w) - (unsigned long long)__double_as_longlong(kMagic);
-    return x >= floor ? bits : 0;
+    const unsigned long long w =
+        (unsigned long long)__double_as_longlong(shifted(x)) - (unsigned long long)__double_as_longlong(kMagic);
+    return x >= floor ? w : 0;
   }
 };
 
@@ -112,10 +114,9 @@ struct alignas(16) SampleSmem {
   float2 masses[kSampleMaxCluster];
   int2 steps[kSampleMaxCluster];
   unsigned long long before[kSampleMaxCluster], through[kSampleMaxCluster];
-  unsigned long long best[kSampleMaxCluster], sums[kSampleMaxCluster], above[kSampleMaxCluster],
-      kept[kSampleMaxCluster];
-  float low[kSampleMaxCluster];
-  int bad[kSampleMaxCluster];
+  unsigned long long sums[kSampleMaxCluster], above[kSampleMaxCluster], kept[kSampleMaxCluster];
+  float tops[kSampleMaxCluster], lows[kSampleMaxCluster];
+  int firsts[kSampleMaxCluster];
   // written by one CTA for all
   unsigned long long cut, step_before;
   int step_bin, step_in;
@@ -201,15 +202,14 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   auto started = cluster.barrier_arrive();  // every CTA is there before one writes to another
   const float heat = a.temperature[row], p = a.top_p[row], least = a.min_p[row], u = a.uniform[row];
   const int k = a.top_k[row];
+  const double scale = 16.0 * kLog2eD / double(heat);  // a division in 64 bits: while the row is on its way
   if (tid < 16) s.table[tid] = exp2(tid / 16.0);
   if (tid == 0) s.listed = 0;
   for (int b = tid; b < kSampleBins; b += kSampleThreads) s.hist[b] = 0;
 
   // ---- the slice into shared memory (places off the row: -inf); extremes, non-finite values
   const float nothing = -CUDART_INF_F;
-  float most = nothing, low = CUDART_INF_F;
-  int at_most = 0;
-  int bad = 0;
+  float most = nothing;  // NaN when there is one
   constexpr int kAhead = 4;  // pieces requested together
   for (int v0 = tid * kVec; v0 < a.slice; v0 += kAhead * kSampleThreads * kVec) {
     uint4 raw[kAhead];
@@ -236,54 +236,45 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 #pragma unroll
       for (int j = 0; j < kVec; ++j) {
         const float f = Row::value(t[j]);
-        bad |= !(f < CUDART_INF_F);
-        if (f > most) most = f, at_most = base + v + j;  // the first of equal ones
-        low = fminf(low, f > nothing ? f : low);
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(f));
       }
     }
   }
-  unsigned long long best = rank_of(most, at_most);
+  float top = most;
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
-    const unsigned long long r = __shfl_xor_sync(~0u, best, o);
-    best = r > best ? r : best;
-    low = fminf(low, __shfl_xor_sync(~0u, low, o));
+    const float other = __shfl_xor_sync(~0u, top, o);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
   }
-  if (lane == 0) s.part[warp] = best, s.bounds[warp].x = low;
-  bad = __syncthreads_or(bad);
+  if (lane == 0) s.bounds[warp].x = top;
+  __syncthreads();
   cluster.barrier_wait(std::move(started));
   if (tid < ctas) {  // thread c tells CTA c
     for (int w = 0; w < kSampleWarps; ++w) {
-      best = s.part[w] > best ? s.part[w] : best;
-      low = fminf(low, s.bounds[w].x);
+      const float other = s.bounds[w].x;
+      asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
     }
-    SampleSmem* other = cluster.map_shared_rank(&s, tid);
-    other->best[rank] = best;
-    other->low[rank] = low;
-    other->bad[rank] = bad;
+    cluster.map_shared_rank(&s, tid)->tops[rank] = top;
   }
   cluster.sync();
-  bad = 0;
   for (int c = 0; c < ctas; ++c) {
-    best = s.best[c] > best ? s.best[c] : best;
-    low = fminf(low, s.low[c]);
-    bad |= s.bad[c];
+    const float other = s.tops[c];
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
   }
-  const float top = rank_value(best);
+  const bool bad = !(top < CUDART_INF_F);
   const bool valid = heat >= 0.f && heat < CUDART_INF_F && p >= 0.f && p <= 1.f && least >= 0.f && least <= 1.f &&
                      u >= 0.f && u < 1.f && k >= 0;
-  if (bad || !valid || top == nothing || heat == 0.f) {  // alike in all CTAs
+  if (bad || !valid || top == nothing) {  // alike in all CTAs
     if (rank == 0 && tid == 0) {
       if (bad) flag(a.err, DSR_ERR_NONFINITE);
       else if (!valid) flag(a.err, DSR_ERR_ID);
-      const bool greedy = !bad && valid && top != nothing;
-      a.tokens[row] = greedy ? int32_t(0xffffffffu - uint32_t(best)) : -1;
-      a.chances[row] = greedy ? 1.f : 0.f;
+      a.tokens[row] = -1;
+      a.chances[row] = 0.f;
     }
     return;
   }
   // 2^-60 is exp(-41.6); -inf stays out also where that lies below all finite numbers
-  const Weight weight{s.table, double(top), 16.0 * kLog2eD / double(heat), fmaxf(top - 41.6f * heat, -FLT_MAX)};
+  const Weight weight{s.table, double(top), scale, fmaxf(top - 41.6f * heat, -FLT_MAX)};
 
   // Weights are formed four at a time, without branches: a 64-bit operation has tens of
   // cycles of latency.
@@ -307,6 +298,25 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       for (int j = 0; j < kFour; ++j) f(g[j], i + j);
     });
   };
+
+  if (heat == 0.f) {  // the lowest index of the maximum
+    int index = INT_MAX;
+    each([&](float f, int i) { index = f == top ? min(index, i) : index; });
+    index = __reduce_min_sync(~0u, index);
+    if (lane == 0) s.part[warp] = unsigned(index);
+    __syncthreads();
+    if (tid == 0) {
+      for (int w = 0; w < kSampleWarps; ++w) index = min(index, int(s.part[w]));
+      cluster.map_shared_rank(&s, 0)->firsts[rank] = index;
+    }
+    cluster.sync();
+    if (rank == 0 && tid == 0) {
+      for (int c = 0; c < ctas; ++c) index = min(index, s.firsts[c]);
+      a.tokens[row] = index;
+      a.chances[row] = 1.f;
+    }
+    return;
+  }
 
   // Exact sums of weights by step or digit: words of 15 bits, which hold the 2^17 entries
   // that a slice has at most.  Three 32-bit shared atomics take 7 cycles a warp, one of 64
@@ -562,7 +572,23 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   unsigned long long cut = 0;
   if (by_rank || by_mass) {
     // steps below the maximum: as far as weights count (2^-44), or the row reaches
-    const float reach = fminf(heat * 30.6f, top - low), per_step = reach > 0.f ? float(kSampleBins) / reach : 0.f;
+    float reach = heat * 30.6f;
+    if (heat > 1.5f) {  // the row may end long before: steps of such a temperature would be too wide
+      float low = CUDART_INF_F;
+      each([&](float f, int) { low = fminf(low, f > nothing ? f : low); });
+#pragma unroll
+      for (int o = 16; o; o >>= 1) low = fminf(low, __shfl_xor_sync(~0u, low, o));
+      if (lane == 0) s.bounds[warp].x = low;
+      __syncthreads();
+      if (tid < ctas) {
+        for (int w = 0; w < kSampleWarps; ++w) low = fminf(low, s.bounds[w].x);
+        cluster.map_shared_rank(&s, tid)->lows[rank] = low;
+      }
+      cluster.sync();
+      for (int c = 0; c < ctas; ++c) low = fminf(low, s.lows[c]);
+      reach = fminf(reach, top - low);
+    }
+    const float per_step = reach > 0.f ? float(kSampleBins) / reach : 0.f;
     const float step = reach / float(kSampleBins);  // inverse of per_step
     // one value only, or a temperature whose steps are no normal numbers: all in step 0
     const bool binned = per_step > 0.f && per_step < CUDART_INF_F && heat > 1e-30f;
@@ -735,8 +761,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         for (int j = 0; j < kFour; ++j) w[j] = weight(f[j]);
 #pragma unroll
         for (int j = 0; j < kFour; ++j) {
-          const bool in = f[j] > cut_at || (f[j] == cut_at && rank_of(f[j], i + j) >= cut);
-          w[j] = in ? w[j] : 0;
+          bool in = true;
+          if (cut != 0) {
+            in = f[j] > cut_at || (f[j] == cut_at && rank_of(f[j], i + j) >= cut);
+            w[j] = in ? w[j] : 0;
+          }
           z += w[j];
           const float at = place_of(f[j]);
           over += at < middle ? w[j] : 0;
@@ -819,9 +848,11 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (!__any_sync(~0u, any)) return;
 #pragma unroll
     for (int j = 0; j < kFour; ++j) w[j] = weight(f[j]);
+    if (cut != 0) {
 #pragma unroll
-    for (int j = 0; j < kFour; ++j)
-      if (f[j] < cut_at || (f[j] == cut_at && rank_of(f[j], base + v + j) < cut)) w[j] = 0;
+      for (int j = 0; j < kFour; ++j)
+        if (f[j] < cut_at || (f[j] == cut_at && rank_of(f[j], base + v + j) < cut)) w[j] = 0;
+    }
     if (least > 0.f) {
 #pragma unroll
       for (int j = 0; j < kFour; ++j)
