@@ -17,9 +17,8 @@
 //   up to 100 by rank   the histogram is that of the threads' maxima, 512 a CTA, instead
 //                       of all entries: at least k entries lie in the steps down to the
 //                       one that holds the k-th maximum, and hardly any more
-//   by rank             the counts say which step holds entry k
-//   by mass             the weights of a step are known to within its width, which says
-//                       between which two steps p lies; their exact masses say in which
+//   by rank             the counts of all entries say which step holds entry k
+//   by mass             the steps' exact masses say which one p lies in
 // Entries in question go to a list in the first CTA, which ranks them on the unique
 // 64-bit rank (order-preserving value, inverted index) with exact weights: by comparing
 // all with all where there are few, after a finer histogram where there are more.  Where
@@ -107,19 +106,16 @@ struct alignas(16) SampleSmem {
   unsigned long long list[kSampleList];  // ranks of the entries to sort
   uint32_t wide[3][kSampleBins];         // exact sums of weights (words of 15 bits) or counts, per step or digit
   uint32_t hist[kSampleBins];            // this CTA's counts
-  unsigned long long part[kSampleWarps], part2[kSampleWarps];
-  float2 bounds[kSampleWarps];
+  unsigned long long part[kSampleWarps];
+  float extremes[kSampleWarps];
   // written by every CTA of the cluster for all
-  unsigned long long counts[2][kSampleMaxCluster];  // of a scan, and of the one before
-  float2 masses[kSampleMaxCluster];
-  int2 steps[kSampleMaxCluster];
-  unsigned long long before[kSampleMaxCluster], through[kSampleMaxCluster];
-  unsigned long long sums[kSampleMaxCluster], above[kSampleMaxCluster], kept[kSampleMaxCluster];
+  ulonglong2 counts[2][kSampleMaxCluster];  // of a scan, and of the one before
+  unsigned long long kept[kSampleMaxCluster];
   float tops[kSampleMaxCluster], lows[kSampleMaxCluster];
   int firsts[kSampleMaxCluster];
   // written by one CTA for all
   unsigned long long cut, step_before;
-  int step_bin, step_in;
+  int step_bin, step_ahead, step_in;
   // this CTA's own
   unsigned long long found_before, found_through;
   int found_bin, found_last, listed;
@@ -160,6 +156,18 @@ __device__ __forceinline__ unsigned long long block_scan(SampleSmem& s, unsigned
 __device__ __forceinline__ unsigned long long warp_sum(unsigned long long v) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+  return v;
+}
+
+// The word at p's place in CTA c of the cluster.  (By instruction: the addresses of eight
+// CTAs, kept over loops by the compiler, would not leave registers for anything else.)
+__device__ __forceinline__ uint32_t cluster_word(const uint32_t* p, int c) {
+  uint32_t v;
+  asm volatile(
+      "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %1, %2;\n\tld.shared::cluster.u32 %0, [a];\n\t}"
+      : "=r"(v)
+      : "r"(smem_u32(p)), "r"(c)
+      : "memory");
   return v;
 }
 
@@ -246,12 +254,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const float other = __shfl_xor_sync(~0u, top, o);
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
   }
-  if (lane == 0) s.bounds[warp].x = top;
+  if (lane == 0) s.extremes[warp] = top;
   __syncthreads();
   cluster.barrier_wait(std::move(started));
   if (tid < ctas) {  // thread c tells CTA c
     for (int w = 0; w < kSampleWarps; ++w) {
-      const float other = s.bounds[w].x;
+      const float other = s.extremes[w];
       asm("max.NaN.f32 %0, %0, %1;" : "+f"(top) : "f"(other));
     }
     cluster.map_shared_rank(&s, tid)->tops[rank] = top;
@@ -332,58 +340,60 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
   };
   // This CTA's share of the steps: `share` of them from first_step on, thread t those from
   // first_step + t * per on (threads with t * per >= share: none).
-  static_assert(kSamplePer == 4, "a thread's piece is 16 bytes");
   const int share = kSampleBins / ctas, first_step = rank * share;
   const int per = share > kSampleThreads ? share / kSampleThreads : 1, my_step = first_step + tid * per;
   const bool mine_any = tid * per < share;
-  // Adds the cluster's sums of this thread's steps, shifted: every thread fetches 16 bytes
-  // of one CTA's words.  After a cluster barrier; `words` must not change until the next.
+  // Adds the cluster's sums of this thread's steps, shifted.  After a cluster barrier;
+  // `words` must not change until the next.
   auto gather_words = [&](const uint32_t* words, unsigned long long (&sum)[kSamplePer], int bits) {
-    const int pieces = share / 4, c = tid / pieces, q = tid % pieces;
-    uint4* stage = reinterpret_cast<uint4*>(s.list);  // 8 KB
-    __syncthreads();
-    stage[tid] = *reinterpret_cast<const uint4*>(cluster.map_shared_rank(words + first_step + 4 * q, c));
-    __syncthreads();
-    const uint32_t* staged = reinterpret_cast<const uint32_t*>(s.list);
-    if (mine_any) {
+    if (!mine_any) return;
 #pragma unroll
-      for (int j = 0; j < kSamplePer; ++j)
-        if (j < per)
-          for (int o = 0; o < ctas; ++o)
-            sum[j] += static_cast<unsigned long long>(staged[o * share + tid * per + j]) << bits;
+    for (int j = 0; j < kSamplePer; ++j) {
+      if (j >= per) break;
+      uint32_t h[kSampleMaxCluster];  // requested together
+#pragma unroll
+      for (int c = 0; c < kSampleMaxCluster; ++c)
+        h[c] = c < ctas ? cluster_word(words + my_step + j, c) : 0;
+#pragma unroll
+      for (int c = 0; c < kSampleMaxCluster; ++c) sum[j] += static_cast<unsigned long long>(h[c]) << bits;
     }
-    __syncthreads();
   };
-  // Sums of this CTA's share before this thread's steps become sums over the cluster's
-  // steps; `total`: over all.
+  // Sums over the cluster's steps before this thread's, and over all.  A cluster barrier.
+  struct Sum {
+    unsigned long long v, n;  // a measure (mass, count), entries
+  };
   int scans = 0;
-  auto cluster_scan = [&](const unsigned long long (&v)[kSamplePer], unsigned long long& total) {
-    unsigned long long sum;
-    unsigned long long at = block_scan(s, (v[0] + v[1]) + (v[2] + v[3]), sum);
+  auto cluster_scan = [&](Sum own, bool counts_alone, Sum& total) {
+    Sum sum, at;
+    at.n = block_scan(s, own.n, sum.n);
+    at.v = at.n, sum.v = sum.n;
+    if (!counts_alone) at.v = block_scan(s, own.v, sum.v);
     scans ^= 1;
-    if (tid < ctas) cluster.map_shared_rank(&s, tid)->counts[scans][rank] = sum;
+    if (tid < ctas) cluster.map_shared_rank(&s, tid)->counts[scans][rank] = make_ulonglong2(sum.v, sum.n);
     cluster.sync();
-    total = 0;
+    total = Sum{0, 0};
     for (int c = 0; c < ctas; ++c) {
-      if (c < rank) at += s.counts[scans][c];
-      total += s.counts[scans][c];
+      const ulonglong2 other = s.counts[scans][c];
+      if (c < rank) at.v += other.x, at.n += other.y;
+      total.v += other.x, total.n += other.y;
     }
     return at;
   };
-  // The step in which the sums reach target, what lies before it and in it: the thread
-  // that has it tells everybody.  A barrier of the cluster.
-  auto find_step = [&](unsigned long long at, const unsigned long long (&v)[kSamplePer], unsigned long long target,
-                       const unsigned long long (&in)[kSamplePer]) {
+  // The step in which the measure reaches target, what lies before it, the entries before
+  // it and in it: the thread that has it tells everybody.  A cluster barrier.
+  auto find_step = [&](Sum at, const unsigned long long (&v)[kSamplePer], const unsigned long long (&n)[kSamplePer],
+                       unsigned long long target) {
 #pragma unroll
     for (int j = 0; j < kSamplePer; ++j) {
-      if (at < target && at + v[j] >= target)
+      if (at.v < target && at.v + v[j] >= target)
         for (int c = 0; c < ctas; ++c) {
           SampleSmem* other = cluster.map_shared_rank(&s, c);
           other->step_bin = my_step + j;
-          other->step_before = at;
-          other->step_in = int(in[j]);
+          other->step_before = at.v;
+          other->step_ahead = int(at.n);
+          other->step_in = int(n[j]);
         }
-      at += v[j];
+      at.v += v[j], at.n += n[j];
     }
     cluster.sync();
   };
@@ -402,11 +412,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         else atomicAdd(&s.wide[0][b], 1u);
       });
       cluster.sync();
-      unsigned long long digit[kSamplePer] = {0, 0, 0, 0}, total;
+      unsigned long long digit[kSamplePer] = {0, 0, 0, 0};
       gather_words(s.wide[0], digit, 0);
       if (mass) gather_words(s.wide[1], digit, 15), gather_words(s.wide[2], digit, 30);
-      const unsigned long long at = before + cluster_scan(digit, total);
-      find_step(at, digit, target, digit);
+      const unsigned long long own = (digit[0] + digit[1]) + (digit[2] + digit[3]);
+      Sum total, at = cluster_scan(Sum{own, own}, true, total);
+      at.v += before;
+      find_step(at, digit, digit, target);
       known = (known << 11) | unsigned(kSampleBins - 1 - s.step_bin);
       before = s.step_before;
       __syncthreads();
@@ -440,8 +452,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     const unsigned long long t = (unsigned long long)(ceil(double(p) * double(mass)));
     return t < 1 ? 1ull : (t > mass ? mass : t);
   };
-  // whether a weight passes min-p (compared in steps of 2^-44)
-  auto enough = [&](float f) { return least == 0.f || weight.shifted(f) - Weight::kMagic >= double(least); };
+  // weights that pass min-p, in steps of 2^-44
+  const unsigned long long enough = (unsigned long long)ceil(double(least) * double(1ull << kWeightBits));
 
   const bool by_rank = k > 0 && k < a.vocab, by_mass = p < 1.f;
   auto draw = [&](int i, unsigned long long w, unsigned long long all) {
@@ -477,7 +489,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     unsigned long long all;
     block_scan(s, in && part == 0 ? w : 0, all);  // also: the weights have been read
     const unsigned long long target = by_mass ? mass_target(mass == 0 ? all : mass) : ~0ull;
-    const unsigned long long stays = in && above < target && enough(rank_value(r)) ? w : 0;
+    const unsigned long long stays = in && above < target && w >= enough ? w : 0;
     if (part == 0) weights[e] = stays;
     __syncthreads();
     unsigned long long before = 0;
@@ -578,10 +590,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       each([&](float f, int) { low = fminf(low, f > nothing ? f : low); });
 #pragma unroll
       for (int o = 16; o; o >>= 1) low = fminf(low, __shfl_xor_sync(~0u, low, o));
-      if (lane == 0) s.bounds[warp].x = low;
+      if (lane == 0) s.extremes[warp] = low;
       __syncthreads();
       if (tid < ctas) {
-        for (int w = 0; w < kSampleWarps; ++w) low = fminf(low, s.bounds[w].x);
+        for (int w = 0; w < kSampleWarps; ++w) low = fminf(low, s.extremes[w]);
         cluster.map_shared_rank(&s, tid)->lows[rank] = low;
       }
       cluster.sync();
@@ -589,7 +601,6 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       reach = fminf(reach, top - low);
     }
     const float per_step = reach > 0.f ? float(kSampleBins) / reach : 0.f;
-    const float step = reach / float(kSampleBins);  // inverse of per_step
     // one value only, or a temperature whose steps are no normal numbers: all in step 0
     const bool binned = per_step > 0.f && per_step < CUDART_INF_F && heat > 1e-30f;
     // where f lies among the steps; its step; whether that is at most b, or below it
@@ -601,16 +612,18 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         return int(fminf(fmaxf((place_of(f) - float(bin)) * float(kSampleBins), 0.f), float(kSampleBins - 1)));
       };
     };
-    unsigned long long count[kSamplePer] = {0, 0, 0, 0}, total;
+    unsigned long long count[kSamplePer] = {0, 0, 0, 0};
+    Sum total;
 
     if (by_rank && k <= 100) {
       // the steps of the threads' maxima
       if (most != nothing) atomicAdd(&s.hist[bin_of(most)], 1u);
       cluster.sync();
       gather_words(s.hist, count, 0);
-      const unsigned long long at = cluster_scan(count, total);
-      if (unsigned(k) <= total) {
-        find_step(at, count, unsigned(k), count);
+      const unsigned long long own = (count[0] + count[1]) + (count[2] + count[3]);
+      const Sum at = cluster_scan(Sum{own, own}, true, total);
+      if (unsigned(k) <= total.n) {
+        find_step(at, count, count, unsigned(k));
         const float bound = bound_after(s.step_bin);
         each([&](float f, int i) {
           if (place_of(f) < bound && f != nothing) keep(f, i);
@@ -626,200 +639,91 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
       for (int j = 0; j < kSamplePer; ++j) count[j] = 0;
       __syncthreads();
     }
-    // the last step holds all that is far below (a mask's low value): counted by thread
-    uint32_t tail = 0;
-    each([&](float f, int) {
-      const float at = place_of(f);
-      const bool counts = f != nothing;  // -inf is never drawn, and all that lies off the row
-      if (at >= float(kSampleBins - 1) || !binned) tail += counts;
-      else if (counts) atomicAdd(&s.hist[int(at)], 1u);
-    });
-    tail = __reduce_add_sync(~0u, tail);
-    if (lane == 0 && tail > 0) atomicAdd(&s.hist[binned ? kSampleBins - 1 : 0], tail);
-    cluster.sync();
-    gather_words(s.hist, count, 0);
-    const unsigned long long at = cluster_scan(count, total);
-
-    if (by_rank && unsigned(k) < total) {
-      find_step(at, count, unsigned(k), count);
-      const int bin = s.step_bin, before = int(s.step_before), in = s.step_in;
-      __syncthreads();
-      if (in <= kSampleList) {
-        const float from = float(bin), bound = bound_after(bin);
-        each([&](float f, int i) {
-          const float at = place_of(f);
-          if (at >= from && at < bound && f != nothing) keep(f, i);
-        });
-        cluster.sync();
-        const int n = bring();
-        if (rank == 0) rank_listed(n, false, unsigned(k - before), part_of(bin));
-        cluster.sync();
-        cut = s.cut;
-        if (tid == 0) s.listed = 0;
-        __syncthreads();
-      } else {
-        cut = descend(false, unsigned(k), 0);
-      }
-      // the counts of the prefix, for the mass below
-#pragma unroll
-      for (int j = 0; j < kSamplePer; ++j) {
-        const int b = my_step + j;
-        if (b == bin && count[j] > 0) count[j] = unsigned(k - before);  // 0: not this thread's
-        else if (b > bin) count[j] = 0;
+    if (by_rank) {
+      // the last step holds all that is far below (a mask's low value): counted by thread
+      uint32_t tail = 0;
+      each([&](float f, int) {
+        const float at = place_of(f);
+        const bool counts = f != nothing;  // -inf is never drawn, and all that lies off the row
+        if (at >= float(kSampleBins - 1) || !binned) tail += counts;
+        else if (counts) atomicAdd(&s.hist[int(at)], 1u);
+      });
+      tail = __reduce_add_sync(~0u, tail);
+      if (lane == 0 && tail > 0) atomicAdd(&s.hist[binned ? kSampleBins - 1 : 0], tail);
+      cluster.sync();
+      gather_words(s.hist, count, 0);
+      const unsigned long long own = (count[0] + count[1]) + (count[2] + count[3]);
+      const Sum at = cluster_scan(Sum{own, own}, true, total);
+      if (unsigned(k) < total.n) {
+        find_step(at, count, count, unsigned(k));
+        const int bin = s.step_bin, before = s.step_ahead, in = s.step_in;
+        if (in <= kSampleList) {
+          const float from = float(bin), bound = bound_after(bin);
+          each([&](float f, int i) {
+            const float at = place_of(f);
+            if (at >= from && at < bound && f != nothing) keep(f, i);
+          });
+          cluster.sync();
+          const int n = bring();
+          if (rank == 0) rank_listed(n, false, unsigned(k - before), part_of(bin));
+          cluster.sync();
+          cut = s.cut;
+        } else {
+          cut = descend(false, unsigned(k), 0);
+        }
       }
     }
     if (by_mass) {
-      // bounds of the mass up to and including each step, from its counts
-      const float fall = step / heat;
-      float lo[kSamplePer], hi[kSamplePer], lo_own = 0.f, hi_own = 0.f;
-#pragma unroll
-      for (int j = 0; j < kSamplePer; ++j) {
-        const int b = my_step + j;
-        // a hundredth of a step covers the rounding of the step's number
-        if (count[j] > 0) {
-          hi_own += float(count[j]) * expf(-fmaxf(float(b) - 0.01f, 0.f) * fall) * 1.0001f;
-          if (b < kSampleBins - 1) lo_own += float(count[j]) * expf(-(float(b) + 1.01f) * fall) * 0.9999f;
-        }
-        lo[j] = lo_own, hi[j] = hi_own;
-      }
-      float lo_run = lo_own, hi_run = hi_own;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const float l = __shfl_up_sync(~0u, lo_run, d), h = __shfl_up_sync(~0u, hi_run, d);
-        if (lane >= d) lo_run += l, hi_run += h;
-      }
-      if (lane == 31) s.bounds[warp] = make_float2(lo_run, hi_run);
+      // the exact masses of the steps' entries in the prefix, and their number
       __syncthreads();
-      float lo_at = lo_run - lo_own, hi_at = hi_run - hi_own, lo_all = 0.f, hi_all = 0.f;
-#pragma unroll
-      for (int w = 0; w < kSampleWarps; ++w) {
-        const float2 v = s.bounds[w];
-        if (w < warp) lo_at += v.x, hi_at += v.y;
-        lo_all += v.x, hi_all += v.y;
-      }
-      if (tid < ctas) cluster.map_shared_rank(&s, tid)->masses[rank] = make_float2(lo_all, hi_all);
-      unsigned long long upto = cluster_scan(count, total);  // its barrier covers the masses
-      lo_all = hi_all = 0.f;
-      for (int c = 0; c < ctas; ++c) {
-        const float2 v = s.masses[c];
-        if (c < rank) lo_at += v.x, hi_at += v.y;
-        lo_all += v.x, hi_all += v.y;
-      }
-      // the cut lies past every step whose upper bound is below p times the total's
-      // lower one, and no later than the first whose lower bound reaches p times the
-      // total's upper one (the sums' own rounding: below 10^-4)
-      const float below = p * lo_all * 0.999f, reached = p * hi_all * 1.001f;
-      if (tid == 0) s.found_bin = s.found_last = kSampleBins, s.found_before = s.found_through = total;
-      __syncthreads();
-      if (mine_any) {
-        int first_bin = kSampleBins, last_bin = kSampleBins;
-#pragma unroll
-        for (int j = kSamplePer - 1; j >= 0; --j) {
-          if (j < per && hi_at + hi[j] >= below) first_bin = my_step + j;
-          if (j < per && lo_at + lo[j] >= reached) last_bin = my_step + j;
-        }
-        if (first_bin < kSampleBins) atomicMin(&s.found_bin, first_bin);
-        if (last_bin < kSampleBins) atomicMin(&s.found_last, last_bin);
-      }
-      __syncthreads();
-      if (mine_any) {
-#pragma unroll
-        for (int j = 0; j < kSamplePer; ++j)
-          if (j < per) {
-            if (my_step + j == s.found_bin) s.found_before = upto;
-            upto += count[j];
-            if (my_step + j == s.found_last) s.found_through = upto;
-          }
-      }
-      __syncthreads();
-      if (tid < ctas) {
-        SampleSmem* other = cluster.map_shared_rank(&s, tid);
-        other->steps[rank] = make_int2(s.found_bin, s.found_last);
-        other->before[rank] = s.found_before;
-        other->through[rank] = s.found_through;
-      }
-      cluster.sync();
-      // the first step of each kind that a CTA has found; without one, or without steps, all
-      int from = 0, to = kSampleBins - 1;
-      unsigned long long before = 0, through = total;
-      if (binned) {
-        for (int c = ctas - 1; c >= 0; --c) {
-          if (s.steps[c].x < kSampleBins) from = s.steps[c].x, before = s.before[c];
-          if (s.steps[c].y < kSampleBins) to = s.steps[c].y, through = s.through[c];
-        }
-      }
-      const bool whole = cut == 0 && through <= kSampleFew, some = whole || through - before <= kSampleList;
-      const float begin = whole ? 0.f : float(from), middle = float(from), bound = bound_after(to);
-      // one pass: the exact mass of the prefix and of its part before step `from`, and the
-      // entries of the steps between, where they fit the list, else the steps' exact masses
-      if (!some) clear_wide();
-      unsigned long long z = 0, over = 0;
+      if (tid == 0) s.listed = 0;
+      for (int b = tid; b < kSampleBins; b += kSampleThreads) s.hist[b] = 0;
+      clear_wide();
       const float cut_at = cut == 0 ? nothing : rank_value(cut);
       each_four([&](const float (&f)[kFour], int i) {
+        if (cut != 0) {
+          bool any = false;
+#pragma unroll
+          for (int j = 0; j < kFour; ++j) any |= f[j] >= cut_at;
+          if (!any) return;
+        }
         unsigned long long w[kFour];
 #pragma unroll
         for (int j = 0; j < kFour; ++j) w[j] = weight(f[j]);
 #pragma unroll
         for (int j = 0; j < kFour; ++j) {
-          bool in = true;
-          if (cut != 0) {
-            in = f[j] > cut_at || (f[j] == cut_at && rank_of(f[j], i + j) >= cut);
-            w[j] = in ? w[j] : 0;
-          }
-          z += w[j];
-          const float at = place_of(f[j]);
-          over += at < middle ? w[j] : 0;
-          if (in && at >= begin && at < bound && f[j] != nothing) {
-            if (some) keep(f[j], i + j);
-            else add_wide(bin_of(f[j]), w[j]);
-          }
+          if (w[j] == 0 || (cut != 0 && (f[j] < cut_at || rank_of(f[j], i + j) < cut))) continue;
+          const int b = bin_of(f[j]);
+          atomicAdd(&s.hist[b], 1u);
+          add_wide(b, w[j]);
         }
       });
-      z = warp_sum(z), over = warp_sum(over);
-      if (lane == 0) s.part[warp] = z, s.part2[warp] = over;
-      __syncthreads();
-      if (tid < ctas) {
-        z = over = 0;
-        for (int w = 0; w < kSampleWarps; ++w) z += s.part[w], over += s.part2[w];
-        SampleSmem* other = cluster.map_shared_rank(&s, tid);
-        other->sums[rank] = z;
-        other->above[rank] = over;
-      }
       cluster.sync();
-      z = over = 0;
-      for (int c = 0; c < ctas; ++c) z += s.sums[c], over += s.above[c];
-      if (whole && finish_alone(kSampleFew, z)) return;
-      const unsigned long long target = mass_target(z);
-      // the step that the target lies in, and its entries
-      bool fits = some;
-      int bin = from;
-      auto parts = [&](float f) {  // of the listed entries' steps
-        return fits && some ? int(fminf(fmaxf((place_of(f) - float(from)) / float(to - from + 1) * float(kSampleBins), 0.f),
-                                        float(kSampleBins - 1)))
-                            : part_of(bin)(f);
-      };
-      if (!some) {
-        unsigned long long mass[kSamplePer] = {0, 0, 0, 0};
-        gather_words(s.wide[0], mass, 0);
-        gather_words(s.wide[1], mass, 15);
-        gather_words(s.wide[2], mass, 30);
-        const unsigned long long run = over + cluster_scan(mass, total);
-        find_step(run, mass, target, count);
-        bin = s.step_bin;
-        fits = s.step_in <= kSampleList;
-        over = s.step_before;
-        if (fits) {
-          const float low_end = float(bin), high_end = bound_after(bin);
-          each([&](float f, int i) {
-            const float at = place_of(f);
-            if (at >= low_end && at < high_end && f != nothing && rank_of(f, i) >= cut) keep(f, i);
-          });
-        }
+      unsigned long long mass[kSamplePer] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < kSamplePer; ++j) count[j] = 0;
+      gather_words(s.hist, count, 0);
+      gather_words(s.wide[0], mass, 0);
+      gather_words(s.wide[1], mass, 15);
+      gather_words(s.wide[2], mass, 30);
+      const Sum at = cluster_scan(Sum{(mass[0] + mass[1]) + (mass[2] + mass[3]), (count[0] + count[1]) + (count[2] + count[3])},
+                                  false, total);
+      const unsigned long long target = mass_target(total.v);
+      // the step that the target lies in, and its entries (with all above them, if they are few)
+      find_step(at, mass, count, target);
+      const int bin = s.step_bin, ahead = s.step_ahead, in = s.step_in;
+      const unsigned long long over = s.step_before;
+      const bool whole = cut == 0 && ahead + in <= kSampleFew;
+      if (in <= kSampleList) {
+        const float from = whole ? 0.f : float(bin), bound = bound_after(bin);
+        each([&](float f, int i) {
+          const float at = place_of(f);
+          if (at >= from && at < bound && f >= weight.floor && (cut == 0 || rank_of(f, i) >= cut)) keep(f, i);
+        });
         cluster.sync();
-      }
-      if (fits) {
+        if (whole && finish_alone(kSampleFew, total.v)) return;
         const int n = bring();
-        if (rank == 0) rank_listed(n, true, target - over, parts);
+        if (rank == 0) rank_listed(n, true, target - over, part_of(bin));
         cluster.sync();
         cut = s.cut;
       } else {
@@ -830,8 +734,12 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
 
   // ---- the kept weights, warp by warp in vocabulary order, four consecutive places a lane
   const float cut_at = cut == 0 ? nothing : rank_value(cut);
-  auto kept = [&](int v, unsigned long long (&w)[kFour]) {  // of places first + v ..
-    float f[kFour] = {nothing, nothing, nothing, nothing};
+  // below it no weight passes min-p (the margin covers the rounding of all three terms)
+  const float lowest =
+      least > 0.f ? fmaxf(weight.floor, top + heat * logf(least) - 1e-6f * (fabsf(top) + heat * 120.f)) : weight.floor;
+  auto values = [&](int v, float (&f)[kFour]) {  // of places first + v ..
+#pragma unroll
+    for (int j = 0; j < kFour; ++j) f[j] = nothing;
     if (v < a.slice) {  // a multiple of four
       if constexpr (W) {
         const float4 g = *reinterpret_cast<const float4*>(held + v);
@@ -842,9 +750,13 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         f[2] = __uint_as_float(g.y << 16), f[3] = __uint_as_float(g.y & 0xffff0000u);
       }
     }
+  };
+  auto kept = [&](int v, unsigned long long (&w)[kFour]) {
+    float f[kFour];
+    values(v, f);
     bool any = false;
 #pragma unroll
-    for (int j = 0; j < kFour; ++j) any |= f[j] >= cut_at && f[j] >= weight.floor, w[j] = 0;
+    for (int j = 0; j < kFour; ++j) any |= f[j] >= cut_at && f[j] >= lowest, w[j] = 0;
     if (!__any_sync(~0u, any)) return;
 #pragma unroll
     for (int j = 0; j < kFour; ++j) w[j] = weight(f[j]);
@@ -856,16 +768,59 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     if (least > 0.f) {
 #pragma unroll
       for (int j = 0; j < kFour; ++j)
-        if (!enough(f[j])) w[j] = 0;
+        if (w[j] < enough) w[j] = 0;
     }
   };
   constexpr int kTurn = 32 * kFour;  // places of a warp at a time
   const int seg = ((a.slice + kSampleWarps - 1) / kSampleWarps + kTurn - 1) / kTurn * kTurn, start = warp * seg;
   unsigned long long own = 0, all = 0;
-  for (int v = start + lane * kFour; v < start + seg; v += kTurn) {
-    unsigned long long w[kFour];
-    kept(v, w);
-    own += (w[0] + w[1]) + (w[2] + w[3]);
+  if (cut == 0 && least == 0.f) {
+    for (int v = start + lane * kFour; v < start + seg; v += kTurn) {
+      unsigned long long w[kFour];
+      kept(v, w);
+      own += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+  } else {
+    // the kept values side by side first, so that weights are formed of them alone
+    constexpr int kRoom = kSampleList * 8 / 4 / kSampleWarps / 4 * 4;  // 248 of a warp
+    static_assert(kRoom >= kTurn - 8 + 64, "two rows of 32 fit behind what is not formed yet");
+    float* side = reinterpret_cast<float*>(s.list) + warp * kRoom;
+    int n = 0;
+    auto form = [&](int m) {  // the first m <= kTurn
+#pragma unroll
+      for (int j = 0; j < kFour; ++j) {
+        const float f = j * 32 + lane < m ? side[j * 32 + lane] : nothing;
+        const unsigned long long w = weight(f);
+        own += w >= enough ? w : 0;
+      }
+    };
+    __syncthreads();
+    for (int v = start + lane * kFour; v - lane * kFour < start + seg; v += kTurn) {
+      float f[kFour];
+      values(v, f);
+#pragma unroll
+      for (int j = 0; j < kFour; ++j) {
+        const bool stays = f[j] >= lowest && f[j] >= cut_at &&
+                           (f[j] > cut_at || rank_of(f[j], base + v + j) >= cut);
+        const unsigned who = __ballot_sync(~0u, stays);
+        if (stays) side[n + __popc(who & ((1u << lane) - 1))] = f[j];
+        n += __popc(who);
+        if (j % 2 == 1 && n >= kTurn - 8) {  // at most 64 more come before the next look
+          __syncwarp();
+          form(min(n, kTurn));
+          __syncwarp();
+          const int rest = n - min(n, kTurn);
+          const float moved = lane < rest ? side[kTurn + lane] : 0.f, moved2 = lane + 32 < rest ? side[kTurn + 32 + lane] : 0.f;
+          __syncwarp();
+          if (lane < rest) side[lane] = moved;
+          if (lane + 32 < rest) side[32 + lane] = moved2;
+          n = rest;
+          __syncwarp();
+        }
+      }
+    }
+    __syncwarp();
+    form(n);
   }
   own = warp_sum(own);
   __syncthreads();
