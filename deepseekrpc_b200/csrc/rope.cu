@@ -53,7 +53,7 @@ __device__ __forceinline__ float2 rotate(float a, float b, float2 cs) {
 // 16 bytes as floats (4 fp32 or 8 bf16) and back
 template <bool W>
 __device__ __forceinline__ void unpack(const uint4& v, float* f) {
-  if (W) {
+  if constexpr (W) {
     f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y), f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
   } else {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -63,13 +63,16 @@ __device__ __forceinline__ void unpack(const uint4& v, float* f) {
 }
 template <bool W>
 __device__ __forceinline__ uint4 pack(const float* f) {
-  if (W) return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
-  uint32_t w[4];
+  if constexpr (W) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  } else {
+    uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __bfloat16_as_ushort(__float2bfloat16_rn(f[2 * i])) |
-           (uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * i + 1]))) << 16);
-  return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int i = 0; i < 4; ++i)
+      w[i] = __bfloat16_as_ushort(__float2bfloat16_rn(f[2 * i])) |
+             (uint32_t(__bfloat16_as_ushort(__float2bfloat16_rn(f[2 * i + 1]))) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
 }
 
 // Item k of one head: rotated items first, then copied ones.

@@ -521,9 +521,18 @@ std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens,
   TORCH_CHECK(tokens >= 0 && tokens < (int64_t(1) << 31), "paged_plan: invalid token count");
   const c10::cuda::CUDAGuard guard(lengths.device());
   auto error = status_or(status, lengths);
-  auto seq = fresh({tokens}, at::kInt, lengths), positions = fresh({tokens}, at::kInt, lengths);
-  auto slots = fresh({tokens}, at::kInt, lengths), cu = fresh({batch + 1}, at::kInt, lengths);
-  auto visible = fresh({batch}, at::kInt, lengths);
+  // one allocation for the five outputs, each from a 16-byte boundary
+  const auto rounded = [](int64_t n) { return (n + 3) / 4 * 4; };
+  const at::Tensor store = fresh({3 * rounded(tokens) + rounded(batch + 1) + rounded(batch)}, at::kInt, lengths);
+  int64_t used = 0;
+  const auto part = [&](int64_t n) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(store.storage()), store.key_set(), store.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(used);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    used += rounded(n);
+    return t;
+  };
+  auto seq = part(tokens), positions = part(tokens), slots = part(tokens), cu = part(batch + 1), visible = part(batch);
   ok(dsr_paged_plan(lengths.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
                     block_table.data_ptr<int32_t>(), block_table.size(1), free_ring.data_ptr<int32_t>(),
                     ring_state.data_ptr<int32_t>(), free_ring.size(0), seq.data_ptr<int32_t>(),
