@@ -156,42 +156,92 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
 
   const int64_t step = int64_t(gridDim.x) * kPlanThreads, first = int64_t(blockIdx.x) * kPlanThreads + tid;
   auto ring_at = [&](int64_t i) { return int64_t(i < a.blocks ? i : i - a.blocks); };
-  // ---- the map of the new tokens
+  // ---- the map of the new tokens, four consecutive ones a thread
   const int64_t mapped = ok ? all.tokens : 0;
-  for (int64_t i = first; i < a.tokens; i += step) {
-    int32_t s = -1, p = -1, slot = -1;
-    if (i < mapped) {
-      s = plan_owner(cu_tokens, a.batch, int32_t(i));
-      p = a.lengths[s] + int32_t(i) - cu_tokens[s];
-      const int32_t j = p >> kBlockShift, have = a.held[s];
-      const int32_t blk = j < have ? a.table[int64_t(s) * a.stride + j]
-                                   : a.ring[ring_at(head + cu_take[s] + (j - have))];
-      if (blk >= 0 && blk < a.blocks) slot = blk * DSR_BLOCK_TOKENS + (p & (DSR_BLOCK_TOKENS - 1));
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.seq) | reinterpret_cast<uintptr_t>(a.positions) |
+                     reinterpret_cast<uintptr_t>(a.slots)) & 15u) == 0;
+  for (int64_t i0 = first * 4; i0 < a.tokens; i0 += step * 4) {
+    int32_t seq[4], pos[4], slot[4];
+    int32_t s = i0 < mapped ? plan_owner(cu_tokens, a.batch, int32_t(i0)) : 0;
+    int32_t len = 0, have = 0, start = 0, next = 0, last_j = -1, blk = -1;
+    bool fetch = true;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t i = i0 + q;
+      seq[q] = pos[q] = slot[q] = -1;
+      if (i >= mapped) continue;
+      if (!fetch && i >= next) {
+        do ++s;
+        while (cu_tokens[s + 1] <= i);
+        fetch = true;
+      }
+      if (fetch) {
+        len = a.lengths[s], have = a.held[s], start = cu_tokens[s], next = cu_tokens[s + 1];
+        last_j = -1;
+        fetch = false;
+      }
+      const int32_t p = len + int32_t(i) - start, j = p >> kBlockShift;
+      if (j != last_j) {
+        blk = j < have ? a.table[int64_t(s) * a.stride + j] : a.ring[ring_at(head + cu_take[s] + (j - have))];
+        last_j = j;
+      }
+      seq[q] = s;
+      pos[q] = p;
+      if (blk >= 0 && blk < a.blocks) slot[q] = blk * DSR_BLOCK_TOKENS + (p & (DSR_BLOCK_TOKENS - 1));
       else flag(a.err, DSR_ERR_ID);
     }
-    a.seq[i] = s;
-    a.positions[i] = p;
-    a.slots[i] = slot;
+    if (vec && i0 + 4 <= a.tokens) {
+      *reinterpret_cast<int4*>(a.seq + i0) = make_int4(seq[0], seq[1], seq[2], seq[3]);
+      *reinterpret_cast<int4*>(a.positions + i0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(a.slots + i0) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (i0 + q < a.tokens) a.seq[i0 + q] = seq[q], a.positions[i0 + q] = pos[q], a.slots[i0 + q] = slot[q];
+    }
   }
   if (ok) {
-    // ---- blocks taken from the ring's head
-    for (int64_t i = first; i < all.take; i += step) {
-      const int b = plan_owner(cu_take, a.batch, int32_t(i));
-      int32_t blk = a.ring[ring_at(head + i)];
-      if (blk < 0 || blk >= a.blocks) {
-        flag(a.err, DSR_ERR_ID);
-        blk = -1;
+    // ---- blocks moved, four of a thread at a time: their chains of reads run side by side
+    constexpr int kMoves = 4;
+    // taken from the ring's head
+    for (int64_t i0 = first; i0 < all.take; i0 += step * kMoves) {
+      int32_t blk[kMoves], *entry[kMoves];
+#pragma unroll
+      for (int q = 0; q < kMoves; ++q) {
+        const int64_t i = i0 + q * step;
+        entry[q] = nullptr;
+        if (i >= all.take) continue;
+        blk[q] = a.ring[ring_at(head + i)];
+        const int b = plan_owner(cu_take, a.batch, int32_t(i));
+        entry[q] = a.table + int64_t(b) * a.stride + a.held[b] + (int32_t(i) - cu_take[b]);
       }
-      a.table[int64_t(b) * a.stride + a.held[b] + (int32_t(i) - cu_take[b])] = blk;
+#pragma unroll
+      for (int q = 0; q < kMoves; ++q) {
+        if (entry[q] == nullptr) continue;
+        const bool good = blk[q] >= 0 && blk[q] < a.blocks;
+        if (!good) flag(a.err, DSR_ERR_ID);
+        *entry[q] = good ? blk[q] : -1;
+      }
     }
-    // ---- blocks given back behind its tail
-    for (int64_t i = first; i < all.give; i += step) {
-      const int b = plan_owner(cu_give, a.batch, int32_t(i));
-      int32_t len, fresh, have, need;
-      plan_request(a, b, len, fresh, have, need);
-      int32_t* entry = a.table + int64_t(b) * a.stride + need + (int32_t(i) - cu_give[b]);
-      a.ring[ring_at(ring_at(head + count) + i)] = *entry;
-      *entry = -1;
+    // given back behind its tail
+    for (int64_t i0 = first; i0 < all.give; i0 += step * kMoves) {
+      int32_t blk[kMoves], *entry[kMoves];
+#pragma unroll
+      for (int q = 0; q < kMoves; ++q) {
+        const int64_t i = i0 + q * step;
+        entry[q] = nullptr;
+        if (i >= all.give) continue;
+        const int b = plan_owner(cu_give, a.batch, int32_t(i));
+        const int32_t need = (a.lengths[b] + a.new_tokens[b] + DSR_BLOCK_TOKENS - 1) >> kBlockShift;
+        entry[q] = a.table + int64_t(b) * a.stride + need + (int32_t(i) - cu_give[b]);
+        blk[q] = *entry[q];
+      }
+#pragma unroll
+      for (int q = 0; q < kMoves; ++q) {
+        if (entry[q] == nullptr) continue;
+        a.ring[ring_at(ring_at(head + count) + i0 + q * step)] = blk[q];
+        *entry[q] = -1;
+      }
     }
   }
   // ---- the last CTA to get here writes what every CTA has read
@@ -244,10 +294,11 @@ extern "C" int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens,
   if (set != DSR_OK) return set;
   const PlanArgs a{lengths, new_tokens, held,  block_table, table_stride, free_ring, ring_state,  pool_blocks, seq,
                    positions, slots,    cu_tokens, visible, err,          tokens,    int(batch)};
-  // a CTA for every kPlanThreads x 4 tokens, or requests' block moves (unknown here:
-  // at most two per request are usual), up to one per SM
-  const int64_t work = tokens > 2 * batch ? tokens : 2 * batch;
-  int64_t grid = (work + kPlanThreads * 4 - 1) / (kPlanThreads * 4);
+  // a CTA for every four tokens a thread, and for the moves of blocks, whose number is not
+  // known here, one for every 32 table entries a thread; up to one per SM
+  const int64_t by_tokens = (tokens + kPlanThreads * 4 - 1) / (kPlanThreads * 4);
+  const int64_t by_table = (batch * table_stride + kPlanThreads * 32 - 1) / (kPlanThreads * 32);
+  int64_t grid = by_tokens > by_table ? by_tokens : by_table;
   if (grid > sm_count()) grid = sm_count();
   plan_kernel<<<unsigned(grid), kPlanThreads, smem, as_stream(stream)>>>(a);
   return launch_status("paged_plan launch");
