@@ -15,20 +15,22 @@
 //
 // A job is one group over a segment of consecutive tiles.  Every CTA finds the same
 // segment length (tree_plan) from the lengths on the device; a request's tiles are
-// cut into equal segments, and job j, in the order (request, segment, group), goes to
-// CTA j modulo the grid: the groups of a segment then run side by side and share its
-// rows in L2.  (Runs of units in the order request, group, tile balance better, but
+// cut into equal segments, and the jobs, in the order (request, segment, group), the
+// longest requests' segments first, are dealt to the CTAs to and fro: the groups of a
+// segment run side by side and share its rows in L2, and a CTA with a long job gets a
+// short one next (for 32 ragged requests the busiest CTA has 4 to 6% more than its
+// share in two rounds; dealt in the order of requests it had 14% in four).  (Runs of units in the order request, group, tile balance better, but
 // read the rows once per group: 1213 us against 1010 us for 32 requests of 3 to 6
 // groups.)  A group of several segments leaves partials (m, l, unnormalised O in
 // FP32) that tree_combine_kernel joins.
 //
-//   warps 0..7  query -> shared memory, softmax over the tile's keys (running
+//   warps 0..7  (FP32 query -> shared memory,) softmax over the tile's keys (running
 //               maximum; O is rescaled only when a maximum grows by more than 2^8),
 //               output.  Warps 0..3 have the first half of the group's rows, warps
 //               4..7 the second; warp w and w + 4 hold the tensor memory's lanes
 //               (keys, value columns) 32 w and up
 //   warp 8      TMEM and the MMAs
-//   warp 9      key tiles by TMA: column blocks 0..7 (the value columns) through a
+//   warp 9      query and key tiles by TMA: column blocks 0..7 (the value columns) through a
 //               ring of block pairs that the O MMA frees pair by pair, block 8 (the
 //               rotary columns) in a buffer that P^T takes over once S^T is done
 #include <math_constants.h>
@@ -117,8 +119,8 @@ __device__ __forceinline__ int32_t tree_segments(const TreeSeq& s, int32_t lengt
 // ---- the jobs of a call
 constexpr int kTreeSearchBatch = 2048;  // larger batches take the even share (the search reads every request)
 constexpr int kTreeSlotsPerCta = 4;  // partial slots, per CTA of the grid
-// A job's cost beside its tiles, in tiles: query load, first copies, output.
-constexpr float kTreeJobCost = 2.f;
+// A round's cost beside its tiles, in tiles: first copies, output, its part of the join.
+constexpr float kTreeJobCost = 8.f;
 
 // A segment length for `waves` jobs per CTA at most: starts at the even share and
 // grows until the jobs (requests' tiles rounded up to whole segments) and the partial
@@ -142,9 +144,9 @@ __device__ __forceinline__ float tree_length(const TreeArgs& a, int64_t units, i
       slots += __shfl_xor_sync(~0u, slots, o);
     }
     if (jobs <= room && slots <= int64_t(kTreeSlotsPerCta) * a.ctas) {
-      // full waves of equal jobs, or list scheduling's mean plus half a job
+      // one round lasts as long as its longest job; several come near the mean
       const float mean = float(units) / float(a.ctas);
-      return fminf(float(waves) * len, mean + 0.5f * len) + float(waves) * kTreeJobCost;
+      return (waves == 1 ? len : fminf(float(waves) * len, mean + 0.1f * len)) + float(waves) * kTreeJobCost;
     }
     len += fmaxf(floorf(len * (1.f - float(room) / float(jobs))), 1.f);
   }
@@ -156,11 +158,12 @@ template <int N>
 struct TreeWalk {
   const TreeArgs& a;
   const int32_t *chunk_jobs, *chunk_slots;  // [kTreeThreads] before each chunk of `per` requests
-  int32_t length, jobs, job;
+  int32_t length, jobs;
+  int round;
   int per;
   // up to 32 requests: lane b keeps request b, and the jobs and slots before it
   TreeSeq own;
-  int32_t own_jobs, own_slots;
+  int32_t own_jobs, own_count, own_slots;
   int b, group, tile0, count, slot;  // slot < 0: the group's only segment
   TreeSeq s;
   __device__ __forceinline__ void at_job(int32_t at, int32_t segments, int32_t slots) {
@@ -170,12 +173,14 @@ struct TreeWalk {
     tile0 = segment * whole + min(segment, longer);
     count = whole + (segment < longer);
     slot = segments > 1 ? slots + at : -1;
-    job += gridDim.x;
   }
   __device__ __forceinline__ bool next() {
+    // to and fro: odd rounds from the last CTA to the first
+    const int32_t job = round * int(gridDim.x) + (round & 1 ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
     if (job >= jobs) return false;
+    ++round;
     if (a.batch <= 32) {
-      b = 31 - __clz(__ballot_sync(~0u, own_jobs <= job));  // the last request that starts at or before the job
+      b = __ffs(__ballot_sync(~0u, job >= own_jobs && job - own_jobs < own_count)) - 1;
       s.node0 = __shfl_sync(~0u, own.node0, b);
       s.nodes = __shfl_sync(~0u, own.nodes, b);
       s.context = __shfl_sync(~0u, own.context, b);
@@ -366,7 +371,8 @@ __device__ __forceinline__ bool tree_store(const TreeArgs& a, int64_t row, int r
 
 template <int N>
 __global__ void __launch_bounds__(kTreeThreads, 1)
-    tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ TreeArgs a) {
+    tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
+                    const __grid_constant__ TreeArgs a) {
   using L = TreeLayout<N>;
   constexpr int kHalf = N / 2, C = kHalf / 8;  // rows of a half of the softmax warps, in chunks of 8
   constexpr int W = kHalf < 16 ? kHalf : 16;   // rows taken from O^T at a time
@@ -380,7 +386,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   uint64_t* bar_s = bar_r + 1;              // S^T complete (commit)
   uint64_t* bar_p = bar_r + 2;              // P^T written (kTreeSoftmax arrivals)
   uint64_t* bar_o = bar_r + 3;              // the tile's O MMAs complete (commit)
-  uint64_t* bar_q = bar_r + 4;              // query in place (kTreeSoftmax arrivals)
+  uint64_t* bar_q = bar_r + 4;              // query in place (TMA bytes + 1; FP32: kTreeSoftmax arrivals)
   uint64_t* bar_free = bar_r + 5;           // O^T read by the epilogue (kTreeSoftmax arrivals)
   uint64_t* masks = reinterpret_cast<uint64_t*>(smem + L::kMaskOff);
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
@@ -389,6 +395,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
   int* loaded = reinterpret_cast<int*>(smem + L::kMiscOff + 8);     // block pairs requested, for an abort
   int* loaded_r = reinterpret_cast<int*>(smem + L::kMiscOff + 12);  // rotary blocks
+  int* loaded_q = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // queries
   int32_t* chunk_jobs = reinterpret_cast<int32_t*>(smem + L::kChunkOff);
   int32_t* chunk_slots = chunk_jobs + kTreeThreads;
   // before the ring is used: [10] sums of the warps (units, groups), [4] estimates and lengths
@@ -400,15 +407,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 
   if (tid == 0) {
     tma_prefetch_desc(&kv_map);
+    if (!a.q_wide) tma_prefetch_desc(&q_map);
     for (int i = 0; i < L::kPairs; ++i) mbar_init(full + i, 1), mbar_init(empty + i, 1);
     mbar_init(bar_r, 1);
     mbar_init(bar_s, 1);
     mbar_init(bar_p, kTreeSoftmax);
     mbar_init(bar_o, 1);
-    mbar_init(bar_q, kTreeSoftmax);
+    mbar_init(bar_q, a.q_wide ? kTreeSoftmax : 1);
     mbar_init(bar_free, kTreeSoftmax);
     *abort = 0;
-    *loaded = *loaded_r = 0;
+    *loaded = *loaded_r = *loaded_q = 0;
     fence_barrier_init();
   }
   if (warp == 8) {
@@ -417,7 +425,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   }
 
   // ---- the work of all requests
-  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, 1, 0, int32_t(blockIdx.x), 1, TreeSeq{}, 0, 0};
+  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, 1, 0, 0, 1, TreeSeq{}, 0, 0, 0};
   const bool small = a.batch <= 32;
   const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;  // else: requests of a thread's chunk
   const int r0 = small ? lane : min(tid * per, a.batch), r1 = small ? min(lane + 1, a.batch) : min(r0 + per, a.batch);
@@ -467,19 +475,26 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     jobs += n;
     if (s.tiles > length) slots += n;
   }
-  int32_t jobs_upto = jobs, slots_upto = slots;
-#pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
-    if (lane >= d) jobs_upto += u, slots_upto += v;
-  }
   walk.length = length;
-  walk.own_jobs = jobs_upto - jobs;
-  walk.own_slots = slots_upto - slots;
   if (small) {
-    walk.jobs = __shfl_sync(~0u, jobs_upto, 31);
-    if (lane >= a.batch) walk.own_jobs = INT32_MAX;
+    // those of the requests with longer segments come first
+    const float mine = jobs > 0 ? float(walk.own.tiles) / float(tree_segments(walk.own, length)) : 0.f;
+    walk.own_count = jobs;
+    for (int b = 0; b < a.batch; ++b) {
+      const float other = __shfl_sync(~0u, mine, b);
+      const int32_t n = __shfl_sync(~0u, jobs, b), m = __shfl_sync(~0u, slots, b);
+      if (other > mine || (other == mine && b < lane)) walk.own_jobs += n, walk.own_slots += m;
+      walk.jobs += n;
+    }
   } else {
+    int32_t jobs_upto = jobs, slots_upto = slots;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
+      if (lane >= d) jobs_upto += u, slots_upto += v;
+    }
+    walk.own_jobs = jobs_upto - jobs;
+    walk.own_slots = slots_upto - slots;
     __syncthreads();  // the sums above have been read
     if (lane == 31) warp_units[warp] = jobs_upto, warp_groups[warp] = slots_upto;
     __syncthreads();
@@ -515,35 +530,34 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const TreeSeq s = walk.s;
       const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
       const int64_t qrow = int64_t(s.node0) * a.heads + row0;
-      // ---- query rows -> bf16, K-major, 128-byte swizzle
-      constexpr int kVec = N * (kTreeD / 8), kBatch = kVec / kTreeSoftmax < 9 ? 5 : 9;
-      for (int i0 = tid; i0 < kVec; i0 += kTreeSoftmax * kBatch) {
-        uint4 v[kBatch];
+      if (a.q_wide) {
+        // ---- FP32 query rows -> bf16, K-major, 128-byte swizzle (BF16 ones come by TMA)
+        constexpr int kVec = N * (kTreeD / 8), kBatch = 3;
+        for (int i0 = tid; i0 < kVec; i0 += kTreeSoftmax * kBatch) {
+          uint4 v[kBatch];
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8);
-          v[j] = make_uint4(0, 0, 0, 0);
-          if (i < kVec && r < rows) {
-            const int64_t at = (qrow + r) * kTreeD + (i - r * (kTreeD / 8)) * 8;
-            if (a.q_wide) {
-              const float4 lo = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at));
-              const float4 hi = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(a.q) + at) + 1);
+          for (int j = 0; j < kBatch; ++j) {
+            const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8);
+            v[j] = make_uint4(0, 0, 0, 0);
+            if (i < kVec && r < rows) {
+              const float4* src = reinterpret_cast<const float4*>(
+                  static_cast<const float*>(a.q) + (qrow + r) * kTreeD + (i - r * (kTreeD / 8)) * 8);
+              const float4 lo = __ldg(src), hi = __ldg(src + 1);
               v[j] = make_uint4(bf16x2(lo.x, lo.y), bf16x2(lo.z, lo.w), bf16x2(hi.x, hi.y), bf16x2(hi.z, hi.w));
-            } else {
-              v[j] = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + at));
             }
           }
-        }
 #pragma unroll
-        for (int j = 0; j < kBatch; ++j) {
-          const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8), d = (i - r * (kTreeD / 8)) * 8;
-          if (i < kVec)
-            *reinterpret_cast<uint4*>(smem + L::kQOff + (d >> 6) * (N * 128) + sw128_offset(r, d & 63)) = v[j];
+          for (int j = 0; j < kBatch; ++j) {
+            const int i = i0 + kTreeSoftmax * j, r = i / (kTreeD / 8), d = (i - r * (kTreeD / 8)) * 8;
+            if (i < kVec)
+              *reinterpret_cast<uint4*>(smem + L::kQOff + (d >> 6) * (N * 128) + sw128_offset(r, d & 63)) = v[j];
+          }
         }
+        fence_proxy_async_smem();
+        mbar_arrive(bar_q);
       }
       if (tid < N) masks[tid] = tid < rows ? uint64_t(a.masks[s.node0 + (row0 + tid) / a.heads]) : 0ull;
-      fence_proxy_async_smem();
-      mbar_arrive(bar_q);
+      asm volatile("bar.sync 3, %0;" ::"n"(kTreeSoftmax) : "memory");  // the masks are there for both halves
 
       // a maximum follows when a score passes it by more than the slack (or is the first)
       auto limit = [](float m) { return m + kTreeSlack; };
@@ -848,6 +862,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         }
         return int32_t(blk * DSR_BLOCK_TOKENS);
       };
+      if (!a.q_wide) {
+        // the query, once the last S MMA of the job before has read the one there
+        if (n > 0) ok = __shfl_sync(~0u, int(tree_wait(bar_s, (n - 1) & 1, abort, a.err)), 0) != 0;
+        if (!ok) break;
+        if (lane == 0) {
+          const int32_t qrow = s.node0 * a.heads + walk.group * N;
+          mbar_arrive_expect_tx(bar_q, 9 * N * 128);
+          for (int c = 0; c < 9; ++c) tma_load_2d(sbase + L::kQOff + c * (N * 128), &q_map, bar_q, c * 64, qrow);
+          ++*loaded_q;
+        }
+      }
       int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
       for (int i = 0; lane == 0 && i < walk.count && ok; ++i, ++n) {
         const int32_t x0 = y0, x1 = y1;
@@ -872,7 +897,13 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         tma_load_2d(sbase + L::kROff, &kv_map, bar_r, 512, x0);
         tma_load_2d(sbase + L::kROff + 8192, &kv_map, bar_r, 512, x1);
         *loaded_r = n + 1;
+        if (i + 1 < walk.count)  // the next tile's rows into L2 (209 to 199 us for 8 nodes over 131072 rows)
+          for (int c = 0; c < 9; ++c) {
+            tma_prefetch_2d(&kv_map, c * 64, y0);
+            tma_prefetch_2d(&kv_map, c * 64, y1);
+          }
       }
+      n = __shfl_sync(~0u, n, 0);
       ok = __shfl_sync(~0u, int(ok), 0) != 0;
     }
   }
@@ -882,6 +913,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     // a wait gave up: let the copies in flight land before exit
     for (int k = max(0, *loaded - L::kPairs); k < *loaded; ++k) mbar_drain(full + k % L::kPairs, (k / L::kPairs) & 1);
     if (*loaded_r > 0) mbar_drain(bar_r, (*loaded_r - 1) & 1);
+    if (*loaded_q > 0) mbar_drain(bar_q, (*loaded_q - 1) & 1);
   }
   if (warp == 8) {
     tc_fence_after();
@@ -997,7 +1029,12 @@ int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStrea
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_start_bytes(a.batch));
   a.part_m = a.part_o + size_t(kTreeSlotsPerCta) * a.ctas * N * kTreeDv;
   a.part_l = a.part_m + size_t(kTreeSlotsPerCta) * a.ctas * N;
-  tree_mla_kernel<N><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, a);
+  CUtensorMap q_map = map;  // FP32 queries are converted, not copied
+  if (!a.q_wide) {
+    rc = encode_tmap_bf16_2d(&q_map, a.q, kTreeD, uint64_t(a.nodes) * a.heads, 64, N);
+    if (rc != DSR_OK) return rc;
+  }
+  tree_mla_kernel<N><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, q_map, a);
   rc = launch_status("tree_mla_decode launch");
   if (rc != DSR_OK) return rc;
   cudaLaunchConfig_t cfg = {};
