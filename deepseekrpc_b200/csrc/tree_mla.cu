@@ -57,8 +57,8 @@ struct TreeLayout {
   static constexpr int kQOff = kROff + 16384;           // 9 x N x 128 B
   static constexpr int kBarOff = kQOff + 9 * N * 128;
   static constexpr int kBars = 2 * kPairs + 6;
-  static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N] seen-masks of the rows
-  static constexpr int kRedOff = kMaskOff + N * 8;      // f32[4][N] per-warp maxima, then sums
+  static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N + 1] seen-masks of the rows, their union
+  static constexpr int kRedOff = kMaskOff + (N + 1) * 8;  // f32[4][N] per-warp maxima, then sums
   static constexpr int kStatOff = kRedOff + 4 * N * 4;  // f32[N] factors / reciprocals
   static constexpr int kChunkOff = kStatOff + N * 4;    // i32[2][kTreeThreads]
   static constexpr int kMiscOff = kChunkOff + 2 * kTreeThreads * 4;
@@ -556,7 +556,16 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         fence_proxy_async_smem();
         mbar_arrive(bar_q);
       }
-      if (tid < N) masks[tid] = tid < rows ? uint64_t(a.masks[s.node0 + (row0 + tid) / a.heads]) : 0ull;
+      if (warp == 0) {  // the rows' masks, and what any of them sees
+        uint64_t any = 0;
+        for (int r = lane; r < N; r += 32) {
+          const uint64_t word = r < rows ? uint64_t(a.masks[s.node0 + (row0 + r) / a.heads]) : 0ull;
+          masks[r] = word;
+          any |= word;
+        }
+        const uint32_t low = __reduce_or_sync(~0u, uint32_t(any)), high = __reduce_or_sync(~0u, uint32_t(any >> 32));
+        if (lane == 0) masks[N] = uint64_t(high) << 32 | low;
+      }
       asm volatile("bar.sync 3, %0;" ::"n"(kTreeSoftmax) : "memory");  // the masks are there for both halves
 
       // a maximum follows when a score passes it by more than the slack (or is the first)
@@ -597,18 +606,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
                   if (d >= 0 && (d >= s.nodes || !(word >> d & 1))) v[c][j][e] = -CUDART_INF_F;
                 }
               }
-            // a row that no node of the group sees may hold anything: it is cleared,
-            // since 0 x NaN would reach the output
-            uint64_t any = 0;
-            for (int r = 0; r < N; ++r) any |= masks[r];
+            // a row that no node of the group sees may hold anything: it is cleared, since
+            // 0 x NaN would reach the output.  Eight lanes a row: a thread per row would
+            // send the 32 lanes of a store to the same banks (4.7 us for one such tile)
+            const uint64_t any = masks[N];
             const int32_t d = drafted + t;
-            if (d >= 0 && (d >= s.nodes || !(any >> d & 1))) {
+            const uint32_t hidden = __ballot_sync(~0u, d >= 0 && (d >= s.nodes || !(any >> d & 1)));
+            if (hidden != 0) {
 #pragma unroll 1
               for (int c = 4 * half; c < 4 * half + 4; ++c) {
                 const int pair = (4 * n + (c >> 1)) % L::kPairs;
-                uint4* dst = reinterpret_cast<uint4*>(smem + L::kRingOff + pair * 32768 + (c & 1) * 16384 + t * 128);
+                uint8_t* block = smem + L::kRingOff + pair * 32768 + (c & 1) * 16384 + (warp & 3) * 32 * 128;
 #pragma unroll
-                for (int x = 0; x < 8; ++x) dst[x] = make_uint4(0, 0, 0, 0);
+                for (int x = 0; x < 8; ++x) {
+                  const int r = 4 * x + (lane >> 3);
+                  if (hidden >> r & 1)
+                    *reinterpret_cast<uint4*>(block + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
+                }
               }
             }
           }
@@ -940,12 +954,14 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
   const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
   const int tid = threadIdx.x, d = blockIdx.y * kJoinThreads + tid;
-  // the request of the node: the largest b with cu_nodes[b] <= node
-  int lo = 0, hi = a.batch;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (a.cu_nodes[mid] <= node) lo = mid;
-    else hi = mid;
+  // the request of the node: the largest b with cu_nodes[b] <= node, 32 ways a step
+  int lo = 0;
+  for (int n = a.batch; n > 1;) {
+    const int stride = (n + 31) / 32, at = (tid & 31) * stride;
+    const unsigned below = __ballot_sync(~0u, at < n && a.cu_nodes[lo + at] <= node);
+    const int last = below == 0 ? 0 : (31 - __clz(below)) * stride;
+    lo += last;
+    n = min(stride, n - last);
   }
   const TreeSeq s = tree_seq<N>(a, lo);
   if (node < s.node0 || node >= s.node0 + s.nodes) return;
