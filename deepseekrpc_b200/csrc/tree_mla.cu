@@ -59,7 +59,7 @@ struct TreeLayout {
   static constexpr int kBars = 2 * kPairs + 6;
   static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N + 1] seen-masks of the rows, their union
   static constexpr int kRedOff = kMaskOff + (N + 1) * 8;  // f32[4][N] per-warp maxima, then sums
-  static constexpr int kStatOff = kRedOff + 4 * N * 4;  // f32[N] factors / reciprocals
+  static constexpr int kStatOff = (kRedOff + 4 * N * 4 + 15) / 16 * 16;  // f32[N] factors / reciprocals
   static constexpr int kChunkOff = kStatOff + N * 4;    // i32[2][kTreeThreads]
   static constexpr int kMiscOff = kChunkOff + 2 * kTreeThreads * 4;
   static constexpr int kBytes = kMiscOff + 64;
@@ -117,32 +117,22 @@ __device__ __forceinline__ int32_t tree_segments(const TreeSeq& s, int32_t lengt
 }
 
 // ---- the jobs of a call
-constexpr int kTreeSearchBatch = 2048;  // larger batches take the even share (the search reads every request)
 constexpr int kTreeSlotsPerCta = 4;  // partial slots, per CTA of the grid
 // A round's cost beside its tiles, in tiles: first copies, output, its part of the join.
 constexpr float kTreeJobCost = 8.f;
 
 // A segment length for `waves` jobs per CTA at most: starts at the even share and
 // grows until the jobs (requests' tiles rounded up to whole segments) and the partial
-// slots fit.  One warp; estimates the time in tiles (infinite when none was found).
-template <int N>
-__device__ __forceinline__ float tree_length(const TreeArgs& a, int64_t units, int waves, int lane, int32_t& length) {
+// slots fit.  One warp, lane b with request b; estimates the time in tiles (infinite when
+// none was found).
+__device__ __forceinline__ float tree_length(const TreeArgs& a, const TreeSeq& s, int64_t units, int waves,
+                                             int32_t& length) {
   const int64_t room = int64_t(waves) * a.ctas;
   float len = fmaxf(ceilf(float(units) / float(room)), 1.f);
   for (int tries = 0; tries < 8; ++tries) {
     length = int32_t(len);
-    int64_t jobs = 0, slots = 0;
-    for (int b = lane; b < a.batch; b += 32) {
-      const TreeSeq s = tree_seq<N>(a, b);
-      const int64_t n = int64_t(s.groups) * tree_segments(s, length);
-      jobs += n;
-      if (s.tiles > length) slots += n;
-    }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-      jobs += __shfl_xor_sync(~0u, jobs, o);
-      slots += __shfl_xor_sync(~0u, slots, o);
-    }
+    const int32_t n = s.groups * tree_segments(s, length);
+    const int32_t jobs = __reduce_add_sync(~0u, n), slots = __reduce_add_sync(~0u, s.tiles > length ? n : 0);
     if (jobs <= room && slots <= int64_t(kTreeSlotsPerCta) * a.ctas) {
       // one round lasts as long as its longest job; several come near the mean
       const float mean = float(units) / float(a.ctas);
@@ -154,16 +144,18 @@ __device__ __forceinline__ float tree_length(const TreeArgs& a, int64_t units, i
 }
 
 // ---- a CTA's jobs, one after another (every warp walks them for itself)
+// Up to 32 requests: what they are, the jobs and slots before each, in shared memory.
+struct TreeEntry {
+  TreeSeq s;
+  int32_t jobs, count, slots;
+};
 template <int N>
 struct TreeWalk {
   const TreeArgs& a;
-  const int32_t *chunk_jobs, *chunk_slots;  // [kTreeThreads] before each chunk of `per` requests
+  const TreeEntry* entries;                 // [batch <= 32]
+  const int32_t *chunk_jobs, *chunk_slots;  // else: [kTreeThreads] before each chunk of `per` requests
   int32_t length, jobs;
-  int round;
-  int per;
-  // up to 32 requests: lane b keeps request b, and the jobs and slots before it
-  TreeSeq own;
-  int32_t own_jobs, own_count, own_slots;
+  int round, per;
   int b, group, tile0, count, slot;  // slot < 0: the group's only segment
   TreeSeq s;
   __device__ __forceinline__ void at_job(int32_t at, int32_t segments, int32_t slots) {
@@ -180,13 +172,15 @@ struct TreeWalk {
     if (job >= jobs) return false;
     ++round;
     if (a.batch <= 32) {
-      b = __ffs(__ballot_sync(~0u, job >= own_jobs && job - own_jobs < own_count)) - 1;
-      s.node0 = __shfl_sync(~0u, own.node0, b);
-      s.nodes = __shfl_sync(~0u, own.nodes, b);
-      s.context = __shfl_sync(~0u, own.context, b);
-      s.tiles = __shfl_sync(~0u, own.tiles, b);
-      s.groups = __shfl_sync(~0u, own.groups, b);
-      at_job(job - __shfl_sync(~0u, own_jobs, b), tree_segments(s, length), __shfl_sync(~0u, own_slots, b));
+      const int lane = threadIdx.x & 31;
+      bool has = false;
+      if (lane < a.batch) {
+        const int32_t at = job - entries[lane].jobs;
+        has = at >= 0 && at < entries[lane].count;
+      }
+      b = __ffs(__ballot_sync(~0u, has)) - 1;
+      s = entries[b].s;
+      at_job(job - entries[b].jobs, tree_segments(s, length), entries[b].slots);
       return true;
     }
     int lo = 0, hi = kTreeThreads;  // the last chunk that starts at or before the job
@@ -339,36 +333,6 @@ __device__ __forceinline__ float tree_total(const TreeArgs& a, int head, float t
   return over > 100.f ? sink : (top + log2f(total)) / kTreeLog2e;
 }
 
-// Value column d = this thread's of W consecutive rows (of which `rows` exist);
-// returns whether one is not finite.
-template <int W>
-__device__ __forceinline__ bool tree_store(const TreeArgs& a, int64_t row, int rows, int d, int lane,
-                                           const float (&x)[W]) {
-  bool bad = false;
-  if (a.out_wide) {
-    float* dst = static_cast<float*>(a.out) + row * kTreeDv + d;
-#pragma unroll
-    for (int y = 0; y < W; ++y)
-      if (y < rows) {
-        dst[int64_t(y) * kTreeDv] = x[y];
-        bad |= !isfinite(x[y]);
-      }
-  } else {
-    // lanes 2i and 2i + 1 swap halves of two rows: each stores two columns of one
-    const int odd = lane & 1;
-    uint16_t* dst = static_cast<uint16_t*>(a.out) + (row + odd) * kTreeDv + (d - odd);
-#pragma unroll
-    for (int y = 0; y < W; y += 2) {
-      const float mine = odd ? x[y + 1] : x[y], other = __shfl_xor_sync(~0u, odd ? x[y] : x[y + 1], 1);
-      if (y + odd < rows) {
-        *reinterpret_cast<uint32_t*>(dst + int64_t(y) * kTreeDv) = odd ? bf16x2(other, mine) : bf16x2(mine, other);
-        bad |= !isfinite(mine) || !isfinite(other);
-      }
-    }
-  }
-  return bad;
-}
-
 template <int N>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
@@ -425,7 +389,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   }
 
   // ---- the work of all requests
-  TreeWalk<N> walk{a, chunk_jobs, chunk_slots, 1, 0, 0, 1, TreeSeq{}, 0, 0, 0};
+  TreeEntry* entries = reinterpret_cast<TreeEntry*>(smem + L::kChunkOff);  // in the chunks' place
+  static_assert(32 * sizeof(TreeEntry) <= 2 * kTreeThreads * 4, "");
+  TreeWalk<N> walk{a, entries, chunk_jobs, chunk_slots, 1, 0, 0, 1};
+  TreeSeq own_seq{};
   const bool small = a.batch <= 32;
   const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;  // else: requests of a thread's chunk
   const int r0 = small ? lane : min(tid * per, a.batch), r1 = small ? min(lane + 1, a.batch) : min(r0 + per, a.batch);
@@ -437,7 +404,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
     units += int64_t(s.groups) * s.tiles;
     groups += s.groups;
-    walk.own = s;
+    own_seq = s;
   }
   // sums over the warp: low and high parts of the units by themselves
   units = (int64_t(__reduce_add_sync(~0u, uint32_t(units >> 24))) << 24) +
@@ -453,10 +420,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   // ---- the segment length: one tile when that fills no more than the grid, else the
   // best of four wave counts
   int32_t length = units <= a.ctas ? 1 : 0;
-  if (length == 0 && a.batch <= kTreeSearchBatch) {
+  if (length == 0 && small) {
     if (warp < 4) {
       int32_t len = 1;
-      const float e = tree_length<N>(a, units, (groups + a.ctas - 1) / a.ctas + warp, lane, len);
+      const float e = tree_length(a, own_seq, units, (groups + a.ctas - 1) / a.ctas + warp, len);
       if (lane == 0) estimate[warp] = e, estimated[warp] = len;
     }
     __syncthreads();
@@ -465,27 +432,29 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       if (estimate[w] < best) best = estimate[w], length = estimated[w];
   }
   // or the even share of two jobs per CTA, whose partials always fit: a cut request's
-  // groups have at most 2 U / length of them
+  // groups have at most 2 U / length of them.  More than 32 requests take that (the search
+  // reads every request several times: 4 us of a CTA for 300), as do those without a find
   if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
   // ---- jobs and partial slots before each lane's request, or each thread's chunk
   int32_t jobs = 0, slots = 0;
   for (int b = r0; b < r1; ++b) {
-    const TreeSeq s = small ? walk.own : tree_seq<N>(a, b);
+    const TreeSeq s = small ? own_seq : tree_seq<N>(a, b);
     const int32_t n = s.groups * tree_segments(s, length);
     jobs += n;
     if (s.tiles > length) slots += n;
   }
   walk.length = length;
+  int32_t jobs_before = 0, slots_before = 0;
   if (small) {
     // those of the requests with longer segments come first
-    const float mine = jobs > 0 ? float(walk.own.tiles) / float(tree_segments(walk.own, length)) : 0.f;
-    walk.own_count = jobs;
+    const float mine = jobs > 0 ? float(own_seq.tiles) / float(tree_segments(own_seq, length)) : 0.f;
     for (int b = 0; b < a.batch; ++b) {
       const float other = __shfl_sync(~0u, mine, b);
       const int32_t n = __shfl_sync(~0u, jobs, b), m = __shfl_sync(~0u, slots, b);
-      if (other > mine || (other == mine && b < lane)) walk.own_jobs += n, walk.own_slots += m;
+      if (other > mine || (other == mine && b < lane)) jobs_before += n, slots_before += m;
       walk.jobs += n;
     }
+    if (warp == 0 && lane < a.batch) entries[lane] = TreeEntry{own_seq, jobs_before, jobs, slots_before};
   } else {
     int32_t jobs_upto = jobs, slots_upto = slots;
 #pragma unroll
@@ -493,24 +462,23 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
       if (lane >= d) jobs_upto += u, slots_upto += v;
     }
-    walk.own_jobs = jobs_upto - jobs;
-    walk.own_slots = slots_upto - slots;
+    jobs_before = jobs_upto - jobs;
+    slots_before = slots_upto - slots;
     __syncthreads();  // the sums above have been read
     if (lane == 31) warp_units[warp] = jobs_upto, warp_groups[warp] = slots_upto;
     __syncthreads();
     for (int w = 0; w < kTreeThreads / 32; ++w) {
-      if (w < warp) walk.own_jobs += int32_t(warp_units[w]), walk.own_slots += int32_t(warp_groups[w]);
+      if (w < warp) jobs_before += int32_t(warp_units[w]), slots_before += int32_t(warp_groups[w]);
       walk.jobs += int32_t(warp_units[w]);
     }
-    chunk_jobs[tid] = walk.own_jobs;
-    chunk_slots[tid] = walk.own_slots;
+    chunk_jobs[tid] = jobs_before;
+    chunk_slots[tid] = slots_before;
   }
   if (blockIdx.x == 0 && (!small || warp == 0)) {
-    int32_t before = walk.own_slots;
     for (int b = r0; b < r1; ++b) {
-      const TreeSeq s = small ? walk.own : tree_seq<N>(a, b);
-      a.slot_start[b] = before;
-      if (s.tiles > length) before += s.groups * tree_segments(s, length);
+      const TreeSeq s = small ? own_seq : tree_seq<N>(a, b);
+      a.slot_start[b] = slots_before;
+      if (s.tiles > length) slots_before += s.groups * tree_segments(s, length);
     }
     if (tid == 0) a.slot_start[a.batch] = length;
   }
@@ -526,8 +494,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     const int quad = lane >> 2, mine = row_h + 2 * (lane & 3);        // key of a fragment, first of its two rows
     int n = 0;
     bool ok = true;
-    while (ok && walk.next()) {
+    bool more = walk.next();
+    while (ok && more) {
       const TreeSeq s = walk.s;
+      const int tile0 = walk.tile0, count = walk.count, slot = walk.slot;
       const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
       const int64_t qrow = int64_t(s.node0) * a.heads + row0;
       if (a.q_wide) {
@@ -573,8 +543,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       float m[C][2], l[C][2];
 #pragma unroll
       for (int c = 0; c < C; ++c) m[c][0] = m[c][1] = -CUDART_INF_F, l[c][0] = l[c][1] = 0.f;
-      for (int i = 0; i < walk.count; ++i, ++n) {
-        const int32_t p0 = (walk.tile0 + i) * kTreeKeys;
+      for (int i = 0; i < count; ++i, ++n) {
+        const int32_t p0 = (tile0 + i) * kTreeKeys;
         ok = tree_wait(bar_s, n & 1, abort, a.err);
         // ---- scores of keys 32 (warp % 4) + quad + 8j, rows row_h + 8c + 2 (lane % 4) + e
         float v[C][4][2];
@@ -721,8 +691,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 
       // ---- output of the segment: sums over the keys' threads, then O^T.  The last O
       // MMA follows every thread's last use of red and stat
+      more = walk.next();  // while they run
       ok = tree_wait(bar_o, (n - 1) & 1, abort, a.err);
-      const int slot = walk.slot;
       const bool whole = slot < 0;
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -756,7 +726,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       }
       softmax_sync(half, true);
       tc_fence_after();
-      bool bad = false;
+      float finite = 0.f;  // stays zero
 #pragma unroll 1
       for (int x0 = 0; x0 < 4 * kHalf; x0 += W) {
         uint32_t o[W];
@@ -765,17 +735,32 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         tmem_wait_ld();
         float x[W];
 #pragma unroll
-        for (int y = 0; y < W; ++y) x[y] = __uint_as_float(o[y]) * stat[r + y];
+        for (int y = 0; y < W; y += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(stat + r + y);
+          x[y] = __uint_as_float(o[y]) * f.x, x[y + 1] = __uint_as_float(o[y + 1]) * f.y;
+          x[y + 2] = __uint_as_float(o[y + 2]) * f.z, x[y + 3] = __uint_as_float(o[y + 3]) * f.w;
+        }
         if (!whole) {
           float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * N + r) * kTreeDv) + d;
 #pragma unroll
           for (int y = 0; y < W; y += 4)
             if (r + y < rows) dst[y / 4 * kTreeDv] = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
+        } else if (a.out_wide) {
+          float* dst = static_cast<float*>(a.out) + (qrow + r) * kTreeDv + d;
+#pragma unroll
+          for (int y = 0; y < W; ++y)
+            if (r + y < rows) dst[y * kTreeDv] = x[y], finite = fmaf(x[y], 0.f, finite);
         } else {
-          bad |= tree_store<W>(a, qrow + r, rows - r, d, lane, x);
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + (qrow + r) * kTreeDv + d;
+#pragma unroll
+          for (int y = 0; y < W; ++y)
+            if (r + y < rows) {
+              dst[y * kTreeDv] = __bfloat16_as_ushort(__float2bfloat16_rn(x[y]));
+              finite = fmaf(x[y], 0.f, finite);
+            }
         }
       }
-      if (bad) flag(a.err, DSR_ERR_NONFINITE);
+      if (finite != 0.f) flag(a.err, DSR_ERR_NONFINITE);
       tc_fence_before();
       mbar_arrive(bar_free);
     }
