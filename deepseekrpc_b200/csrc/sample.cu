@@ -606,7 +606,10 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
     // where f lies among the steps; its step; whether that is at most b, or below it
     auto place_of = [&](float f) { return binned ? (top - f) * per_step : 0.f; };
     auto bin_of = [&](float f) { return int(fminf(place_of(f), float(kSampleBins - 1))); };
-    auto bound_after = [&](int b) { return b < kSampleBins - 1 ? float(b + 1) : CUDART_INF_F; };  // place < it: step <= b
+    // up_to(place, bound_after(b)): step <= b.  Places may be infinite (a mask's lowest value
+    // over a small step), and all of them are in the last step: no bound, as a NaN
+    auto bound_after = [&](int b) { return b < kSampleBins - 1 ? float(b + 1) : CUDART_NAN_F; };
+    auto up_to = [](float place, float bound) { return !(place >= bound); };
     auto part_of = [&](int bin) {  // of step `bin`, in kSampleBins parts
       return [=](float f) {
         return int(fminf(fmaxf((place_of(f) - float(bin)) * float(kSampleBins), 0.f), float(kSampleBins - 1)));
@@ -626,7 +629,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         find_step(at, count, count, unsigned(k));
         const float bound = bound_after(s.step_bin);
         each([&](float f, int i) {
-          if (place_of(f) < bound && f != nothing) keep(f, i);
+          if (up_to(place_of(f), bound) && f != nothing) keep(f, i);
         });
         cluster.sync();
         if (finish_alone(k, 0)) return;
@@ -661,7 +664,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
           const float from = float(bin), bound = bound_after(bin);
           each([&](float f, int i) {
             const float at = place_of(f);
-            if (at >= from && at < bound && f != nothing) keep(f, i);
+            if (at >= from && up_to(at, bound) && f != nothing) keep(f, i);
           });
           cluster.sync();
           const int n = bring();
@@ -718,7 +721,7 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const float from = whole ? 0.f : float(bin), bound = bound_after(bin);
         each([&](float f, int i) {
           const float at = place_of(f);
-          if (at >= from && at < bound && f >= weight.floor && (cut == 0 || rank_of(f, i) >= cut)) keep(f, i);
+          if (at >= from && up_to(at, bound) && f >= weight.floor && (cut == 0 || rank_of(f, i) >= cut)) keep(f, i);
         });
         cluster.sync();
         if (whole && finish_alone(kSampleFew, total.v)) return;

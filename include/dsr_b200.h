@@ -521,9 +521,11 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
  * with w_i >= min_p; tokens i32[rows] = the first kept index in vocabulary order
  * whose cumulative weight exceeds uniform times the kept weight, chances f32[rows]
  * its share of the kept weight.  temperature 0: the arg max (lowest index), chance
- * 1.  Settings per row: temperature >= 0, top_k >= 0, top_p, min_p in [0, 1],
- * uniform in [0, 1); others give status 1.  -inf logits are never drawn; a row of
- * them alone gives token -1 and chance 0; NaN or +inf gives status 2; a row with
+ * 1.  Weights are multiples of 2^-44 of the row's largest: an entry of less than
+ * half of one is never drawn, not even by uniform = 0.  Settings per row:
+ * temperature >= 0, top_k >= 0, top_p, min_p in [0, 1], uniform in [0, 1); others
+ * give status 1.  -inf logits are never drawn; a row of them alone gives token -1
+ * and chance 0; NaN or +inf gives status 2; a row with
  * a status has token -1.  vocab <= 262144. */
 int dsr_sample(const void* logits, int dtype, int64_t row_stride, int64_t vocab,
                const float* temperature, const int32_t* top_k, const float* top_p,
