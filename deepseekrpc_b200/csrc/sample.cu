@@ -721,7 +721,8 @@ __global__ void __launch_bounds__(kSampleThreads, 2) sample_kernel(const SampleA
         const float from = whole ? 0.f : float(bin), bound = bound_after(bin);
         each([&](float f, int i) {
           const float at = place_of(f);
-          if (at >= from && up_to(at, bound) && f >= weight.floor && (cut == 0 || rank_of(f, i) >= cut)) keep(f, i);
+          // what the steps counted, and nothing else: the list has room for that
+          if (at >= from && up_to(at, bound) && (cut == 0 || rank_of(f, i) >= cut) && weight(f) != 0) keep(f, i);
         });
         cluster.sync();
         if (whole && finish_alone(kSampleFew, total.v)) return;

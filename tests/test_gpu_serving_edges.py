@@ -69,6 +69,18 @@ def test_sampling_prefix_ends_among_entries_of_the_lowest_value(cuda, dtype, voc
         sample(logits, temperature, top_k, top_p=0.9, uniform=u)
 
 
+@pytest.mark.parametrize("temperature", [1e-31, 1e-32])
+@pytest.mark.parametrize("top_k", [0, 150])
+def test_sampling_of_tiny_values_at_a_tiny_temperature(cuda, temperature, top_k):
+    """One step holds all: thousands of entries whose weight rounds to none."""
+    gen = torch.Generator("cuda").manual_seed(9)
+    x = -torch.rand((3, 40000), generator=gen, device="cuda", dtype=torch.float64) * 10 - 31.6
+    x[:, ::1000] += 31.6  # 40 entries with weight; the others at 2^-45.6 to 2^-60
+    logits = (x * temperature).float()
+    for p in (0.5, 0.9, 1.0):
+        sample(logits, temperature, top_k, p, uniform=0.7)
+
+
 @pytest.mark.parametrize("temperature", [1e-30, 3e37, 3e38])
 def test_sampling_extreme_temperatures(cuda, temperature):
     gen = torch.Generator("cuda").manual_seed(3)
