@@ -239,7 +239,9 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
 #pragma unroll
       for (int q = 0; q < kMoves; ++q) {
         if (entry[q] == nullptr) continue;
-        a.ring[ring_at(ring_at(head + count) + i0 + q * step)] = blk[q];
+        const bool good = blk[q] >= 0 && blk[q] < a.blocks;
+        if (!good) flag(a.err, DSR_ERR_ID);
+        a.ring[ring_at(ring_at(head + count) + i0 + q * step)] = good ? blk[q] : -1;
         *entry[q] = -1;
       }
     }

@@ -35,7 +35,10 @@ def paged_plan(lengths, new_tokens, held, table, ring, state, tokens):
                 block, status = -1, 1
             table[b, j] = block
         for j in range(need[b], held[b]):
-            ring[tail % blocks] = table[b, j]
+            block = table[b, j]
+            if not 0 <= block < blocks:
+                block, status = -1, 1
+            ring[tail % blocks] = block
             tail += 1
             table[b, j] = -1
         for p in range(lengths[b], total[b]):

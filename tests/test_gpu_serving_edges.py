@@ -107,3 +107,38 @@ def test_sampling_replays_with_other_values(cuda):
         graph.replay()
         fresh = call()
         assert torch.equal(out[0], fresh[0]) and torch.equal(out[1], fresh[1])
+
+
+# ------------------------------------------------------------------------ plan
+def test_plan_reports_bad_blocks_that_are_given_back(cuda):
+    args = [np.array([0, 10], np.int32), np.array([0, 1], np.int32), np.array([3, 1], np.int32),
+            np.array([[4, 99, -5, -1], [2, -1, -1, -1]], np.int32), np.array([7, 6, 5, 0, 0, 0, 0, 0], np.int32),
+            np.array([0, 3, 0, 0], np.int32)]
+    expect = serving.paged_plan(*args, 1)
+    d = [torch.from_numpy(a).cuda() for a in args]
+    *_, status = cuda_ops.extension().paged_plan(*d, 1)
+    assert int(status.item()) == expect[-1] == 1
+    for got, want in zip(d[2:], expect[:4]):
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
+def test_plan_writes_outputs_off_the_16_byte_grid(cuda):
+    """The C call takes any int32 pointers: four tokens a store only where all three allow."""
+    from deepseekrpc_b200 import _native
+    p = _native.ptr
+    lengths, new = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([5, 100], [70, 9]))
+    held = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    table = torch.tensor([[3, -1, -1], [0, 1, -1]], dtype=torch.int32, device="cuda")
+    ring = torch.tensor([2, 4, 5, 6, 7, 0, 0, 0], dtype=torch.int32, device="cuda")
+    state = torch.tensor([0, 5, 0, 0], dtype=torch.int32, device="cuda")
+    expect = serving.paged_plan(*(t.cpu().numpy() for t in (lengths, new, held, table, ring, state)), 83)
+    store = torch.full((3, 100), -9, dtype=torch.int32, device="cuda")
+    maps = [store[i, i + 1:i + 84] for i in range(3)]
+    rest, err = torch.zeros(8, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    rc = _native.library().dsr_paged_plan(p(lengths), p(new), p(held), p(table), 3, p(ring), p(state), 8, p(maps[0]),
+                                          p(maps[1]), p(maps[2]), 83, p(rest), p(rest[4:]), p(err), 2,
+                                          _native.stream_handle())
+    assert rc == 0 and int(err.item()) == 0
+    for i in range(3):
+        assert np.array_equal(maps[i].cpu().numpy(), expect[4][i])
+        assert torch.all(store[i, :i + 1] == -9) and torch.all(store[i, i + 84:] == -9)
