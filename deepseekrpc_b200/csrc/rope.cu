@@ -199,6 +199,11 @@ extern "C" int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int
     const bool in_place = s.x == s.out;
     DSR_REQUIRE(!in_place || (s.x_token == s.out_token && s.x_head == s.out_head),
                 "rope: an in-place rotation needs equal strides");
+    DSR_REQUIRE((s.out_token != 0 || tokens == 1) && (s.out_head != 0 || s.heads == 1),
+                "rope: rows of an output overlap");
+    for (int m = 0; m < count; ++m)
+      DSR_REQUIRE(m == n || (s.out != tensors[m].out && s.out != tensors[m].x),
+                  "rope: tensor %d's output is tensor %d's input or output", n, m);
     const int size = s.dtype == DSR_F32 ? 4 : 2, v = 16 / size;
     DSR_REQUIRE((reinterpret_cast<uintptr_t>(s.x) | reinterpret_cast<uintptr_t>(s.out)) % size == 0,
                 "rope: misaligned tensor");

@@ -464,7 +464,7 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
 /* One tensor of dsr_rope: x and out [tokens, heads, width] of type dtype with unit
  * column stride and token and head strides in elements (any sign; rows of one
  * tensor must not overlap).  out == x rotates in place (equal strides), otherwise
- * x and out must not overlap. */
+ * x and out must not overlap; nor may an output and another tensor of the call. */
 typedef struct {
   const void* x;
   void* out;
