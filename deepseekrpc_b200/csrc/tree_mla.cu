@@ -57,8 +57,8 @@ struct TreeLayout {
   static constexpr int kQOff = kROff + 16384;           // 9 x N x 128 B
   static constexpr int kBarOff = kQOff + 9 * N * 128;
   static constexpr int kBars = 2 * kPairs + 6;
-  static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[N + 1] seen-masks of the rows, their union
-  static constexpr int kRedOff = kMaskOff + (N + 1) * 8;  // f32[4][N] per-warp maxima, then sums
+  static constexpr int kMaskOff = kBarOff + kBars * 8;  // u64[2][N + 1] seen-masks of the rows, their union, per half
+  static constexpr int kRedOff = kMaskOff + 2 * (N + 1) * 8;  // f32[4][N] per-warp maxima, then sums
   static constexpr int kStatOff = (kRedOff + 4 * N * 4 + 15) / 16 * 16;  // f32[N] factors / reciprocals
   static constexpr int kChunkOff = kStatOff + N * 4;    // i32[2][kTreeThreads]
   static constexpr int kMiscOff = kChunkOff + 2 * kTreeThreads * 4;
@@ -352,7 +352,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   uint64_t* bar_o = bar_r + 3;              // the tile's O MMAs complete (commit)
   uint64_t* bar_q = bar_r + 4;              // query in place (TMA bytes + 1; FP32: kTreeSoftmax arrivals)
   uint64_t* bar_free = bar_r + 5;           // O^T read by the epilogue (kTreeSoftmax arrivals)
-  uint64_t* masks = reinterpret_cast<uint64_t*>(smem + L::kMaskOff);
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   float* stat = reinterpret_cast<float*>(smem + L::kStatOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
@@ -490,6 +489,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   if (warp < 8) {
     // ------------------------------------------------------------ softmax
     const int half = warp >> 2, row_h = half * kHalf, t = tid & 127;  // t: key, or value column
+    uint64_t* masks = reinterpret_cast<uint64_t*>(smem + L::kMaskOff) + half * (N + 1);
     const uint32_t lanes = uint32_t(warp & 3) * 32 << 16;             // this warp's TMEM lanes
     const int quad = lane >> 2, mine = row_h + 2 * (lane & 3);        // key of a fragment, first of its two rows
     int n = 0;
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         fence_proxy_async_smem();
         mbar_arrive(bar_q);
       }
-      if (warp == 0) {  // the rows' masks, and what any of them sees
+      if ((warp & 3) == 0) {  // the rows' masks, and what any of them sees
         uint64_t any = 0;
         for (int r = lane; r < N; r += 32) {
           const uint64_t word = r < rows ? uint64_t(a.masks[s.node0 + (row0 + r) / a.heads]) : 0ull;
@@ -536,7 +536,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         const uint32_t low = __reduce_or_sync(~0u, uint32_t(any)), high = __reduce_or_sync(~0u, uint32_t(any >> 32));
         if (lane == 0) masks[N] = uint64_t(high) << 32 | low;
       }
-      asm volatile("bar.sync 3, %0;" ::"n"(kTreeSoftmax) : "memory");  // the masks are there for both halves
+      // a half has its own, since it leaves alone when one of its waits gives up: a barrier
+      // of both would then never be complete
+      softmax_sync(half, true);
 
       // a maximum follows when a score passes it by more than the slack (or is the first)
       auto limit = [](float m) { return m + kTreeSlack; };
