@@ -782,11 +782,12 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     const uint64_t desc_p = umma_desc_sw128(sb + L::kROff, 16, 1024);
     int n = 0, segment = 0, pair = 0;  // pair: ring position of the tile's first block pair
     uint32_t lap = 0;                  // the ring's phase there
-    bool ok = true;
+    bool ok = true, committed = false;  // committed: the tile's S MMAs
     auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tree_wait(bar, parity, abort, a.err)); };
     while (ok) {
       if (!walk.next()) break;  // alike in all lanes
       const int count = __shfl_sync(~0u, walk.count, 0);
+      committed = false;
       ok = wait(bar_q, segment & 1);
       for (int i = 0; i < count && ok; ++i, ++n) {
         // S^T: column blocks 0..7 pair by pair, then the rotary block.  A step of 16
@@ -794,6 +795,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         // to a descriptor's address field (units of 16 bytes)
         int at = pair;
         uint32_t phase = lap;
+        committed = false;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           ok = ok && wait(full + at, phase);
@@ -818,6 +820,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             umma_bf16(ts, desc_s + L::kROff / 16 + 2 * x, desc_q + 8 * (N * 128 / 16) + 2 * x, idesc_s, 1u);
           umma_commit(bar_s);
         }
+        committed = true;
         ok = wait(bar_p, n & 1);
         // the previous segment's O^T has been read
         if (ok && i == 0 && segment > 0) ok = wait(bar_free, (segment - 1) & 1);
@@ -846,6 +849,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     }
     // the last MMAs retire before TMEM is released (commits cover all before them)
     if (n > 0) mbar_drain(bar_o, (n - 1) & 1);
+    if (!ok) {  // a wait gave up: nor may S MMAs of the tile it was in outlive TMEM
+      if (!committed && leader) umma_commit(bar_s);
+      mbar_drain(bar_s, n & 1);
+    }
   } else if (warp == 9) {
     // ------------------------------------------------------------ key tiles
     int n = 0;
