@@ -958,8 +958,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
     n = min(stride, n - last);
   }
   const TreeSeq s = tree_seq<N>(a, lo);
+  pdl_wait();  // before any CTA leaves: the join must not end ahead of the attention
   if (node < s.node0 || node >= s.node0 + s.nodes) return;
-  pdl_wait();
   const int parts = tree_segments(s, __ldcg(a.slot_start + a.batch));
   if (parts <= 1) return;  // written by its job
   const int in = int(row - int64_t(s.node0) * a.heads), group = in / N, r = in % N;

@@ -501,8 +501,8 @@ int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int32_t* posit
  * product; sums and statistics are FP32.  Output rows at or past cu_nodes[batch]
  * are not written.  Status 1: a context or node range that is negative, larger
  * than max_nodes, `nodes` or the table (that request's rows are not written), or a
- * block id outside the pool (its keys count as zeros); status 2: a NaN or infinite
- * score, sink or output.  Cached rows that no node sees may hold anything.
+ * block id outside the pool (its keys count as zeros); status 2: a NaN or +infinite
+ * score (one of -infinity is not seen), an infinite or NaN sink or output.  Cached rows that no node sees may hold anything.
  * Scratch: dsr_tree_mla_workspace_bytes() on the current device, 256-byte
  * aligned, need not be cleared; calls sharing it must not overlap. */
 size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes);

@@ -142,3 +142,105 @@ def test_plan_writes_outputs_off_the_16_byte_grid(cuda):
     for i in range(3):
         assert np.array_equal(maps[i].cpu().numpy(), expect[4][i])
         assert torch.all(store[i, :i + 1] == -9) and torch.all(store[i, i + 84:] == -9)
+
+
+# ------------------------------------------------------------------ attention
+def attend(lengths, counts, heads, seed, wide=False, padding=0, stream=None):
+    """Requests of lengths (cached) and counts (drafted) with a page table in random order;
+    NaN in every pool row that nobody sees and in the padding queries."""
+    rng = np.random.default_rng(seed)
+    gen = torch.Generator("cuda").manual_seed(seed)
+    batch, total = len(lengths), int(sum(counts))
+    blocks = [-(-(c + n) // 64) for c, n in zip(lengths, counts)]
+    ids = rng.permutation(sum(blocks) + 1)
+    pool = torch.full(((sum(blocks) + 1) * 64, 576), float("nan"), device="cuda").bfloat16()
+    table = np.full((batch, max(max(blocks), 1)), -1, np.int32)
+    q = torch.randn((total + padding, heads, 576), generator=gen, device="cuda")
+    q[total:] = float("nan")
+    q = q if wide else q.bfloat16()
+    sink = torch.randn(heads, generator=gen, device="cuda")
+    masks, keys, at = [], [], 0
+    for b in range(batch):
+        table[b, :blocks[b]] = ids[at:at + blocks[b]]
+        at += blocks[b]
+        n = lengths[b] + counts[b]
+        rows = torch.randn((n, 576), generator=gen, device="cuda").bfloat16()
+        where = torch.from_numpy((table[b][np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64)).cuda()
+        pool[where] = rows
+        keys.append(rows.double().cpu().numpy())
+        masks.append([int(rng.integers(0, 2 ** 62)) for _ in range(counts[b])])
+    cu = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    scale = 1 / math.sqrt(192)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    words = torch.tensor([w for m in masks for w in m] + [0] * padding, dtype=torch.int64, device="cuda")
+    call = [q, pool, torch.from_numpy(table).cuda(), torch.tensor(lengths, dtype=torch.int32, device="cuda"),
+            torch.from_numpy(cu).cuda(), words, max(max(counts), 1), scale]
+    out = torch.full((total + padding, heads, 512), 7.0, device="cuda")
+    cuda_ops.extension().tree_mla_decode(*call, sink=sink, out=out, status=status)
+    assert int(status.item()) == 0
+    assert torch.all(out[total:] == 7)
+    q64 = q.bfloat16().double().cpu().numpy()
+    for b in range(batch):
+        at = slice(cu[b], cu[b + 1])
+        if counts[b] == 0:
+            continue
+        ref, _ = serving.tree_attention(q64[at], keys[b], lengths[b], masks[b], sink.double().cpu().numpy(), scale)
+        got = out[at].double().cpu().numpy()
+        size = np.abs(keys[b]).max()
+        assert np.all(np.abs(got - ref) <= (2.0 ** -8 + 2.0 ** -11) * size), b
+        assert np.linalg.norm(got - ref) <= 2.0 ** -7 * np.linalg.norm(ref) + 1e-30, b
+
+
+@pytest.mark.parametrize("batch", [32, 33, 320, 321, 700])
+@pytest.mark.parametrize("wide", [False, True])
+def test_attention_of_many_requests(cuda, batch, wide):
+    rng = np.random.default_rng(batch)
+    lengths = rng.integers(0, 300, batch).tolist()
+    counts = rng.integers(0, 4, batch).tolist()
+    lengths[batch // 2], counts[batch // 2] = 5000, 3
+    attend(lengths, counts, 16, batch, wide, padding=5)
+
+
+@pytest.mark.parametrize("nodes,heads", [(1, 32), (2, 16), (64, 16), (5, 128)])
+def test_attention_of_long_contexts_in_each_group_size(cuda, nodes, heads):
+    attend([20001, 64, 0], [nodes, nodes, max(nodes - 1, 1)], heads, nodes)
+
+
+def test_attention_writes_nothing_where_no_request_has_nodes(cuda):
+    out = torch.full((4, 16, 512), 3.0, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = torch.zeros((4, 16, 576), device="cuda").bfloat16()
+    pool = torch.zeros((128, 576), device="cuda").bfloat16()
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    none = torch.zeros(3, dtype=torch.int32, device="cuda")
+    mask = torch.zeros(4, dtype=torch.int64, device="cuda")
+    for _ in range(3):
+        cuda_ops.extension().tree_mla_decode(q, pool, table, none[:2] + 10, none, mask, 4, 0.1, out=out, status=status)
+    assert int(status.item()) == 0 and torch.all(out == 3)
+    # a bad request's status is there for the next operation on the stream
+    bad = torch.tensor([0, 4, 9], dtype=torch.int32, device="cuda")
+    cuda_ops.extension().tree_mla_decode(q, pool, table, none[:2] - 5, bad, mask, 4, 0.1, out=out, status=status)
+    seen = status.clone()
+    assert int(seen.item()) == 1 and torch.all(out == 3)
+
+
+def test_attention_on_two_streams_at_once(cuda):
+    """Each call has its own workspace."""
+    gen = torch.Generator("cuda").manual_seed(5)
+    pool = torch.randn((8192, 576), generator=gen, device="cuda").bfloat16()
+    table = torch.randperm(128, generator=gen, device="cuda").to(torch.int32)[None]
+    context = torch.tensor([8100], dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 8], dtype=torch.int32, device="cuda")
+    mask = torch.full((8,), 255, dtype=torch.int64, device="cuda")
+    qs = [torch.randn((8, 64, 576), generator=gen, device="cuda").bfloat16() for _ in range(2)]
+    call = lambda q: cuda_ops.extension().tree_mla_decode(q, pool, table, context, cu, mask, 8, 0.07)[0]  # noqa: E731
+    alone = [call(q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):
+        both = []
+        for q, s in zip(qs, streams):
+            with torch.cuda.stream(s):
+                both.append(call(q))
+        torch.cuda.synchronize()
+        assert torch.equal(both[0], alone[0]) and torch.equal(both[1], alone[1])
