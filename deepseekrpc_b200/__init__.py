@@ -4,6 +4,7 @@ Layers:
   include/dsr_b200.h / libdsr_b200.so   C ABI over the hand-written kernels (_native: ctypes)
   deepseekrpc_cuda (torch extension)    the reference module's op names on that ABI
   cuda_ops, index_selection             host-side mirrors of the reference modules
+  rotary                                frequencies of rotary positions, long-context scaling
   sharded                               sequence sharding across GPUs (NCCL)
   workloads                             seeded BASELINE-config inputs
 """

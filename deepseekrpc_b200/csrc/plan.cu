@@ -16,7 +16,9 @@
 // and given back behind its tail, which are disjoint entries.  What all CTAs read
 // and the call changes (held, the ring's head and count) is written by the last
 // CTA to finish (a ticket in the ring state).  Bound by latency: one scan, one
-// dependent read of the block id, one store.
+// dependent read of the block id, one store.  Measured: 7 us a call for 1 request as for
+// 256 with 8 tokens each (launch and the extension's allocation); 1M tokens of 256
+// requests 15.6 us, 12 MB written (0.8 TB/s).
 #include "common.cuh"
 #include "host_common.h"
 
@@ -156,7 +158,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
 
   const int64_t step = int64_t(gridDim.x) * kPlanThreads, first = int64_t(blockIdx.x) * kPlanThreads + tid;
   auto ring_at = [&](int64_t i) { return int64_t(i < a.blocks ? i : i - a.blocks); };
-  // ---- the map of the new tokens, four consecutive ones a thread
+  // ---- the map of the new tokens, four consecutive ones a thread, stored 16 bytes at a time
+  // where all three outputs allow (1M tokens: 15.6 us, off that grid 19.8; 16K: 10.3 both)
   const int64_t mapped = ok ? all.tokens : 0;
   const bool vec = ((reinterpret_cast<uintptr_t>(a.seq) | reinterpret_cast<uintptr_t>(a.positions) |
                      reinterpret_cast<uintptr_t>(a.slots)) & 15u) == 0;

@@ -14,7 +14,11 @@
 // takes one token (or a share of one: few tokens have to fill the GPU too) and
 // forms its cosines once for all heads of all tensors.  Bound by memory: every
 // value is read and written once, in 16-byte pieces wherever pointers, strides and
-// columns allow.
+// columns allow (one tensor of 64 heads, 64 of 576 columns rotated in place, 8192 tokens:
+// 41 us; off the 16-byte grid, column by column, 90).  Measured: 8192 tokens of four
+// tensors, 560 MB, 127 us = 4.4 TB/s, 67% of a plain copy; 999 tokens, 44 MB, 14.5 us = 3.0
+// TB/s; 1 token 5.9 us, a launch.  Two to four pieces a thread ahead, streaming hints, loops
+// per tensor and several tokens a CTA were all slower (129 to 186 us of the first).
 #include "common.cuh"
 #include "host_common.h"
 

@@ -33,6 +33,14 @@
 //   warp 9      query and key tiles by TMA: column blocks 0..7 (the value columns) through a
 //               ring of block pairs that the O MMA frees pair by pair, block 8 (the
 //               rotary columns) in a buffer that P^T takes over once S^T is done
+//
+// Bound by shared memory at 64 rows: an MMA of 128 x 64 x 16 takes 48 cycles, not 32, to read
+// its operands, which is two thirds of the tensor cores' rate at best.  Measured: 8 nodes of
+// 64 heads over 131072 rows 186 to 192 us (770 TFLOP/s, 47% of a measured BF16 GEMM); 32
+// requests of 6 nodes over up to 65536 rows 0.93 to 1.03 ms (0.72 to 0.80 PFLOP/s).  Bound by
+// memory at 16 rows: 32 requests of one node and 16 heads over 65536 rows 378 us, 6.4 TB/s,
+// 97% of a plain copy.  Bound by latency for little: one node over 4096 rows 17.5 us in two
+// launches.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -1017,7 +1025,8 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
 }
 
 // Rows per group: all of a request's rows in one group when that fits, since a
-// group reads every key tile once.
+// group reads every key tile once, and no more, since the MMAs of empty rows cost as much
+// (16 rows over 131072: 64 us in groups of 16, 88 of 32, 92 of 64).
 int tree_rows(int64_t heads, int64_t max_nodes) {
   const int64_t rows = heads * max_nodes;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
