@@ -70,11 +70,14 @@ struct TreeLayout {
   static constexpr int kStatOff = (kRedOff + 4 * N * 4 + 15) / 16 * 16;  // f32[N] factors / reciprocals
   static constexpr int kChunkOff = kStatOff + N * 4;    // i32[2][kTreeThreads]
   static constexpr int kMiscOff = kChunkOff + 2 * kTreeThreads * 4;
-  static constexpr int kBytes = kMiscOff + 64;
+  static constexpr int kScratchOff = kMiscOff + 64;     // the schedule's sums, see tree_mla_kernel
+  static constexpr int kBytes = kScratchOff + 2 * (kTreeThreads / 32) * 8 + 2 * 4 * 4;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr uint32_t kTmemCols = N == 64 ? 512 : (N == 32 ? 256 : 128);  // >= 5 N
   static_assert(2 * N * 128 <= 16384, "P^T fits the rotary block's buffer");
   static_assert(kAlloc <= 232448, "shared memory of one CTA");
+  // ordinary accesses and TMA's are not ordered by a barrier alone
+  static_assert(kScratchOff >= kQOff + 9 * N * 128 && kScratchOff % 8 == 0, "the scratch is no place that TMA writes");
 };
 
 struct TreeArgs {
@@ -369,8 +372,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   int* loaded_q = reinterpret_cast<int*>(smem + L::kMiscOff + 16);  // queries
   int32_t* chunk_jobs = reinterpret_cast<int32_t*>(smem + L::kChunkOff);
   int32_t* chunk_slots = chunk_jobs + kTreeThreads;
-  // before the ring is used: [10] sums of the warps (units, groups), [4] estimates and lengths
-  int64_t* warp_units = reinterpret_cast<int64_t*>(smem);
+  // [10] sums of the warps (units, groups), [4] estimates and lengths
+  int64_t* warp_units = reinterpret_cast<int64_t*>(smem + L::kScratchOff);
   int64_t* warp_groups = warp_units + kTreeThreads / 32;
   float* estimate = reinterpret_cast<float*>(warp_groups + kTreeThreads / 32);
   int32_t* estimated = reinterpret_cast<int32_t*>(estimate + 4);
