@@ -239,6 +239,13 @@ __device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volati
   }
 }
 
+// The same for a whole warp, with one answer for all lanes: a lane may see the phase
+// complete while another gives up, and what follows a wait (tcgen05.ld, votes, shuffles) is
+// for all lanes or none.
+__device__ __forceinline__ bool tree_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  return __all_sync(~0u, tree_wait(bar, parity, abort, err));
+}
+
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t r;
@@ -558,7 +565,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       for (int c = 0; c < C; ++c) m[c][0] = m[c][1] = -CUDART_INF_F, l[c][0] = l[c][1] = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
         const int32_t p0 = (tile0 + i) * kTreeKeys;
-        ok = tree_wait(bar_s, n & 1, abort, a.err);
+        ok = tree_wait_warp(bar_s, n & 1, abort, a.err);
         // ---- scores of keys 32 (warp % 4) + quad + 8j, rows row_h + 8c + 2 (lane % 4) + e
         float v[C][4][2];
         if (ok) {
@@ -705,7 +712,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       // ---- output of the segment: sums over the keys' threads, then O^T.  The last O
       // MMA follows every thread's last use of red and stat
       more = walk.next();  // while they run
-      ok = tree_wait(bar_o, (n - 1) & 1, abort, a.err);
+      ok = tree_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
       const bool whole = slot < 0;
 #pragma unroll
       for (int c = 0; c < C; ++c)
@@ -794,7 +801,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     int n = 0, segment = 0, pair = 0;  // pair: ring position of the tile's first block pair
     uint32_t lap = 0;                  // the ring's phase there
     bool ok = true, committed = false;  // committed: the tile's S MMAs
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, tree_wait(bar, parity, abort, a.err)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return tree_wait_warp(bar, parity, abort, a.err); };
     while (ok) {
       if (!walk.next()) break;  // alike in all lanes
       const int count = __shfl_sync(~0u, walk.count, 0);
@@ -883,7 +890,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       };
       if (!a.q_wide) {
         // the query, once the last S MMA of the job before has read the one there
-        if (n > 0) ok = __shfl_sync(~0u, int(tree_wait(bar_s, (n - 1) & 1, abort, a.err)), 0) != 0;
+        if (n > 0) ok = tree_wait_warp(bar_s, (n - 1) & 1, abort, a.err);
         if (!ok) break;
         if (lane == 0) {
           const int32_t qrow = s.node0 * a.heads + walk.group * N;

@@ -21,3 +21,16 @@ def test_the_schedules_scratch_is_no_place_that_tma_writes():
     assert re.search(r"static_assert\(kScratchOff >= kQOff \+ 9 \* N \* 128", text)
     # every generic pointer into the block names a place of its own
     assert not re.search(r"reinterpret_cast<[^>]*\*>\(smem\)", text)
+
+
+def test_a_warp_has_one_answer_to_a_wait():
+    """A wait that gives up may answer one lane otherwise than another; an aligned
+    instruction behind it would then run in a part of the warp.  Outside the helper that
+    asks all lanes, only the copying lane, alone in its branch, waits by itself."""
+    text = code()
+    helper = re.search(r"bool tree_wait_warp\([^{]*\{(.*?)\n\}", text, re.S)
+    assert helper and "__all_sync(~0u, tree_wait(" in helper.group(1)
+    alone = re.search(r"for \([^;]*; lane == 0 && .*?\n      \}\n", text, re.S)
+    assert alone and alone.group(0).count("tree_wait(") == 2
+    rest = text.replace(helper.group(0), "").replace(alone.group(0), "")
+    assert len(re.findall(r"\btree_wait\(", rest)) == 1  # its definition
