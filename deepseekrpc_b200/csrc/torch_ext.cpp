@@ -493,6 +493,15 @@ int element_type(const at::Tensor& t, const char* what) {
   return t.scalar_type() == at::kFloat ? DSR_F32 : DSR_BF16;
 }
 
+// A tensor of the caller's that is written through its pointer: autograd would take what was
+// there before for its value, so one with a history (or a leaf) is refused, as torch refuses
+// it, and one that autograd may have saved is marked as changed.
+void overwrite(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), what,
+              ": the output requires a gradient, which this call does not track");
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // An uninitialised tensor without the dispatcher's round trip (a small call is made of these).
 at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dtype, const at::Tensor& anchor) {
   return at::detail::empty_cuda(sizes, dtype, anchor.device(), c10::nullopt);
@@ -579,6 +588,7 @@ at::Tensor ds_rope(std::vector<at::Tensor> x, std::vector<at::Tensor> out, at::T
     desc[i].interleaved = interleaved[i];
     desc[i].dtype = element_type(a, "rope");
   }
+  for (const at::Tensor& b : out) overwrite(b, "rope");
   ok(dsr_rope(desc, int64_t(x.size()), positions.data_ptr<int32_t>(), frequencies.data_ptr<double>(),
               frequencies.size(0), static_cast<float>(mscale), inverse, error.data_ptr<int32_t>(), tokens,
               current_stream()));
@@ -617,6 +627,7 @@ std::vector<at::Tensor> ds_tree_mla_decode(at::Tensor q, at::Tensor kv_pool, at:
     TORCH_CHECK(result.dim() == 3 && result.size(0) == nodes && result.size(1) == heads &&
                     result.size(2) == DSR_V_DIM,
                 "tree_mla_decode: out [nodes, heads, 512] expected");
+    overwrite(result, "tree_mla_decode");
   } else {
     result = fresh({nodes, heads, DSR_V_DIM}, q.scalar_type(), q);
   }

@@ -118,12 +118,22 @@ def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float
     """Rotates 1 to 4 tensors [tokens(, heads), width] by their positions in one launch.
 
     offsets and interleaved: first rotated column and layout of each tensor.  out:
-    where to write (the tensors themselves rotate in place); new tensors without it.
-    inverse: the transposed rotation, which is the gradient's.
+    where to write (the tensors themselves rotate in place); new tensors without it,
+    which carry the gradient of those that require one.  inverse: the transposed
+    rotation, which is the gradient's.  There is no gradient of the frequencies, none
+    through `out`, and no writing into a tensor that requires one.
     """
+    import torch
     tensors = list(tensors)
+    if torch.is_grad_enabled():
+        if frequencies.requires_grad:
+            raise ValidationError("the gradient of rotary frequencies is not provided")
+        if out is None and any(t.requires_grad for t in tensors):
+            from .rotary import Rotation
+            return list(Rotation.apply(positions, frequencies, list(offsets), list(interleaved), mscale, inverse,
+                                       True, *tensors))
     if out is None:
-        out = [t.clone() for t in tensors]  # padding rows keep their values
+        out = [t.detach().clone() for t in tensors]  # padding rows keep their values
     _status(extension().rope(tensors, list(out), positions, frequencies, list(offsets), list(interleaved),
                              mscale=mscale, inverse=inverse))
     return list(out)

@@ -1,7 +1,9 @@
-"""Frequencies of rotary positions, with the usual scalings for long contexts.
+"""Frequencies of rotary positions, with the usual scalings for long contexts, and the
+rotation's gradient.
 
 `rope_frequencies` gives what `cuda_ops.rope` (dsr_rope) takes: one angular
 frequency per rotated pair, in 64 bits, and the amplitude of the rotated columns.
+`Rotation` is that call for tensors that require a gradient.
 """
 from __future__ import annotations
 
@@ -9,7 +11,7 @@ import math
 
 import torch
 
-from .cuda_ops import ValidationError
+from .cuda_ops import ValidationError, _status, extension
 
 SCALINGS = ("none", "linear", "ntk", "yarn")
 
@@ -52,3 +54,34 @@ def rope_frequencies(dim: int, *, base: float = 10000.0, scaling: str = "none", 
     high = min(math.ceil(pair_of(beta_slow)), dim - 1)
     ramp = ((torch.arange(pairs, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
     return frequencies * (1 - ramp) + frequencies / factor * ramp, 0.1 * math.log(factor) + 1.0
+
+
+class Rotation(torch.autograd.Function):
+    """cuda_ops.rope into new tensors.  The rotation is linear, so its gradient is the
+    transposed one: the same amplitude, the angles negated; padding rows pass as they are."""
+
+    @staticmethod
+    def forward(ctx, positions, frequencies, offsets, interleaved, mscale, inverse, check, *tensors):
+        out = [t.detach().clone() for t in tensors]
+        status = extension().rope(list(tensors), out, positions, frequencies, offsets, interleaved, mscale=mscale,
+                                  inverse=inverse)
+        if check:
+            _status(status)
+        ctx.save_for_backward(positions, frequencies)
+        ctx.settings = offsets, interleaved, mscale, inverse
+        ctx.set_materialize_grads(False)
+        ctx.mark_non_differentiable(*(o for o, needed in zip(out, ctx.needs_input_grad[7:]) if not needed))
+        return tuple(out)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        positions, frequencies = ctx.saved_tensors
+        offsets, interleaved, mscale, inverse = ctx.settings
+        at = [i for i, g in enumerate(grads) if g is not None and ctx.needs_input_grad[7 + i]]
+        result = [None] * len(grads)
+        if at:  # the positions have passed the forward's check
+            turned = Rotation.apply(positions, frequencies, [offsets[i] for i in at], [interleaved[i] for i in at],
+                                    mscale, not inverse, False, *(grads[i].contiguous() for i in at))
+            for i, g in zip(at, turned):
+                result[i] = g
+        return (None,) * 7 + tuple(result)
