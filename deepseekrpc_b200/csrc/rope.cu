@@ -21,6 +21,7 @@
 // per tensor and several tokens a CTA were all slower (129 to 186 us of the first).
 #include "common.cuh"
 #include "host_common.h"
+#include "strided.h"
 
 namespace dsr {
 namespace {
@@ -230,6 +231,26 @@ extern "C" int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int
     DSR_REQUIRE(items < (int64_t(1) << 30), "rope: too many columns for one call");
     t.items = int(own);
   }
+  // CTAs of different tokens, and threads of different tensors, run in no order: what one
+  // writes no other may read or write.  In place only the rotated columns are touched.
+  StridedBytes in[kRopeMaxTensors], out[kRopeMaxTensors];
+  for (int n = 0; n < count; ++n) {
+    const dsr_rope_tensor& s = tensors[n];
+    const int size = s.dtype == DSR_F32 ? 4 : 2;
+    const bool in_place = s.x == s.out;
+    const int64_t first = in_place ? int64_t(s.offset) * size : 0, width = in_place ? 2 * pairs : s.width;
+    out[n] = StridedBytes(static_cast<const uint8_t*>(s.out) + first, width, tokens, s.out_token, s.heads, s.out_head,
+                          size);
+    in[n] = in_place ? out[n] : StridedBytes(s.x, width, tokens, s.x_token, s.heads, s.x_head, size);
+    DSR_REQUIRE(!out[n].folds(), "rope: rows of an output overlap");
+  }
+  for (int n = 0; n < count; ++n)
+    for (int m = 0; m < count; ++m) {
+      if (m != n || tensors[n].x != tensors[n].out)
+        DSR_REQUIRE(!StridedBytes::meet(out[n], in[m]), "rope: tensor %d's output overlaps tensor %d's input", n, m);
+      if (m > n)
+        DSR_REQUIRE(!StridedBytes::meet(out[n], out[m]), "rope: tensor %d's output overlaps tensor %d's output", n, m);
+    }
   a.positions = positions;
   a.frequencies = frequencies;
   a.err = err;

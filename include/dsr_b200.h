@@ -462,9 +462,11 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
                    int32_t* err, int64_t batch, void* stream);
 
 /* One tensor of dsr_rope: x and out [tokens, heads, width] of type dtype with unit
- * column stride and token and head strides in elements (any sign; rows of one
- * tensor must not overlap).  out == x rotates in place (equal strides), otherwise
- * x and out must not overlap; nor may an output and another tensor of the call. */
+ * column stride and token and head strides in elements (any sign).  out == x
+ * rotates in place (equal strides; only the rotated columns count as written).
+ * Rows of an output that overlap, and an output that overlaps its own or another
+ * tensor's x or another out, are refused: views of one buffer may lie between one
+ * another, as the slabs of one projection do, but share no element. */
 typedef struct {
   const void* x;
   void* out;
