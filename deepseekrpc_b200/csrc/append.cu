@@ -44,6 +44,7 @@ __global__ void __launch_bounds__(128) append_kernel(
   const int i = blockIdx.x;
   pdl_wait();
   const int32_t s = seq[i], p = positions[i];
+  if (s == -1 && p == -1) return;  // padding: no row
   int64_t kv_row, ix_row;
   append_rows(kv, ix, nseq, s, p, kv_row, ix_row);
   const bool in = kv_row >= 0 && ix_row >= 0;

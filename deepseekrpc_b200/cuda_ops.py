@@ -96,7 +96,9 @@ def decode_step(idx_q, idx_w, index_pool, query, kv_pool, block_table, visible, 
 
 def append_kv_index(kv_pool, index_pool, generations, block_table, seq, positions, expected, kv_values,
                     index_values, swa=None):
-    """Generation-checked append; a refused row raises ValidationError and was not written."""
+    """Generation-checked append; a refused row raises ValidationError and was not written.
+
+    Rows whose seq and position are both -1 (paged_plan's padding) are skipped."""
     _status(extension().append_kv_index(kv_pool, index_pool, generations, block_table, seq, positions,
                                         expected, kv_values, index_values, swa))
 

@@ -268,7 +268,8 @@ int dsr_lse_combine_packed(const float* packed, int64_t world, const float* sink
  * DeviceRowPool.write calls of publish_source plus the SWA ring write
  * (attention_state.py:183-192, cache_pool.py:289-313, vllm_attention.py:261).
  * block_table i32[table_rows,table_stride]; seq i32[n] sequence of each new
- * row (< table_rows); positions i32[n] its logical position;
+ * row (< table_rows); positions i32[n] its logical position; both -1: padding (as
+ * dsr_paged_plan marks it), skipped without a status;
  * generations i64[pool_blocks*64] per physical row; expected i64[n].
  * A row is written only if its physical row is in bounds, not repeated by an
  * earlier row of the batch, generations[row]==expected[i] and both value rows
@@ -373,7 +374,7 @@ int dsr_decode_step_ring(const float* idx_q, const float* idx_w, int64_t idx_hea
  * rows are in bounds, neither repeats an earlier row's target in its pool,
  * kv_generations[kv row] == kv_expected[i], index_generations[index row] ==
  * index_expected[i] and both value rows are finite; then both generations are
- * bumped to expected + 1.  Otherwise status 3 (bounds / repeat / stale) or 2
+ * bumped to expected + 1.  seq and position both -1: padding, skipped.  Otherwise status 3 (bounds / repeat / stale) or 2
  * (non-finite) and nothing of that row is written.  Replaces publish_source's
  * two DeviceRowPool.write calls (attention_state.py:183-192); the SWA windows
  * pool stays the caller's (DeviceRowPool.write over dsr_pool_write).

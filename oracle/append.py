@@ -26,6 +26,9 @@ only when its scatter status is 0 (with status 0 both agree).
 Status: the device reports the first failing row's code in an unspecified order;
 `append_kv_index` returns the set of codes raised, and a batch whose rows fail
 with one code only has a definite status.
+
+A row whose sequence and position are both -1 is padding of a batch of fixed size
+(nothing the reference has): it is skipped without a code.
 """
 from __future__ import annotations
 
@@ -85,6 +88,8 @@ def append_kv_index(kv_pool, index_pool, generations, rows, seq, positions, expe
     ring_of = (list(np.asarray(swa_rows).tolist()) if swa_rows is not None
                else [p % SWA_ROWS for p in positions])
     for i, row in enumerate(rows):
+        if seq[i] == positions[i] == -1:
+            continue
         # scatter_kernel's checks (operations.cu:149-153)
         valid = row >= 0 and row not in rows[:i]
         if valid and swa is not None:
