@@ -93,7 +93,7 @@ struct TreeArgs {
   void* out;
   float* lse;  // nullable
   int32_t* err;
-  int32_t* slot_start;  // [batch + 1] first partial slot of each request; the segment length
+  int32_t* slot_start;  // [batch + 1] first partial slot of each request; the segment length (negative: a request was refused)
   float* part_o;        // [slots][N / 4][512][4]: value columns of four rows side by side
   float* part_m;        // [slots][N]
   float* part_l;
@@ -416,9 +416,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   walk.per = per;
   int64_t units = 0;
   int32_t groups = 0;
+  bool fine = true;  // no request is refused: the node sums rise
   for (int b = r0; b < r1; ++b) {
     const TreeSeq s = tree_seq<N>(a, b);
     if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
+    fine = fine && s.ok;
     units += int64_t(s.groups) * s.tiles;
     groups += s.groups;
     own_seq = s;
@@ -427,10 +429,11 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   units = (int64_t(__reduce_add_sync(~0u, uint32_t(units >> 24))) << 24) +
           __reduce_add_sync(~0u, uint32_t(units) & 0xffffffu);
   groups = __reduce_add_sync(~0u, groups);
+  fine = __all_sync(~0u, fine);
   tc_fence_before();
   if (!small) {
     if (lane == 0) warp_units[warp] = units, warp_groups[warp] = groups;
-    __syncthreads();
+    fine = __syncthreads_and(fine);
     units = groups = 0;
     for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
   }
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       a.slot_start[b] = slots_before;
       if (s.tiles > length) slots_before += s.groups * tree_segments(s, length);
     }
-    if (tid == 0) a.slot_start[a.batch] = length;
+    if (tid == 0) a.slot_start[a.batch] = fine ? length : -length;
   }
   __syncthreads();
   tc_fence_after();
@@ -963,6 +966,7 @@ template <int N>
 __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid_constant__ TreeArgs a) {
   __shared__ float weight[4][kTreeMaxParts];
   __shared__ float inverse[4];
+  __shared__ int owner;
   const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
   const int tid = threadIdx.x, d = blockIdx.y * kJoinThreads + tid;
@@ -975,10 +979,25 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
     lo += last;
     n = min(stride, n - last);
   }
-  const TreeSeq s = tree_seq<N>(a, lo);
+  TreeSeq s = tree_seq<N>(a, lo);
   pdl_wait();  // before any CTA leaves: the join must not end ahead of the attention
-  if (node < s.node0 || node >= s.node0 + s.nodes) return;
-  const int parts = tree_segments(s, __ldcg(a.slot_start + a.batch));
+  const int32_t length = __ldcg(a.slot_start + a.batch);
+  if (node < s.node0 || node >= s.node0 + s.nodes) {
+    // a padding row.  Where a request was refused the sums may be in disorder and the search
+    // may have missed the request that has the row: every one is asked
+    if (length > 0) return;
+    if (tid == 0) owner = -1;
+    __syncthreads();
+    for (int b = tid; b < a.batch; b += kJoinThreads) {
+      const TreeSeq other = tree_seq<N>(a, b);
+      if (node >= other.node0 && node < other.node0 + other.nodes) atomicMax(&owner, b);
+    }
+    __syncthreads();
+    lo = owner;
+    if (lo < 0) return;
+    s = tree_seq<N>(a, lo);
+  }
+  const int parts = tree_segments(s, abs(length));
   if (parts <= 1) return;  // written by its job
   const int in = int(row - int64_t(s.node0) * a.heads), group = in / N, r = in % N;
   const int64_t first = int64_t(__ldcg(a.slot_start + lo)) + group;
