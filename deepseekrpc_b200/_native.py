@@ -27,7 +27,7 @@ class RopeTensor(ctypes.Structure):
                 ("reserved", ctypes.c_int32)]
 
 
-DSR_BF16, DSR_F32 = 0, 1
+DSR_BF16, DSR_F32, DSR_ZERO_UNUSED = 0, 1, 256
 
 # name -> (restype, argtypes); mirrors include/dsr_b200.h exactly
 SIGNATURES = {

@@ -631,14 +631,17 @@ std::vector<at::Tensor> ds_tree_mla_decode(at::Tensor q, at::Tensor kv_pool, at:
   } else {
     result = fresh({nodes, heads, DSR_V_DIM}, q.scalar_type(), q);
   }
-  at::Tensor lse = return_lse ? fresh({nodes, heads}, at::kFloat, q) : at::Tensor();
+  // what this call allocates has no row that nobody wrote; the caller's rows stay
+  const int unused = out ? 0 : DSR_ZERO_UNUSED;
+  at::Tensor lse;
+  if (return_lse) lse = out ? at::full({nodes, heads}, -INFINITY, q.options().dtype(at::kFloat)) : fresh({nodes, heads}, at::kFloat, q);
   const size_t ws_bytes = dsr_tree_mla_workspace_bytes(batch, heads, max_nodes);
   auto ws = fresh({int64_t(ws_bytes)}, at::kByte, q);
   ok(dsr_tree_mla_decode(q.data_ptr(), dtype, bf16(kv_pool), kv_pool.size(0) / DSR_BLOCK_TOKENS,
                          block_table.data_ptr<int32_t>(), block_table.size(1), context.data_ptr<int32_t>(),
                          cu_nodes.data_ptr<int32_t>(), tree_mask.data_ptr<int64_t>(), max_nodes,
                          sink ? sink->data_ptr<float>() : nullptr, static_cast<float>(scale), result.data_ptr(),
-                         element_type(result, "tree_mla_decode"), return_lse ? lse.data_ptr<float>() : nullptr,
+                         element_type(result, "tree_mla_decode") | unused, return_lse ? lse.data_ptr<float>() : nullptr,
                          ws.data_ptr(), ws_bytes, error.data_ptr<int32_t>(), batch, nodes, heads, current_stream()));
   if (return_lse) return {result, error, lse};
   return {result, error};

@@ -83,6 +83,7 @@ struct TreeLayout {
 struct TreeArgs {
   const void* q;
   bool q_wide, out_wide;  // fp32 (else bf16)
+  bool zero_unused;       // rows of no request: zeros (else left)
   const int32_t* table;
   int64_t stride, pool_rows;
   const int32_t* context;
@@ -985,16 +986,27 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
   if (node < s.node0 || node >= s.node0 + s.nodes) {
     // a padding row.  Where a request was refused the sums may be in disorder and the search
     // may have missed the request that has the row: every one is asked
-    if (length > 0) return;
-    if (tid == 0) owner = -1;
-    __syncthreads();
-    for (int b = tid; b < a.batch; b += kJoinThreads) {
-      const TreeSeq other = tree_seq<N>(a, b);
-      if (node >= other.node0 && node < other.node0 + other.nodes) atomicMax(&owner, b);
+    lo = -1;
+    if (length < 0) {
+      if (tid == 0) owner = -1;
+      __syncthreads();
+      for (int b = tid; b < a.batch; b += kJoinThreads) {
+        const TreeSeq other = tree_seq<N>(a, b);
+        if (node >= other.node0 && node < other.node0 + other.nodes) atomicMax(&owner, b);
+      }
+      __syncthreads();
+      lo = owner;
     }
-    __syncthreads();
-    lo = owner;
-    if (lo < 0) return;
+    if (lo < 0) {
+      if (!a.zero_unused) return;
+      for (int y = 0; y < 4; ++y) {
+        const int64_t at = (row + y) * kTreeDv + d;
+        if (a.out_wide) static_cast<float*>(a.out)[at] = 0.f;
+        else static_cast<uint16_t*>(a.out)[at] = 0;
+      }
+      if (a.lse != nullptr && blockIdx.y == 0 && tid < 4) a.lse[row + tid] = -CUDART_INF_F;
+      return;
+    }
     s = tree_seq<N>(a, lo);
   }
   const int parts = tree_segments(s, abs(length));
@@ -1122,6 +1134,8 @@ extern "C" int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* k
   if (rc != DSR_OK) return rc;
   DSR_REQUIRE(q && kv_pool && context && cu_nodes && tree_mask && out && workspace && err,
               "tree_mla_decode: null pointer");
+  const bool zero_unused = (out_dtype & DSR_ZERO_UNUSED) != 0;
+  out_dtype &= ~DSR_ZERO_UNUSED;
   DSR_REQUIRE((q_dtype == DSR_BF16 || q_dtype == DSR_F32) && (out_dtype == DSR_BF16 || out_dtype == DSR_F32),
               "tree_mla_decode: unknown element type");
   DSR_REQUIRE(heads == 16 || heads == 32 || heads == 64 || heads == 128,
@@ -1141,6 +1155,7 @@ extern "C" int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* k
   a.q = q;
   a.q_wide = q_dtype == DSR_F32;
   a.out_wide = out_dtype == DSR_F32;
+  a.zero_unused = zero_unused;
   a.table = block_table;
   a.stride = table_stride;
   a.pool_rows = pa.rows;

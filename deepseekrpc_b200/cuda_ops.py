@@ -143,7 +143,10 @@ def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float
 
 def tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes: int, *, scale: float,
                     sink=None, out=None, return_lse: bool = False):
-    """Attention of drafted tokens over their request's cached rows and their own branch."""
+    """Attention of drafted tokens over their request's cached rows and their own branch.
+
+    Rows at or past cu_nodes[-1] (padding) are zeros, their lse -inf; those of `out` stay.
+    """
     if not math.isfinite(scale) or scale <= 0:
         raise ValidationError("invalid attention scale")
     result = extension().tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes, scale,

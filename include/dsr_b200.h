@@ -435,6 +435,9 @@ int dsr_pool_restore(uint16_t* data, int64_t* generations, int64_t slots, int64_
 /* Element types of the entry points that take more than one. */
 #define DSR_BF16 0
 #define DSR_F32 1
+/* Added to out_dtype of dsr_tree_mla_decode: output rows of no request become
+ * zeros and their lse -inf, instead of staying as they are. */
+#define DSR_ZERO_UNUSED 256
 
 /* Gives every request of a paged batch the pool blocks that its length needs and
  * maps its new tokens to pool rows.  lengths i32[batch] tokens already cached,
@@ -502,8 +505,8 @@ int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int32_t* posit
  * f32[nodes,heads] (nullable): the logarithm of the denominator (-inf for zero).
  * q is contracted as BF16 and the weights e^s are rounded to BF16 before the value
  * product; sums and statistics are FP32.  Output rows at or past cu_nodes[batch]
- * are not written.  Status 1: a context or node range that is negative, larger
- * than max_nodes, `nodes` or the table (that request's rows are not written), or a
+ * are not written, or zeros (DSR_ZERO_UNUSED).  Status 1: a context or node range that is negative, larger
+ * than max_nodes, `nodes` or the table (that request's rows count as unused), or a
  * block id outside the pool (its keys count as zeros); status 2: a NaN or +infinite
  * score (one of -infinity is not seen), an infinite or NaN sink or output.  Cached rows that no node sees may hold anything.
  * Scratch: dsr_tree_mla_workspace_bytes() on the current device, 256-byte
