@@ -129,22 +129,35 @@ __device__ __forceinline__ int32_t tree_segments(const TreeSeq& s, int32_t lengt
 }
 
 // ---- the jobs of a call
+// Requests of a search at most.  It reads every request several times, and many requests
+// share evenly without it.  Its time over the even share's, mean (and range) over contexts of
+// 500 to 32000 rows and 1 to 4 nodes of 16 to 128 heads: 96 requests 0.93 (0.76 to 1.15), 128
+// 0.94 (0.79 to 1.06), 160 0.96 (0.80 to 1.03), 200 1.00 (0.92 to 1.10), 300 1.02 (0.86 to 1.10)
+constexpr int kTreeSearchBatch = 160;
 constexpr int kTreeSlotsPerCta = 4;  // partial slots, per CTA of the grid
 // A round's cost beside its tiles, in tiles: first copies, output, its part of the join.
 constexpr float kTreeJobCost = 8.f;
 
 // A segment length for `waves` jobs per CTA at most: starts at the even share and
 // grows until the jobs (requests' tiles rounded up to whole segments) and the partial
-// slots fit.  One warp, lane b with request b; estimates the time in tiles (infinite when
-// none was found).
-__device__ __forceinline__ float tree_length(const TreeArgs& a, const TreeSeq& s, int64_t units, int waves,
+// slots fit.  One warp (`own`: of up to 32 requests, lane b's is request b); estimates the
+// time in tiles (infinite when none was found).
+template <int N>
+__device__ __forceinline__ float tree_length(const TreeArgs& a, const TreeSeq& own, int64_t units, int waves,
                                              int32_t& length) {
   const int64_t room = int64_t(waves) * a.ctas;
   float len = fmaxf(ceilf(float(units) / float(room)), 1.f);
   for (int tries = 0; tries < 8; ++tries) {
     length = int32_t(len);
-    const int32_t n = s.groups * tree_segments(s, length);
-    const int32_t jobs = __reduce_add_sync(~0u, n), slots = __reduce_add_sync(~0u, s.tiles > length ? n : 0);
+    int32_t jobs = 0, slots = 0;
+    for (int b = threadIdx.x & 31; b < a.batch; b += 32) {
+      const TreeSeq s = a.batch <= 32 ? own : tree_seq<N>(a, b);
+      const int32_t n = s.groups * tree_segments(s, length);
+      jobs += n;
+      if (s.tiles > length) slots += n;
+    }
+    jobs = __reduce_add_sync(~0u, jobs);
+    slots = __reduce_add_sync(~0u, slots);
     if (jobs <= room && slots <= int64_t(kTreeSlotsPerCta) * a.ctas) {
       // one round lasts as long as its longest job; several come near the mean
       const float mean = float(units) / float(a.ctas);
@@ -441,10 +454,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   // ---- the segment length: one tile when that fills no more than the grid, else the
   // best of four wave counts
   int32_t length = units <= a.ctas ? 1 : 0;
-  if (length == 0 && small) {
+  if (length == 0 && a.batch <= kTreeSearchBatch) {
     if (warp < 4) {
       int32_t len = 1;
-      const float e = tree_length(a, own_seq, units, (groups + a.ctas - 1) / a.ctas + warp, len);
+      const float e = tree_length<N>(a, own_seq, units, (groups + a.ctas - 1) / a.ctas + warp, len);
       if (lane == 0) estimate[warp] = e, estimated[warp] = len;
     }
     __syncthreads();
@@ -453,8 +466,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       if (estimate[w] < best) best = estimate[w], length = estimated[w];
   }
   // or the even share of two jobs per CTA, whose partials always fit: a cut request's
-  // groups have at most 2 U / length of them.  More than 32 requests take that (the search
-  // reads every request several times: 4 us of a CTA for 300), as do those without a find
+  // groups have at most 2 U / length of them.  Batches beyond the search's take that, as do
+  // those without a find
   if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
   // ---- jobs and partial slots before each lane's request, or each thread's chunk
   int32_t jobs = 0, slots = 0;
