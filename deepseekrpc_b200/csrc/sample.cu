@@ -26,9 +26,12 @@
 // ranks, 11 bits a level.
 //
 // Bound by the passes over the row in shared memory, and for a few rows by the 7 to 14
-// barriers of a cluster (some 0.6 us each).  Measured, FP32, T = 0.8: 1 row of
-// 128000, top_k 50 and top_p 0.95, 16.4 us; 148 rows 80 us; 511 rows 244 us = 1.1 TB/s; 148
-// rows by top_p alone, which forms every weight, 188 us.
+// barriers of a cluster (some 0.6 us each).  By mass every entry's weight is formed at least
+// twice, ten 64-bit operations each, and costs four shared atomics; 48 rows so (76 to 84 us)
+// are 384 CTAs on 296 places: a second wave, one third full, is near half of that.
+// Measured, FP32, T = 0.8: 1 row of 128000, top_k 50 and top_p 0.95, 16.4 us; 148 rows 80
+// us; 511 rows 244 us = 1.1 TB/s; 148 rows by top_p alone 188 us.  T = 0, 1, 48 and 511
+// (BF16) rows of 128K: 12.3, 24.6 and 79.9 us.
 #include <cooperative_groups.h>
 #include <math_constants.h>
 

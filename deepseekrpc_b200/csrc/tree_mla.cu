@@ -14,15 +14,17 @@
 // then MN-major) and O^T of 64 rows takes half of the tensor memory.
 //
 // A job is one group over a segment of consecutive tiles.  Every CTA finds the same
-// segment length (tree_plan) from the lengths on the device; a request's tiles are
-// cut into equal segments, and the jobs, in the order (request, segment, group), the
-// longest requests' segments first, are dealt to the CTAs to and fro: the groups of a
-// segment run side by side and share its rows in L2, and a CTA with a long job gets a
-// short one next (for 32 ragged requests the busiest CTA has 4 to 6% more than its
-// share in two rounds; dealt in the order of requests it had 14% in four).  (Runs of units in the order request, group, tile balance better, but
-// read the rows once per group: 1213 us against 1010 us for 32 requests of 3 to 6
-// groups.)  A group of several segments leaves partials (m, l, unnormalised O in
-// FP32) that tree_combine_kernel joins.
+// segment length from the lengths on the device (tree_length, a search; more than
+// kTreeSearchBatch requests take an even share); a request's tiles are cut into equal
+// segments, and the jobs, in the order (request, segment, group), are dealt to the CTAs
+// to and fro: the groups of a segment run side by side and share its rows in L2, and a
+// CTA with a long job gets a short one next.  Up to 32 requests go with the longest
+// segments first (ragged ones: the busiest CTA has 4 to 6% more than its share in two
+// rounds; dealt in the order of requests it had 14% in four), more in their own order
+// (counted for ragged requests of 8192 to 65536 rows: 20% for 33, 37% for 128).  (Runs of
+// units in the order request, group, tile balance better, but read the rows once per
+// group: 1213 us against 1010 us for 32 requests of 3 to 6 groups.)  A group of several
+// segments leaves partials (m, l, unnormalised O in FP32) that tree_combine_kernel joins.
 //
 //   warps 0..7  (FP32 query -> shared memory,) softmax over the tile's keys (running
 //               maximum; O is rescaled only when a maximum grows by more than 2^8),
@@ -34,13 +36,15 @@
 //               ring of block pairs that the O MMA frees pair by pair, block 8 (the
 //               rotary columns) in a buffer that P^T takes over once S^T is done
 //
-// Bound by shared memory at 64 rows: an MMA of 128 x 64 x 16 takes 48 cycles, not 32, to read
-// its operands, which is two thirds of the tensor cores' rate at best.  Measured: 8 nodes of
-// 64 heads over 131072 rows 186 to 192 us (770 TFLOP/s, 47% of a measured BF16 GEMM); 32
-// requests of 6 nodes over up to 65536 rows 0.93 to 1.03 ms (0.72 to 0.80 PFLOP/s).  Bound by
-// memory at 16 rows: 32 requests of one node and 16 heads over 65536 rows 378 us, 6.4 TB/s,
-// 97% of a plain copy.  Bound by latency for little: one node over 4096 rows 17.5 us in two
-// launches.
+// Bound at 64 rows by two things of about equal weight.  An MMA of 128 x 64 x 16 takes 48
+// cycles, not 32, to read its operands from shared memory: the 68 of a tile 3264 cycles.  And
+// a tile takes nearly 6000: there is one S^T, and the ring holds one tile, so that the MMAs
+// wait through every softmax.  Measured: 8 nodes of 64 heads over 131072 rows 186 to 194 us
+// (750 to 785 TFLOP/s, 46 to 48% of a measured BF16 GEMM), FP32 queries cost no more; 32
+// requests of 6 nodes over up to 65536 rows 0.91 to 1.03 ms (0.72 to 0.82 PFLOP/s), 33 of them
+// 1.11 ms, 64 2.07, 128 5.06.  Bound by memory at 16 rows: 32 requests of one node and 16 heads
+// over 65536 rows 378 to 406 us from box to box, 6.0 to 6.4 TB/s, 91 to 97% of a plain copy.
+// Bound by latency for little: one node over 4096 rows 16.4 to 18.4 us in two launches.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -536,7 +540,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
       const int64_t qrow = int64_t(s.node0) * a.heads + row0;
       if (a.q_wide) {
-        // ---- FP32 query rows -> bf16, K-major, 128-byte swizzle (BF16 ones come by TMA)
+        // ---- FP32 query rows -> bf16, K-major, 128-byte swizzle (BF16 ones come by TMA).  As
+        // in the sparse attention: the keys are BF16, and one product takes one type.  It moves
+        // the output by 1.8e-3 to 2.7e-3 of its norm (60000 to 500 rows); FP32 in and out saves
+        // the caller a cast, no more
         constexpr int kVec = N * (kTreeD / 8), kBatch = 3;
         for (int i0 = tid; i0 < kVec; i0 += kTreeSoftmax * kBatch) {
           uint4 v[kBatch];
@@ -634,7 +641,10 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             }
           }
         }
-        // ---- weights against the running maxima as they stand, their sums, P^T
+        // ---- weights against the running maxima as they stand, their sums, P^T.  The sums are
+        // of the weights as formed; for the product with V they are rounded to BF16, the type
+        // the tensor cores take beside V's (by 2^-8 of a weight at most: measured over 500 to
+        // 60000 rows 4e-4 to 9e-4 of an output's norm, where an output in BF16 rounds by 1.7e-3)
         float sum[C][2];
         bool fits = ok && i > 0;
         auto weigh = [&] {

@@ -108,7 +108,8 @@ def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, to
     """Blocks for every request's new tokens and the map of those tokens to pool rows.
 
     Updates held, block_table, free_ring and ring_state in place; returns
-    (seq, positions, slots, cu_tokens, visible).  A refused batch changes nothing.
+    (seq, positions, slots, cu_tokens, visible).  A batch whose counts are refused changes
+    nothing; one that met a block id outside the pool raises too, and has -1 in its place.
     """
     *value, status = extension().paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens)
     _status(status)

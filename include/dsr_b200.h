@@ -453,7 +453,8 @@ int dsr_pool_restore(uint16_t* data, int64_t* generations, int64_t slots, int64_
  * next call on.  All four are updated in place.
  * Outputs: seq, positions, slots i32[tokens] of the new tokens, request by
  * request (slots = block*64 + position%64), -1 behind the last; cu_tokens
- * i32[batch+1] their exclusive sums; visible i32[batch] = lengths + new_tokens.
+ * i32[batch+1] their exclusive sums; visible i32[batch] = lengths + new_tokens
+ * (no output may be one of the inputs).
  * Refused with status 1, the four tables unchanged, no token mapped (-1, sums 0)
  * and visible = lengths: counts out of range, more new tokens than `tokens`, too
  * few free blocks, a ring state out of range.  A block id outside the pool met on
@@ -504,11 +505,14 @@ int dsr_rope(const dsr_rope_tensor* tensors, int64_t count, const int32_t* posit
  * sink (NULL) that term is absent.  A row that sees nothing gives zeros.  lse
  * f32[nodes,heads] (nullable): the logarithm of the denominator (-inf for zero).
  * q is contracted as BF16 and the weights e^s are rounded to BF16 before the value
- * product; sums and statistics are FP32.  Output rows at or past cu_nodes[batch]
+ * product; sums and statistics are FP32.  (Of an output's norm the weights'
+ * rounding is 4e-4 to 9e-4, an FP32 q's 1.8e-3 to 2.7e-3.)  Output rows at or past cu_nodes[batch]
  * are not written, or zeros (DSR_ZERO_UNUSED).  Status 1: a context or node range that is negative, larger
  * than max_nodes, `nodes` or the table (that request's rows count as unused), or a
  * block id outside the pool (its keys count as zeros); status 2: a NaN or +infinite
- * score (one of -infinity is not seen), an infinite or NaN sink or output.  Cached rows that no node sees may hold anything.
+ * score (one of -infinity is not seen), an infinite or NaN sink or output.
+ * Cached rows that no node sees may hold anything.  Where the sums of cu_nodes
+ * give a row to two requests, either may write it.  batch <= 65535.
  * Scratch: dsr_tree_mla_workspace_bytes() on the current device, 256-byte
  * aligned, need not be cleared; calls sharing it must not overlap. */
 size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes);
@@ -532,7 +536,7 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
  * temperature >= 0, top_k >= 0, top_p, min_p in [0, 1], uniform in [0, 1); others
  * give status 1.  -inf logits are never drawn; a row of them alone gives token -1
  * and chance 0; NaN or +inf gives status 2; a row with
- * a status has token -1.  vocab <= 262144. */
+ * a status has token -1.  vocab <= 262144, rows <= 65535. */
 int dsr_sample(const void* logits, int dtype, int64_t row_stride, int64_t vocab,
                const float* temperature, const int32_t* top_k, const float* top_p,
                const float* min_p, const float* uniform, int32_t* tokens, float* chances,
