@@ -17,11 +17,11 @@
 // heads, 64 of 576 columns rotated in place, 8192 tokens: 41 us; off the 16-byte grid,
 // column by column, 90).  Bound by instructions as much as by memory: 173 warp
 // instructions for 32 items of one or two pieces, mostly the way from an item to its
-// tensor, head and column, which every token walks anew; issue slots are 62% busy, DRAM 51%.  Measured: 8192 tokens
-// of four tensors in BF16, 560 MB, 127 us = 4.4 TB/s, 67% of a plain copy, in FP32, 1.1 GB,
-// 207 us = 5.3 TB/s; 999 tokens, 44 MB, 14.5 us = 3.0 TB/s; 1 token 5.8 us, a launch.  Two
-// to four pieces a thread ahead, streaming hints, loops per tensor and several tokens a CTA
-// were all slower (129 to 186 us of the first).
+// tensor, head and column, which every token walks anew; issue slots are 62% busy, DRAM
+// 51%.  Measured: 8192 tokens of four tensors in BF16, 560 MB, 127 us = 4.4 TB/s, 67% of a
+// plain copy, in FP32, 1.1 GB, 207 us = 5.3 TB/s; 999 tokens, 44 MB, 14.5 us = 3.0 TB/s; 1
+// token 5.8 us, a launch.  Two to four pieces a thread ahead, streaming hints, loops per
+// tensor and several tokens a CTA were all slower (129 to 186 us of the first).
 #include "common.cuh"
 #include "host_common.h"
 #include "strided.h"
