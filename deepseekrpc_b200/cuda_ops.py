@@ -135,11 +135,11 @@ def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float
             from .rotary import Rotation
             return list(Rotation.apply(positions, frequencies, list(offsets), list(interleaved), mscale, inverse,
                                        True, *tensors))
-    if out is None:
-        out = [t.detach().clone() for t in tensors]  # padding rows keep their values
-    _status(extension().rope(tensors, list(out), positions, frequencies, list(offsets), list(interleaved),
-                             mscale=mscale, inverse=inverse))
-    return list(out)
+    # new tensors are copies, so that padding rows keep their values
+    out = [t.detach().clone() for t in tensors] if out is None else list(out)
+    _status(extension().rope(tensors, out, positions, frequencies, list(offsets), list(interleaved), mscale=mscale,
+                             inverse=inverse))
+    return out
 
 
 def tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes: int, *, scale: float,
