@@ -90,6 +90,12 @@ SIGNATURES = {
                                          _P, _P, _P, c_int64, _P]),
     "dsr_paged_plan": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64,
                                _P]),
+    "dsr_paged_fork": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P]),
+    "dsr_paged_release_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "dsr_paged_release": (c_int, [_P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_size_t, _P, c_int64, _P]),
+    "dsr_paged_compact_workspace_bytes": (c_size_t, [c_int64]),
+    "dsr_paged_compact": (c_int, [_P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_size_t, _P, c_int64, _P]),
+    "dsr_paged_copy": (c_int, [_P, _P, c_int64, _P, c_int64, c_int64, _P, _P, c_int64, _P, _P]),
     "dsr_rope": (c_int, [POINTER(RopeTensor), c_int64, _P, _P, c_int64, c_float, c_int, _P, c_int64, _P]),
     "dsr_tree_mla_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "dsr_tree_mla_decode": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, c_float, _P, c_int,

@@ -10,6 +10,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <utility>
 #include <vector>
 
 #include "dsr_b200.h"
@@ -550,6 +552,119 @@ std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens,
   return {seq, positions, slots, cu, visible, error};
 }
 
+// ---- blocks that several requests map
+// The five tables of a paged cache: their shapes, and what they are called with.
+struct PageTables {
+  at::Tensor held, table, ring, state, shares;
+  int64_t batch, stride, blocks;
+  PageTables(const at::Tensor& held_, const at::Tensor& table_, const at::Tensor& ring_, const at::Tensor& state_,
+             const at::Tensor& shares_)
+      : held(held_), table(table_), ring(ring_), state(state_), shares(shares_) {
+    const char* shapes =
+        "held [batch], block_table [batch, blocks], free_ring [pool blocks], ring_state [4] and shares [pool blocks] "
+        "expected";
+    check_vector(held, at::kInt, held.numel(), held, shapes);
+    check(table, at::kInt, held);
+    batch = held.numel();
+    TORCH_CHECK(table.dim() == 2 && table.size(0) == batch, shapes);
+    check_vector(ring, at::kInt, ring.numel(), held, shapes);
+    check_vector(state, at::kInt, 4, held, shapes);
+    check_vector(shares, at::kInt, ring.numel(), held, shapes);
+    stride = table.size(1), blocks = ring.numel();
+  }
+};
+
+// moves [n, 4] and count [1], of one allocation.
+std::pair<at::Tensor, at::Tensor> move_list(int64_t n, const at::Tensor& anchor) {
+  const at::Tensor store = fresh({4 * n + 4}, at::kInt, anchor);
+  const auto part = [&](int64_t offset, at::IntArrayRef sizes) {
+    auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(store.storage()), store.key_set(), store.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(offset);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  };
+  return {part(4, {n, 4}), part(0, {1})};
+}
+
+std::vector<at::Tensor> ds_paged_fork(at::Tensor parent, at::Tensor lengths, at::Tensor held, at::Tensor block_table,
+                                      at::Tensor free_ring, at::Tensor ring_state, at::Tensor shares,
+                                      c10::optional<at::Tensor> status) {
+  PageTables t(held, block_table, free_ring, ring_state, shares);
+  check_vector(parent, at::kInt, t.batch, held, "paged_fork: parent [batch] expected");
+  check_vector(lengths, at::kInt, t.batch, held, "paged_fork: lengths [batch] expected");
+  const c10::cuda::CUDAGuard guard(held.device());
+  auto error = status_or(status, held);
+  auto [moves, count] = move_list(t.batch, held);
+  ok(dsr_paged_fork(parent.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
+                    block_table.data_ptr<int32_t>(), t.stride, free_ring.data_ptr<int32_t>(),
+                    ring_state.data_ptr<int32_t>(), shares.data_ptr<int32_t>(), t.blocks, moves.data_ptr<int32_t>(),
+                    count.data_ptr<int32_t>(), error.data_ptr<int32_t>(), t.batch, current_stream()));
+  return {moves, count, error};
+}
+
+std::vector<at::Tensor> ds_paged_release(at::Tensor lengths, at::Tensor held, at::Tensor block_table,
+                                         at::Tensor free_ring, at::Tensor ring_state, at::Tensor shares,
+                                         c10::optional<at::Tensor> status) {
+  PageTables t(held, block_table, free_ring, ring_state, shares);
+  check_vector(lengths, at::kInt, t.batch, held, "paged_release: lengths [batch] expected");
+  const c10::cuda::CUDAGuard guard(held.device());
+  auto error = status_or(status, held);
+  auto [moves, count] = move_list(t.batch, held);
+  const size_t ws_bytes = dsr_paged_release_workspace_bytes(t.batch, t.blocks);
+  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, held);
+  ok(dsr_paged_release(lengths.data_ptr<int32_t>(), held.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(),
+                       t.stride, free_ring.data_ptr<int32_t>(), ring_state.data_ptr<int32_t>(),
+                       shares.data_ptr<int32_t>(), t.blocks, moves.data_ptr<int32_t>(), count.data_ptr<int32_t>(),
+                       ws.data_ptr(), ws_bytes, error.data_ptr<int32_t>(), t.batch, current_stream()));
+  return {moves, count, error};
+}
+
+std::vector<at::Tensor> ds_paged_compact(at::Tensor held, at::Tensor block_table, at::Tensor free_ring,
+                                         at::Tensor ring_state, at::Tensor shares, c10::optional<at::Tensor> status) {
+  PageTables t(held, block_table, free_ring, ring_state, shares);
+  const c10::cuda::CUDAGuard guard(held.device());
+  auto error = status_or(status, held);
+  auto [moves, count] = move_list(std::max<int64_t>(t.blocks / 2, 1), held);
+  const size_t ws_bytes = dsr_paged_compact_workspace_bytes(t.blocks);
+  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, held);
+  ok(dsr_paged_compact(held.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), t.stride,
+                       free_ring.data_ptr<int32_t>(), ring_state.data_ptr<int32_t>(), shares.data_ptr<int32_t>(),
+                       t.blocks, moves.data_ptr<int32_t>(), count.data_ptr<int32_t>(), ws.data_ptr(), ws_bytes,
+                       error.data_ptr<int32_t>(), t.batch, current_stream()));
+  return {moves, count, error};
+}
+
+at::Tensor ds_paged_copy(std::vector<at::Tensor> pools, std::vector<at::Tensor> generations, at::Tensor moves,
+                         at::Tensor count, c10::optional<at::Tensor> status) {
+  check(moves, at::kInt, moves);
+  TORCH_CHECK(moves.dim() == 2 && moves.size(1) == 4, "paged_copy: moves [n, 4] expected");
+  check_vector(count, at::kInt, 1, moves, "paged_copy: count [1] expected");
+  const c10::cuda::CUDAGuard guard(moves.device());
+  auto error = status_or(status, moves);
+  if (pools.empty() && generations.empty()) return error;
+  const int64_t rows = (pools.empty() ? generations : pools)[0].size(0);
+  for (const at::Tensor& p : pools) {
+    check(p, p.scalar_type(), moves);
+    TORCH_CHECK(p.dim() == 2 && p.size(0) == rows, "paged_copy: pools [rows, width] of as many rows expected");
+  }
+  for (const at::Tensor& g : generations)
+    check_vector(g, at::kLong, rows, moves, "paged_copy: generations [rows] of the pools' rows expected");
+  for (const at::Tensor& p : pools) overwrite(p, "paged_copy");
+  constexpr size_t most = 64;  // of a launch
+  for (size_t i = 0; i < std::max(pools.size(), generations.size()); i += most) {
+    std::vector<void*> data;
+    std::vector<int64_t> bytes;
+    std::vector<int64_t*> gens;
+    for (size_t j = i; j < std::min(i + most, pools.size()); ++j)
+      data.push_back(pools[j].data_ptr()), bytes.push_back(pools[j].size(1) * pools[j].element_size());
+    for (size_t j = i; j < std::min(i + most, generations.size()); ++j) gens.push_back(generations[j].data_ptr<int64_t>());
+    ok(dsr_paged_copy(data.data(), bytes.data(), int64_t(data.size()), gens.data(), int64_t(gens.size()), rows,
+                      moves.data_ptr<int32_t>(), count.data_ptr<int32_t>(), moves.size(0), error.data_ptr<int32_t>(),
+                      current_stream()));
+  }
+  return error;
+}
+
 at::Tensor ds_rope(std::vector<at::Tensor> x, std::vector<at::Tensor> out, at::Tensor positions,
                    at::Tensor frequencies, std::vector<int64_t> offsets, std::vector<bool> interleaved, double mscale,
                    bool inverse, c10::optional<at::Tensor> status) {
@@ -706,6 +821,15 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_values"), py::arg("index_values"));
   m.def("paged_plan", &ds_paged_plan, py::arg("lengths"), py::arg("new_tokens"), py::arg("held"),
         py::arg("block_table"), py::arg("free_ring"), py::arg("ring_state"), py::arg("tokens"),
+        py::arg("status") = py::none());
+  m.def("paged_fork", &ds_paged_fork, py::arg("parent"), py::arg("lengths"), py::arg("held"),
+        py::arg("block_table"), py::arg("free_ring"), py::arg("ring_state"), py::arg("shares"),
+        py::arg("status") = py::none());
+  m.def("paged_release", &ds_paged_release, py::arg("lengths"), py::arg("held"), py::arg("block_table"),
+        py::arg("free_ring"), py::arg("ring_state"), py::arg("shares"), py::arg("status") = py::none());
+  m.def("paged_compact", &ds_paged_compact, py::arg("held"), py::arg("block_table"), py::arg("free_ring"),
+        py::arg("ring_state"), py::arg("shares"), py::arg("status") = py::none());
+  m.def("paged_copy", &ds_paged_copy, py::arg("pools"), py::arg("generations"), py::arg("moves"), py::arg("count"),
         py::arg("status") = py::none());
   m.def("rope", &ds_rope, py::arg("x"), py::arg("out"), py::arg("positions"), py::arg("frequencies"),
         py::arg("offsets"), py::arg("interleaved"), py::arg("mscale") = 1.0, py::arg("inverse") = false,

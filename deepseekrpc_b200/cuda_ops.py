@@ -116,6 +116,40 @@ def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, to
     return tuple(value)
 
 
+def paged_fork(parent, lengths, held, block_table, free_ring, ring_state, shares):
+    """Requests with a parent become its first `lengths` tokens, on the parent's whole blocks.
+
+    Updates the five tables in place; returns (moves, count), the rows of partial last
+    blocks that paged_copy has to copy in every pool.  A refused batch changes nothing.
+    """
+    *value, status = extension().paged_fork(parent, lengths, held, block_table, free_ring, ring_state, shares)
+    _status(status)
+    return tuple(value)
+
+
+def paged_release(lengths, held, block_table, free_ring, ring_state, shares):
+    """Cuts every request to `lengths` tokens; blocks that nobody maps any more are free again.
+
+    Returns (moves, count): a partial last block that others map too is exchanged for a
+    fresh one, whose rows paged_copy has to copy.  A refused batch changes nothing.
+    """
+    *value, status = extension().paged_release(lengths, held, block_table, free_ring, ring_state, shares)
+    _status(status)
+    return tuple(value)
+
+
+def paged_compact(held, block_table, free_ring, ring_state, shares):
+    """The blocks in use get the lowest ids; returns (moves, count) of the blocks to copy."""
+    *value, status = extension().paged_compact(held, block_table, free_ring, ring_state, shares)
+    _status(status)
+    return tuple(value)
+
+
+def paged_copy(pools, generations, moves, count):
+    """Copies the rows of the moves in every pool [rows, width] and bumps their generations."""
+    _status(extension().paged_copy(list(pools), list(generations), moves, count))
+
+
 def rope(tensors, positions, frequencies, *, offsets, interleaved, mscale: float = 1.0, inverse: bool = False,
          out=None):
     """Rotates 1 to 4 tensors [tokens(, heads), width] by their positions in one launch.

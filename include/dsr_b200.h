@@ -466,6 +466,70 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
                    int32_t* slots, int64_t tokens, int32_t* cu_tokens, int32_t* visible,
                    int32_t* err, int64_t batch, void* stream);
 
+/* Blocks that several requests map.  shares i32[pool_blocks] holds, for every block,
+ * the number of table entries that map it beyond the first (all zeros without shared
+ * blocks; dsr_paged_plan, which maps free blocks only, leaves it alone).  held,
+ * block_table, free_ring, ring_state as in dsr_paged_plan; all five are updated in
+ * place, and calls on them must not overlap on the GPU.  Where blocks are shared,
+ * dsr_paged_release gives blocks back; a request that dsr_paged_plan finds holding
+ * more than it needs would put a block that others map into the ring.
+ * moves i32[batch][4], 16-byte aligned: (source row, destination row, rows, 0) of the
+ * rows to copy, in request order, (-1,-1,0,0) behind the last; count i32[1] how many.
+ * The caller copies them (dsr_paged_copy) in every pool that the table maps, before
+ * anything is appended.  batch <= 16384.  Refused with status 1, the tables unchanged
+ * and count 0: what each call says, too few free blocks for the copies, a held or a
+ * ring state out of range.  A block id outside the pool met on the way gives status 1,
+ * -1 in the new entries and no move. */
+
+/* Forks requests: request b with parent[b] = p >= 0 becomes the first lengths[b] tokens
+ * of request p.  Its whole blocks are p's (shares + 1), the rows of a last, partial one
+ * are to be copied to a block taken from the ring's head; held[b] becomes
+ * ceil(lengths[b]/64).  parent i32[batch] is -1 for every other request, which stays as
+ * it is; p must not be a child of the same call, held[b] must be 0 and lengths[b] at
+ * most lengths[p], which p's blocks must hold (else refused). */
+int dsr_paged_fork(const int32_t* parent, const int32_t* lengths, int32_t* held,
+                   int32_t* block_table, int64_t table_stride, int32_t* free_ring,
+                   int32_t* ring_state, int32_t* shares, int64_t pool_blocks, int32_t* moves,
+                   int32_t* count, int32_t* err, int64_t batch, void* stream);
+
+/* Cuts every request to its first lengths[b] <= 64 held[b] tokens (0: it ends; more is
+ * refused): entries behind the last needed block become -1, their blocks lose a share,
+ * and those that nobody maps any more go behind the ring's tail, in the order of their
+ * ids, free from the next call on.  A partial last block that others map too is
+ * exchanged for one from the ring's head, its rows to be copied, so that what is
+ * appended next is seen by this request alone.  A block whose count is too low for its
+ * entries gives status 1.  Scratch: 256-byte aligned, need not be cleared; calls
+ * sharing it must not overlap. */
+size_t dsr_paged_release_workspace_bytes(int64_t batch, int64_t pool_blocks);
+int dsr_paged_release(const int32_t* lengths, int32_t* held, int32_t* block_table,
+                      int64_t table_stride, int32_t* free_ring, int32_t* ring_state,
+                      int32_t* shares, int64_t pool_blocks, int32_t* moves, int32_t* count,
+                      void* workspace, size_t workspace_bytes, int32_t* err, int64_t batch,
+                      void* stream);
+
+/* Moves the blocks in use to the lowest ids.  With L blocks mapped by the entries below
+ * held (of all `batch` rows of the table), the i-th mapped id from L on becomes the i-th
+ * id below L that is not mapped; entries and shares follow, the ring is rebuilt as
+ * L .. pool_blocks-1 (state {0, pool_blocks-L}, -1 behind them).  A block that no entry
+ * maps is free afterwards, whether the ring had it or not.  moves is
+ * i32[max(1, pool_blocks/2)][4]: whole blocks, by ascending source.  pool_blocks <= 8388608.  Scratch as above. */
+size_t dsr_paged_compact_workspace_bytes(int64_t pool_blocks);
+int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t table_stride,
+                      int32_t* free_ring, int32_t* ring_state, int32_t* shares,
+                      int64_t pool_blocks, int32_t* moves, int32_t* count, void* workspace,
+                      size_t workspace_bytes, int32_t* err, int64_t batch, void* stream);
+
+/* Copies the rows of the first *count moves in each of up to 64 pools of pool_rows rows
+ * (row_bytes[i] a multiple of 16, at most 65536; 16-byte aligned) and adds 1 to the
+ * written rows' entries of up to 64 generations i64[pool_rows] (an append's bump).  The
+ * three host arrays are read by the call.  A move of more than 64 rows, or with rows
+ * outside the pool, and a count outside [0, max_moves] give status 1 and are skipped.
+ * No destination may be another move's source or destination. */
+int dsr_paged_copy(void* const* pools, const int64_t* row_bytes, int64_t pool_count,
+                   int64_t* const* generations, int64_t generation_count, int64_t pool_rows,
+                   const int32_t* moves, const int32_t* count, int64_t max_moves, int32_t* err,
+                   void* stream);
+
 /* One tensor of dsr_rope: x and out [tokens, heads, width] of type dtype with unit
  * column stride and token and head strides in elements (any sign).  out == x
  * rotates in place (equal strides; only the rotated columns count as written).
