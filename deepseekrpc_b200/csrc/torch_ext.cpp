@@ -762,6 +762,62 @@ std::vector<at::Tensor> ds_tree_mla_decode(at::Tensor q, at::Tensor kv_pool, at:
   return {result, error};
 }
 
+std::vector<at::Tensor> ds_prefix_mla_decode(at::Tensor q, at::Tensor kv_pool, at::Tensor block_table,
+                                             at::Tensor context, at::Tensor cu_nodes, at::Tensor tree_mask,
+                                             int64_t max_nodes, at::Tensor prefix, at::Tensor holder, double scale,
+                                             c10::optional<at::Tensor> sink, bool return_lse,
+                                             c10::optional<at::Tensor> out, c10::optional<at::Tensor> status) {
+  const int dtype = element_type(q, "prefix_mla_decode");
+  check(q, q.scalar_type(), q);
+  check_cache(kv_pool, q);
+  check(block_table, at::kInt, q);
+  TORCH_CHECK(q.dim() == 3 && q.size(0) > 0 && q.size(2) == DSR_KV_DIM,
+              "prefix_mla_decode: q [nodes, heads, 576] expected");
+  const int64_t nodes = q.size(0), heads = q.size(1), batch = context.numel();
+  const char* shapes =
+      "prefix_mla_decode: context, prefix, holder [batch], cu_nodes [batch + 1], tree_mask [nodes], block_table "
+      "[batch or more, blocks], kv_pool [blocks*64, 576] and sink [heads] expected";
+  check_vector(context, at::kInt, batch, q, shapes);
+  check_vector(prefix, at::kInt, batch, q, shapes);
+  check_vector(holder, at::kInt, batch, q, shapes);
+  check_vector(cu_nodes, at::kInt, batch + 1, q, shapes);
+  check_vector(tree_mask, at::kLong, nodes, q, shapes);
+  TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) >= batch && kv_pool.dim() == 2 &&
+                  kv_pool.size(1) == DSR_KV_DIM && kv_pool.size(0) % DSR_BLOCK_TOKENS == 0,
+              shapes);
+  if (sink) check_vector(*sink, at::kFloat, heads, q, shapes);
+  const c10::cuda::CUDAGuard guard(q.device());
+  auto error = status_or(status, q);
+  at::Tensor result;
+  if (out) {
+    result = *out;
+    element_type(result, "prefix_mla_decode");
+    check(result, result.scalar_type(), q);
+    TORCH_CHECK(result.dim() == 3 && result.size(0) == nodes && result.size(1) == heads &&
+                    result.size(2) == DSR_V_DIM,
+                "prefix_mla_decode: out [nodes, heads, 512] expected");
+    overwrite(result, "prefix_mla_decode");
+  } else {
+    result = fresh({nodes, heads, DSR_V_DIM}, q.scalar_type(), q);
+  }
+  const int unused = out ? 0 : DSR_ZERO_UNUSED;  // as in tree_mla_decode
+  at::Tensor lse;
+  if (return_lse && out) lse = at::full({nodes, heads}, -INFINITY, q.options().dtype(at::kFloat));
+  else if (return_lse) lse = fresh({nodes, heads}, at::kFloat, q);
+  const size_t ws_bytes = dsr_prefix_mla_workspace_bytes(batch, nodes, heads, max_nodes);
+  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, q);
+  ok(dsr_prefix_mla_decode(q.data_ptr(), dtype, bf16(kv_pool), kv_pool.size(0) / DSR_BLOCK_TOKENS,
+                           block_table.data_ptr<int32_t>(), block_table.size(0), block_table.size(1),
+                           context.data_ptr<int32_t>(), cu_nodes.data_ptr<int32_t>(), tree_mask.data_ptr<int64_t>(),
+                           max_nodes, prefix.data_ptr<int32_t>(), holder.data_ptr<int32_t>(),
+                           sink ? sink->data_ptr<float>() : nullptr, static_cast<float>(scale), result.data_ptr(),
+                           element_type(result, "prefix_mla_decode") | unused,
+                           return_lse ? lse.data_ptr<float>() : nullptr, ws.data_ptr(), ws_bytes,
+                           error.data_ptr<int32_t>(), batch, nodes, heads, current_stream()));
+  if (return_lse) return {result, error, lse};
+  return {result, error};
+}
+
 std::vector<at::Tensor> ds_sample_logits(at::Tensor logits, at::Tensor temperature, at::Tensor top_k,
                                          at::Tensor top_p, at::Tensor min_p, at::Tensor uniform,
                                          c10::optional<at::Tensor> status) {
@@ -838,6 +894,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("context"), py::arg("cu_nodes"), py::arg("tree_mask"), py::arg("max_nodes"), py::arg("scale"),
         py::arg("sink") = py::none(), py::arg("return_lse") = false, py::arg("out") = py::none(),
         py::arg("status") = py::none());
+  m.def("prefix_mla_decode", &ds_prefix_mla_decode, py::arg("q"), py::arg("kv_pool"), py::arg("block_table"),
+        py::arg("context"), py::arg("cu_nodes"), py::arg("tree_mask"), py::arg("max_nodes"), py::arg("prefix"),
+        py::arg("holder"), py::arg("scale"), py::arg("sink") = py::none(), py::arg("return_lse") = false,
+        py::arg("out") = py::none(), py::arg("status") = py::none());
   m.def("sample_logits", &ds_sample_logits, py::arg("logits"), py::arg("temperature"), py::arg("top_k"),
         py::arg("top_p"), py::arg("min_p"), py::arg("uniform"), py::arg("status") = py::none());
 }

@@ -45,10 +45,11 @@
 // 1.11 ms, 64 2.07, 128 5.06.  Bound by memory at 16 rows: 32 requests of one node and 16 heads
 // over 65536 rows 378 to 406 us from box to box, 6.0 to 6.4 TB/s, 91 to 97% of a plain copy.
 // Bound by latency for little: one node over 4096 rows 16.4 to 18.4 us in two launches.
-#include <math_constants.h>
+#include <type_traits>
 
 #include "common.cuh"
 #include "host_common.h"
+#include "tree_jobs.cuh"
 
 namespace dsr {
 namespace {
@@ -58,7 +59,6 @@ constexpr int kTreeThreads = kTreeSoftmax + 64;
 constexpr int kTreeKeys = 128;
 constexpr int kTreeD = DSR_KV_DIM, kTreeDv = DSR_V_DIM;
 constexpr int kTreeMaxNodes = 64;
-constexpr float kTreeLog2e = 1.4426950408889634f;
 constexpr float kTreeSlack = 8.f;  // log2 units a row's maximum may lag behind
 
 template <int N>
@@ -104,6 +104,7 @@ struct TreeArgs {
   float* part_l;
   int64_t nodes;
   int batch, heads, max_nodes, ctas;
+  TreeListed list;  // of a Listed kernel, in place of what its jobs follow from
 };
 
 // ---- the work of request b
@@ -232,6 +233,40 @@ struct TreeWalk {
   }
 };
 
+// The jobs of a list, dealt like those of a walk.
+struct TreeList {
+  const TreeJob* jobs;
+  int32_t count;
+  int round;
+  TreeJob job;
+  __device__ __forceinline__ bool next() {
+    const int at = round * int(gridDim.x) + (round & 1 ? int(gridDim.x) - 1 - int(blockIdx.x) : int(blockIdx.x));
+    if (at >= count) return false;
+    ++round;
+    const int4* words = reinterpret_cast<const int4*>(jobs + at);
+    const int4 x = __ldcg(words), y = __ldcg(words + 1), z = __ldcg(words + 2);
+    job = TreeJob{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, {}};
+    return true;
+  }
+};
+
+// What the job at hand is, for all warps.
+struct TreeWork {
+  int32_t table, block0, node0, row0, rows, drafts, context, tile0, count;
+  int32_t part;  // first row of its partials
+  bool whole;    // or none: the group's only segment
+};
+template <int N>
+__device__ __forceinline__ TreeWork tree_work(const TreeWalk<N>& w) {
+  return TreeWork{w.b,       0,           w.s.node0, w.group * N, min(N, w.s.nodes * w.a.heads - w.group * N),
+                  w.s.nodes, w.s.context, w.tile0,   w.count,     w.slot * N,
+                  w.slot < 0};
+}
+__device__ __forceinline__ TreeWork tree_work(const TreeList& l) {
+  const TreeJob& j = l.job;
+  return TreeWork{j.table, j.block0, j.node0, j.row0, j.rows, j.drafts, j.context, j.tile0, j.count, j.part, false};
+}
+
 // mbar_wait whose polls sleep in the barrier unit until the phase completes (or a few
 // microseconds pass): the ten warps that wait here would otherwise poll shared memory
 // all the time, whose bandwidth the MMAs of 64 columns need to the last byte.
@@ -269,12 +304,6 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 // 16 TMEM lanes x 8 C columns: thread i holds lanes i/4 and i/4 + 8 (of the 16),
@@ -354,22 +383,8 @@ __device__ __forceinline__ bool softmax_sync(int half, bool ok) {
   return r != 0;
 }
 
-// A row's total with its head's sink (in units of 2^top), and the logarithm of its sum.
-__device__ __forceinline__ float tree_total(const TreeArgs& a, int head, float top, float sum, float& total) {
-  total = sum;
-  if (a.sink == nullptr) return top == -CUDART_INF_F ? top : (top + log2f(sum)) / kTreeLog2e;
-  float sink = a.sink[head];
-  if (!isfinite(sink)) {
-    flag(a.err, DSR_ERR_NONFINITE);
-    sink = 0.f;
-  }
-  if (top == -CUDART_INF_F) return sink;
-  const float over = sink * kTreeLog2e - top;  // the sink's weight, log2
-  total = sum + ex2(over);
-  return over > 100.f ? sink : (top + log2f(total)) / kTreeLog2e;
-}
-
-template <int N>
+// Listed: the jobs are a list that a kernel before this one wrote, and all leave partials.
+template <int N, bool Listed>
 __global__ void __launch_bounds__(kTreeThreads, 1)
     tree_mla_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
                     const __grid_constant__ TreeArgs a) {
@@ -424,101 +439,110 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   }
 
   // ---- the work of all requests
+  if constexpr (Listed)
+    if (a.list.after_plan) pdl_wait();
   TreeEntry* entries = reinterpret_cast<TreeEntry*>(smem + L::kChunkOff);  // in the chunks' place
   static_assert(32 * sizeof(TreeEntry) <= 2 * kTreeThreads * 4, "");
-  TreeWalk<N> walk{a, entries, chunk_jobs, chunk_slots, 1, 0, 0, 1};
-  TreeSeq own_seq{};
-  const bool small = a.batch <= 32;
-  const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;  // else: requests of a thread's chunk
-  const int r0 = small ? lane : min(tid * per, a.batch), r1 = small ? min(lane + 1, a.batch) : min(r0 + per, a.batch);
-  walk.per = per;
-  int64_t units = 0;
-  int32_t groups = 0;
-  bool fine = true;  // no request is refused: the node sums rise
-  for (int b = r0; b < r1; ++b) {
-    const TreeSeq s = tree_seq<N>(a, b);
-    if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
-    fine = fine && s.ok;
-    units += int64_t(s.groups) * s.tiles;
-    groups += s.groups;
-    own_seq = s;
-  }
-  // sums over the warp: low and high parts of the units by themselves
-  units = (int64_t(__reduce_add_sync(~0u, uint32_t(units >> 24))) << 24) +
-          __reduce_add_sync(~0u, uint32_t(units) & 0xffffffu);
-  groups = __reduce_add_sync(~0u, groups);
-  fine = __all_sync(~0u, fine);
-  tc_fence_before();
-  if (!small) {
-    if (lane == 0) warp_units[warp] = units, warp_groups[warp] = groups;
-    fine = __syncthreads_and(fine);
-    units = groups = 0;
-    for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
-  }
-  // ---- the segment length: one tile when that fills no more than the grid, else the
-  // best of four wave counts
-  int32_t length = units <= a.ctas ? 1 : 0;
-  if (length == 0 && a.batch <= kTreeSearchBatch) {
-    if (warp < 4) {
-      int32_t len = 1;
-      const float e = tree_length<N>(a, own_seq, units, (groups + a.ctas - 1) / a.ctas + warp, len);
-      if (lane == 0) estimate[warp] = e, estimated[warp] = len;
+  auto walk = [&] {
+    if constexpr (Listed) return TreeList{a.list.jobs, __ldcg(a.list.count), 0, {}};
+    else return TreeWalk<N>{a, entries, chunk_jobs, chunk_slots, 1, 0, 0, 1};
+  }();
+  if constexpr (!Listed) {
+    TreeSeq own_seq{};
+    const bool small = a.batch <= 32;
+    const int per = (a.batch + kTreeThreads - 1) / kTreeThreads;  // else: requests of a thread's chunk
+    const int r0 = small ? lane : min(tid * per, a.batch), r1 = small ? min(lane + 1, a.batch) : min(r0 + per, a.batch);
+    walk.per = per;
+    int64_t units = 0;
+    int32_t groups = 0;
+    bool fine = true;  // no request is refused: the node sums rise
+    for (int b = r0; b < r1; ++b) {
+      const TreeSeq s = tree_seq<N>(a, b);
+      if (!s.ok && blockIdx.x == 0) flag(a.err, DSR_ERR_ID);
+      fine = fine && s.ok;
+      units += int64_t(s.groups) * s.tiles;
+      groups += s.groups;
+      own_seq = s;
     }
-    __syncthreads();
-    float best = CUDART_INF_F;
-    for (int w = 0; w < 4; ++w)
-      if (estimate[w] < best) best = estimate[w], length = estimated[w];
-  }
-  // or the even share of two jobs per CTA, whose partials always fit: a cut request's
-  // groups have at most 2 U / length of them.  Batches beyond the search's take that, as do
-  // those without a find
-  if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
-  // ---- jobs and partial slots before each lane's request, or each thread's chunk
-  int32_t jobs = 0, slots = 0;
-  for (int b = r0; b < r1; ++b) {
-    const TreeSeq s = small ? own_seq : tree_seq<N>(a, b);
-    const int32_t n = s.groups * tree_segments(s, length);
-    jobs += n;
-    if (s.tiles > length) slots += n;
-  }
-  walk.length = length;
-  int32_t jobs_before = 0, slots_before = 0;
-  if (small) {
-    // those of the requests with longer segments come first
-    const float mine = jobs > 0 ? float(own_seq.tiles) / float(tree_segments(own_seq, length)) : 0.f;
-    for (int b = 0; b < a.batch; ++b) {
-      const float other = __shfl_sync(~0u, mine, b);
-      const int32_t n = __shfl_sync(~0u, jobs, b), m = __shfl_sync(~0u, slots, b);
-      if (other > mine || (other == mine && b < lane)) jobs_before += n, slots_before += m;
-      walk.jobs += n;
+    // sums over the warp: low and high parts of the units by themselves
+    units = (int64_t(__reduce_add_sync(~0u, uint32_t(units >> 24))) << 24) +
+            __reduce_add_sync(~0u, uint32_t(units) & 0xffffffu);
+    groups = __reduce_add_sync(~0u, groups);
+    fine = __all_sync(~0u, fine);
+    tc_fence_before();
+    if (!small) {
+      if (lane == 0) warp_units[warp] = units, warp_groups[warp] = groups;
+      fine = __syncthreads_and(fine);
+      units = groups = 0;
+      for (int w = 0; w < kTreeThreads / 32; ++w) units += warp_units[w], groups += warp_groups[w];
     }
-    if (warp == 0 && lane < a.batch) entries[lane] = TreeEntry{own_seq, jobs_before, jobs, slots_before};
-  } else {
-    int32_t jobs_upto = jobs, slots_upto = slots;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
-      if (lane >= d) jobs_upto += u, slots_upto += v;
+    // ---- the segment length: one tile when that fills no more than the grid, else the
+    // best of four wave counts
+    int32_t length = units <= a.ctas ? 1 : 0;
+    if (length == 0 && a.batch <= kTreeSearchBatch) {
+      if (warp < 4) {
+        int32_t len = 1;
+        const float e = tree_length<N>(a, own_seq, units, (groups + a.ctas - 1) / a.ctas + warp, len);
+        if (lane == 0) estimate[warp] = e, estimated[warp] = len;
+      }
+      __syncthreads();
+      float best = CUDART_INF_F;
+      for (int w = 0; w < 4; ++w)
+        if (estimate[w] < best) best = estimate[w], length = estimated[w];
     }
-    jobs_before = jobs_upto - jobs;
-    slots_before = slots_upto - slots;
-    __syncthreads();  // the sums above have been read
-    if (lane == 31) warp_units[warp] = jobs_upto, warp_groups[warp] = slots_upto;
-    __syncthreads();
-    for (int w = 0; w < kTreeThreads / 32; ++w) {
-      if (w < warp) jobs_before += int32_t(warp_units[w]), slots_before += int32_t(warp_groups[w]);
-      walk.jobs += int32_t(warp_units[w]);
-    }
-    chunk_jobs[tid] = jobs_before;
-    chunk_slots[tid] = slots_before;
-  }
-  if (blockIdx.x == 0 && (!small || warp == 0)) {
+    // or the even share of two jobs per CTA, whose partials always fit: a cut request's
+    // groups have at most 2 U / length of them.  Batches beyond the search's take that, as do
+    // those without a find
+    if (length == 0) length = max(int32_t((units + 2 * a.ctas - 1) / (2 * a.ctas)), 1);
+    // ---- jobs and partial slots before each lane's request, or each thread's chunk
+    int32_t jobs = 0, slots = 0;
     for (int b = r0; b < r1; ++b) {
       const TreeSeq s = small ? own_seq : tree_seq<N>(a, b);
-      a.slot_start[b] = slots_before;
-      if (s.tiles > length) slots_before += s.groups * tree_segments(s, length);
+      const int32_t n = s.groups * tree_segments(s, length);
+      jobs += n;
+      if (s.tiles > length) slots += n;
     }
-    if (tid == 0) a.slot_start[a.batch] = fine ? length : -length;
+    walk.length = length;
+    int32_t jobs_before = 0, slots_before = 0;
+    if (small) {
+      // those of the requests with longer segments come first
+      const float mine = jobs > 0 ? float(own_seq.tiles) / float(tree_segments(own_seq, length)) : 0.f;
+      for (int b = 0; b < a.batch; ++b) {
+        const float other = __shfl_sync(~0u, mine, b);
+        const int32_t n = __shfl_sync(~0u, jobs, b), m = __shfl_sync(~0u, slots, b);
+        if (other > mine || (other == mine && b < lane)) jobs_before += n, slots_before += m;
+        walk.jobs += n;
+      }
+      if (warp == 0 && lane < a.batch) entries[lane] = TreeEntry{own_seq, jobs_before, jobs, slots_before};
+    } else {
+      int32_t jobs_upto = jobs, slots_upto = slots;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int32_t u = __shfl_up_sync(~0u, jobs_upto, d), v = __shfl_up_sync(~0u, slots_upto, d);
+        if (lane >= d) jobs_upto += u, slots_upto += v;
+      }
+      jobs_before = jobs_upto - jobs;
+      slots_before = slots_upto - slots;
+      __syncthreads();  // the sums above have been read
+      if (lane == 31) warp_units[warp] = jobs_upto, warp_groups[warp] = slots_upto;
+      __syncthreads();
+      for (int w = 0; w < kTreeThreads / 32; ++w) {
+        if (w < warp) jobs_before += int32_t(warp_units[w]), slots_before += int32_t(warp_groups[w]);
+        walk.jobs += int32_t(warp_units[w]);
+      }
+      chunk_jobs[tid] = jobs_before;
+      chunk_slots[tid] = slots_before;
+    }
+    if (blockIdx.x == 0 && (!small || warp == 0)) {
+      for (int b = r0; b < r1; ++b) {
+        const TreeSeq s = small ? own_seq : tree_seq<N>(a, b);
+        a.slot_start[b] = slots_before;
+        if (s.tiles > length) slots_before += s.groups * tree_segments(s, length);
+      }
+      if (tid == 0) a.slot_start[a.batch] = fine ? length : -length;
+    }
+  } else {
+    tc_fence_before();
   }
   __syncthreads();
   tc_fence_after();
@@ -535,10 +559,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     bool ok = true;
     bool more = walk.next();
     while (ok && more) {
-      const TreeSeq s = walk.s;
-      const int tile0 = walk.tile0, count = walk.count, slot = walk.slot;
-      const int row0 = walk.group * N, rows = min(N, s.nodes * a.heads - row0);
-      const int64_t qrow = int64_t(s.node0) * a.heads + row0;
+      const TreeWork s = tree_work(walk);
+      const int count = s.count, rows = s.rows;
+      const int64_t qrow = int64_t(s.node0) * a.heads + s.row0;
       if (a.q_wide) {
         // ---- FP32 query rows -> bf16, K-major, 128-byte swizzle (BF16 ones come by TMA).  As
         // in the sparse attention: the keys are BF16, and one product takes one type.  It moves
@@ -571,7 +594,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       if ((warp & 3) == 0) {  // the rows' masks, and what any of them sees
         uint64_t any = 0;
         for (int r = lane; r < N; r += 32) {
-          const uint64_t word = r < rows ? uint64_t(a.masks[s.node0 + (row0 + r) / a.heads]) : 0ull;
+          const uint64_t word = r < rows ? uint64_t(a.masks[s.node0 + (s.row0 + r) / a.heads]) : 0ull;
           masks[r] = word;
           any |= word;
         }
@@ -588,7 +611,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
       for (int c = 0; c < C; ++c) m[c][0] = m[c][1] = -CUDART_INF_F, l[c][0] = l[c][1] = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
-        const int32_t p0 = (tile0 + i) * kTreeKeys;
+        const int32_t p0 = s.block0 * DSR_BLOCK_TOKENS + (s.tile0 + i) * kTreeKeys;
         ok = tree_wait_warp(bar_s, n & 1, abort, a.err);
         // ---- scores of keys 32 (warp % 4) + quad + 8j, rows row_h + 8c + 2 (lane % 4) + e
         float v[C][4][2];
@@ -617,7 +640,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                   const int32_t d = drafted + (warp & 3) * 32 + quad + 8 * j;
-                  if (d >= 0 && (d >= s.nodes || !(word >> d & 1))) v[c][j][e] = -CUDART_INF_F;
+                  if (d >= 0 && (d >= s.drafts || !(word >> d & 1))) v[c][j][e] = -CUDART_INF_F;
                 }
               }
             // a row that no node of the group sees may hold anything: it is cleared, since
@@ -625,7 +648,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
             // send the 32 lanes of a store to the same banks (4.7 us for one such tile)
             const uint64_t any = masks[N];
             const int32_t d = drafted + t;
-            const uint32_t hidden = __ballot_sync(~0u, d >= 0 && (d >= s.nodes || !(any >> d & 1)));
+            const uint32_t hidden = __ballot_sync(~0u, d >= 0 && (d >= s.drafts || !(any >> d & 1)));
             if (hidden != 0) {
 #pragma unroll 1
               for (int c = 4 * half; c < 4 * half + 4; ++c) {
@@ -740,7 +763,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
       // MMA follows every thread's last use of red and stat
       more = walk.next();  // while they run
       ok = tree_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
-      const bool whole = slot < 0;
+      const bool whole = s.whole;
 #pragma unroll
       for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -762,12 +785,14 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         if (r < rows && !(sum < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
         if (whole) {
           float total;
-          const float lse = tree_total(a, (row0 + r) % a.heads, top, sum, total);
+          const float lse = tree_total(a.sink, a.err, (s.row0 + r) % a.heads, top, sum, total);
           stat[r] = total > 0.f ? 1.f / total : 0.f;
           if (a.lse != nullptr && r < rows) a.lse[qrow + r] = lse;
         } else {
-          a.part_m[int64_t(slot) * N + r] = top;
-          a.part_l[int64_t(slot) * N + r] = sum;
+          if (!Listed || r < rows) {
+            a.part_m[int64_t(s.part) + r] = top;
+            a.part_l[int64_t(s.part) + r] = sum;
+          }
           stat[r] = 1.f;
         }
       }
@@ -788,7 +813,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
           x[y + 2] = __uint_as_float(o[y + 2]) * f.z, x[y + 3] = __uint_as_float(o[y + 3]) * f.w;
         }
         if (!whole) {
-          float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(slot) * N + r) * kTreeDv) + d;
+          float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(s.part) + r) * kTreeDv) + d;
 #pragma unroll
           for (int y = 0; y < W; y += 4)
             if (r + y < rows) dst[y / 4 * kTreeDv] = make_float4(x[y], x[y + 1], x[y + 2], x[y + 3]);
@@ -831,7 +856,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     auto wait = [&](uint64_t* bar, uint32_t parity) { return tree_wait_warp(bar, parity, abort, a.err); };
     while (ok) {
       if (!walk.next()) break;  // alike in all lanes
-      const int count = __shfl_sync(~0u, walk.count, 0);
+      const int count = __shfl_sync(~0u, tree_work(walk).count, 0);
       committed = false;
       ok = wait(bar_q, segment & 1);
       for (int i = 0; i < count && ok; ++i, ++n) {
@@ -903,9 +928,9 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     int n = 0;
     bool ok = true;
     while (ok && walk.next()) {
-      const TreeSeq s = walk.s;
-      const int32_t* table = a.table + int64_t(walk.b) * a.stride;
-      const int32_t blocks = int32_t((int64_t(s.context) + s.nodes + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS);
+      const TreeWork s = tree_work(walk);
+      const int32_t* table = a.table + int64_t(s.table) * a.stride;
+      const int32_t blocks = int32_t((int64_t(s.context) + s.drafts + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS);
       auto row_of = [&](int32_t j) -> int32_t {  // first pool row of block j; past the pool: reads zeros
         if (j >= blocks || lane != 0) return int32_t(a.pool_rows);
         const int64_t blk = table[j];
@@ -920,16 +945,17 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         if (n > 0) ok = tree_wait_warp(bar_s, (n - 1) & 1, abort, a.err);
         if (!ok) break;
         if (lane == 0) {
-          const int32_t qrow = s.node0 * a.heads + walk.group * N;
+          const int32_t qrow = s.node0 * a.heads + s.row0;
           mbar_arrive_expect_tx(bar_q, 9 * N * 128);
           for (int c = 0; c < 9; ++c) tma_load_2d(sbase + L::kQOff + c * (N * 128), &q_map, bar_q, c * 64, qrow);
           ++*loaded_q;
         }
       }
-      int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
-      for (int i = 0; lane == 0 && i < walk.count && ok; ++i, ++n) {
+      const int32_t block0 = s.block0 + 2 * s.tile0;
+      int32_t y0 = row_of(block0), y1 = row_of(block0 + 1);
+      for (int i = 0; lane == 0 && i < s.count && ok; ++i, ++n) {
         const int32_t x0 = y0, x1 = y1;
-        if (i + 1 < walk.count) y0 = row_of(2 * (walk.tile0 + i) + 2), y1 = row_of(2 * (walk.tile0 + i) + 3);
+        if (i + 1 < s.count) y0 = row_of(block0 + 2 * i + 2), y1 = row_of(block0 + 2 * i + 3);
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           const int k = 4 * n + c, pair = k % L::kPairs;
@@ -950,7 +976,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
         tma_load_2d(sbase + L::kROff, &kv_map, bar_r, 512, x0);
         tma_load_2d(sbase + L::kROff + 8192, &kv_map, bar_r, 512, x1);
         *loaded_r = n + 1;
-        if (i + 1 < walk.count)  // the next tile's rows into L2 (209 to 199 us for 8 nodes over 131072 rows)
+        if (i + 1 < s.count)  // the next tile's rows into L2 (209 to 199 us for 8 nodes over 131072 rows)
           for (int c = 0; c < 9; ++c) {
             tma_prefetch_2d(&kv_map, c * 64, y0);
             tma_prefetch_2d(&kv_map, c * 64, y1);
@@ -972,6 +998,8 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem_o, L::kTmemCols);
   }
+  if constexpr (Listed)
+    if (!a.list.after_plan) pdl_wait();  // so that what waits for this kernel waits for the one before it
 }
 
 // ---------------------------------------------------------------------------
@@ -982,7 +1010,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
 // The statistics and a thread's first values are requested together, so that few
 // parts take one memory round trip.
 // ---------------------------------------------------------------------------
-constexpr int kTreeMaxCtas = 256;
 constexpr int kTreeMaxParts = kTreeSlotsPerCta * kTreeMaxCtas;  // of one row
 constexpr int kJoinThreads = 128, kJoinBatch = 8;  // kJoinBatch: parts requested together
 
@@ -1062,7 +1089,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
     if (lane == 0) {
       float total;
-      const float lse = tree_total(a, int((row + w) % a.heads), top, sum, total);
+      const float lse = tree_total(a.sink, a.err, int((row + w) % a.heads), top, sum, total);
       inverse[w] = total > 0.f ? 1.f / total : 0.f;
       if (a.lse != nullptr && blockIdx.y == 0) a.lse[row + w] = lse;
     }
@@ -1091,33 +1118,39 @@ __global__ void __launch_bounds__(kJoinThreads) tree_combine_kernel(const __grid
 // Rows per group: all of a request's rows in one group when that fits, since a
 // group reads every key tile once, and no more, since the MMAs of empty rows cost as much
 // (16 rows over 131072: 64 us in groups of 16, 88 of 32, 92 of 64).
+}  // namespace
 int tree_rows(int64_t heads, int64_t max_nodes) {
   const int64_t rows = heads * max_nodes;
   return rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
 }
 
 int tree_ctas() { return sm_count() < kTreeMaxCtas ? sm_count() : kTreeMaxCtas; }
+namespace {
 
 size_t tree_start_bytes(int64_t batch) { return (size_t(batch + 1) * 4 + 255) / 256 * 256; }
+
+// The tensor maps: one page by 64 columns, and a group's queries (FP32 ones are converted, not copied).
+template <int N>
+int tree_maps(const TreeArgs& a, const uint16_t* kv_pool, CUtensorMap& map, CUtensorMap& q_map) {
+  const int rc = encode_tmap_bf16_2d(&map, kv_pool, kTreeD, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
+  if (rc != DSR_OK) return rc;
+  q_map = map;
+  return a.q_wide ? DSR_OK : encode_tmap_bf16_2d(&q_map, a.q, kTreeD, uint64_t(a.nodes) * a.heads, 64, N);
+}
 
 template <int N>
 int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStream_t stream) {
   using L = TreeLayout<N>;
-  int rc = set_max_smem(tree_mla_kernel<N>, L::kAlloc, "tree_mla_decode");
+  int rc = set_max_smem(tree_mla_kernel<N, false>, L::kAlloc, "tree_mla_decode");
   if (rc != DSR_OK) return rc;
-  CUtensorMap map;  // one page by 64 columns
-  rc = encode_tmap_bf16_2d(&map, kv_pool, kTreeD, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
+  CUtensorMap map, q_map;
+  rc = tree_maps<N>(a, kv_pool, map, q_map);
   if (rc != DSR_OK) return rc;
   a.slot_start = static_cast<int32_t*>(workspace);
   a.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + tree_start_bytes(a.batch));
   a.part_m = a.part_o + size_t(kTreeSlotsPerCta) * a.ctas * N * kTreeDv;
   a.part_l = a.part_m + size_t(kTreeSlotsPerCta) * a.ctas * N;
-  CUtensorMap q_map = map;  // FP32 queries are converted, not copied
-  if (!a.q_wide) {
-    rc = encode_tmap_bf16_2d(&q_map, a.q, kTreeD, uint64_t(a.nodes) * a.heads, 64, N);
-    if (rc != DSR_OK) return rc;
-  }
-  tree_mla_kernel<N><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, q_map, a);
+  tree_mla_kernel<N, false><<<unsigned(a.ctas), kTreeThreads, L::kAlloc, stream>>>(map, q_map, a);
   rc = launch_status("tree_mla_decode launch");
   if (rc != DSR_OK) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -1134,7 +1167,58 @@ int launch_tree(TreeArgs& a, const uint16_t* kv_pool, void* workspace, cudaStrea
   return DSR_OK;
 }
 
+template <int N>
+int launch_listed(const TreeArgs& a, const uint16_t* kv_pool, cudaStream_t stream) {
+  using L = TreeLayout<N>;
+  int rc = set_max_smem(tree_mla_kernel<N, true>, L::kAlloc, "prefix_mla_decode");
+  if (rc != DSR_OK) return rc;
+  CUtensorMap map, q_map;
+  rc = tree_maps<N>(a, kv_pool, map, q_map);
+  if (rc != DSR_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.ctas), 1, 1);
+  cfg.blockDim = dim3(kTreeThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kAlloc;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_mla_kernel<N, true>, map, q_map, a);
+  if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode launch: %s", cudaGetErrorString(e));
+  return DSR_OK;
+}
+
 }  // namespace
+
+int launch_tree_listed(const TreeListedCall& c, cudaStream_t stream) {
+  TreeArgs a = {};
+  a.q = c.q;
+  a.q_wide = c.q_dtype == DSR_F32;
+  a.table = c.table;
+  a.stride = c.stride;
+  a.pool_rows = c.pool_rows;
+  a.masks = c.masks;
+  a.scale_log2 = c.scale_log2;
+  a.err = c.err;
+  a.part_o = c.part_o;
+  a.part_m = c.part_m;
+  a.part_l = c.part_l;
+  a.nodes = c.nodes;
+  a.heads = c.heads;
+  a.ctas = tree_ctas();
+  a.list = c.list;
+  switch (c.rows) {
+    case 16:
+      return launch_listed<16>(a, c.kv_pool, stream);
+    case 32:
+      return launch_listed<32>(a, c.kv_pool, stream);
+    default:
+      return launch_listed<64>(a, c.kv_pool, stream);
+  }
+}
+
 }  // namespace dsr
 
 extern "C" size_t dsr_tree_mla_workspace_bytes(int64_t batch, int64_t heads, int64_t max_nodes) {

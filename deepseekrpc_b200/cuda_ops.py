@@ -190,6 +190,21 @@ def tree_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, m
     return (result[0], result[2]) if return_lse else result[0]
 
 
+def prefix_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes: int, prefix, holder, *,
+                      scale: float, sink=None, out=None, return_lse: bool = False):
+    """tree_mla_decode for requests that continue common prompts.
+
+    The whole blocks of a request's first `prefix` positions are read through block_table's
+    row `holder`, once for all requests in a row that have the same.
+    """
+    if not math.isfinite(scale) or scale <= 0:
+        raise ValidationError("invalid attention scale")
+    result = extension().prefix_mla_decode(query, kv_pool, block_table, context, cu_nodes, tree_mask, max_nodes, prefix,
+                                           holder, scale, sink=sink, return_lse=return_lse, out=out)
+    _status(result[1])
+    return (result[0], result[2]) if return_lse else result[0]
+
+
 def sample_logits(logits, temperature, top_k, top_p, min_p, uniform):
     """One token per row after temperature, top-k, top-p and min-p; returns (tokens, chances)."""
     tokens, chances, status = extension().sample_logits(logits, temperature, top_k, top_p, min_p, uniform)

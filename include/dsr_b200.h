@@ -587,6 +587,31 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
                         void* workspace, size_t workspace_bytes, int32_t* err, int64_t batch,
                         int64_t nodes, int64_t heads, void* stream);
 
+/* dsr_tree_mla_decode for requests that continue common prompts: the first S =
+ * 64 floor(prefix[b]/64) positions of request b are read through row holder[b] of
+ * block_table i32[table_rows,table_stride] (any row: a request's, or one that only keeps
+ * a prompt), the others through its own row b < batch <= table_rows.  prefix and holder
+ * are i32[batch]; prefix[b] <= context[b], and with S = 0 holder[b] is not looked at.
+ * Requests one after another with the same holder and the same S are computed together:
+ * their shared rows are read and multiplied once for all of their query rows, so a batch
+ * is best in the order of its prompts.  The result does not depend on the grouping
+ * beyond the order of FP32 sums; all else, and the status, as in dsr_tree_mla_decode.
+ * Status 1 also for a prefix or holder out of range (that request's rows count as
+ * unused), and where disordered sums of cu_nodes give rows to several requests (then
+ * all may count as unused).  batch <= 16384, nodes * heads <= 2^24.
+ * Scratch: dsr_prefix_mla_workspace_bytes() on the current device, 256-byte aligned,
+ * need not be cleared; calls sharing it must not overlap. */
+size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads,
+                                      int64_t max_nodes);
+int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool,
+                          int64_t pool_blocks, const int32_t* block_table, int64_t table_rows,
+                          int64_t table_stride, const int32_t* context, const int32_t* cu_nodes,
+                          const int64_t* tree_mask, int64_t max_nodes, const int32_t* prefix,
+                          const int32_t* holder, const float* sink, float scale, void* out,
+                          int out_dtype, float* lse, void* workspace, size_t workspace_bytes,
+                          int32_t* err, int64_t batch, int64_t nodes, int64_t heads,
+                          void* stream);
+
 /* One token per row of logits [rows, vocab] (dtype, row_stride elements apart, 0:
  * all rows the same):
  * with w_i = exp((x_i - max)/temperature) and the order (value descending, index
