@@ -30,10 +30,24 @@ static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 struct alignas(16) PrefixRequest {
   int32_t node0, nodes;
   int32_t own_part, own_segments;              // its rows' parts: own_part + segment * rows
-  int32_t run_part, run_rows, run_segments;    // its run's: run_part + segment * run_rows
+  int32_t run_part, run_rows, run_segments;    // its run's: run_part + segment * run_rows, or -1 - its pair run
   int32_t run_node0;
 };
 static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
+
+// A run whose rows, in groups of 128, the pairs of CTAs take.  Its units (group x tile) are
+// numbered from unit0 on, tile by tile of one group after another; pair c has the units
+// [c share, (c + 1) share) of all runs, in one piece per group.  Piece (group g, pair c)
+// leaves its partials at part + 128 (g + c), since g or c rises from piece to piece.
+struct alignas(16) PairRun {
+  int64_t unit0;
+  int32_t groups, blocks;
+  int32_t row0, rows;  // query rows
+  int32_t table, part;
+  __device__ __forceinline__ int32_t tiles() const { return (blocks + kPrefixTileBlocks - 1) / kPrefixTileBlocks; }
+};
+static_assert(sizeof(PairRun) == 32, "two 16-byte words");
+constexpr int kPairRows = 128;
 
 struct PrefixArgs {
   const int32_t* table;
@@ -47,14 +61,17 @@ struct PrefixArgs {
   bool out_wide, zero_unused;
   float* lse;
   int32_t* err;
-  int32_t* head;  // {jobs, 1 when no request was refused}
+  int32_t* head;  // {jobs, 1 when no request was refused, pair runs, units of a pair}
   PrefixRequest* requests;
-  int32_t* places;  // the plan's own
+  PairRun* pair_runs;
+  int32_t* places;  // the plan's own: [batch] a run's pair run, [2 batch] an item's partials
   TreeJob* jobs;
   float *part_o, *part_m, *part_l;
   int64_t nodes;
   int batch, heads, max_nodes, ctas;
-  int rows;  // of a job's group
+  int rows;   // of a job's group
+  int pairs;  // of CTAs that take the runs of more rows than that (0: none does)
+  int32_t pair_part;  // where their partials begin
 };
 
 // ---- request b: what it has to itself, and the blocks that it reads through `holder`
@@ -94,14 +111,16 @@ __device__ __forceinline__ PrefixItem own_item(const PrefixArgs& a, int b) {
   }
   return it;
 }
-__device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, int b0, int b1) {
+// (`paired`: what the pairs take, in groups of their own size, else what they do not.)
+__device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, int b0, int b1, bool paired) {
   const PrefixSeq s = prefix_seq(a, b0);
   PrefixItem it{s.holder, 0, s.node0, 0, 0, s.shared * DSR_BLOCK_TOKENS, 0, 0};
   if (!s.ok || s.shared == 0) return it;
-  it.rows = (a.cu_nodes[b1] - s.node0) * a.heads;
-  if (it.rows == 0) return it;
+  const int32_t rows = (a.cu_nodes[b1] - s.node0) * a.heads;
+  if (rows == 0 || (a.pairs > 0 && rows > a.rows) != paired) return it;
+  it.rows = rows;
   it.tiles = (s.shared + kPrefixTileBlocks - 1) / kPrefixTileBlocks;
-  it.groups = (it.rows + a.rows - 1) / a.rows;
+  it.groups = (rows + (paired ? kPairRows : a.rows) - 1) / (paired ? kPairRows : a.rows);
   return it;
 }
 
@@ -139,7 +158,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
   extern __shared__ int32_t plan_smem[];
   int32_t* starts = plan_smem;               // [batch + 1] first request of each run
   int32_t* cu_jobs = starts + a.batch + 1;   // [2 batch + 1] jobs before each item
-  int32_t* parts = a.places;                 // [2 batch] where its partials are
+  int32_t* parts = a.places + a.batch;       // [2 batch] where its partials are
   __shared__ PlanPair part[kPlanThreads / 32];
   __shared__ unsigned long long counted[kPlanWaves];
   __shared__ int longest;
@@ -167,7 +186,36 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
   __syncthreads();
   // ---- units and groups of all items
   const int items = runs + a.batch;
-  auto item = [&](int i) { return i < runs ? run_item(a, starts[i], starts[i + 1]) : own_item(a, i - runs); };
+  auto item = [&](int i) { return i < runs ? run_item(a, starts[i], starts[i + 1], false) : own_item(a, i - runs); };
+  // ---- those of the pairs: units, then {records, rows}
+  const int per_run = (runs + kPlanThreads - 1) / kPlanThreads;
+  const int r0 = min(tid * per_run, runs), r1 = min(r0 + per_run, runs);
+  int64_t pair_units = 0, pair_rows = 0;
+  int pair_runs = 0;
+  if (a.pairs > 0) {
+    PlanPair units{0, 0}, records{0, 0}, totals;
+    for (int r = r0; r < r1; ++r) {
+      const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
+      units.x += int64_t(it.groups) * it.tiles;
+      records = records + PlanPair{it.groups > 0, it.rows};
+    }
+    units = plan_scan(units, part, totals);
+    pair_units = totals.x;
+    records = plan_scan(records, part, totals);
+    pair_runs = int(totals.x), pair_rows = totals.y;
+    if (pair_rows <= a.nodes * a.heads)
+      for (int r = r0; r < r1; ++r) {
+        const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
+        a.places[r] = -1;
+        if (it.groups == 0) continue;
+        a.places[r] = int32_t(records.x);
+        a.pair_runs[records.x] = PairRun{units.x, it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows, it.table,
+                                         a.pair_part + int32_t(records.y)};
+        units.x += int64_t(it.groups) * it.tiles;
+        records = records + PlanPair{1, it.rows};
+      }
+  }
+  const int64_t share = a.pairs > 0 ? (pair_units + a.pairs - 1) / a.pairs : 0;
   const int per_item = (items + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(tid * per_item, items), i1 = min(i0 + per_item, items);
   PlanPair mine{0, 0};
@@ -180,9 +228,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
   atomicMax(&longest, most);
   plan_scan(mine, part, all);
   const int64_t units = all.x;
-  if (all.y > 2 * a.nodes * a.heads) {
+  if (all.y > 2 * a.nodes * a.heads || pair_rows > a.nodes * a.heads || share > INT32_MAX) {
     // sums in disorder that give rows to several requests, more than there are partials for
-    if (tid == 0) a.head[0] = 0, a.head[1] = 1;
+    if (tid == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
     for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
     return;
   }
@@ -227,15 +275,16 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
   }
   if (tid == 0) cu_jobs[items] = int32_t(all.x);
   const int32_t jobs = int32_t(all.x);
-  if (tid == 0) a.head[0] = jobs, a.head[1] = fine;
+  if (tid == 0) a.head[0] = jobs, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
   __syncthreads();
   // ---- the requests' records
   for (int b = b0, r = run0 - 1; b < b1; ++b) {
     if (r + 1 < runs && starts[r + 1] == b) ++r;
-    const PrefixItem it = own_item(a, b), run = run_item(a, starts[r], starts[r + 1]);
+    const PrefixItem it = own_item(a, b), run = run_item(a, starts[r], starts[r + 1], false);
     const PrefixSeq s = prefix_seq(a, b);
+    const int paired = a.pairs > 0 ? a.places[r] : -1;
     a.requests[b] = PrefixRequest{s.node0, s.nodes, parts[runs + b], segments(it.tiles, length), parts[r], run.rows,
-                                  segments(run.tiles, length), run.node0};
+                                  paired >= 0 ? -1 - paired : segments(run.tiles, length), run.node0};
   }
   // ---- the jobs: an item's segments one after another, the groups of one side by side
   for (int32_t j = tid; j < jobs; j += kPlanThreads) {
@@ -252,6 +301,563 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
     a.jobs[j] = TreeJob{it.table, it.block0, it.node0, row0, min(a.rows, it.rows - row0), it.drafts, it.context,
                         segment * whole + min(segment, longer), whole + (segment < longer),
                         parts[lo] + segment * it.rows + row0, {}};
+  }
+}
+
+__device__ __forceinline__ PairRun load_pair_run(const PairRun* run) {
+  const int4* words = reinterpret_cast<const int4*>(run);
+  const int4 x = __ldcg(words), y = __ldcg(words + 1);
+  return PairRun{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+
+// ---------------------------------------------------------------------------
+// The shared rows of a run, by pairs of CTAs (clusters of two).  A unit is one group of 128
+// query rows x one 128-key tile, 64 rows of it in either CTA; the MMAs are the pair's
+// (cta_group::2, M = 128), issued by CTA 0:
+//   S[row, key]   = Q[row, :576] K[key, :576]      (N = 128 keys, 64 from either CTA)
+//   O[row, dim]  += P[row, key] V[key, dim]        (N = 256 dims x 2, 128 from either CTA)
+// so that an SM reads of every operand its own half only: 4 KB of shared memory for an MMA
+// of 32 cycles, 6 KB for one of 64 (a CTA alone, with 64 rows: 6 KB for 32).  For S a CTA has
+// its 64 keys of the tile with all columns, for O all 128 keys with its half of the value
+// columns, which are fetched once more, from L2.
+// An accumulator of 64 rows takes tensor memory's lanes twice: lanes 0..63 have the rows and
+// the first half of the columns, lanes 64..127 the same rows and the second half.
+//   warps 0..3  (FP32 query -> shared memory,) softmax: warp w has rows 32 (w % 2) .. of
+//               this CTA and the keys, value columns of half w / 2; the running maximum of a
+//               row is followed only when it grows by more than 2^8
+//   warp 4      tensor memory; in CTA 0 the MMAs: S of the next tile, then O of this one, so
+//               that they run through the softmax between
+//   warp 5      query, keys and values by TMA; what arrives in either CTA is counted by CTA
+//               0's barriers
+// ---------------------------------------------------------------------------
+constexpr int kPairSoftmax = 128, kPairThreads = kPairSoftmax + 64;
+constexpr int kPairKeys = 128;
+constexpr int kKStages = 5;  // pairs of 64-column blocks, the rotary block alone
+constexpr float kPairSlack = 8.f;  // log2 units a row's maximum may lag behind
+
+struct PairLayout {
+  static constexpr int kBlock = 64 * 128;                    // 64 rows x 64 columns
+  static constexpr int kQOff = 0;                            // 9 blocks
+  static constexpr int kKOff = kQOff + 9 * kBlock;           // 9 blocks
+  static constexpr int kVOff = kKOff + 9 * kBlock;           // 2 x [2 blocks of 128 keys x 64 columns]
+  static constexpr int kPOff = kVOff + 8 * kBlock;           // 2 blocks of 64 rows x 64 keys
+  static constexpr int kBarOff = kPOff + 2 * kBlock;
+  static constexpr int kBars = 2 * kKStages + 2 * 2 + 2 + 5;
+  static constexpr int kRedOff = kBarOff + (kBars * 8 + 15) / 16 * 16;  // f32[2][64]
+  static constexpr int kMiscOff = kRedOff + 2 * 64 * 4;
+  static constexpr int kBytes = kMiscOff + 16;
+  static constexpr int kAlloc = kBytes + 1024;
+  static constexpr uint32_t kTmemCols = 512;  // O: 256 columns, S: two of 64
+  static_assert(kAlloc <= 232448, "shared memory of one CTA");
+};
+
+struct PairArgs {
+  const void* q;
+  bool q_wide;  // fp32 (else bf16)
+  const int32_t* table;
+  int64_t stride, pool_rows;
+  float scale_log2;
+  float *part_o, *part_m, *part_l;
+  const int32_t* head;
+  const PairRun* runs;
+  int32_t* err;
+};
+
+// A pair's pieces, one after another (every warp walks them for itself).
+struct PairWalk {
+  const PairRun* runs;
+  int64_t unit, end;
+  int32_t at, pair;
+  PairRun run;
+  int32_t row0, rows, tile0, count, part;  // of the piece at hand
+  __device__ __forceinline__ PairWalk(const PairArgs& a, int pair_) : runs(a.runs), at(0), pair(pair_) {
+    const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head));
+    const int64_t share = head.w;
+    unit = share * pair;
+    end = unit;
+    if (head.z == 0) return;
+    const PairRun last = load_pair_run(runs + head.z - 1);
+    end = min(unit + share, last.unit0 + int64_t(last.groups) * last.tiles());
+    if (unit >= end) return;
+    // the last run that starts at or before the unit, 32 ways a step
+    for (int n = head.z; n > 1;) {
+      const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
+      const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&runs[at + i].unit0) <= unit);
+      const int lead = (31 - __clz(below)) * stride;
+      at += lead;
+      n = min(stride, n - lead);
+    }
+    run = load_pair_run(runs + at);
+  }
+  __device__ __forceinline__ bool next() {
+    if (unit >= end) return false;
+    if (unit >= run.unit0 + int64_t(run.groups) * run.tiles()) run = load_pair_run(runs + ++at);
+    const int64_t in = unit - run.unit0;
+    const int32_t tiles = run.tiles(), group = int32_t(in / tiles);
+    tile0 = int32_t(in - int64_t(group) * tiles);
+    count = int32_t(min(int64_t(tiles - tile0), end - unit));
+    row0 = run.row0 + group * kPairRows;
+    rows = min(kPairRows, run.rows - group * kPairRows);
+    part = run.part + (group + pair) * kPairRows;
+    unit += count;
+    return true;
+  }
+};
+
+// ---- barriers of a pair
+__device__ __forceinline__ uint32_t pair_address(const void* p, uint32_t cta) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(cta));
+  return r;
+}
+__device__ __forceinline__ void pair_sync() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrives at a barrier of either CTA (an address from pair_address).
+__device__ __forceinline__ void pair_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait for what the other CTA may have done, whose polls sleep in the barrier unit.
+__device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  const uint64_t start = global_ns();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if (*abort) return false;
+    if (global_ns() - start > kWaitNs) {
+      *abort = 1;
+      flag(err, DSR_ERR_TIMEOUT);
+      return false;
+    }
+  }
+}
+// The same for a whole warp, with one answer for all lanes.
+__device__ __forceinline__ bool pair_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  return __all_sync(~0u, pair_wait(bar, parity, abort, err));
+}
+// A copy to this CTA that a barrier of CTA 0 (an address from pair_address) counts.
+__device__ __forceinline__ void pair_load(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      : "memory");
+}
+__device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Arrives on `bar` of both CTAs once all MMAs issued so far are complete.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"(uint16_t(3))
+      : "memory");
+}
+// The 64 softmax threads of one half of a CTA's rows: a barrier, and whether every one is fine.
+__device__ __forceinline__ bool rows_sync(int half, bool ok) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"(uint32_t(ok)), "r"(1 + half)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__global__ void __launch_bounds__(kPairThreads, 1)
+    prefix_pair_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
+                       const __grid_constant__ PairArgs a) {
+  using L = PairLayout;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align_smem_1024(smem_raw);
+  const uint32_t sbase = smem_u32(smem);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+  // CTA 0's are waited for
+  uint64_t* full_k = bars;                  // [kKStages] in both CTAs (TMA bytes + 1)
+  uint64_t* full_v = full_k + kKStages;     // [2]
+  uint64_t* bar_p = full_v + 2;             // P written in both CTAs (a warp arrives)
+  uint64_t* bar_q = bar_p + 1;              // query in place (TMA bytes + 1; FP32: a warp arrives)
+  uint64_t* bar_free = bar_p + 2;           // O read by the output (a warp arrives)
+  uint64_t* bar_end = bar_p + 3;            // all MMAs complete (commit)
+  // each CTA has its own
+  uint64_t* empty_k = bar_p + 4;            // [kKStages] read by the S MMAs (commit)
+  uint64_t* empty_v = empty_k + kKStages;   // [2] read by the O MMAs (commit)
+  uint64_t* bar_s = empty_v + 2;            // [2] S complete (commit)
+  uint64_t* bar_o = bar_s + 2;              // the tile's O MMAs complete (commit)
+  static_assert(2 * kKStages + 2 * 2 + 2 + 5 == L::kBars, "");
+  float* red = reinterpret_cast<float*>(smem + L::kRedOff);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = int(blockIdx.x & 1), pair = int(blockIdx.x >> 1);  // clusters of two along x
+
+  if (tid == 0) {
+    tma_prefetch_desc(&kv_map);
+    if (!a.q_wide) tma_prefetch_desc(&q_map);
+    for (int i = 0; i < kKStages; ++i) mbar_init(full_k + i, 1), mbar_init(empty_k + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(full_v + i, 1), mbar_init(empty_v + i, 1), mbar_init(bar_s + i, 1);
+    mbar_init(bar_p, 8);
+    mbar_init(bar_q, a.q_wide ? 8 : 1);
+    mbar_init(bar_free, 8);
+    mbar_init(bar_end, 1);
+    mbar_init(bar_o, 1);
+    *abort = 0;
+    fence_barrier_init();
+  }
+  if (warp == 4) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(L::kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();  // the other CTA's barriers and tensor memory are there
+  tc_fence_after();
+  const uint32_t tmem_o = *tmem_slot, tmem_s = tmem_o + 256;
+  pdl_wait();
+  pdl_launch_dependents();
+  PairWalk walk(a, pair);
+
+  if (warp < 4) {
+    // ------------------------------------------------------------ softmax
+    const int half = warp >> 1, pack = warp & 1, r = 32 * pack + lane;  // this thread's row of the CTA's
+    const uint32_t lanes = uint32_t(warp) * 32 << 16;                  // this warp's TMEM lanes
+    const uint32_t to_p = pair_address(bar_p, 0), to_q = pair_address(bar_q, 0), to_free = pair_address(bar_free, 0);
+    int n = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const int count = walk.count, mine = 64 * rank + r;  // the row in its group
+      if (a.q_wide) {
+        // FP32 query rows -> bf16, K-major, 128-byte swizzle (as in the tree attention).  The
+        // S MMAs of the piece before have been waited for with its last tile
+        const float* src = static_cast<const float*>(a.q) + int64_t(walk.row0 + 64 * rank) * DSR_KV_DIM;
+        constexpr int kVec = 64 * (DSR_KV_DIM / 8);
+        for (int i = tid; i < kVec; i += kPairSoftmax) {
+          const int row = i / (DSR_KV_DIM / 8), d = (i - row * (DSR_KV_DIM / 8)) * 8;
+          uint4 v = make_uint4(0, 0, 0, 0);
+          if (64 * rank + row < walk.rows) {
+            const float4* at = reinterpret_cast<const float4*>(src + int64_t(row) * DSR_KV_DIM + d);
+            const float4 lo = __ldg(at), hi = __ldg(at + 1);
+            v = make_uint4(pack_bf16(lo.x, lo.y), pack_bf16(lo.z, lo.w), pack_bf16(hi.x, hi.y), pack_bf16(hi.z, hi.w));
+          }
+          *reinterpret_cast<uint4*>(smem + L::kQOff + (d >> 6) * L::kBlock + sw128_offset(row, d & 63)) = v;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) pair_arrive(to_q);
+      }
+      const int32_t blocks = walk.run.blocks;
+      float m = -CUDART_INF_F, l = 0.f;
+      for (int i = 0; i < count; ++i, ++n) {
+        ok = ok && pair_wait_warp(bar_s + (n & 1), (n >> 1) & 1, abort, a.err);
+        float v[64];
+        float top = -CUDART_INF_F;
+        if (ok) {
+          tc_fence_after();
+          uint32_t t0[32], t1[32];
+          tmem_ld32(tmem_s + (n & 1) * 64 + lanes, t0);
+          tmem_ld32(tmem_s + (n & 1) * 64 + 32 + lanes, t1);
+          tmem_wait_ld();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]), v[32 + c] = __uint_as_float(t1[c]);
+          if (half == 1 && kPrefixTileBlocks * (walk.tile0 + i) + 1 >= blocks) {  // the last tile has one page
+#pragma unroll
+            for (int c = 0; c < 64; ++c) v[c] = -CUDART_INF_F;
+          }
+#pragma unroll
+          for (int c = 0; c < 64; ++c) top = fmaxf(top, v[c]);
+          top *= a.scale_log2;
+        }
+        // weights against the running maximum as it stands; their sums are of the weights as
+        // formed, for the product with V they are rounded to BF16 (as in the tree attention)
+        uint32_t packed[32];
+        float sum = 0.f;
+        auto weigh = [&] {
+          const float base = m == -CUDART_INF_F ? 0.f : m;
+          float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            const float x = ex2(fmaf(v[2 * c], a.scale_log2, -base)), y = ex2(fmaf(v[2 * c + 1], a.scale_log2, -base));
+            s0 += x;
+            s1 += y;
+            packed[c] = pack_bf16(x, y);
+          }
+          sum = s0 + s1;
+        };
+        bool fits = ok && i > 0 && !(top > m + kPairSlack);
+        if (ok && i > 0) weigh();
+        // most tiles end here: no row's maximum has to follow
+        if (!rows_sync(pack, fits)) {
+          ok = rows_sync(pack, ok);
+          if (!ok) break;
+          red[64 * half + r] = top;
+          rows_sync(pack, true);
+          top = fmaxf(top, red[64 * (half ^ 1) + r]);
+          float f = 1.f;
+          if (top > m + kPairSlack) f = ex2(m - top), l *= f, m = top;  // f: 0 when the row had seen nothing
+          if (i > 0) {
+            ok = rows_sync(pack, pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < 256; c += 32) {
+              uint32_t o[32];
+              tmem_ld32(tmem_o + c + lanes, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tmem_st32(tmem_o + c + lanes, o);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          }
+          weigh();
+        }
+        l += sum;
+        // P, once the O MMAs of the tile before have read theirs.  (A warp whose wait gives up
+        // says so in the next vote: its rows' other warp must not wait there alone.)
+        if (n > 0) ok = pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
+        if (!ok) continue;
+#pragma unroll
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(smem + L::kPOff + half * L::kBlock + sw128_offset(r, 8 * c)) =
+              make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
+        fence_proxy_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) pair_arrive(to_p);
+      }
+      if (!ok) break;
+
+      // ---- the piece's partials
+      ok = ok && pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
+      if (half == 1) red[64 + r] = l;
+      ok = rows_sync(pack, ok);
+      if (!ok) break;
+      const bool valid = mine < walk.rows;
+      if (half == 0 && valid) {
+        const float total = l + red[64 + r];
+        if (!(total < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
+        a.part_m[int64_t(walk.part) + mine] = m;
+        a.part_l[int64_t(walk.part) + mine] = total;
+      }
+      tc_fence_after();
+      // four rows side by side: a quad's 4 x 4 values are transposed, so that a thread has
+      // one column of its four rows
+      const int q = lane & 3;
+      float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(walk.part) + (mine & ~3)) * DSR_V_DIM);
+#pragma unroll 1
+      for (int c0 = 0; c0 < 256; c0 += 32) {
+        uint32_t o[32];
+        tmem_ld32(tmem_o + c0 + lanes, o);
+        tmem_wait_ld();
+        const int d0 = (c0 >> 7) * 256 + half * 128 + (c0 & 127);
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          // exchange with the neighbour, then with the other two
+          uint32_t w[4] = {o[c], o[c + 1], o[c + 2], o[c + 3]};
+          const uint32_t a0 = __shfl_xor_sync(~0u, q & 1 ? w[0] : w[1], 1), a1 = __shfl_xor_sync(~0u, q & 1 ? w[2] : w[3], 1);
+          if (q & 1) w[0] = a0, w[2] = a1;
+          else w[1] = a0, w[3] = a1;
+          const uint32_t b0 = __shfl_xor_sync(~0u, q & 2 ? w[0] : w[2], 2), b1 = __shfl_xor_sync(~0u, q & 2 ? w[1] : w[3], 2);
+          if (q & 2) w[0] = b0, w[1] = b1;
+          else w[2] = b0, w[3] = b1;
+          if (valid)
+            dst[d0 + c + q] = make_float4(__uint_as_float(w[0]), __uint_as_float(w[1]), __uint_as_float(w[2]),
+                                          __uint_as_float(w[3]));
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) pair_arrive(to_free);
+    }
+  } else if (warp == 4) {
+    if (rank == 0) {
+      // ------------------------------------------------------------ MMA issuer
+      // The whole warp runs the loop and one lane issues, on values that are the same in all
+      // lanes: descriptors then stay in uniform registers
+      constexpr uint32_t idesc_s = umma_idesc_bf16(kPairRows, kPairKeys, false, false);
+      constexpr uint32_t idesc_o = umma_idesc_bf16(kPairRows, 256, false, true);
+      const uint32_t sb = __shfl_sync(~0u, sbase, 0);
+      const uint32_t ts = __shfl_sync(~0u, tmem_s, 0), to = __shfl_sync(~0u, tmem_o, 0);
+      uint32_t elected;
+      asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
+      const bool leader = elected != 0;
+      const uint64_t desc_q = umma_desc_sw128(sb + L::kQOff, 16, 1024), desc_k = umma_desc_sw128(sb + L::kKOff, 16, 1024);
+      const uint64_t desc_p = umma_desc_sw128(sb + L::kPOff, 16, 1024);
+      const uint64_t desc_v = umma_desc_sw128(sb + L::kVOff, 2 * L::kBlock, 1024);
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
+      int n = 0, piece = 0;
+      bool ok = true;
+      // S of tile k: a step of 16 columns moves both operands by 32 bytes
+      auto scores = [&](int k) {
+#pragma unroll
+        for (int c = 0; c < kKStages; ++c) {
+          ok = ok && wait(full_k + c, k & 1);
+          if (!ok) return;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int x = 0; x < (c < 4 ? 8 : 4); ++x)
+              pair_umma(ts + (k & 1) * 64, desc_q + (2 * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3),
+                        desc_k + (2 * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3), idesc_s, (c | x) != 0 ? 1u : 0u);
+            pair_commit(empty_k + c);
+          }
+        }
+        if (leader) pair_commit(bar_s + (k & 1));
+      };
+      while (ok) {
+        if (!walk.next()) break;  // alike in all lanes
+        const int count = __shfl_sync(~0u, walk.count, 0);
+        ok = wait(bar_q, piece & 1);
+        if (ok) scores(n);
+        for (int i = 0; i < count && ok; ++i, ++n) {
+          if (i + 1 < count) scores(n + 1);
+          ok = ok && wait(bar_p, n & 1);
+          // the output of the piece before has read O
+          if (ok && i == 0 && piece > 0) ok = wait(bar_free, (piece - 1) & 1);
+          if (!ok) break;
+          const uint32_t accumulate = i > 0;
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            ok = ok && wait(full_v + c, n & 1);
+            if (!ok) break;
+            tc_fence_after();
+            if (leader) {
+#pragma unroll
+              for (int ks = 0; ks < kPairKeys / 16; ++ks)
+                pair_umma(to + c * 128, desc_p + (ks >> 2) * (L::kBlock / 16) + 2 * (ks & 3),
+                          desc_v + c * (4 * L::kBlock / 16) + ks * (2048 / 16), idesc_o, ks > 0 ? 1u : accumulate);
+              pair_commit(empty_v + c);
+            }
+          }
+          if (leader && ok) pair_commit(bar_o);
+        }
+        ++piece;
+      }
+      // the last MMAs retire before TMEM is released
+      if (leader)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
+                         smem_u32(bar_end))
+                     : "memory");
+      mbar_drain(bar_end, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ copies
+    uint32_t to_k[kKStages], to_v[2];
+    for (int c = 0; c < kKStages; ++c) to_k[c] = pair_address(full_k + c, 0);
+    for (int c = 0; c < 2; ++c) to_v[c] = pair_address(full_v + c, 0);
+    const uint32_t to_q = pair_address(bar_q, 0);
+    int n = 0;
+    bool ok = true;
+    while (ok && walk.next()) {
+      const int32_t* table = a.table + int64_t(walk.run.table) * a.stride;
+      const int32_t blocks = walk.run.blocks;
+      auto row_of = [&](int32_t j) -> int32_t {  // first pool row of block j; past the pool: reads zeros
+        if (j >= blocks || lane != 0) return int32_t(a.pool_rows);
+        const int64_t blk = table[j];
+        if (blk < 0 || blk * DSR_BLOCK_TOKENS >= a.pool_rows) {
+          flag(a.err, DSR_ERR_ID);
+          return int32_t(a.pool_rows);
+        }
+        return int32_t(blk * DSR_BLOCK_TOKENS);
+      };
+      if (!a.q_wide) {
+        // the query, once the last S MMA of the piece before has read the one there
+        if (n > 0) ok = pair_wait_warp(bar_s + ((n - 1) & 1), ((n - 1) >> 1) & 1, abort, a.err);
+        if (!ok) break;
+        if (lane == 0) {
+          if (rank == 0) mbar_arrive_expect_tx(bar_q, 2 * 9 * L::kBlock);
+          for (int c = 0; c < 9; ++c)
+            pair_load(sbase + L::kQOff + c * L::kBlock, &q_map, to_q, c * 64, walk.row0 + 64 * rank);
+        }
+      }
+      // keys of tile i from page `rank` of the tile's two, values of both
+      auto keys = [&](int k, int32_t y) {
+#pragma unroll 1
+        for (int c = 0; c < kKStages && ok; ++c) {
+          ok = pair_wait(empty_k + c, (k & 1) ^ 1, abort, a.err);
+          if (!ok) return;
+          const int wide = c < 4 ? 2 : 1;
+          if (rank == 0) mbar_arrive_expect_tx(full_k + c, 2 * wide * L::kBlock);
+          for (int h = 0; h < wide; ++h)
+            pair_load(sbase + L::kKOff + (2 * c + h) * L::kBlock, &kv_map, to_k[c], (2 * c + h) * 64, y);
+        }
+      };
+      auto values = [&](int k, int32_t y0, int32_t y1) {
+#pragma unroll 1
+        for (int c = 0; c < 2 && ok; ++c) {
+          ok = pair_wait(empty_v + c, (k & 1) ^ 1, abort, a.err);
+          if (!ok) return;
+          if (rank == 0) mbar_arrive_expect_tx(full_v + c, 2 * 4 * L::kBlock);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t dst = sbase + L::kVOff + (4 * c + 2 * h) * L::kBlock;
+            const int32_t x = c * 256 + rank * 128 + h * 64;
+            pair_load(dst, &kv_map, to_v[c], x, y0);
+            pair_load(dst + L::kBlock, &kv_map, to_v[c], x, y1);
+          }
+        }
+      };
+      if (lane == 0) {
+        int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
+        keys(n, rank == 0 ? y0 : y1);
+        for (int i = 0; i < walk.count && ok; ++i, ++n) {
+          const int32_t x0 = y0, x1 = y1;
+          if (i + 1 < walk.count) {
+            y0 = row_of(2 * (walk.tile0 + i) + 2), y1 = row_of(2 * (walk.tile0 + i) + 3);
+            keys(n + 1, rank == 0 ? y0 : y1);
+          }
+          if (ok) values(n, x0, x1);
+        }
+      }
+      n = __shfl_sync(~0u, n, 0);
+      ok = __shfl_sync(~0u, int(ok), 0) != 0;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (*abort && tid == 0) {
+    // a wait gave up: copies that nobody waits for any more land meanwhile
+    const uint64_t start = global_ns();
+    while (global_ns() - start < 2000000) __nanosleep(1000);
+  }
+  __syncthreads();
+  pair_sync();  // neither CTA leaves while the other's copies, commits or MMAs may reach it
+  if (warp == 4) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_o), "r"(L::kTmemCols) : "memory");
   }
 }
 
@@ -313,7 +919,17 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
   }
   const int32_t own_rows = s.nodes * a.heads;
   const int64_t own0 = s.own_part + row - int64_t(s.node0) * a.heads;
-  const int64_t run0 = s.run_part + row - int64_t(s.run_node0) * a.heads;
+  int64_t run0 = s.run_part + row - int64_t(s.run_node0) * a.heads;
+  if (s.run_segments < 0) {
+    const PairRun run = load_pair_run(a.pair_runs - 1 - s.run_segments);
+    const int64_t share = __ldcg(a.head + 3);
+    const int32_t in = int32_t(row - run.row0);
+    const int64_t unit = run.unit0 + int64_t(in / kPairRows) * run.tiles();
+    const int32_t first = int32_t(unit / share), last = int32_t((unit + run.tiles() - 1) / share);
+    run0 = run.part + in + int64_t(kPairRows) * first;
+    s.run_rows = kPairRows;
+    s.run_segments = last - first + 1;
+  }
   const int own = s.own_segments, parts = own + s.run_segments;
   auto place = [&](int p) { return p < own ? own0 + int64_t(p) * own_rows : run0 + int64_t(p - own) * s.run_rows; };
   float4 v[kJoinBatch];
@@ -367,12 +983,45 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
   }
 }
 
-// ---- scratch: {jobs, fine}, the requests' records, the jobs, the partials
+int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaStream_t stream) {
+  int rc = set_max_smem(prefix_pair_kernel, PairLayout::kAlloc, "prefix_mla_decode");
+  if (rc != DSR_OK) return rc;
+  CUtensorMap kv_map, q_map;  // one page, and a CTA's rows of a group, by 64 columns
+  rc = encode_tmap_bf16_2d(&kv_map, kv_pool, DSR_KV_DIM, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
+  if (rc != DSR_OK) return rc;
+  q_map = kv_map;
+  if (!a.q_wide) {
+    rc = encode_tmap_bf16_2d(&q_map, a.q, DSR_KV_DIM, uint64_t(rows), 64, kPairRows / 2);
+    if (rc != DSR_OK) return rc;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(2 * (tree_ctas() / 2)), 1, 1);
+  cfg.blockDim = dim3(kPairThreads, 1, 1);
+  cfg.dynamicSmemBytes = PairLayout::kAlloc;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_pair_kernel, kv_map, q_map, a);
+  if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode pair launch: %s", cudaGetErrorString(e));
+  return DSR_OK;
+}
+
+// ---- scratch: the head, the requests' records, the plan's own, the pair runs, the jobs, the
+// partials
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
+
+int pair_count() { return tree_ctas() / 2; }
 
 struct PrefixSizes {
   int rows;
-  size_t requests, places, jobs, parts;  // bytes, and rows
+  size_t requests, places, pair_runs, jobs;  // bytes
+  size_t parts, pair_part;                   // rows of partials, and where the pairs' begin
 };
 PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t max_nodes) {
   PrefixSizes s;
@@ -381,9 +1030,11 @@ PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t ma
   // last group may be short of rows
   const size_t groups = 2 * (size_t(nodes) * heads / s.rows + size_t(batch)), cut = size_t(kPlanWaves) * tree_ctas();
   s.requests = rounded(size_t(batch) * sizeof(PrefixRequest));
-  s.places = rounded(size_t(batch) * 2 * sizeof(int32_t));
+  s.places = rounded(size_t(batch) * 3 * sizeof(int32_t));
+  s.pair_runs = size_t(batch) * sizeof(PairRun);
   s.jobs = rounded((groups + cut) * sizeof(TreeJob));
-  s.parts = 2 * size_t(nodes) * heads + cut * s.rows;
+  s.pair_part = 2 * size_t(nodes) * heads + cut * s.rows;
+  s.parts = s.pair_part + size_t(nodes) * heads + size_t(kPairRows) * pair_count();
   return s;
 }
 
@@ -396,7 +1047,7 @@ extern "C" size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, i
   using namespace dsr;
   if (batch <= 0 || nodes <= 0 || heads <= 0 || max_nodes <= 0) return 0;
   const PrefixSizes s = prefix_sizes(batch, nodes, heads, max_nodes);
-  return 256 + s.requests + s.places + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
+  return 256 + s.requests + s.places + rounded(s.pair_runs) + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
 }
 
 extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
@@ -453,8 +1104,11 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.head = reinterpret_cast<int32_t*>(ws);
   a.requests = reinterpret_cast<PrefixRequest*>(ws + 256);
   a.places = reinterpret_cast<int32_t*>(ws + 256 + sizes.requests);
-  a.jobs = reinterpret_cast<TreeJob*>(ws + 256 + sizes.requests + sizes.places);
-  a.part_o = reinterpret_cast<float*>(ws + 256 + sizes.requests + sizes.places + sizes.jobs);
+  uint8_t* at = ws + 256 + sizes.requests + sizes.places;
+  a.pair_runs = reinterpret_cast<PairRun*>(at);
+  at += rounded(sizes.pair_runs);
+  a.jobs = reinterpret_cast<TreeJob*>(at);
+  a.part_o = reinterpret_cast<float*>(at + sizes.jobs);
   a.part_m = a.part_o + sizes.parts * DSR_V_DIM;
   a.part_l = a.part_m + sizes.parts;
   a.nodes = nodes;
@@ -463,11 +1117,19 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.max_nodes = int(max_nodes);
   a.ctas = tree_ctas();
   a.rows = sizes.rows;
+  a.pairs = nodes * heads > sizes.rows ? pair_count() : 0;  // else no run has rows enough
+  a.pair_part = int32_t(sizes.pair_part);
   rc = set_max_smem(prefix_plan_kernel, plan_smem_bytes(kPrefixMaxBatch), "prefix_mla_decode");
   if (rc != DSR_OK) return rc;
   prefix_plan_kernel<<<1, kPlanThreads, plan_smem_bytes(batch), as_stream(stream)>>>(a);
   rc = launch_status("prefix_mla_decode launch");
   if (rc != DSR_OK) return rc;
+  if (a.pairs > 0) {
+    rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, scale * kTreeLog2e, a.part_o,
+                               a.part_m, a.part_l, a.head, a.pair_runs, err},
+                      kv_pool, nodes * heads, as_stream(stream));
+    if (rc != DSR_OK) return rc;
+  }
   TreeListedCall call = {};
   call.q = q;
   call.q_dtype = q_dtype;
@@ -480,7 +1142,7 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   call.nodes = nodes;
   call.heads = int(heads);
   call.rows = sizes.rows;
-  call.list = TreeListed{a.jobs, a.head, true};
+  call.list = TreeListed{a.jobs, a.head, a.pairs == 0};
   call.part_o = a.part_o;
   call.part_m = a.part_m;
   call.part_l = a.part_l;
