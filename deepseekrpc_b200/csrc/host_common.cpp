@@ -111,6 +111,21 @@ int encode_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint
   return DSR_OK;
 }
 
+int encode_tmap_bf16_blocks(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_rows,
+                            uint32_t box_blocks) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(DSR_ECUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {64, outer, inner / 64};
+  const cuuint64_t strides[2] = {inner * 2, 128};
+  const cuuint32_t box[3] = {64, box_rows, box_blocks};
+  const cuuint32_t elem[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, elem,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(DSR_ECUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return DSR_OK;
+}
+
 }  // namespace dsr
 
 extern "C" const char* dsr_last_error(void) { return dsr::g_message.c_str(); }

@@ -45,6 +45,11 @@ inline int set_max_smem(F* fn, size_t bytes, const char* what) {
 int encode_tmap_bf16_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer,
                         uint32_t box_inner, uint32_t box_outer);
 
+// The same as a 3-D map of its 64-column blocks: coordinates (0, row, block), so that one
+// copy brings box_rows rows of box_blocks blocks, a block after another.
+int encode_tmap_bf16_blocks(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint32_t box_rows,
+                            uint32_t box_blocks);
+
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

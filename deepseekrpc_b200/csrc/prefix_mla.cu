@@ -332,14 +332,15 @@ __device__ __forceinline__ PairRun load_pair_run(const PairRun* run) {
 // ---------------------------------------------------------------------------
 constexpr int kPairSoftmax = 128, kPairThreads = kPairSoftmax + 64;
 constexpr int kPairKeys = 128;
-constexpr int kKStages = 5;  // pairs of 64-column blocks, the rotary block alone
+constexpr int kKStages = 3, kKBlocks = 3;  // 64-column blocks of a copy: the nine of a key,
+constexpr int kVBlocks = 2;                // and a CTA's of a pass over 256 value columns
 constexpr float kPairSlack = 8.f;  // log2 units a row's maximum may lag behind
 
 struct PairLayout {
   static constexpr int kBlock = 64 * 128;                    // 64 rows x 64 columns
   static constexpr int kQOff = 0;                            // 9 blocks
   static constexpr int kKOff = kQOff + 9 * kBlock;           // 9 blocks
-  static constexpr int kVOff = kKOff + 9 * kBlock;           // 2 x [2 blocks of 128 keys x 64 columns]
+  static constexpr int kVOff = kKOff + 9 * kBlock;           // 2 passes x 2 pages x 2 blocks
   static constexpr int kPOff = kVOff + 8 * kBlock;           // 2 blocks of 64 rows x 64 keys
   static constexpr int kBarOff = kPOff + 2 * kBlock;
   static constexpr int kBars = 2 * kKStages + 2 * 2 + 2 + 5;
@@ -414,23 +415,29 @@ __device__ __forceinline__ void pair_sync() {
   __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrives at a barrier of either CTA (an address from pair_address).
+// Arrives at a barrier of either CTA (an address from pair_address).  At the scope of this
+// CTA: no thread of the other one reads what this one's threads write, only the tensor core
+// of this SM does, behind a proxy fence.  (A release to the cluster took some 1000 cycles.)
 __device__ __forceinline__ void pair_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// mbar_wait for what the other CTA may have done, whose polls sleep in the barrier unit.
+// mbar_wait whose polls sleep in the barrier unit.
+__device__ __forceinline__ bool pair_try(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
+  if (pair_try(bar, parity)) return true;
   const uint64_t start = global_ns();
   for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
-        : "memory");
-    if (ok) return true;
+    if (pair_try(bar, parity)) return true;
     if (*abort) return false;
     if (global_ns() - start > kWaitNs) {
       *abort = 1;
@@ -443,12 +450,13 @@ __device__ __forceinline__ bool pair_wait(uint64_t* bar, uint32_t parity, volati
 __device__ __forceinline__ bool pair_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int32_t* err) {
   return __all_sync(~0u, pair_wait(bar, parity, abort, err));
 }
-// A copy to this CTA that a barrier of CTA 0 (an address from pair_address) counts.
-__device__ __forceinline__ void pair_load(uint32_t dst, const void* tmap, uint32_t bar, int32_t x, int32_t y) {
+// A copy to this CTA that a barrier of CTA 0 (an address from pair_address) counts: 64 rows
+// from y on of the 64-column blocks from z on, a block after another.
+__device__ __forceinline__ void pair_load(uint32_t dst, const void* tmap, uint32_t bar, int32_t y, int32_t z) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
-      " [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(x), "r"(y)
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(0), "r"(y), "r"(z)
       : "memory");
 }
 __device__ __forceinline__ void pair_umma(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -467,6 +475,12 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
           smem_u32(bar)),
       "h"(uint16_t(3))
       : "memory");
+}
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
 }
 // The 64 softmax threads of one half of a CTA's rows: a barrier, and whether every one is fine.
 __device__ __forceinline__ bool rows_sync(int half, bool ok) {
@@ -497,8 +511,8 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 }
 
 __global__ void __launch_bounds__(kPairThreads, 1)
-    prefix_pair_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap q_map,
-                       const __grid_constant__ PairArgs a) {
+    prefix_pair_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                       const __grid_constant__ CUtensorMap q_map, const __grid_constant__ PairArgs a) {
   using L = PairLayout;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align_smem_1024(smem_raw);
@@ -524,7 +538,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   const int rank = int(blockIdx.x & 1), pair = int(blockIdx.x >> 1);  // clusters of two along x
 
   if (tid == 0) {
-    tma_prefetch_desc(&kv_map);
+    tma_prefetch_desc(&k_map);
+    tma_prefetch_desc(&v_map);
     if (!a.q_wide) tma_prefetch_desc(&q_map);
     for (int i = 0; i < kKStages; ++i) mbar_init(full_k + i, 1), mbar_init(empty_k + i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(full_v + i, 1), mbar_init(empty_v + i, 1), mbar_init(bar_s + i, 1);
@@ -683,7 +698,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         uint32_t o[32];
         tmem_ld32(tmem_o + c0 + lanes, o);
         tmem_wait_ld();
-        const int d0 = (c0 >> 7) * 256 + half * 128 + (c0 & 127);
+        const int d0 = half * 256 + c0;  // a pass has 128 columns of either CTA's 256
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
           // exchange with the neighbour, then with the other two
@@ -712,12 +727,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       constexpr uint32_t idesc_o = umma_idesc_bf16(kPairRows, 256, false, true);
       const uint32_t sb = __shfl_sync(~0u, sbase, 0);
       const uint32_t ts = __shfl_sync(~0u, tmem_s, 0), to = __shfl_sync(~0u, tmem_o, 0);
-      uint32_t elected;
-      asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(elected));
-      const bool leader = elected != 0;
+      const bool leader = elect_lane();
       const uint64_t desc_q = umma_desc_sw128(sb + L::kQOff, 16, 1024), desc_k = umma_desc_sw128(sb + L::kKOff, 16, 1024);
       const uint64_t desc_p = umma_desc_sw128(sb + L::kPOff, 16, 1024);
-      const uint64_t desc_v = umma_desc_sw128(sb + L::kVOff, 2 * L::kBlock, 1024);
+      const uint64_t desc_v = umma_desc_sw128(sb + L::kVOff, L::kBlock, 1024);
       auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
       int n = 0, piece = 0;
       bool ok = true;
@@ -730,9 +743,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tc_fence_after();
           if (leader) {
 #pragma unroll
-            for (int x = 0; x < (c < 4 ? 8 : 4); ++x)
-              pair_umma(ts + (k & 1) * 64, desc_q + (2 * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3),
-                        desc_k + (2 * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3), idesc_s, (c | x) != 0 ? 1u : 0u);
+            for (int x = 0; x < 4 * kKBlocks; ++x)
+              pair_umma(ts + (k & 1) * 64, desc_q + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3),
+                        desc_k + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3), idesc_s,
+                        (c | x) != 0 ? 1u : 0u);
             pair_commit(empty_k + c);
           }
         }
@@ -759,7 +773,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
               for (int ks = 0; ks < kPairKeys / 16; ++ks)
                 pair_umma(to + c * 128, desc_p + (ks >> 2) * (L::kBlock / 16) + 2 * (ks & 3),
-                          desc_v + c * (4 * L::kBlock / 16) + ks * (2048 / 16), idesc_o, ks > 0 ? 1u : accumulate);
+                          desc_v + (4 * c + 2 * (ks >> 2)) * (L::kBlock / 16) + (ks & 3) * (2048 / 16), idesc_o,
+                          ks > 0 ? 1u : accumulate);
               pair_commit(empty_v + c);
             }
           }
@@ -776,74 +791,82 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ copies
-    uint32_t to_k[kKStages], to_v[2];
-    for (int c = 0; c < kKStages; ++c) to_k[c] = pair_address(full_k + c, 0);
-    for (int c = 0; c < 2; ++c) to_v[c] = pair_address(full_v + c, 0);
-    const uint32_t to_q = pair_address(bar_q, 0);
+    const uint32_t sb = __shfl_sync(~0u, sbase, 0);
+    const uint32_t to_k = __shfl_sync(~0u, pair_address(full_k, 0), 0);
+    const uint32_t to_v = __shfl_sync(~0u, pair_address(full_v, 0), 0);
+    const uint32_t to_q = __shfl_sync(~0u, pair_address(bar_q, 0), 0);
+    const bool leader = elect_lane();
     int n = 0;
     bool ok = true;
     while (ok && walk.next()) {
       const int32_t* table = a.table + int64_t(walk.run.table) * a.stride;
       const int32_t blocks = walk.run.blocks;
-      auto row_of = [&](int32_t j) -> int32_t {  // first pool row of block j; past the pool: reads zeros
-        if (j >= blocks || lane != 0) return int32_t(a.pool_rows);
-        const int64_t blk = table[j];
-        if (blk < 0 || blk * DSR_BLOCK_TOKENS >= a.pool_rows) {
+      const int32_t none = int32_t(a.pool_rows);  // past the pool: reads zeros
+      // the tile's two pages; what a block id means is seen when they are used
+      auto pages = [&](int32_t tile) {
+        const int32_t j = kPrefixTileBlocks * tile;
+        return make_int2(j < blocks ? table[j] : INT32_MIN, j + 1 < blocks ? table[j + 1] : INT32_MIN);
+      };
+      auto row_of = [&](int32_t blk) {
+        if (blk == INT32_MIN) return none;
+        if (blk < 0 || blk * int64_t(DSR_BLOCK_TOKENS) >= a.pool_rows) {
           flag(a.err, DSR_ERR_ID);
-          return int32_t(a.pool_rows);
+          return none;
         }
         return int32_t(blk * DSR_BLOCK_TOKENS);
       };
+      // The whole warp runs the loop and one lane issues, as the MMAs are: a copy from a
+      // one-lane branch takes some 200 cycles to be on its way
+      auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
       if (!a.q_wide) {
         // the query, once the last S MMA of the piece before has read the one there
-        if (n > 0) ok = pair_wait_warp(bar_s + ((n - 1) & 1), ((n - 1) >> 1) & 1, abort, a.err);
+        if (n > 0) ok = wait(bar_s + ((n - 1) & 1), ((n - 1) >> 1) & 1);
         if (!ok) break;
-        if (lane == 0) {
+        if (leader) {
           if (rank == 0) mbar_arrive_expect_tx(bar_q, 2 * 9 * L::kBlock);
-          for (int c = 0; c < 9; ++c)
-            pair_load(sbase + L::kQOff + c * L::kBlock, &q_map, to_q, c * 64, walk.row0 + 64 * rank);
+          for (int c = 0; c < kKStages; ++c)
+            pair_load(sb + L::kQOff + kKBlocks * c * L::kBlock, &q_map, to_q, walk.row0 + 64 * rank, kKBlocks * c);
         }
       }
       // keys of tile i from page `rank` of the tile's two, values of both
       auto keys = [&](int k, int32_t y) {
-#pragma unroll 1
-        for (int c = 0; c < kKStages && ok; ++c) {
-          ok = pair_wait(empty_k + c, (k & 1) ^ 1, abort, a.err);
+#pragma unroll
+        for (int c = 0; c < kKStages; ++c) {
+          ok = ok && wait(empty_k + c, (k & 1) ^ 1);
           if (!ok) return;
-          const int wide = c < 4 ? 2 : 1;
-          if (rank == 0) mbar_arrive_expect_tx(full_k + c, 2 * wide * L::kBlock);
-          for (int h = 0; h < wide; ++h)
-            pair_load(sbase + L::kKOff + (2 * c + h) * L::kBlock, &kv_map, to_k[c], (2 * c + h) * 64, y);
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(full_k + c, 2 * kKBlocks * L::kBlock);
+            pair_load(sb + L::kKOff + kKBlocks * c * L::kBlock, &k_map, to_k + 8 * c, y, kKBlocks * c);
+          }
         }
       };
       auto values = [&](int k, int32_t y0, int32_t y1) {
-#pragma unroll 1
-        for (int c = 0; c < 2 && ok; ++c) {
-          ok = pair_wait(empty_v + c, (k & 1) ^ 1, abort, a.err);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          ok = ok && wait(empty_v + c, (k & 1) ^ 1);
           if (!ok) return;
-          if (rank == 0) mbar_arrive_expect_tx(full_v + c, 2 * 4 * L::kBlock);
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t dst = sbase + L::kVOff + (4 * c + 2 * h) * L::kBlock;
-            const int32_t x = c * 256 + rank * 128 + h * 64;
-            pair_load(dst, &kv_map, to_v[c], x, y0);
-            pair_load(dst + L::kBlock, &kv_map, to_v[c], x, y1);
+          if (leader) {
+            if (rank == 0) mbar_arrive_expect_tx(full_v + c, 2 * 4 * L::kBlock);
+            const int32_t z = 4 * rank + kVBlocks * c;
+            pair_load(sb + L::kVOff + 4 * c * L::kBlock, &v_map, to_v + 8 * c, y0, z);
+            pair_load(sb + L::kVOff + (4 * c + 2) * L::kBlock, &v_map, to_v + 8 * c, y1, z);
           }
         }
       };
-      if (lane == 0) {
-        int32_t y0 = row_of(2 * walk.tile0), y1 = row_of(2 * walk.tile0 + 1);
-        keys(n, rank == 0 ? y0 : y1);
-        for (int i = 0; i < walk.count && ok; ++i, ++n) {
-          const int32_t x0 = y0, x1 = y1;
-          if (i + 1 < walk.count) {
-            y0 = row_of(2 * (walk.tile0 + i) + 2), y1 = row_of(2 * (walk.tile0 + i) + 3);
-            keys(n + 1, rank == 0 ? y0 : y1);
-          }
-          if (ok) values(n, x0, x1);
+      const int count = __shfl_sync(~0u, walk.count, 0);
+      int2 now = pages(walk.tile0), next = count > 1 ? pages(walk.tile0 + 1) : now;
+      int32_t x0 = __shfl_sync(~0u, row_of(now.x), 0), x1 = __shfl_sync(~0u, row_of(now.y), 0);
+      keys(n, rank == 0 ? x0 : x1);
+      for (int i = 0; i < count && ok; ++i, ++n) {
+        int32_t y0 = none, y1 = none;
+        if (i + 1 < count) {
+          y0 = __shfl_sync(~0u, row_of(next.x), 0), y1 = __shfl_sync(~0u, row_of(next.y), 0);
+          if (i + 2 < count) next = pages(walk.tile0 + i + 2);  // a tile ahead
+          keys(n + 1, rank == 0 ? y0 : y1);
         }
+        if (ok) values(n, x0, x1);
+        x0 = y0, x1 = y1;
       }
-      n = __shfl_sync(~0u, n, 0);
-      ok = __shfl_sync(~0u, int(ok), 0) != 0;
     }
   }
   tc_fence_before();
@@ -986,12 +1009,14 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
 int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaStream_t stream) {
   int rc = set_max_smem(prefix_pair_kernel, PairLayout::kAlloc, "prefix_mla_decode");
   if (rc != DSR_OK) return rc;
-  CUtensorMap kv_map, q_map;  // one page, and a CTA's rows of a group, by 64 columns
-  rc = encode_tmap_bf16_2d(&kv_map, kv_pool, DSR_KV_DIM, uint64_t(a.pool_rows), 64, DSR_BLOCK_TOKENS);
+  CUtensorMap k_map, v_map, q_map;  // 64 rows (a page, a CTA's of a group) of some 64-column blocks
+  rc = encode_tmap_bf16_blocks(&k_map, kv_pool, DSR_KV_DIM, uint64_t(a.pool_rows), DSR_BLOCK_TOKENS, kKBlocks);
   if (rc != DSR_OK) return rc;
-  q_map = kv_map;
+  rc = encode_tmap_bf16_blocks(&v_map, kv_pool, DSR_KV_DIM, uint64_t(a.pool_rows), DSR_BLOCK_TOKENS, kVBlocks);
+  if (rc != DSR_OK) return rc;
+  q_map = k_map;
   if (!a.q_wide) {
-    rc = encode_tmap_bf16_2d(&q_map, a.q, DSR_KV_DIM, uint64_t(rows), 64, kPairRows / 2);
+    rc = encode_tmap_bf16_blocks(&q_map, a.q, DSR_KV_DIM, uint64_t(rows), kPairRows / 2, kKBlocks);
     if (rc != DSR_OK) return rc;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1007,7 +1032,7 @@ int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaS
   attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 2;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_pair_kernel, kv_map, q_map, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_pair_kernel, k_map, v_map, q_map, a);
   if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode pair launch: %s", cudaGetErrorString(e));
   return DSR_OK;
 }
