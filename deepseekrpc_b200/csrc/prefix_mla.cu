@@ -21,7 +21,6 @@ namespace {
 
 constexpr int kPrefixMaxBatch = 16384;
 constexpr int kPrefixTileBlocks = 2;  // 128-key tiles of 64-row blocks
-constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = 4;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
@@ -124,133 +123,133 @@ __device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, int b0, int 
   return it;
 }
 
-struct PlanPair {
-  int64_t x, y;
-};
-__device__ __forceinline__ PlanPair operator+(const PlanPair& a, const PlanPair& b) {
-  return PlanPair{a.x + b.x, a.y + b.y};
-}
-// Exclusive sums over the CTA's threads; `all` the totals.
-__device__ __forceinline__ PlanPair plan_scan(const PlanPair& mine, PlanPair* part, PlanPair& all) {
+// Exclusive sums of K values over the CTA's threads, and their totals.  `part` [K][32] is not
+// used by the scan before this one.
+template <int Threads, int K>
+__device__ __forceinline__ void plan_scan(int64_t (&v)[K], int64_t (&all)[K], int64_t (*part)[32]) {
+  constexpr int kWarps = Threads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  PlanPair run = mine;
+  auto inclusive = [&](int64_t x) {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const PlanPair up{__shfl_up_sync(~0u, run.x, d), __shfl_up_sync(~0u, run.y, d)};
-    if (lane >= d) run = run + up;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(~0u, x, d);
+      if (lane >= d) x += up;
+    }
+    return x;
+  };
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t sum = inclusive(v[k]);
+    if (lane == 31) part[k][warp] = sum;
+    v[k] = sum - v[k];
   }
-  if (lane == 31) part[warp] = run;
   __syncthreads();
-  PlanPair before{0, 0};
-  all = PlanPair{0, 0};
-  for (int w = 0; w < kPlanThreads / 32; ++w) {
-    if (w < warp) before = before + part[w];
-    all = all + part[w];
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int64_t mine = lane < kWarps ? part[k][lane] : 0, upto = inclusive(mine);
+    v[k] += __shfl_sync(~0u, upto - mine, warp);
+    all[k] = __shfl_sync(~0u, upto, 31);
   }
-  __syncthreads();
-  return PlanPair{before.x + run.x - mine.x, before.y + run.y - mine.y};
 }
 
 // Lays the jobs out.  An item's tiles are cut into segments of at most `length` tiles:
 // one tile each when all units (group x tile) fit the grid, else the best of a few lengths by
 // the time that the busiest CTA takes.
-__global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
+template <int Threads>
+__global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
   extern __shared__ int32_t plan_smem[];
   int32_t* starts = plan_smem;               // [batch + 1] first request of each run
   int32_t* cu_jobs = starts + a.batch + 1;   // [2 batch + 1] jobs before each item
   int32_t* parts = a.places + a.batch;       // [2 batch] where its partials are
-  __shared__ PlanPair part[kPlanThreads / 32];
+  __shared__ int64_t sums[2][5][32];
   __shared__ unsigned long long counted[kPlanWaves];
   __shared__ int longest;
   const int tid = threadIdx.x;
-  const int per = (a.batch + kPlanThreads - 1) / kPlanThreads;
+  const int per = (a.batch + Threads - 1) / Threads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
   if (tid < kPlanWaves) counted[tid] = 0;
   if (tid == 0) longest = 0;
   // ---- the runs
-  int first = 0;
+  int64_t first[1] = {0}, found[1];
   bool fine = true;
   for (int b = b0; b < b1; ++b) {
-    first += prefix_starts(a, b);
+    first[0] += prefix_starts(a, b);
     if (!prefix_seq(a, b).ok) {
       fine = false;
       flag(a.err, DSR_ERR_ID);
     }
   }
-  fine = __syncthreads_and(fine);
-  PlanPair all;
-  const int run0 = int(plan_scan(PlanPair{first, 0}, part, all).x), runs = int(all.x);
+  plan_scan<Threads>(first, found, sums[0]);
+  const int run0 = int(first[0]), runs = int(found[0]);
   for (int b = b0, r = run0; b < b1; ++b)
     if (prefix_starts(a, b)) starts[r++] = b;
   if (tid == 0) starts[runs] = a.batch;
-  __syncthreads();
-  // ---- units and groups of all items
+  fine = __syncthreads_and(fine);
+  // ---- what the pairs take: units, records, rows; and the units and rows of all items
   const int items = runs + a.batch;
   auto item = [&](int i) { return i < runs ? run_item(a, starts[i], starts[i + 1], false) : own_item(a, i - runs); };
-  // ---- those of the pairs: units, then {records, rows}
-  const int per_run = (runs + kPlanThreads - 1) / kPlanThreads;
+  const int per_item = (items + Threads - 1) / Threads, per_run = (runs + Threads - 1) / Threads;
+  const int i0 = min(tid * per_item, items), i1 = min(i0 + per_item, items);
   const int r0 = min(tid * per_run, runs), r1 = min(r0 + per_run, runs);
-  int64_t pair_units = 0, pair_rows = 0;
-  int pair_runs = 0;
-  if (a.pairs > 0) {
-    PlanPair units{0, 0}, records{0, 0}, totals;
+  int64_t v[5] = {}, all[5];
+  if (a.pairs > 0)
     for (int r = r0; r < r1; ++r) {
       const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
-      units.x += int64_t(it.groups) * it.tiles;
-      records = records + PlanPair{it.groups > 0, it.rows};
+      v[0] += int64_t(it.groups) * it.tiles;
+      v[1] += it.groups > 0;
+      v[2] += it.rows;
     }
-    units = plan_scan(units, part, totals);
-    pair_units = totals.x;
-    records = plan_scan(records, part, totals);
-    pair_runs = int(totals.x), pair_rows = totals.y;
-    if (pair_rows <= a.nodes * a.heads)
-      for (int r = r0; r < r1; ++r) {
-        const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
-        a.places[r] = -1;
-        if (it.groups == 0) continue;
-        a.places[r] = int32_t(records.x);
-        a.pair_runs[records.x] = PairRun{units.x, it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows, it.table,
-                                         a.pair_part + int32_t(records.y)};
-        units.x += int64_t(it.groups) * it.tiles;
-        records = records + PlanPair{1, it.rows};
-      }
-  }
-  const int64_t share = a.pairs > 0 ? (pair_units + a.pairs - 1) / a.pairs : 0;
-  const int per_item = (items + kPlanThreads - 1) / kPlanThreads;
-  const int i0 = min(tid * per_item, items), i1 = min(i0 + per_item, items);
-  PlanPair mine{0, 0};
   int most = 0;
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
-    mine = mine + PlanPair{int64_t(it.groups) * it.tiles, it.groups > 0 ? it.rows : 0};
+    v[3] += int64_t(it.groups) * it.tiles;
+    v[4] += it.groups > 0 ? it.rows : 0;
     most = max(most, it.tiles);
   }
-  atomicMax(&longest, most);
-  plan_scan(mine, part, all);
-  const int64_t units = all.x;
-  if (all.y > 2 * a.nodes * a.heads || pair_rows > a.nodes * a.heads || share > INT32_MAX) {
+  most = __reduce_max_sync(~0u, most);
+  if ((tid & 31) == 0) atomicMax(&longest, most);
+  plan_scan<Threads>(v, all, sums[1]);
+  const int64_t share = a.pairs > 0 ? (all[0] + a.pairs - 1) / a.pairs : 0, units = all[3];
+  const int32_t pair_runs = int32_t(all[1]);
+  if (all[4] > 2 * a.nodes * a.heads || all[2] > a.nodes * a.heads || share > INT32_MAX) {
     // sums in disorder that give rows to several requests, more than there are partials for
     if (tid == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
     for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
     return;
   }
+  if (a.pairs > 0)
+    for (int r = r0; r < r1; ++r) {
+      const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
+      a.places[r] = it.groups > 0 ? int32_t(v[1]) : -1;
+      if (it.groups == 0) continue;
+      a.pair_runs[v[1]] = PairRun{v[0], it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows, it.table,
+                                  a.pair_part + int32_t(v[2])};
+      v[0] += int64_t(it.groups) * it.tiles;
+      ++v[1];
+      v[2] += it.rows;
+    }
+  // ---- the segments' length
   auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
   int32_t length = 1;
   if (units > a.ctas) {
     int32_t tried[kPlanWaves];
     int64_t jobs[kPlanWaves] = {};
+#pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
-      const int64_t room = int64_t(w + 1) * a.ctas, share = (units + room - 1) / room;
-      tried[w] = int32_t(min(share, int64_t(1) << 24));  // no item has more tiles
+      const int64_t room = int64_t(w + 1) * a.ctas;
+      tried[w] = int32_t(min((units + room - 1) / room, int64_t(1) << 24));  // no item has more tiles
     }
     for (int i = i0; i < i1; ++i) {
       const PrefixItem it = item(i);
+#pragma unroll
       for (int w = 0; w < kPlanWaves; ++w) jobs[w] += int64_t(it.groups) * segments(it.tiles, tried[w]);
     }
+#pragma unroll
     for (int w = 0; w < kPlanWaves; ++w)
       if (jobs[w] > 0) atomicAdd(counted + w, (unsigned long long)jobs[w]);
     __syncthreads();
     float best = CUDART_INF_F;
+#pragma unroll
     for (int w = 0; w < kPlanWaves; ++w) {
       // a job costs some 8 tiles beside its own: first copies, output, its part of the join
       const float rounds = ceilf(float(counted[w]) / float(a.ctas));
@@ -259,23 +258,27 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
     }
   }
   // ---- jobs and partials before each item
-  mine = PlanPair{0, 0};
+  int64_t at[2] = {}, totals[2];
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
     const int32_t n = segments(it.tiles, length);
-    mine = mine + PlanPair{int64_t(it.groups) * n, int64_t(it.rows) * n};
+    at[0] += int64_t(it.groups) * n;
+    at[1] += int64_t(it.rows) * n;
   }
-  PlanPair at = plan_scan(mine, part, all);
+  plan_scan<Threads>(at, totals, sums[0]);
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
     const int32_t n = segments(it.tiles, length);
-    cu_jobs[i] = int32_t(at.x);
-    parts[i] = int32_t(at.y);
-    at = at + PlanPair{int64_t(it.groups) * n, int64_t(it.rows) * n};
+    cu_jobs[i] = int32_t(at[0]);
+    parts[i] = int32_t(at[1]);
+    at[0] += int64_t(it.groups) * n;
+    at[1] += int64_t(it.rows) * n;
   }
-  if (tid == 0) cu_jobs[items] = int32_t(all.x);
-  const int32_t jobs = int32_t(all.x);
-  if (tid == 0) a.head[0] = jobs, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+  const int32_t jobs = int32_t(totals[0]);
+  if (tid == 0) {
+    cu_jobs[items] = jobs;
+    a.head[0] = jobs, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+  }
   __syncthreads();
   // ---- the requests' records
   for (int b = b0, r = run0 - 1; b < b1; ++b) {
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) prefix_plan_kernel(const __gr
                                   paired >= 0 ? -1 - paired : segments(run.tiles, length), run.node0};
   }
   // ---- the jobs: an item's segments one after another, the groups of one side by side
-  for (int32_t j = tid; j < jobs; j += kPlanThreads) {
+  for (int32_t j = tid; j < jobs; j += Threads) {
     int lo = 0, hi = items;  // cu_jobs[lo] <= j < cu_jobs[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -1050,7 +1053,8 @@ struct PrefixSizes {
 };
 PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t max_nodes) {
   PrefixSizes s;
-  s.rows = tree_rows(heads, max_nodes);
+  // rows of a group: a request's, as in the tree attention; all of them where that is one group
+  s.rows = tree_rows(heads, nodes * heads <= 64 ? nodes : max_nodes);
   // a segment or more per group: a cut adds at most kPlanWaves jobs a CTA, and an item's
   // last group may be short of rows
   const size_t groups = 2 * (size_t(nodes) * heads / s.rows + size_t(batch)), cut = size_t(kPlanWaves) * tree_ctas();
@@ -1144,9 +1148,14 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.rows = sizes.rows;
   a.pairs = nodes * heads > sizes.rows ? pair_count() : 0;  // else no run has rows enough
   a.pair_part = int32_t(sizes.pair_part);
-  rc = set_max_smem(prefix_plan_kernel, plan_smem_bytes(kPrefixMaxBatch), "prefix_mla_decode");
-  if (rc != DSR_OK) return rc;
-  prefix_plan_kernel<<<1, kPlanThreads, plan_smem_bytes(batch), as_stream(stream)>>>(a);
+  // few requests: scans over few warps
+  if (batch <= 1024) {
+    prefix_plan_kernel<256><<<1, 256, plan_smem_bytes(batch), as_stream(stream)>>>(a);
+  } else {
+    rc = set_max_smem(prefix_plan_kernel<1024>, plan_smem_bytes(kPrefixMaxBatch), "prefix_mla_decode");
+    if (rc != DSR_OK) return rc;
+    prefix_plan_kernel<1024><<<1, 1024, plan_smem_bytes(batch), as_stream(stream)>>>(a);
+  }
   rc = launch_status("prefix_mla_decode launch");
   if (rc != DSR_OK) return rc;
   if (a.pairs > 0) {
