@@ -21,7 +21,9 @@ namespace {
 
 constexpr int kPrefixMaxBatch = 16384;
 constexpr int kPrefixTileBlocks = 2;  // 128-key tiles of 64-row blocks
-constexpr int kPlanWaves = 4;
+constexpr int kPlanWaves = 4, kPlanTried = kPlanWaves + 1;
+// A job's cost beside its tiles, in tiles: first copies, output, its part of the join.
+constexpr float kPlanJobTiles = 4.f;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // What the join has to know of a request: its query rows, where its own parts are, and
@@ -89,10 +91,8 @@ __device__ __forceinline__ PrefixSeq prefix_seq(const PrefixArgs& a, int b) {
   return s;
 }
 // A refused request is a run of its own.
-__device__ __forceinline__ bool prefix_starts(const PrefixArgs& a, int b) {
-  if (b == 0) return true;
-  const PrefixSeq s = prefix_seq(a, b), t = prefix_seq(a, b - 1);
-  return !s.ok || !t.ok || s.shared != t.shared || s.holder != t.holder;
+__device__ __forceinline__ bool prefix_continues(const PrefixSeq& before, const PrefixSeq& s) {
+  return s.ok && before.ok && s.shared == before.shared && s.holder == before.holder;
 }
 
 // ---- an item of the plan: a run's shared rows (items 0 .. runs - 1), then a request's own
@@ -100,8 +100,7 @@ struct PrefixItem {
   int32_t table, block0, node0, rows, drafts, context;
   int32_t tiles, groups;
 };
-__device__ __forceinline__ PrefixItem own_item(const PrefixArgs& a, int b) {
-  const PrefixSeq s = prefix_seq(a, b);
+__device__ __forceinline__ PrefixItem own_item(const PrefixArgs& a, int b, const PrefixSeq& s) {
   PrefixItem it{b, s.shared, s.node0, s.nodes * a.heads, s.nodes, s.context, 0, 0};
   const int32_t keys = s.context + s.nodes - s.shared * DSR_BLOCK_TOKENS;
   if (s.nodes > 0 && keys > 0) {
@@ -110,12 +109,13 @@ __device__ __forceinline__ PrefixItem own_item(const PrefixArgs& a, int b) {
   }
   return it;
 }
-// (`paired`: what the pairs take, in groups of their own size, else what they do not.)
-__device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, int b0, int b1, bool paired) {
-  const PrefixSeq s = prefix_seq(a, b0);
+// Of a run's first and last request.  (`paired`: what the pairs take, in groups of their own
+// size, else what they do not.)
+__device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, const PrefixSeq& s, const PrefixSeq& last,
+                                               bool paired) {
   PrefixItem it{s.holder, 0, s.node0, 0, 0, s.shared * DSR_BLOCK_TOKENS, 0, 0};
   if (!s.ok || s.shared == 0) return it;
-  const int32_t rows = (a.cu_nodes[b1] - s.node0) * a.heads;
+  const int32_t rows = (last.node0 + last.nodes - s.node0) * a.heads;
   if (rows == 0 || (a.pairs > 0 && rows > a.rows) != paired) return it;
   it.rows = rows;
   it.tiles = (s.shared + kPrefixTileBlocks - 1) / kPrefixTileBlocks;
@@ -152,29 +152,43 @@ __device__ __forceinline__ void plan_scan(int64_t (&v)[K], int64_t (&all)[K], in
   }
 }
 
-// Lays the jobs out.  An item's tiles are cut into segments of at most `length` tiles:
-// one tile each when all units (group x tile) fit the grid, else the best of a few lengths by
-// the time that the busiest CTA takes.
-template <int Threads>
+// Lays the jobs out.  An item's tiles are cut into segments of at most `length` tiles: one
+// tile each when all units (group x tile) fit the grid, else the best of a few lengths by the
+// time that the busiest CTA takes.  Jobs with long segments come first in the list, so that a
+// CTA with a long one gets a short one next; within that their order does not matter.
+// Threads: 256 for up to 1024 requests, whose sequences are then kept in shared memory.
+constexpr int kPlanCached = 1024, kPlanBuckets = 64;
+template <int Threads, bool Cached>
 __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
-  extern __shared__ int32_t plan_smem[];
-  int32_t* starts = plan_smem;               // [batch + 1] first request of each run
-  int32_t* cu_jobs = starts + a.batch + 1;   // [2 batch + 1] jobs before each item
-  int32_t* parts = a.places + a.batch;       // [2 batch] where its partials are
-  __shared__ int64_t sums[2][5][32];
-  __shared__ unsigned long long counted[kPlanWaves];
-  __shared__ int longest;
-  const int tid = threadIdx.x;
+  extern __shared__ int32_t plan_smem[];     // [batch + 1] first request of each run
+  int32_t* starts = plan_smem;
+  int32_t* parts = a.places + a.batch;       // [2 batch] where an item's partials are
+  __shared__ PrefixSeq cache[Cached ? kPlanCached : 1];
+  __shared__ int64_t sums[2][3][32];
+  __shared__ unsigned long long totals[2];   // units, rows
+  __shared__ int counted[kPlanTried], longest, bucket[kPlanBuckets];
+  const int tid = threadIdx.x, lane = tid & 31;
+  pdl_launch_dependents();
   const int per = (a.batch + Threads - 1) / Threads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-  if (tid < kPlanWaves) counted[tid] = 0;
-  if (tid == 0) longest = 0;
+  if (tid < kPlanTried) counted[tid] = 0;
+  if (tid < kPlanBuckets) bucket[tid] = 0;
+  if (tid == 0) longest = 0, totals[0] = totals[1] = 0;
+  auto seq = [&](int b) {
+    if constexpr (Cached) return cache[b];
+    else return prefix_seq(a, b);
+  };
   // ---- the runs
+  if constexpr (Cached) {
+    for (int b = tid; b < a.batch; b += Threads) cache[b] = prefix_seq(a, b);
+    __syncthreads();
+  }
+  auto starts_run = [&](int b) { return b == 0 || !prefix_continues(seq(b - 1), seq(b)); };
   int64_t first[1] = {0}, found[1];
   bool fine = true;
   for (int b = b0; b < b1; ++b) {
-    first[0] += prefix_starts(a, b);
-    if (!prefix_seq(a, b).ok) {
+    first[0] += starts_run(b);
+    if (!seq(b).ok) {
       fine = false;
       flag(a.err, DSR_ERR_ID);
     }
@@ -182,36 +196,49 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
   plan_scan<Threads>(first, found, sums[0]);
   const int run0 = int(first[0]), runs = int(found[0]);
   for (int b = b0, r = run0; b < b1; ++b)
-    if (prefix_starts(a, b)) starts[r++] = b;
+    if (starts_run(b)) starts[r++] = b;
   if (tid == 0) starts[runs] = a.batch;
   fine = __syncthreads_and(fine);
   // ---- what the pairs take: units, records, rows; and the units and rows of all items
   const int items = runs + a.batch;
-  auto item = [&](int i) { return i < runs ? run_item(a, starts[i], starts[i + 1], false) : own_item(a, i - runs); };
+  auto run = [&](int r, bool paired) { return run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), paired); };
+  auto item = [&](int i) { return i < runs ? run(i, false) : own_item(a, i - runs, seq(i - runs)); };
   const int per_item = (items + Threads - 1) / Threads, per_run = (runs + Threads - 1) / Threads;
   const int i0 = min(tid * per_item, items), i1 = min(i0 + per_item, items);
   const int r0 = min(tid * per_run, runs), r1 = min(r0 + per_run, runs);
-  int64_t v[5] = {}, all[5];
-  if (a.pairs > 0)
+  {
+    int most = 0;
+    int64_t units = 0, rows = 0;
+    for (int i = i0; i < i1; ++i) {
+      const PrefixItem it = item(i);
+      units += int64_t(it.groups) * it.tiles;
+      rows += it.groups > 0 ? it.rows : 0;
+      most = max(most, it.tiles);
+    }
+    most = __reduce_max_sync(~0u, most);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) units += __shfl_xor_sync(~0u, units, d), rows += __shfl_xor_sync(~0u, rows, d);
+    if (lane == 0 && most > 0) {
+      atomicMax(&longest, most);
+      atomicAdd(totals, (unsigned long long)units);
+      atomicAdd(totals + 1, (unsigned long long)rows);
+    }
+  }
+  int64_t v[3] = {}, all[3] = {};
+  if (a.pairs > 0) {
     for (int r = r0; r < r1; ++r) {
-      const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
+      const PrefixItem it = run(r, true);
       v[0] += int64_t(it.groups) * it.tiles;
       v[1] += it.groups > 0;
       v[2] += it.rows;
     }
-  int most = 0;
-  for (int i = i0; i < i1; ++i) {
-    const PrefixItem it = item(i);
-    v[3] += int64_t(it.groups) * it.tiles;
-    v[4] += it.groups > 0 ? it.rows : 0;
-    most = max(most, it.tiles);
+    plan_scan<Threads>(v, all, sums[1]);
+  } else {
+    __syncthreads();
   }
-  most = __reduce_max_sync(~0u, most);
-  if ((tid & 31) == 0) atomicMax(&longest, most);
-  plan_scan<Threads>(v, all, sums[1]);
-  const int64_t share = a.pairs > 0 ? (all[0] + a.pairs - 1) / a.pairs : 0, units = all[3];
+  const int64_t share = a.pairs > 0 ? (all[0] + a.pairs - 1) / a.pairs : 0, units = int64_t(totals[0]);
   const int32_t pair_runs = int32_t(all[1]);
-  if (all[4] > 2 * a.nodes * a.heads || all[2] > a.nodes * a.heads || share > INT32_MAX) {
+  if (int64_t(totals[1]) > 2 * a.nodes * a.heads || all[2] > a.nodes * a.heads || share > INT32_MAX) {
     // sums in disorder that give rows to several requests, more than there are partials for
     if (tid == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
     for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
@@ -219,7 +246,7 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
   }
   if (a.pairs > 0)
     for (int r = r0; r < r1; ++r) {
-      const PrefixItem it = run_item(a, starts[r], starts[r + 1], true);
+      const PrefixItem it = run(r, true);
       a.places[r] = it.groups > 0 ? int32_t(v[1]) : -1;
       if (it.groups == 0) continue;
       a.pair_runs[v[1]] = PairRun{v[0], it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows, it.table,
@@ -232,78 +259,109 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
   auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
   int32_t length = 1;
   if (units > a.ctas) {
-    int32_t tried[kPlanWaves];
-    int64_t jobs[kPlanWaves] = {};
+    int32_t tried[kPlanTried], jobs[kPlanTried] = {};  // at most kPlanWaves * ctas more than groups
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) {
+    for (int w = 0; w < kPlanTried; ++w) {
       const int64_t room = int64_t(w + 1) * a.ctas;
-      tried[w] = int32_t(min((units + room - 1) / room, int64_t(1) << 24));  // no item has more tiles
+      // the even share of so many jobs a CTA, or no cut at all
+      tried[w] = w < kPlanWaves ? int32_t(min((units + room - 1) / room, int64_t(longest))) : longest;
     }
     for (int i = i0; i < i1; ++i) {
       const PrefixItem it = item(i);
 #pragma unroll
-      for (int w = 0; w < kPlanWaves; ++w) jobs[w] += int64_t(it.groups) * segments(it.tiles, tried[w]);
+      for (int w = 0; w < kPlanTried; ++w) jobs[w] += it.groups * segments(it.tiles, tried[w]);
     }
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w)
-      if (jobs[w] > 0) atomicAdd(counted + w, (unsigned long long)jobs[w]);
+    for (int w = 0; w < kPlanTried; ++w) {
+      jobs[w] = __reduce_add_sync(~0u, jobs[w]);
+      if (lane == 0) atomicAdd(counted + w, jobs[w]);
+    }
     __syncthreads();
     float best = CUDART_INF_F;
 #pragma unroll
-    for (int w = 0; w < kPlanWaves; ++w) {
-      // a job costs some 8 tiles beside its own: first copies, output, its part of the join
-      const float rounds = ceilf(float(counted[w]) / float(a.ctas));
-      const float time = rounds * (float(min(tried[w], longest)) + 8.f);
+    for (int w = 0; w < kPlanTried; ++w) {
+      // the longest job, or a CTA's share of all
+      const float time = fmaxf(float(tried[w]) + kPlanJobTiles,
+                               (float(units) + kPlanJobTiles * float(counted[w])) / float(a.ctas));
       if (time < best) best = time, length = tried[w];
     }
   }
-  // ---- jobs and partials before each item
-  int64_t at[2] = {}, totals[2];
+  // ---- partials before each item, and the jobs of each length of segments
+  int64_t at[1] = {}, parts_all[1];
+  auto bucket_of = [&](const PrefixItem& it, int32_t n) {
+    // a segment's share of the longest
+    return kPlanBuckets - 1 - min(int(float(it.tiles) * float(kPlanBuckets - 1) / (float(n) * float(length))), kPlanBuckets - 1);
+  };
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
     const int32_t n = segments(it.tiles, length);
-    at[0] += int64_t(it.groups) * n;
-    at[1] += int64_t(it.rows) * n;
+    at[0] += int64_t(it.rows) * n;
+    if (n > 0) atomicAdd(bucket + bucket_of(it, n), it.groups * n);
   }
-  plan_scan<Threads>(at, totals, sums[0]);
+  plan_scan<Threads>(at, parts_all, sums[0]);
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
-    const int32_t n = segments(it.tiles, length);
-    cu_jobs[i] = int32_t(at[0]);
-    parts[i] = int32_t(at[1]);
-    at[0] += int64_t(it.groups) * n;
-    at[1] += int64_t(it.rows) * n;
-  }
-  const int32_t jobs = int32_t(totals[0]);
-  if (tid == 0) {
-    cu_jobs[items] = jobs;
-    a.head[0] = jobs, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+    parts[i] = int32_t(at[0]);
+    at[0] += int64_t(it.rows) * segments(it.tiles, length);
   }
   __syncthreads();
+  if (tid < 32) {  // jobs before each bucket
+    static_assert(kPlanBuckets == 64, "two a lane");
+    const int x = bucket[2 * tid], y = bucket[2 * tid + 1];
+    int sum = x + y;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, sum, d);
+      if (tid >= d) sum += up;
+    }
+    bucket[2 * tid] = sum - x - y;
+    bucket[2 * tid + 1] = sum - y;
+    if (tid == 31) a.head[0] = sum, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+  }
+  __syncthreads();
+  // ---- the jobs: a warp takes 32 items at a time.  An item's segments come one after another,
+  // the groups of one side by side
+  for (int base = (tid - lane); base < items; base += Threads) {
+    PrefixItem it{};
+    int32_t n = 0, place = 0;
+    if (base + lane < items) {
+      it = item(base + lane);
+      n = segments(it.tiles, length);
+      if (n > 0) place = atomicAdd(bucket + bucket_of(it, n), it.groups * n);
+    }
+    int upto = it.groups * n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += up;
+    }
+    const int jobs = __shfl_sync(~0u, upto, 31), before = upto - it.groups * n;
+    for (int j0 = 0; j0 < jobs; j0 += 32) {
+      const int j = j0 + lane;
+      int lo = 0;  // the first item whose jobs end behind j
+#pragma unroll
+      for (int d = 16; d; d >>= 1)
+        if (__shfl_sync(~0u, upto, lo + d - 1) <= j) lo += d;
+      lo = min(lo, 31);
+      const int32_t in = j - __shfl_sync(~0u, before, lo), to = __shfl_sync(~0u, place, lo) + in;
+      const int32_t count = __shfl_sync(~0u, n, lo);
+      if (j >= jobs) continue;
+      const PrefixItem own = item(base + lo);
+      const int32_t segment = in / own.groups, group = in - segment * own.groups;
+      const int32_t whole = own.tiles / count, longer = own.tiles - whole * count, row0 = group * a.rows;
+      a.jobs[to] = TreeJob{own.table, own.block0, own.node0, row0, min(a.rows, own.rows - row0), own.drafts, own.context,
+                           segment * whole + min(segment, longer), whole + (segment < longer),
+                           parts[base + lo] + segment * own.rows + row0, {}};
+    }
+  }
   // ---- the requests' records
   for (int b = b0, r = run0 - 1; b < b1; ++b) {
     if (r + 1 < runs && starts[r + 1] == b) ++r;
-    const PrefixItem it = own_item(a, b), run = run_item(a, starts[r], starts[r + 1], false);
-    const PrefixSeq s = prefix_seq(a, b);
+    const PrefixSeq s = seq(b);
+    const PrefixItem it = own_item(a, b, s), shared = run(r, false);
     const int paired = a.pairs > 0 ? a.places[r] : -1;
-    a.requests[b] = PrefixRequest{s.node0, s.nodes, parts[runs + b], segments(it.tiles, length), parts[r], run.rows,
-                                  paired >= 0 ? -1 - paired : segments(run.tiles, length), run.node0};
-  }
-  // ---- the jobs: an item's segments one after another, the groups of one side by side
-  for (int32_t j = tid; j < jobs; j += Threads) {
-    int lo = 0, hi = items;  // cu_jobs[lo] <= j < cu_jobs[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (cu_jobs[mid] <= j) lo = mid;
-      else hi = mid;
-    }
-    const PrefixItem it = item(lo);
-    const int32_t n = segments(it.tiles, length), in = j - cu_jobs[lo];
-    const int32_t segment = in / it.groups, group = in - segment * it.groups;
-    const int32_t whole = it.tiles / n, longer = it.tiles - whole * n, row0 = group * a.rows;
-    a.jobs[j] = TreeJob{it.table, it.block0, it.node0, row0, min(a.rows, it.rows - row0), it.drafts, it.context,
-                        segment * whole + min(segment, longer), whole + (segment < longer),
-                        parts[lo] + segment * it.rows + row0, {}};
+    a.requests[b] = PrefixRequest{s.node0, s.nodes, parts[runs + b], segments(it.tiles, length), parts[r], shared.rows,
+                                  paired >= 0 ? -1 - paired : segments(shared.tiles, length), shared.node0};
   }
 }
 
@@ -891,16 +949,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // Joins the parts of a row: one CTA per four query rows (of one node, since heads come in
 // sixteens) and 128 value columns, a thread one column of all four.
 // ---------------------------------------------------------------------------
-constexpr int kJoinThreads = 128, kJoinBatch = 8;  // kJoinBatch: parts requested together
+constexpr int kJoinThreads = 128, kJoinValues = 8;  // kJoinValues: of the parts, requested together
 constexpr int kJoinMaxParts = kPlanWaves * kTreeMaxCtas + 16;
 
+template <int Columns>
 __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
+  constexpr int kBatch = kJoinValues / Columns;  // parts requested together
   __shared__ float weight[4][kJoinMaxParts];
   __shared__ float inverse[4];
   __shared__ int owner;
   const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
-  const int tid = threadIdx.x, d = blockIdx.y * kJoinThreads + tid;
+  const int tid = threadIdx.x, d = blockIdx.y * Columns * kJoinThreads + tid;  // the first column
   // the request of the node: the largest b with cu_nodes[b] <= node, 32 ways a step
   int lo = 0;
   for (int n = a.batch; n > 1;) {
@@ -933,8 +993,8 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
     }
     if (lo < 0) {
       if (!a.zero_unused) return;
-      for (int y = 0; y < 4; ++y) {
-        const int64_t at = (row + y) * DSR_V_DIM + d;
+      for (int x = 0; x < 4 * Columns; ++x) {
+        const int64_t at = (row + x % 4) * DSR_V_DIM + d + x / 4 * kJoinThreads;
         if (a.out_wide) static_cast<float*>(a.out)[at] = 0.f;
         else static_cast<uint16_t*>(a.out)[at] = 0;
       }
@@ -958,11 +1018,15 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
   }
   const int own = s.own_segments, parts = own + s.run_segments;
   auto place = [&](int p) { return p < own ? own0 + int64_t(p) * own_rows : run0 + int64_t(p - own) * s.run_rows; };
-  float4 v[kJoinBatch];
+  float4 v[kBatch][Columns];
   auto request = [&](int p0) {
 #pragma unroll
-    for (int j = 0; j < kJoinBatch; ++j)
-      if (p0 + j < parts) v[j] = __ldcg(reinterpret_cast<const float4*>(a.part_o + place(p0 + j) * DSR_V_DIM) + d);
+    for (int j = 0; j < kBatch; ++j)
+      if (p0 + j < parts) {
+        const float4* from = reinterpret_cast<const float4*>(a.part_o + place(p0 + j) * DSR_V_DIM) + d;
+#pragma unroll
+        for (int c = 0; c < Columns; ++c) v[j][c] = __ldcg(from + c * kJoinThreads);
+      }
   };
   request(0);
   {
@@ -989,24 +1053,33 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
     }
   }
   __syncthreads();
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += kJoinBatch) {
+  float4 acc[Columns];
+#pragma unroll
+  for (int c = 0; c < Columns; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += kBatch) {
     if (p0 > 0) request(p0);
 #pragma unroll
-    for (int j = 0; j < kJoinBatch; ++j)
-      if (p0 + j < parts) {
-        acc.x = fmaf(weight[0][p0 + j], v[j].x, acc.x), acc.y = fmaf(weight[1][p0 + j], v[j].y, acc.y);
-        acc.z = fmaf(weight[2][p0 + j], v[j].z, acc.z), acc.w = fmaf(weight[3][p0 + j], v[j].w, acc.w);
-      }
-  }
-  const float out[4] = {acc.x * inverse[0], acc.y * inverse[1], acc.z * inverse[2], acc.w * inverse[3]};
+    for (int j = 0; j < kBatch; ++j)
+      if (p0 + j < parts)
 #pragma unroll
-  for (int y = 0; y < 4; ++y) {
-    if (!isfinite(out[y])) flag(a.err, DSR_ERR_NONFINITE);
-    const int64_t at = (row + y) * DSR_V_DIM + d;
-    if (a.out_wide) static_cast<float*>(a.out)[at] = out[y];
-    else static_cast<uint16_t*>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16_rn(out[y]));
+        for (int c = 0; c < Columns; ++c) {
+          acc[c].x = fmaf(weight[0][p0 + j], v[j][c].x, acc[c].x), acc[c].y = fmaf(weight[1][p0 + j], v[j][c].y, acc[c].y);
+          acc[c].z = fmaf(weight[2][p0 + j], v[j][c].z, acc[c].z), acc[c].w = fmaf(weight[3][p0 + j], v[j][c].w, acc[c].w);
+        }
   }
+  float finite = 0.f;  // stays zero
+#pragma unroll
+  for (int c = 0; c < Columns; ++c) {
+    const float out[4] = {acc[c].x * inverse[0], acc[c].y * inverse[1], acc[c].z * inverse[2], acc[c].w * inverse[3]};
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      finite = fmaf(out[y], 0.f, finite);
+      const int64_t at = (row + y) * DSR_V_DIM + d + c * kJoinThreads;
+      if (a.out_wide) static_cast<float*>(a.out)[at] = out[y];
+      else static_cast<uint16_t*>(a.out)[at] = __bfloat16_as_ushort(__float2bfloat16_rn(out[y]));
+    }
+  }
+  if (finite != 0.f) flag(a.err, DSR_ERR_NONFINITE);
 }
 
 int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaStream_t stream) {
@@ -1066,8 +1139,6 @@ PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t ma
   s.parts = s.pair_part + size_t(nodes) * heads + size_t(kPairRows) * pair_count();
   return s;
 }
-
-size_t plan_smem_bytes(int64_t batch) { return (size_t(batch) * 3 + 2) * sizeof(int32_t); }
 
 }  // namespace
 }  // namespace dsr
@@ -1149,12 +1220,14 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.pairs = nodes * heads > sizes.rows ? pair_count() : 0;  // else no run has rows enough
   a.pair_part = int32_t(sizes.pair_part);
   // few requests: scans over few warps
-  if (batch <= 1024) {
-    prefix_plan_kernel<256><<<1, 256, plan_smem_bytes(batch), as_stream(stream)>>>(a);
+  const size_t smem = size_t(batch + 1) * sizeof(int32_t);
+  if (batch <= kPlanCached) {
+    prefix_plan_kernel<256, true><<<1, 256, smem, as_stream(stream)>>>(a);
   } else {
-    rc = set_max_smem(prefix_plan_kernel<1024>, plan_smem_bytes(kPrefixMaxBatch), "prefix_mla_decode");
+    rc = set_max_smem(prefix_plan_kernel<1024, false>, size_t(kPrefixMaxBatch + 1) * sizeof(int32_t),
+                      "prefix_mla_decode");
     if (rc != DSR_OK) return rc;
-    prefix_plan_kernel<1024><<<1, 1024, plan_smem_bytes(batch), as_stream(stream)>>>(a);
+    prefix_plan_kernel<1024, false><<<1, 1024, smem, as_stream(stream)>>>(a);
   }
   rc = launch_status("prefix_mla_decode launch");
   if (rc != DSR_OK) return rc;
@@ -1184,7 +1257,9 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   rc = launch_tree_listed(call, as_stream(stream));
   if (rc != DSR_OK) return rc;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(nodes * heads / 4), DSR_V_DIM / kJoinThreads, 1);
+  // a CTA has all columns of its rows where there are rows enough to fill the SMs with those
+  const bool whole = nodes * heads / 4 >= 4 * sm_count();
+  cfg.gridDim = dim3(unsigned(nodes * heads / 4), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
   cfg.blockDim = dim3(kJoinThreads, 1, 1);
   cfg.stream = as_stream(stream);
   cudaLaunchAttribute attr[1];
@@ -1192,7 +1267,7 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, prefix_join_kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, whole ? prefix_join_kernel<4> : prefix_join_kernel<1>, a);
   if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode join launch: %s", cudaGetErrorString(e));
   return DSR_OK;
 }
