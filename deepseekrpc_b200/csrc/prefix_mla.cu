@@ -947,20 +947,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
 // ---------------------------------------------------------------------------
 // Joins the parts of a row: one CTA per four query rows (of one node, since heads come in
-// sixteens) and 128 value columns, a thread one column of all four.
+// sixteens) and 128 Columns value columns, a thread Columns of them of all four and every
+// Split-th part.  Few rows of many parts are bound by the latency of one part after another
+// (32 rows of 34 parts: 10 us by one thread a column, each after eight others).
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 128, kJoinValues = 8;  // kJoinValues: of the parts, requested together
 constexpr int kJoinMaxParts = kPlanWaves * kTreeMaxCtas + 16;
 
-template <int Columns>
-__global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
+template <int Columns, int Split>
+__global__ void __launch_bounds__(kJoinThreads * Split) prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
   constexpr int kBatch = kJoinValues / Columns;  // parts requested together
   __shared__ float weight[4][kJoinMaxParts];
-  __shared__ float inverse[4];
+  __shared__ float inverse[4], tops[4][Split], sums[4][Split];
+  __shared__ float4 others[Split > 1 ? Split - 1 : 1][Columns][kJoinThreads];
   __shared__ int owner;
   const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
-  const int tid = threadIdx.x, d = blockIdx.y * Columns * kJoinThreads + tid;  // the first column
+  const int tid = threadIdx.x, thread = tid % kJoinThreads, turn = tid / kJoinThreads;
+  const int d = blockIdx.y * Columns * kJoinThreads + thread;  // the first column
   // the request of the node: the largest b with cu_nodes[b] <= node, 32 ways a step
   int lo = 0;
   for (int n = a.batch; n > 1;) {
@@ -984,7 +988,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
     if (!__ldcg(a.head + 1)) {
       if (tid == 0) owner = -1;
       __syncthreads();
-      for (int b = tid; b < a.batch; b += kJoinThreads) {
+      for (int b = tid; b < a.batch; b += kJoinThreads * Split) {
         const PrefixRequest other = record(b);
         if (node >= other.node0 && node < other.node0 + other.nodes) atomicMax(&owner, b);
       }
@@ -992,7 +996,7 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
       lo = owner;
     }
     if (lo < 0) {
-      if (!a.zero_unused) return;
+      if (!a.zero_unused || turn > 0) return;
       for (int x = 0; x < 4 * Columns; ++x) {
         const int64_t at = (row + x % 4) * DSR_V_DIM + d + x / 4 * kJoinThreads;
         if (a.out_wide) static_cast<float*>(a.out)[at] = 0.f;
@@ -1022,50 +1026,78 @@ __global__ void __launch_bounds__(kJoinThreads) prefix_join_kernel(const __grid_
   auto request = [&](int p0) {
 #pragma unroll
     for (int j = 0; j < kBatch; ++j)
-      if (p0 + j < parts) {
-        const float4* from = reinterpret_cast<const float4*>(a.part_o + place(p0 + j) * DSR_V_DIM) + d;
+      if (p0 + j * Split < parts) {
+        const float4* from = reinterpret_cast<const float4*>(a.part_o + place(p0 + j * Split) * DSR_V_DIM) + d;
 #pragma unroll
         for (int c = 0; c < Columns; ++c) v[j][c] = __ldcg(from + c * kJoinThreads);
       }
   };
-  request(0);
+  request(turn);
+  // ---- the parts' weights: row w by the warps w + 4 k, a lane every (32 Split)-th part
+  const int w = (tid >> 5) & 3, p_first = turn + Split * (tid & 31);
   {
-    const int w = tid >> 5, lane = tid & 31;  // one warp per row
-    const float m0 = lane < parts ? __ldcg(a.part_m + place(lane) + w) : -CUDART_INF_F;
-    const float l0 = lane < parts ? __ldcg(a.part_l + place(lane) + w) : 0.f;
+    const float m0 = p_first < parts ? __ldcg(a.part_m + place(p_first) + w) : -CUDART_INF_F;
+    const float l0 = p_first < parts ? __ldcg(a.part_l + place(p_first) + w) : 0.f;
     float top = m0, sum = 0.f;
-    for (int p = lane + 32; p < parts; p += 32) top = fmaxf(top, __ldcg(a.part_m + place(p) + w));
+    for (int p = p_first + 32 * Split; p < parts; p += 32 * Split) top = fmaxf(top, __ldcg(a.part_m + place(p) + w));
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
+    if constexpr (Split > 1) {
+      if ((tid & 31) == 0) tops[w][turn] = top;
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < Split; ++k) top = fmaxf(top, tops[w][k]);
+    }
     const float base = top == -CUDART_INF_F ? 0.f : top;
-    for (int p = lane; p < parts; p += 32) {
-      const float e = ex2((p < 32 ? m0 : __ldcg(a.part_m + place(p) + w)) - base);
+    for (int p = p_first; p < parts; p += 32 * Split) {
+      const float e = ex2((p == p_first ? m0 : __ldcg(a.part_m + place(p) + w)) - base);
       weight[w][p] = e;
-      sum += e * (p < 32 ? l0 : __ldcg(a.part_l + place(p) + w));
+      sum += e * (p == p_first ? l0 : __ldcg(a.part_l + place(p) + w));
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-    if (lane == 0) {
-      float total;
-      const float lse = tree_total(a.sink, a.err, int((row + w) % a.heads), top, sum, total);
-      inverse[w] = total > 0.f ? 1.f / total : 0.f;
-      if (a.lse != nullptr && blockIdx.y == 0) a.lse[row + w] = lse;
-    }
+    if ((tid & 31) == 0) sums[w][turn] = sum, tops[w][turn] = top;
   }
   __syncthreads();
+  if (turn == 0 && (tid & 31) == 0) {
+    float total, sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < Split; ++k) sum += sums[w][k];
+    const float lse = tree_total(a.sink, a.err, int((row + w) % a.heads), tops[w][0], sum, total);
+    inverse[w] = total > 0.f ? 1.f / total : 0.f;
+    if (a.lse != nullptr && blockIdx.y == 0) a.lse[row + w] = lse;
+  }
   float4 acc[Columns];
 #pragma unroll
   for (int c = 0; c < Columns; ++c) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += kBatch) {
-    if (p0 > 0) request(p0);
+  for (int p0 = turn; p0 < parts; p0 += kBatch * Split) {
+    if (p0 > turn) request(p0);
 #pragma unroll
-    for (int j = 0; j < kBatch; ++j)
-      if (p0 + j < parts)
+    for (int j = 0; j < kBatch; ++j) {
+      const int p = p0 + j * Split;
+      if (p < parts)
 #pragma unroll
         for (int c = 0; c < Columns; ++c) {
-          acc[c].x = fmaf(weight[0][p0 + j], v[j][c].x, acc[c].x), acc[c].y = fmaf(weight[1][p0 + j], v[j][c].y, acc[c].y);
-          acc[c].z = fmaf(weight[2][p0 + j], v[j][c].z, acc[c].z), acc[c].w = fmaf(weight[3][p0 + j], v[j][c].w, acc[c].w);
+          acc[c].x = fmaf(weight[0][p], v[j][c].x, acc[c].x), acc[c].y = fmaf(weight[1][p], v[j][c].y, acc[c].y);
+          acc[c].z = fmaf(weight[2][p], v[j][c].z, acc[c].z), acc[c].w = fmaf(weight[3][p], v[j][c].w, acc[c].w);
         }
+    }
+  }
+  if constexpr (Split > 1) {
+    if (turn > 0)
+#pragma unroll
+      for (int c = 0; c < Columns; ++c) others[turn - 1][c][thread] = acc[c];
+  }
+  __syncthreads();
+  if (turn > 0) return;
+  if constexpr (Split > 1) {
+#pragma unroll
+    for (int k = 0; k < Split - 1; ++k)
+#pragma unroll
+      for (int c = 0; c < Columns; ++c) {
+        const float4 x = others[k][c][thread];
+        acc[c].x += x.x, acc[c].y += x.y, acc[c].z += x.z, acc[c].w += x.w;
+      }
   }
   float finite = 0.f;  // stays zero
 #pragma unroll
@@ -1260,14 +1292,14 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   // a CTA has all columns of its rows where there are rows enough to fill the SMs with those
   const bool whole = nodes * heads / 4 >= 4 * sm_count();
   cfg.gridDim = dim3(unsigned(nodes * heads / 4), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
-  cfg.blockDim = dim3(kJoinThreads, 1, 1);
+  cfg.blockDim = dim3(kJoinThreads * (whole ? 1 : 4), 1, 1);
   cfg.stream = as_stream(stream);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, whole ? prefix_join_kernel<4> : prefix_join_kernel<1>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, whole ? prefix_join_kernel<4, 1> : prefix_join_kernel<1, 4>, a);
   if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode join launch: %s", cudaGetErrorString(e));
   return DSR_OK;
 }
