@@ -951,12 +951,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // Split-th part.  Few rows of many parts are bound by the latency of one part after another
 // (32 rows of 34 parts: 10 us by one thread a column, each after eight others).
 // ---------------------------------------------------------------------------
-constexpr int kJoinThreads = 128, kJoinValues = 8;  // kJoinValues: of the parts, requested together
+constexpr int kJoinThreads = 128;
 constexpr int kJoinMaxParts = kPlanWaves * kTreeMaxCtas + 16;
 
-template <int Columns, int Split>
+template <int Columns, int Split, int kBatch>  // kBatch: parts requested together
 __global__ void __launch_bounds__(kJoinThreads * Split) prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
-  constexpr int kBatch = kJoinValues / Columns;  // parts requested together
   __shared__ float weight[4][kJoinMaxParts];
   __shared__ float inverse[4], tops[4][Split], sums[4][Split];
   __shared__ float4 others[Split > 1 ? Split - 1 : 1][Columns][kJoinThreads];
@@ -1288,10 +1287,15 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   call.err = err;
   rc = launch_tree_listed(call, as_stream(stream));
   if (rc != DSR_OK) return rc;
+  // a CTA has all columns of its rows where there are rows enough to fill the SMs with those;
+  // with up to eight a SM it is bound by latency, and more parts at once pay (2576 rows: 14 to
+  // 11 us), with more it is not (8192 rows: 17 and 22 us)
+  const int64_t quads = nodes * heads / 4;
+  const bool whole = quads >= 4 * sm_count();
+  const auto join = !whole ? prefix_join_kernel<1, 4, 8>
+                           : quads <= 8 * sm_count() ? prefix_join_kernel<4, 1, 4> : prefix_join_kernel<4, 1, 2>;
   cudaLaunchConfig_t cfg = {};
-  // a CTA has all columns of its rows where there are rows enough to fill the SMs with those
-  const bool whole = nodes * heads / 4 >= 4 * sm_count();
-  cfg.gridDim = dim3(unsigned(nodes * heads / 4), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
+  cfg.gridDim = dim3(unsigned(quads), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
   cfg.blockDim = dim3(kJoinThreads * (whole ? 1 : 4), 1, 1);
   cfg.stream = as_stream(stream);
   cudaLaunchAttribute attr[1];
@@ -1299,7 +1303,7 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, whole ? prefix_join_kernel<4, 1> : prefix_join_kernel<1, 4>, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a);
   if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode join launch: %s", cudaGetErrorString(e));
   return DSR_OK;
 }

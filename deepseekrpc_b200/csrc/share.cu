@@ -8,6 +8,10 @@
 // A move (source row, destination row, rows, 0) names up to one block of rows to copy.
 // The tables are changed once for all layers; dsr_paged_copy then runs per cache, or for
 // the pools of many layers at once.
+//
+// Small calls are bound by their launches: all kernels here are launched while the one
+// before them runs (programmatic dependent launch) and wait for its end before their first
+// access, and small tables are released and compacted by one CTA in one launch.
 #include "common.cuh"
 #include "host_common.h"
 
@@ -44,26 +48,26 @@ __device__ __forceinline__ int64_t ring_at(const ShareArgs& a, int64_t i) { retu
 struct Pair {
   int64_t x, y;
 };
-__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) { return Pair{a.x + b.x, a.y + b.y}; }
 
-// Exclusive sums over the CTA's threads; `all` the totals.  `part` holds one pair a warp.
+// Exclusive sums over the CTA's threads; `all` the totals.  Each warp sums up the warps'
+// totals by itself; the barrier at the end lets `part` be used again.
 template <int Threads>
 __device__ __forceinline__ Pair cta_scan(const Pair& mine, Pair* part, Pair& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  Pair run = mine;
+  auto inclusive = [&](Pair run) {
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const Pair up{__shfl_up_sync(~0u, run.x, d), __shfl_up_sync(~0u, run.y, d)};
-    if (lane >= d) run = run + up;
-  }
+    for (int d = 1; d < 32; d <<= 1) {
+      const Pair up{__shfl_up_sync(~0u, run.x, d), __shfl_up_sync(~0u, run.y, d)};
+      if (lane >= d) run.x += up.x, run.y += up.y;
+    }
+    return run;
+  };
+  const Pair run = inclusive(mine);
   if (lane == 31) part[warp] = run;
   __syncthreads();
-  Pair before{0, 0};
-  all = Pair{0, 0};
-  for (int w = 0; w < Threads / 32; ++w) {
-    if (w < warp) before = before + part[w];
-    all = all + part[w];
-  }
+  const Pair one = lane < Threads / 32 ? part[lane] : Pair{0, 0}, upto = inclusive(one);
+  all = Pair{__shfl_sync(~0u, upto.x, 31), __shfl_sync(~0u, upto.y, 31)};
+  const Pair before{__shfl_sync(~0u, upto.x - one.x, warp), __shfl_sync(~0u, upto.y - one.y, warp)};
   __syncthreads();
   return Pair{before.x + run.x - mine.x, before.y + run.y - mine.y};
 }
@@ -79,25 +83,11 @@ __device__ __forceinline__ int share_owner(const int32_t* cu, int n, int32_t i) 
   return lo;
 }
 
-// True in all threads of the last CTA to get here (a ticket in the ring state).
-__device__ __forceinline__ bool last_cta(const ShareArgs& a, int* last) {
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    *last = gridDim.x == 1;
-    if (!*last) {
-      __threadfence();
-      *last = atomicAdd(a.state + 2, 1) == int(gridDim.x) - 1;
-      __threadfence();
-    }
-  }
-  __syncthreads();
-  return *last != 0;
-}
-
 // ---------------------------------------------------------------------------
 // Fork.  Every CTA scans all requests itself, as the plan does; an entry of a child is
 // read from its parent's row, which no child's is.  held and the ring's state are written
-// by the last CTA, since all have read them.
+// by the CTA that is the last to have read them (a ticket in the ring state, drawn when a
+// CTA has its sums: it runs beside the entries).
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 512;
 
@@ -122,7 +112,9 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
   __shared__ Pair part[kForkThreads / 32];
   __shared__ int bad, last;
   const int tid = threadIdx.x;
+  pdl_launch_dependents();
   if (tid == 0) bad = 0;
+  pdl_wait();
   __syncthreads();
   const int per = (a.batch + kForkThreads - 1) / kForkThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
@@ -130,10 +122,10 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
   for (int b = b0; b < b1; ++b) {
     int32_t parent, len, need;
     if (!fork_request(a, b, parent, len, need)) bad = 1;
-    mine = mine + Pair{need, (len & (DSR_BLOCK_TOKENS - 1)) != 0};
+    mine.x += need, mine.y += (len & (DSR_BLOCK_TOKENS - 1)) != 0;
   }
-  Pair all, at = cta_scan<kForkThreads>(mine, part, all);
   const int64_t head = a.state[0], count = a.state[1];
+  Pair all, at = cta_scan<kForkThreads>(mine, part, all);
   const bool ok = bad == 0 && all.x < (int64_t(1) << 31) && all.y <= count && head >= 0 && head < a.blocks &&
                   count >= 0 && count <= a.blocks;
   if (ok) {
@@ -142,13 +134,14 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
       fork_request(a, b, parent, len, need);
       cu_entry[b] = int32_t(at.x);
       cu_take[b] = int32_t(at.y);
-      at = at + Pair{need, (len & (DSR_BLOCK_TOKENS - 1)) != 0};
+      at.x += need, at.y += (len & (DSR_BLOCK_TOKENS - 1)) != 0;
     }
     if (tid == 0) cu_entry[a.batch] = int32_t(all.x), cu_take[a.batch] = int32_t(all.y);
   } else if (blockIdx.x == 0 && tid == 0) {
     flag(a.err, DSR_ERR_ID);
   }
-  __syncthreads();
+  __syncthreads();  // all of this CTA have read
+  if (tid == 0) last = atomicAdd(a.state + 2, 1) == int(gridDim.x) - 1;
   const int64_t step = int64_t(gridDim.x) * kForkThreads, first = int64_t(blockIdx.x) * kForkThreads + tid;
   const int64_t moved = ok ? all.y : 0;
   for (int64_t i = moved + first; i < a.batch; i += step) a.moves[i] = kNoMove;
@@ -175,7 +168,8 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
       a.table[int64_t(b) * a.stride + j] = blk >= 0 && blk < a.blocks ? blk : -1;
     }
   }
-  if (!last_cta(a, &last)) return;
+  __syncthreads();
+  if (!last) return;
   if (ok) {
     for (int b = b0; b < b1; ++b)
       if (a.parent[b] >= 0) a.held[b] = blocks_of(a.lengths[b]);
@@ -188,20 +182,24 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Release, in two launches.  The first (one CTA) decides: which last blocks are shared,
-// before any count changes, and what is dropped.  The second drops the entries; the last
-// of its CTAs gives the blocks that nobody maps any more to the ring, in the order of
-// their ids, so that the order in which the counts were lowered does not matter.
-// Scratch: {ok, taken, dropped} and cu_drop[batch + 1], then a bit per freed block.
+// Release.  One CTA decides: which last blocks are shared, before any count changes, and
+// what is dropped.  Then the entries are dropped, and the blocks that nobody maps any more
+// go to the ring, in the order of their ids, so that the order in which the counts were
+// lowered does not matter.  Tables of up to kWholeEntries entries: by the same CTA, with
+// its bit per freed block in shared memory; larger ones by two more launches.
+// Scratch of two launches: {ok, taken, dropped} and cu_drop[batch + 1], then the bits.
 // ---------------------------------------------------------------------------
 constexpr int kScanThreads = 1024, kDropThreads = 512;
 constexpr int kScanPer = kShareMaxBatch / kScanThreads;
+static_assert(kScanPer <= 32, "a bit for each of a thread's requests");
+// (One CTA takes some 1 ns an entry, the second launch 5 us and more.)
+constexpr int64_t kWholeEntries = 8192, kWholeBlocks = 65536;  // bits: 8 KB
 
 struct ReleaseScratch {
   int32_t* head;      // {ok, taken, dropped}
   int32_t* cu_drop;   // [batch + 1]
   uint32_t* freed;    // [words]
-  int64_t words;      // a multiple of 4
+  int64_t words;
 };
 
 __device__ __forceinline__ void drop_block(const ShareArgs& a, uint32_t* freed, int32_t blk) {
@@ -214,12 +212,93 @@ __device__ __forceinline__ void drop_block(const ShareArgs& a, uint32_t* freed, 
   if (others <= 0) atomicOr(freed + (blk >> 5), 1u << (blk & 31));
 }
 
+// The dropped entries, `per` of a thread at a time: their chains of accesses run side by side.
+template <int Threads>
+__device__ __forceinline__ void drop_entries(const ShareArgs& a, const int32_t* cu_drop, uint32_t* freed,
+                                             int32_t dropped) {
+  constexpr int kPer = 4;
+  const int64_t step = int64_t(gridDim.x) * Threads;
+  for (int64_t i0 = int64_t(blockIdx.x) * Threads + threadIdx.x; i0 < dropped; i0 += step * kPer) {
+    int32_t blk[kPer];
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+      const int64_t i = i0 + q * step;
+      if (i >= dropped) continue;
+      const int b = share_owner(cu_drop, a.batch, int32_t(i));
+      int32_t* entry = a.table + int64_t(b) * a.stride + blocks_of(a.lengths[b]) + (int32_t(i) - cu_drop[b]);
+      blk[q] = *entry;
+      *entry = -1;
+    }
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      if (i0 + q * step < dropped) drop_block(a, freed, blk[q]);
+  }
+}
+
+// The freed blocks behind the ring's tail, held, and the ring's state.  Every CTA has a run of
+// words and counts the blocks before it itself; a warp takes a word, so that its stores are to
+// neighbours.  The state is written by the CTA that is the last to have read it (a ticket).
+// Own: the bits are this CTA's, in shared memory.
+template <int Threads, bool Own>
+__device__ __forceinline__ void free_blocks(const ShareArgs& a, const uint32_t* freed, int64_t words, int64_t taken,
+                                            Pair* part, int* last) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t head = a.state[0], count = a.state[1];
+  const int64_t slice = (words + gridDim.x - 1) / gridDim.x;
+  const int64_t w0 = min(blockIdx.x * slice, words), w1 = min(w0 + slice, words);
+  auto bits = [&](int64_t w) { return Own ? freed[w] : __ldcg(freed + w); };
+  Pair mine{0, 0}, all;  // blocks before this CTA's, and all
+  for (int64_t w = threadIdx.x; w < words; w += Threads) {
+    const int n = __popc(bits(w));
+    mine.x += w < w0 ? n : 0, mine.y += n;
+  }
+  cta_scan<Threads>(mine, part, all);  // all of this CTA have read the state
+  if (threadIdx.x == 0) *last = gridDim.x == 1 || atomicAdd(a.state + 2, 1) == int(gridDim.x) - 1;
+  int64_t to = head + count + all.x;
+  for (int64_t c = w0; c < w1; c += Threads / 32) {
+    const uint32_t word = lane < Threads / 32 && c + lane < w1 ? bits(c + lane) : 0u;
+    int upto = __popc(word);
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += up;
+    }
+    const uint32_t own = __shfl_sync(~0u, word, warp);
+    const int end = __shfl_sync(~0u, upto, warp);
+    if (own >> lane & 1) {
+      int64_t place = to + end - __popc(own >> lane);
+      while (place >= a.blocks) place -= a.blocks;
+      const int32_t blk = int32_t(c + warp) * 32 + lane;
+      a.ring[place] = blk;
+      a.shares[blk] = 0;
+    }
+    __syncwarp();
+    to += __shfl_sync(~0u, upto, 31);
+  }
+  for (int64_t b = int64_t(blockIdx.x) * Threads + threadIdx.x; b < a.batch; b += int64_t(gridDim.x) * Threads)
+    a.held[b] = blocks_of(a.lengths[b]);
+  __syncthreads();
+  if (*last && threadIdx.x == 0) {
+    const int64_t now = count - taken + all.y;
+    if (now > a.blocks) flag(a.err, DSR_ERR_ID);  // the ring held blocks that were mapped
+    a.state[0] = int32_t((head + taken) % a.blocks);
+    a.state[1] = int32_t(now < a.blocks ? now : a.blocks);
+    a.state[2] = 0;
+  }
+}
+
+template <bool Whole>
 __global__ void __launch_bounds__(kScanThreads, 1) release_scan_kernel(const ShareArgs a, const ReleaseScratch s) {
+  extern __shared__ int32_t release_smem[];  // Whole: cu_drop, then the bits
   __shared__ Pair part[kScanThreads / 32];
-  __shared__ int bad;
+  __shared__ int bad, last;
   const int tid = threadIdx.x;
+  int32_t* cu_drop = Whole ? release_smem : s.cu_drop;
+  uint32_t* freed = Whole ? reinterpret_cast<uint32_t*>(release_smem + a.batch + 1) : s.freed;
+  pdl_launch_dependents();
   if (tid == 0) bad = 0;
-  for (int64_t w = tid; w < s.words; w += kScanThreads) s.freed[w] = 0u;
+  pdl_wait();
+  for (int64_t w = tid; w < s.words; w += kScanThreads) freed[w] = 0u;
   __syncthreads();
   const int per = (a.batch + kScanThreads - 1) / kScanThreads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
@@ -236,101 +315,75 @@ __global__ void __launch_bounds__(kScanThreads, 1) release_scan_kernel(const Sha
       if (blk < 0 || blk >= a.blocks) flag(a.err, DSR_ERR_ID);
       else if (a.shares[blk] > 0) copies |= 1u << (b - b0);
     }
-    mine = mine + Pair{have - need, copies >> (b - b0) & 1};
+    mine.x += have - need, mine.y += copies >> (b - b0) & 1;
   }
-  Pair all, at = cta_scan<kScanThreads>(mine, part, all);
   const int64_t head = a.state[0], count = a.state[1];
+  Pair all, at = cta_scan<kScanThreads>(mine, part, all);
   const bool ok = bad == 0 && all.x < (int64_t(1) << 31) && all.y <= count && head >= 0 && head < a.blocks &&
                   count >= 0 && count <= a.blocks;
   const int64_t moved = ok ? all.y : 0;
   for (int64_t i = moved + tid; i < a.batch; i += kScanThreads) a.moves[i] = kNoMove;
   if (tid == 0) {
-    s.head[0] = ok;
-    s.head[1] = int32_t(moved);
-    s.head[2] = ok ? int32_t(all.x) : 0;
+    if constexpr (!Whole) {
+      s.head[0] = ok;
+      s.head[1] = int32_t(moved);
+      s.head[2] = ok ? int32_t(all.x) : 0;
+    }
     *a.count = int32_t(moved);
     if (!ok) flag(a.err, DSR_ERR_ID);
   }
-  if (ok) {
-    // every count has been read: it may change now
-    for (int b = b0; b < b1; ++b) {
-      const int32_t len = a.lengths[b], need = blocks_of(len);
-      s.cu_drop[b] = int32_t(at.x);
-      at.x += a.held[b] - need;
-      if (!(copies >> (b - b0) & 1)) continue;
-      int32_t* entry = a.table + int64_t(b) * a.stride + need - 1;
-      const int32_t source = *entry, blk = a.ring[ring_at(a, head + at.y)];
-      const bool good = blk >= 0 && blk < a.blocks;
-      if (!good) flag(a.err, DSR_ERR_ID);
-      a.moves[at.y] = good ? make_int4(source * DSR_BLOCK_TOKENS, blk * DSR_BLOCK_TOKENS,
-                                       len & (DSR_BLOCK_TOKENS - 1), 0)
-                           : kNoMove;
-      *entry = good ? blk : -1;
-      drop_block(a, s.freed, source);
-      ++at.y;
-    }
-    if (tid == 0) s.cu_drop[a.batch] = int32_t(all.x);
+  if (!ok) return;
+  // every count has been read: it may change now
+  for (int b = b0; b < b1; ++b) {
+    const int32_t len = a.lengths[b], need = blocks_of(len);
+    cu_drop[b] = int32_t(at.x);
+    at.x += a.held[b] - need;
+    if (!(copies >> (b - b0) & 1)) continue;
+    int32_t* entry = a.table + int64_t(b) * a.stride + need - 1;
+    const int32_t source = *entry, blk = a.ring[ring_at(a, head + at.y)];
+    const bool good = blk >= 0 && blk < a.blocks;
+    if (!good) flag(a.err, DSR_ERR_ID);
+    a.moves[at.y] = good ? make_int4(source * DSR_BLOCK_TOKENS, blk * DSR_BLOCK_TOKENS, len & (DSR_BLOCK_TOKENS - 1), 0)
+                         : kNoMove;
+    *entry = good ? blk : -1;
+    drop_block(a, freed, source);
+    ++at.y;
+  }
+  if (tid == 0) cu_drop[a.batch] = int32_t(all.x);
+  if constexpr (Whole) {
+    __syncthreads();
+    drop_entries<kScanThreads>(a, cu_drop, freed, int32_t(all.x));
+    __syncthreads();
+    free_blocks<kScanThreads, true>(a, freed, s.words, all.y, part, &last);
   }
 }
 
 __global__ void __launch_bounds__(kDropThreads, 1) release_drop_kernel(const ShareArgs a, const ReleaseScratch s) {
   extern __shared__ int32_t drop_smem[];  // cu_drop
+  pdl_launch_dependents();
+  pdl_wait();
+  const int32_t dropped = __ldcg(s.head + 2);
+  if (dropped == 0) return;
+  for (int b = threadIdx.x; b <= a.batch; b += kDropThreads) drop_smem[b] = __ldcg(s.cu_drop + b);
+  __syncthreads();
+  drop_entries<kDropThreads>(a, drop_smem, s.freed, dropped);
+}
+
+__global__ void __launch_bounds__(kDropThreads, 1) release_free_kernel(const ShareArgs a, const ReleaseScratch s) {
   __shared__ Pair part[kDropThreads / 32];
   __shared__ int last;
-  const int tid = threadIdx.x;
+  pdl_launch_dependents();
   pdl_wait();
-  const bool ok = __ldcg(s.head) != 0;
-  const int32_t dropped = __ldcg(s.head + 2);
-  if (ok && dropped > 0) {
-    for (int b = tid; b <= a.batch; b += kDropThreads) drop_smem[b] = __ldcg(s.cu_drop + b);
-    __syncthreads();
-    for (int64_t i = int64_t(blockIdx.x) * kDropThreads + tid; i < dropped; i += int64_t(gridDim.x) * kDropThreads) {
-      const int b = share_owner(drop_smem, a.batch, int32_t(i));
-      int32_t* entry = a.table + int64_t(b) * a.stride + blocks_of(a.lengths[b]) + (int32_t(i) - drop_smem[b]);
-      const int32_t blk = *entry;
-      *entry = -1;
-      drop_block(a, s.freed, blk);
-    }
-  }
-  if (!last_cta(a, &last)) return;
-  if (ok) {
-    const int64_t head = a.state[0], count = a.state[1], taken = __ldcg(s.head + 1);
-    int64_t free = 0;
-    // 128 blocks a thread at a time
-    for (int64_t w0 = 0; w0 < s.words; w0 += 4 * kDropThreads) {
-      const int64_t w = w0 + 4 * tid;
-      uint4 bits = make_uint4(0u, 0u, 0u, 0u);
-      if (w < s.words) bits = __ldcg(reinterpret_cast<const uint4*>(s.freed + w));
-      const int n = __popc(bits.x) + __popc(bits.y) + __popc(bits.z) + __popc(bits.w);
-      if (!__syncthreads_or(n)) continue;
-      Pair all, at = cta_scan<kDropThreads>(Pair{n, 0}, part, all);
-      int64_t to = head + count + free + at.x;
-      const uint32_t word[4] = {bits.x, bits.y, bits.z, bits.w};
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        for (uint32_t left = word[q]; left != 0; left &= left - 1, ++to) {
-          const int32_t blk = int32_t(w + q) * 32 + __ffs(left) - 1;
-          a.ring[to % a.blocks] = blk;
-          a.shares[blk] = 0;
-        }
-      free += all.x;
-    }
-    for (int b = tid; b < a.batch; b += kDropThreads) a.held[b] = blocks_of(a.lengths[b]);
-    if (tid == 0) {
-      const int64_t now = count - taken + free;
-      if (now > a.blocks) flag(a.err, DSR_ERR_ID);  // the ring held blocks that were mapped
-      a.state[0] = int32_t((head + taken) % a.blocks);
-      a.state[1] = int32_t(now < a.blocks ? now : a.blocks);
-    }
-  }
-  if (tid == 0) a.state[2] = 0;
+  if (__ldcg(s.head) == 0) return;  // alike in all CTAs
+  free_blocks<kDropThreads, false>(a, s.freed, s.words, __ldcg(s.head + 1), part, &last);
 }
 
 // ---------------------------------------------------------------------------
 // Compaction.  With L live blocks (mapped by an entry below its row's held), the i-th
 // live id from L on goes to the i-th id below L that is not live: the fewest copies, and
 // no destination is a source.  A bit per live block; every CTA sums the bits of 256-block
-// groups itself and finds ranks and free ids by search.
+// groups itself and finds ranks and free ids by search.  Tables of up to kWholeEntries
+// entries: one CTA, with its bits in shared memory, in one launch.
 // ---------------------------------------------------------------------------
 constexpr int kCompactThreads = 512;
 constexpr int kCompactMaxGroups = 32768;  // of 256 blocks: 128 KB of shared memory
@@ -341,12 +394,12 @@ struct CompactScratch {
   int groups;
 };
 
-__global__ void __launch_bounds__(kCompactThreads) compact_mark_kernel(const ShareArgs a, const CompactScratch s) {
+__device__ __forceinline__ void mark_live(const ShareArgs& a, uint32_t* live, int* bad) {
   const int64_t step = int64_t(gridDim.x) * kCompactThreads, first = int64_t(blockIdx.x) * kCompactThreads + threadIdx.x;
   for (int64_t b = first; b < a.batch; b += step)
     if (a.held[b] < 0 || a.held[b] > a.stride) {
       flag(a.err, DSR_ERR_ID);
-      *s.bad = 1;
+      *bad = 1;
     }
   for (int64_t i = first; i < int64_t(a.batch) * a.stride; i += step) {
     const int64_t b = i / a.stride;
@@ -357,25 +410,43 @@ __global__ void __launch_bounds__(kCompactThreads) compact_mark_kernel(const Sha
       continue;
     }
     const uint32_t bit = 1u << (blk & 31);
-    if (!(__ldcg(s.live + (blk >> 5)) & bit)) atomicOr(s.live + (blk >> 5), bit);
+    if (!(*reinterpret_cast<volatile uint32_t*>(live + (blk >> 5)) & bit)) atomicOr(live + (blk >> 5), bit);
   }
 }
 
+__global__ void __launch_bounds__(kCompactThreads) compact_mark_kernel(const ShareArgs a, const CompactScratch s) {
+  mark_live(a, s.live, s.bad);
+}
+
+template <bool Whole>
 __global__ void __launch_bounds__(kCompactThreads) compact_apply_kernel(const ShareArgs a, const CompactScratch s) {
-  extern __shared__ int32_t before[];  // [groups + 1] live blocks before each group
+  extern __shared__ uint4 compact_smem[];  // Whole: the bits; [groups + 1] live blocks before each group
+  uint32_t* live = Whole ? reinterpret_cast<uint32_t*>(compact_smem) : s.live;
+  int32_t* before = reinterpret_cast<int32_t*>(compact_smem + (Whole ? 2 * s.groups : 0));
   __shared__ Pair part[kCompactThreads / 32];
+  __shared__ int refused;
   const int tid = threadIdx.x;
+  pdl_launch_dependents();
   pdl_wait();
+  if constexpr (Whole) {
+    if (tid == 0) refused = 0;
+    for (int w = tid; w < 8 * s.groups; w += kCompactThreads) live[w] = 0u;
+    __syncthreads();
+    mark_live(a, live, &refused);
+  } else if (tid == 0) {
+    refused = __ldcg(s.bad);
+  }
+  __syncthreads();
   const int64_t step = int64_t(gridDim.x) * kCompactThreads, first = int64_t(blockIdx.x) * kCompactThreads + tid;
   const int64_t room = a.blocks < 2 ? 1 : a.blocks / 2;
-  if (__ldcg(s.bad) != 0) {
+  if (refused != 0) {
     for (int64_t i = first; i < room; i += step) a.moves[i] = kNoMove;
     if (first == 0) *a.count = 0;
     return;
   }
   auto words = [&](int g, uint32_t (&w)[8]) {
-    const uint4 lo = __ldcg(reinterpret_cast<const uint4*>(s.live) + 2 * g);
-    const uint4 hi = __ldcg(reinterpret_cast<const uint4*>(s.live) + 2 * g + 1);
+    const uint4* from = reinterpret_cast<const uint4*>(live) + 2 * g;
+    const uint4 lo = Whole ? from[0] : __ldcg(from), hi = Whole ? from[1] : __ldcg(from + 1);
     w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
   };
   int32_t used = 0;
@@ -443,7 +514,7 @@ __global__ void __launch_bounds__(kCompactThreads) compact_apply_kernel(const Sh
   }
   for (int64_t i = first; i < a.blocks; i += step) a.ring[i] = i < a.blocks - used ? int32_t(i) + used : -1;
   for (int64_t i = used + first; i < a.blocks; i += step) {
-    if (!(__ldcg(s.live + (i >> 5)) >> (i & 31) & 1)) continue;
+    if (!((Whole ? live[i >> 5] : __ldcg(s.live + (i >> 5))) >> (i & 31) & 1)) continue;
     const int32_t n = rank(int32_t(i)) - kept, to = hole(n);
     a.moves[n] = make_int4(int32_t(i) * DSR_BLOCK_TOKENS, to * DSR_BLOCK_TOKENS, DSR_BLOCK_TOKENS, 0);
     a.shares[to] = a.shares[i];
@@ -478,6 +549,7 @@ struct CopyArgs {
 
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constant__ CopyArgs a) {
   const int tid = threadIdx.x;
+  pdl_launch_dependents();
   pdl_wait();
   int32_t n = *a.count;
   if (n < 0 || n > a.room) {
@@ -516,7 +588,7 @@ __global__ void __launch_bounds__(kCopyThreads) copy_kernel(const __grid_constan
 }
 static_assert(kCopyPiece == 4 * 16 * kCopyThreads, "four 16-byte units a thread");
 
-int64_t freed_words(int64_t blocks) { return (blocks + 127) / 128 * 4; }
+int64_t freed_words(int64_t blocks) { return (blocks + 31) / 32; }
 int64_t live_groups(int64_t blocks) { return (blocks + 255) / 256; }
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 
@@ -541,6 +613,11 @@ int check_scratch(const void* workspace, size_t have, size_t need, const char* w
               "%s: workspace must be 256-byte aligned", what);
   DSR_REQUIRE(have >= need, "%s: workspace %zu < %zu bytes", what, have, need);
   return DSR_OK;
+}
+
+// A table that one CTA takes in one launch.
+bool whole_table(int64_t batch, int64_t stride, int64_t blocks) {
+  return batch * stride <= kWholeEntries && blocks <= kWholeBlocks;
 }
 
 // CTAs for `items` of which a thread takes `per`, up to one per SM.
@@ -586,8 +663,8 @@ extern "C" int dsr_paged_fork(const int32_t* parent, const int32_t* lengths, int
   rc = set_max_smem(fork_kernel, 2 * size_t(kShareMaxBatch + 1) * sizeof(int32_t), "paged_fork");
   if (rc != DSR_OK) return rc;
   const unsigned grid = share_grid(batch * table_stride, kForkThreads);
-  fork_kernel<<<grid, kForkThreads, 2 * size_t(batch + 1) * sizeof(int32_t), as_stream(stream)>>>(a);
-  return launch_status("paged_fork launch");
+  return launch_after(fork_kernel, grid, kForkThreads, 2 * size_t(batch + 1) * sizeof(int32_t), as_stream(stream),
+                      "paged_fork", a);
 }
 
 extern "C" size_t dsr_paged_release_workspace_bytes(int64_t batch, int64_t pool_blocks) {
@@ -613,13 +690,22 @@ extern "C" int dsr_paged_release(const int32_t* lengths, int32_t* held, int32_t*
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const ReleaseScratch s{reinterpret_cast<int32_t*>(ws), reinterpret_cast<int32_t*>(ws + 256),
                          reinterpret_cast<uint32_t*>(ws + 256 + rounded(size_t(batch + 1) * 4)), freed_words(pool_blocks)};
+  if (whole_table(batch, table_stride, pool_blocks)) {
+    const size_t smem = (size_t(batch + 1) + size_t(s.words)) * 4, most = (kShareMaxBatch + 1 + kWholeBlocks / 32) * 4;
+    rc = set_max_smem(release_scan_kernel<true>, most, "paged_release");
+    if (rc != DSR_OK) return rc;
+    return launch_after(release_scan_kernel<true>, 1, kScanThreads, smem, as_stream(stream), "paged_release", a, s);
+  }
   rc = set_max_smem(release_drop_kernel, size_t(kShareMaxBatch + 1) * sizeof(int32_t), "paged_release");
   if (rc != DSR_OK) return rc;
-  release_scan_kernel<<<1, kScanThreads, 0, as_stream(stream)>>>(a, s);
-  rc = launch_status("paged_release launch");
+  rc = launch_after(release_scan_kernel<false>, 1, kScanThreads, 0, as_stream(stream), "paged_release", a, s);
   if (rc != DSR_OK) return rc;
-  return launch_after(release_drop_kernel, share_grid(batch * table_stride, kDropThreads), kDropThreads,
-                      size_t(batch + 1) * sizeof(int32_t), as_stream(stream), "paged_release", a, s);
+  rc = launch_after(release_drop_kernel, share_grid(batch * table_stride, kDropThreads), kDropThreads,
+                    size_t(batch + 1) * sizeof(int32_t), as_stream(stream), "paged_release", a, s);
+  if (rc != DSR_OK) return rc;
+  // two words a warp and more
+  return launch_after(release_free_kernel, share_grid(s.words, 2 * kDropThreads / 32), kDropThreads, 0,
+                      as_stream(stream), "paged_release", a, s);
 }
 
 extern "C" size_t dsr_paged_compact_workspace_bytes(int64_t pool_blocks) {
@@ -644,7 +730,13 @@ extern "C" int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t ta
   if (rc != DSR_OK) return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const CompactScratch s{reinterpret_cast<uint32_t*>(ws + 256), reinterpret_cast<int32_t*>(ws), int(groups)};
-  rc = set_max_smem(compact_apply_kernel, size_t(kCompactMaxGroups + 1) * sizeof(int32_t), "paged_compact");
+  if (whole_table(batch, table_stride, pool_blocks)) {
+    const size_t smem = size_t(groups) * 36 + 4;
+    rc = set_max_smem(compact_apply_kernel<true>, kWholeBlocks / 256 * 36 + 4, "paged_compact");
+    if (rc != DSR_OK) return rc;
+    return launch_after(compact_apply_kernel<true>, 1, kCompactThreads, smem, as_stream(stream), "paged_compact", a, s);
+  }
+  rc = set_max_smem(compact_apply_kernel<false>, size_t(kCompactMaxGroups + 1) * sizeof(int32_t), "paged_compact");
   if (rc != DSR_OK) return rc;
   const cudaError_t e = cudaMemsetAsync(ws, 0, need, as_stream(stream));
   if (e != cudaSuccess) return fail(DSR_ECUDA, "paged_compact: %s", cudaGetErrorString(e));
@@ -652,7 +744,7 @@ extern "C" int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t ta
   compact_mark_kernel<<<share_grid(entries, kCompactThreads), kCompactThreads, 0, as_stream(stream)>>>(a, s);
   rc = launch_status("paged_compact launch");
   if (rc != DSR_OK) return rc;
-  return launch_after(compact_apply_kernel, share_grid(entries > pool_blocks ? entries : pool_blocks, kCompactThreads),
+  return launch_after(compact_apply_kernel<false>, share_grid(entries > pool_blocks ? entries : pool_blocks, kCompactThreads),
                       kCompactThreads, size_t(groups + 1) * sizeof(int32_t), as_stream(stream), "paged_compact", a, s);
 }
 

@@ -574,16 +574,22 @@ struct PageTables {
   }
 };
 
-// moves [n, 4] and count [1], of one allocation.
-std::pair<at::Tensor, at::Tensor> move_list(int64_t n, const at::Tensor& anchor) {
-  const at::Tensor store = fresh({4 * n + 4}, at::kInt, anchor);
+// moves [n, 4] and count [1], and a call's scratch, of one allocation.
+struct MoveList {
+  at::Tensor moves, count;
+  void* scratch;
+  size_t scratch_bytes;
+};
+MoveList move_list(int64_t n, const at::Tensor& anchor, size_t scratch_bytes = 0) {
+  const int64_t used = (4 * n + 4 + 63) / 64 * 64;  // 256 bytes
+  const at::Tensor store = fresh({used + int64_t(scratch_bytes + 3) / 4}, at::kInt, anchor);
   const auto part = [&](int64_t offset, at::IntArrayRef sizes) {
     auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(store.storage()), store.key_set(), store.dtype());
     t.unsafeGetTensorImpl()->set_storage_offset(offset);
     t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
     return t;
   };
-  return {part(4, {n, 4}), part(0, {1})};
+  return {part(4, {n, 4}), part(0, {1}), store.data_ptr<int32_t>() + used, scratch_bytes};
 }
 
 std::vector<at::Tensor> ds_paged_fork(at::Tensor parent, at::Tensor lengths, at::Tensor held, at::Tensor block_table,
@@ -594,12 +600,12 @@ std::vector<at::Tensor> ds_paged_fork(at::Tensor parent, at::Tensor lengths, at:
   check_vector(lengths, at::kInt, t.batch, held, "paged_fork: lengths [batch] expected");
   const c10::cuda::CUDAGuard guard(held.device());
   auto error = status_or(status, held);
-  auto [moves, count] = move_list(t.batch, held);
+  const MoveList list = move_list(t.batch, held);
   ok(dsr_paged_fork(parent.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
                     block_table.data_ptr<int32_t>(), t.stride, free_ring.data_ptr<int32_t>(),
-                    ring_state.data_ptr<int32_t>(), shares.data_ptr<int32_t>(), t.blocks, moves.data_ptr<int32_t>(),
-                    count.data_ptr<int32_t>(), error.data_ptr<int32_t>(), t.batch, current_stream()));
-  return {moves, count, error};
+                    ring_state.data_ptr<int32_t>(), shares.data_ptr<int32_t>(), t.blocks, list.moves.data_ptr<int32_t>(),
+                    list.count.data_ptr<int32_t>(), error.data_ptr<int32_t>(), t.batch, current_stream()));
+  return {list.moves, list.count, error};
 }
 
 std::vector<at::Tensor> ds_paged_release(at::Tensor lengths, at::Tensor held, at::Tensor block_table,
@@ -609,14 +615,12 @@ std::vector<at::Tensor> ds_paged_release(at::Tensor lengths, at::Tensor held, at
   check_vector(lengths, at::kInt, t.batch, held, "paged_release: lengths [batch] expected");
   const c10::cuda::CUDAGuard guard(held.device());
   auto error = status_or(status, held);
-  auto [moves, count] = move_list(t.batch, held);
-  const size_t ws_bytes = dsr_paged_release_workspace_bytes(t.batch, t.blocks);
-  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, held);
+  const MoveList list = move_list(t.batch, held, dsr_paged_release_workspace_bytes(t.batch, t.blocks));
   ok(dsr_paged_release(lengths.data_ptr<int32_t>(), held.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(),
                        t.stride, free_ring.data_ptr<int32_t>(), ring_state.data_ptr<int32_t>(),
-                       shares.data_ptr<int32_t>(), t.blocks, moves.data_ptr<int32_t>(), count.data_ptr<int32_t>(),
-                       ws.data_ptr(), ws_bytes, error.data_ptr<int32_t>(), t.batch, current_stream()));
-  return {moves, count, error};
+                       shares.data_ptr<int32_t>(), t.blocks, list.moves.data_ptr<int32_t>(), list.count.data_ptr<int32_t>(),
+                       list.scratch, list.scratch_bytes, error.data_ptr<int32_t>(), t.batch, current_stream()));
+  return {list.moves, list.count, error};
 }
 
 std::vector<at::Tensor> ds_paged_compact(at::Tensor held, at::Tensor block_table, at::Tensor free_ring,
@@ -624,14 +628,13 @@ std::vector<at::Tensor> ds_paged_compact(at::Tensor held, at::Tensor block_table
   PageTables t(held, block_table, free_ring, ring_state, shares);
   const c10::cuda::CUDAGuard guard(held.device());
   auto error = status_or(status, held);
-  auto [moves, count] = move_list(std::max<int64_t>(t.blocks / 2, 1), held);
-  const size_t ws_bytes = dsr_paged_compact_workspace_bytes(t.blocks);
-  auto ws = fresh({int64_t(ws_bytes)}, at::kByte, held);
+  const MoveList list =
+      move_list(std::max<int64_t>(t.blocks / 2, 1), held, dsr_paged_compact_workspace_bytes(t.blocks));
   ok(dsr_paged_compact(held.data_ptr<int32_t>(), block_table.data_ptr<int32_t>(), t.stride,
                        free_ring.data_ptr<int32_t>(), ring_state.data_ptr<int32_t>(), shares.data_ptr<int32_t>(),
-                       t.blocks, moves.data_ptr<int32_t>(), count.data_ptr<int32_t>(), ws.data_ptr(), ws_bytes,
+                       t.blocks, list.moves.data_ptr<int32_t>(), list.count.data_ptr<int32_t>(), list.scratch, list.scratch_bytes,
                        error.data_ptr<int32_t>(), t.batch, current_stream()));
-  return {moves, count, error};
+  return {list.moves, list.count, error};
 }
 
 at::Tensor ds_paged_copy(std::vector<at::Tensor> pools, std::vector<at::Tensor> generations, at::Tensor moves,
