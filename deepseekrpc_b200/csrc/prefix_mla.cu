@@ -123,33 +123,25 @@ __device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, const Prefix
   return it;
 }
 
-// Exclusive sums of K values over the CTA's threads, and their totals.  `part` [K][32] is not
-// used by the scan before this one.
-template <int Threads, int K>
-__device__ __forceinline__ void plan_scan(int64_t (&v)[K], int64_t (&all)[K], int64_t (*part)[32]) {
-  constexpr int kWarps = Threads / 32;
+// Exclusive sums over the CTA's threads, and their total.  `part` is not used by the scan
+// before this one.
+template <int Threads, typename T>
+__device__ __forceinline__ T plan_scan(T mine, T& all, T* part) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto inclusive = [&](int64_t x) {
+  auto inclusive = [&](T x) {
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int64_t up = __shfl_up_sync(~0u, x, d);
+      const T up = __shfl_up_sync(~0u, x, d);
       if (lane >= d) x += up;
     }
     return x;
   };
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t sum = inclusive(v[k]);
-    if (lane == 31) part[k][warp] = sum;
-    v[k] = sum - v[k];
-  }
+  const T sum = inclusive(mine);
+  if (lane == 31) part[warp] = sum;
   __syncthreads();
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t mine = lane < kWarps ? part[k][lane] : 0, upto = inclusive(mine);
-    v[k] += __shfl_sync(~0u, upto - mine, warp);
-    all[k] = __shfl_sync(~0u, upto, 31);
-  }
+  const T one = lane < Threads / 32 ? part[lane] : T(0), upto = inclusive(one);
+  all = __shfl_sync(~0u, upto, 31);
+  return sum - mine + __shfl_sync(~0u, upto - one, warp);
 }
 
 // Lays the jobs out.  An item's tiles are cut into segments of at most `length` tiles: one
@@ -162,9 +154,12 @@ template <int Threads, bool Cached>
 __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
   extern __shared__ int32_t plan_smem[];     // [batch + 1] first request of each run
   int32_t* starts = plan_smem;
-  int32_t* parts = a.places + a.batch;       // [2 batch] where an item's partials are
+  __shared__ int32_t kept[Cached ? 3 * kPlanCached : 1];
+  int32_t* places = Cached ? kept : a.places;  // [batch] a run's pair run, or -1
+  int32_t* parts = places + (Cached ? kPlanCached : a.batch);  // [2 batch] where an item's partials are
   __shared__ PrefixSeq cache[Cached ? kPlanCached : 1];
-  __shared__ int64_t sums[2][3][32];
+  __shared__ int64_t sums[3][32];
+  __shared__ int32_t start_sums[32];
   __shared__ unsigned long long totals[2];   // units, rows
   __shared__ int counted[kPlanTried], longest, bucket[kPlanBuckets];
   const int tid = threadIdx.x, lane = tid & 31;
@@ -184,17 +179,16 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
     __syncthreads();
   }
   auto starts_run = [&](int b) { return b == 0 || !prefix_continues(seq(b - 1), seq(b)); };
-  int64_t first[1] = {0}, found[1];
+  int32_t first = 0, runs;
   bool fine = true;
   for (int b = b0; b < b1; ++b) {
-    first[0] += starts_run(b);
+    first += starts_run(b);
     if (!seq(b).ok) {
       fine = false;
       flag(a.err, DSR_ERR_ID);
     }
   }
-  plan_scan<Threads>(first, found, sums[0]);
-  const int run0 = int(first[0]), runs = int(found[0]);
+  const int32_t run0 = plan_scan<Threads>(first, runs, start_sums);
   for (int b = b0, r = run0; b < b1; ++b)
     if (starts_run(b)) starts[r++] = b;
   if (tid == 0) starts[runs] = a.batch;
@@ -224,21 +218,23 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
       atomicAdd(totals + 1, (unsigned long long)rows);
     }
   }
-  int64_t v[3] = {}, all[3] = {};
+  int64_t pair_unit = 0, pair_at = 0, pair_units = 0, pair_all = 0;  // units; rows and (low) records
+  constexpr int kRowsShift = 16;
+  static_assert(kPrefixMaxBatch < 1 << kRowsShift, "records of a call");
   if (a.pairs > 0) {
     for (int r = r0; r < r1; ++r) {
       const PrefixItem it = run(r, true);
-      v[0] += int64_t(it.groups) * it.tiles;
-      v[1] += it.groups > 0;
-      v[2] += it.rows;
+      pair_unit += int64_t(it.groups) * it.tiles;
+      pair_at += (int64_t(it.rows) << kRowsShift) + (it.groups > 0);
     }
-    plan_scan<Threads>(v, all, sums[1]);
+    pair_unit = plan_scan<Threads>(pair_unit, pair_units, sums[0]);
+    pair_at = plan_scan<Threads>(pair_at, pair_all, sums[1]);
   } else {
     __syncthreads();
   }
-  const int64_t share = a.pairs > 0 ? (all[0] + a.pairs - 1) / a.pairs : 0, units = int64_t(totals[0]);
-  const int32_t pair_runs = int32_t(all[1]);
-  if (int64_t(totals[1]) > 2 * a.nodes * a.heads || all[2] > a.nodes * a.heads || share > INT32_MAX) {
+  const int64_t share = a.pairs > 0 ? (pair_units + a.pairs - 1) / a.pairs : 0, units = int64_t(totals[0]);
+  const int32_t pair_runs = int32_t(pair_all & ((1 << kRowsShift) - 1));
+  if (int64_t(totals[1]) > 2 * a.nodes * a.heads || pair_all >> kRowsShift > a.nodes * a.heads || share > INT32_MAX) {
     // sums in disorder that give rows to several requests, more than there are partials for
     if (tid == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
     for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
@@ -247,13 +243,13 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
   if (a.pairs > 0)
     for (int r = r0; r < r1; ++r) {
       const PrefixItem it = run(r, true);
-      a.places[r] = it.groups > 0 ? int32_t(v[1]) : -1;
+      const int32_t record = int32_t(pair_at & ((1 << kRowsShift) - 1));
+      places[r] = it.groups > 0 ? record : -1;
       if (it.groups == 0) continue;
-      a.pair_runs[v[1]] = PairRun{v[0], it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows, it.table,
-                                  a.pair_part + int32_t(v[2])};
-      v[0] += int64_t(it.groups) * it.tiles;
-      ++v[1];
-      v[2] += it.rows;
+      a.pair_runs[record] = PairRun{pair_unit, it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows,
+                                    it.table, a.pair_part + int32_t(pair_at >> kRowsShift)};
+      pair_unit += int64_t(it.groups) * it.tiles;
+      pair_at += (int64_t(it.rows) << kRowsShift) + 1;
     }
   // ---- the segments' length
   auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
@@ -286,37 +282,50 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
       if (time < best) best = time, length = tried[w];
     }
   }
-  // ---- partials before each item, and the jobs of each length of segments
-  int64_t at[1] = {}, parts_all[1];
-  auto bucket_of = [&](const PrefixItem& it, int32_t n) {
-    // a segment's share of the longest
-    return kPlanBuckets - 1 - min(int(float(it.tiles) * float(kPlanBuckets - 1) / (float(n) * float(length))), kPlanBuckets - 1);
-  };
+  // ---- jobs and partials (low) before each item
+  int64_t at = 0, at_all;
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
     const int32_t n = segments(it.tiles, length);
-    at[0] += int64_t(it.rows) * n;
-    if (n > 0) atomicAdd(bucket + bucket_of(it, n), it.groups * n);
+    at += (int64_t(it.groups * n) << 32) + int64_t(it.rows) * n;
   }
-  plan_scan<Threads>(at, parts_all, sums[0]);
+  at = plan_scan<Threads>(at, at_all, sums[2]);
   for (int i = i0; i < i1; ++i) {
     const PrefixItem it = item(i);
-    parts[i] = int32_t(at[0]);
-    at[0] += int64_t(it.rows) * segments(it.tiles, length);
+    const int32_t n = segments(it.tiles, length);
+    parts[i] = int32_t(at & 0xffffffff);
+    at += (int64_t(it.groups * n) << 32) + int64_t(it.rows) * n;
   }
-  __syncthreads();
-  if (tid < 32) {  // jobs before each bucket
-    static_assert(kPlanBuckets == 64, "two a lane");
-    const int x = bucket[2 * tid], y = bucket[2 * tid + 1];
-    int sum = x + y;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(~0u, sum, d);
-      if (tid >= d) sum += up;
+  const int32_t jobs_all = int32_t(at_all >> 32);
+  if (tid == 0) a.head[0] = jobs_all, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+  // ---- more jobs than CTAs: by the length of their segments
+  const bool sorted = jobs_all > a.ctas;
+  auto bucket_of = [&](const PrefixItem& it, int32_t n) {
+    // a segment's share of the longest
+    const int share = int(float(it.tiles) * float(kPlanBuckets - 1) / (float(n) * float(length)));
+    return kPlanBuckets - 1 - min(share, kPlanBuckets - 1);
+  };
+  if (sorted) {
+    for (int i = i0; i < i1; ++i) {
+      const PrefixItem it = item(i);
+      const int32_t n = segments(it.tiles, length);
+      if (n > 0) atomicAdd(bucket + bucket_of(it, n), it.groups * n);
     }
-    bucket[2 * tid] = sum - x - y;
-    bucket[2 * tid + 1] = sum - y;
-    if (tid == 31) a.head[0] = sum, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
+    __syncthreads();
+    if (tid < 32) {  // jobs before each bucket
+      static_assert(kPlanBuckets == 64, "two a lane");
+      const int x = bucket[2 * tid], y = bucket[2 * tid + 1];
+      int sum = x + y;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int up = __shfl_up_sync(~0u, sum, d);
+        if (tid >= d) sum += up;
+      }
+      bucket[2 * tid] = sum - x - y;
+      bucket[2 * tid + 1] = sum - y;
+    }
+  } else if (tid == 0) {
+    bucket[0] = 0;  // in no order: one counter for all
   }
   __syncthreads();
   // ---- the jobs: a warp takes 32 items at a time.  An item's segments come one after another,
@@ -327,7 +336,7 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
     if (base + lane < items) {
       it = item(base + lane);
       n = segments(it.tiles, length);
-      if (n > 0) place = atomicAdd(bucket + bucket_of(it, n), it.groups * n);
+      if (n > 0) place = atomicAdd(bucket + (sorted ? bucket_of(it, n) : 0), it.groups * n);
     }
     int upto = it.groups * n;
 #pragma unroll
@@ -359,9 +368,137 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
     if (r + 1 < runs && starts[r + 1] == b) ++r;
     const PrefixSeq s = seq(b);
     const PrefixItem it = own_item(a, b, s), shared = run(r, false);
-    const int paired = a.pairs > 0 ? a.places[r] : -1;
+    const int paired = a.pairs > 0 ? places[r] : -1;
     a.requests[b] = PrefixRequest{s.node0, s.nodes, parts[runs + b], segments(it.tiles, length), parts[r], shared.rows,
                                   paired >= 0 ? -1 - paired : segments(shared.tiles, length), shared.node0};
+  }
+}
+
+// The same for up to 32 requests, without a barrier: lane b of every warp has request b and, if
+// one starts there, its run; each warp finds the whole plan and writes its share of the jobs
+// (7 us of the general kernel's scans become 3).
+constexpr int kFewThreads = 256;
+__global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const __grid_constant__ PrefixArgs a) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  const bool here = lane < a.batch;
+  const PrefixSeq s = here ? prefix_seq(a, lane) : PrefixSeq{0, 0, 0, 0, -1, true};
+  const bool fine = __all_sync(~0u, s.ok);
+  if (!s.ok && warp == 0) flag(a.err, DSR_ERR_ID);
+  // ---- the runs: `last` request of the one that starts here, `start` of the one this is in
+  const PrefixSeq before{0, 0, 0, __shfl_up_sync(~0u, s.shared, 1), __shfl_up_sync(~0u, s.holder, 1),
+                         __shfl_up_sync(~0u, int(s.ok), 1) != 0};
+  const bool starts = here && (lane == 0 || !prefix_continues(before, s));
+  const unsigned all_starts = __ballot_sync(~0u, starts);
+  const unsigned later = lane < 31 ? all_starts >> (lane + 1) : 0u;
+  const int last = later != 0 ? lane + __ffs(later) - 1 : a.batch - 1;
+  const int start = 31 - __clz(all_starts & (~0u >> (31 - lane)));
+  const PrefixSeq end{__shfl_sync(~0u, s.node0, last & 31), __shfl_sync(~0u, s.nodes, last & 31), 0, 0, 0, true};
+  const PrefixItem own = here ? own_item(a, lane, s) : PrefixItem{};
+  const PrefixItem run = starts ? run_item(a, s, end, false) : PrefixItem{};
+  const PrefixItem paired = starts && a.pairs > 0 ? run_item(a, s, end, true) : PrefixItem{};
+  auto sum64 = [](int64_t x) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
+    return x;
+  };
+  auto before64 = [&](int64_t x) {  // exclusive sums
+    int64_t upto = x;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int64_t up = __shfl_up_sync(~0u, upto, d);
+      if (lane >= d) upto += up;
+    }
+    return upto - x;
+  };
+  const int64_t units = sum64(int64_t(own.groups) * own.tiles + int64_t(run.groups) * run.tiles);
+  const int32_t rows = __reduce_add_sync(~0u, (own.groups > 0 ? own.rows : 0) + (run.groups > 0 ? run.rows : 0));
+  const int32_t pair_rows = __reduce_add_sync(~0u, paired.rows);
+  const int64_t pair_units = int64_t(paired.groups) * paired.tiles, pair_all = a.pairs > 0 ? sum64(pair_units) : 0;
+  const int64_t share = a.pairs > 0 ? (pair_all + a.pairs - 1) / a.pairs : 0;
+  const unsigned pair_runs = __ballot_sync(~0u, paired.groups > 0);
+  if (rows > 2 * a.nodes * a.heads || pair_rows > a.nodes * a.heads || share > INT32_MAX) {
+    // sums in disorder that give rows to several requests, more than there are partials for
+    if (threadIdx.x == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
+    if (warp == 0 && here) a.requests[lane] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
+    return;
+  }
+  const int record = paired.groups > 0 ? __popc(pair_runs & ((1u << lane) - 1u)) : -1;
+  if (a.pairs > 0 && warp == 0) {
+    const int64_t unit0 = before64(pair_units), row0 = before64(paired.rows);
+    if (record >= 0)
+      a.pair_runs[record] = PairRun{unit0, paired.groups, paired.context / DSR_BLOCK_TOKENS, paired.node0 * a.heads,
+                                    paired.rows, paired.table, a.pair_part + int32_t(row0)};
+  }
+  // ---- the segments' length, as in the general kernel
+  auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
+  int32_t length = 1;
+  if (units > a.ctas) {
+    const int32_t longest = __reduce_max_sync(~0u, max(own.tiles, run.tiles));
+    float best = CUDART_INF_F;
+#pragma unroll
+    for (int w = 0; w < kPlanTried; ++w) {
+      const int64_t room = int64_t(w + 1) * a.ctas;
+      const int32_t tried = w < kPlanWaves ? int32_t(min((units + room - 1) / room, int64_t(longest))) : longest;
+      const int32_t jobs =
+          __reduce_add_sync(~0u, own.groups * segments(own.tiles, tried) + run.groups * segments(run.tiles, tried));
+      const float time = fmaxf(float(tried) + kPlanJobTiles,
+                               (float(units) + kPlanJobTiles * float(jobs)) / float(a.ctas));
+      if (time < best) best = time, length = tried;
+    }
+  }
+  // ---- jobs and partials before each lane's run and request
+  const int32_t run_n = segments(run.tiles, length), own_n = segments(own.tiles, length);
+  const int32_t run_jobs = run.groups * run_n, own_jobs = own.groups * own_n;
+  const int64_t at = before64((int64_t(run_jobs + own_jobs) << 32) + int64_t(run.rows) * run_n + int64_t(own.rows) * own_n);
+  const int32_t first = int32_t(at >> 32), run_part = int32_t(at & 0xffffffff), own_part = run_part + run.rows * run_n;
+  const int32_t jobs = __reduce_add_sync(~0u, run_jobs + own_jobs);
+  // and their places in the list, where CTAs take several: long segments first
+  int32_t run_place = first, own_place = first + run_jobs;
+  if (jobs > a.ctas) {
+    const float run_mine = run_n > 0 ? float(run.tiles) / float(run_n) : 0.f;
+    const float own_mine = own_n > 0 ? float(own.tiles) / float(own_n) : 0.f;
+    run_place = own_place = 0;
+    for (int b = 0; b < a.batch; ++b) {  // equal ones: runs before requests, then by their number
+      const float r = __shfl_sync(~0u, run_mine, b), o = __shfl_sync(~0u, own_mine, b);
+      const int32_t rn = __shfl_sync(~0u, run_jobs, b), on = __shfl_sync(~0u, own_jobs, b);
+      run_place += (r > run_mine || (r == run_mine && b < lane) ? rn : 0) + (o > run_mine ? on : 0);
+      own_place += (r >= own_mine ? rn : 0) + (o > own_mine || (o == own_mine && b < lane) ? on : 0);
+    }
+  }
+  if (threadIdx.x == 0) a.head[0] = jobs, a.head[1] = fine, a.head[2] = __popc(pair_runs), a.head[3] = int32_t(share);
+  // ---- the requests' records
+  const int32_t of_part = __shfl_sync(~0u, run_part, start & 31), of_rows = __shfl_sync(~0u, run.rows, start & 31);
+  const int32_t of_n = __shfl_sync(~0u, run_n, start & 31), of_node0 = __shfl_sync(~0u, s.node0, start & 31);
+  const int32_t of_record = __shfl_sync(~0u, record, start & 31);
+  if (warp == 0 && here)
+    a.requests[lane] = PrefixRequest{s.node0, s.nodes, own_part, own_n, of_part, of_rows,
+                                     of_record >= 0 ? -1 - of_record : of_n, of_node0};
+  // ---- the jobs: an item's segments one after another, the groups of one side by side
+  for (int32_t j0 = warp * 32; j0 < jobs; j0 += kFewThreads) {
+    const int32_t j = min(j0 + lane, jobs - 1);
+    int b = 0;  // the last lane whose jobs start at or before j
+#pragma unroll
+    for (int d = 16; d; d >>= 1)
+      if (__shfl_sync(~0u, first, (b + d) & 31) <= j && b + d < 32) b += d;
+    // (lanes without jobs start where the next one does: the last of those is the one that has j)
+    const int32_t in_lane = j - __shfl_sync(~0u, first, b), of_run = __shfl_sync(~0u, run_jobs, b);
+    const bool shared = in_lane < of_run;
+    auto pick = [&](int32_t r, int32_t o) {
+      const int32_t x = __shfl_sync(~0u, r, b), y = __shfl_sync(~0u, o, b);
+      return shared ? x : y;
+    };
+    const int32_t in = shared ? in_lane : in_lane - of_run;
+    const int32_t groups = pick(run.groups, own.groups), tiles = pick(run.tiles, own.tiles), n = pick(run_n, own_n);
+    const int32_t all_rows = pick(run.rows, own.rows), part = pick(run_part, own_part), place = pick(run_place, own_place);
+    const int32_t table = pick(run.table, lane), block0 = pick(0, own.block0), node0 = pick(run.node0, own.node0);
+    const int32_t drafts = pick(0, own.drafts), context = pick(run.context, own.context);
+    if (j0 + lane >= jobs) continue;
+    const int32_t segment = in / groups, group = in - segment * groups, row0 = group * a.rows;
+    const int32_t whole = tiles / n, longer = tiles - whole * n;
+    a.jobs[place + in] = TreeJob{table, block0, node0, row0, min(a.rows, all_rows - row0), drafts, context,
+                                 segment * whole + min(segment, longer), whole + (segment < longer),
+                                 part + segment * all_rows + row0, {}};
   }
 }
 
@@ -1252,7 +1389,9 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.pair_part = int32_t(sizes.pair_part);
   // few requests: scans over few warps
   const size_t smem = size_t(batch + 1) * sizeof(int32_t);
-  if (batch <= kPlanCached) {
+  if (batch <= 32) {
+    prefix_plan_few_kernel<<<1, kFewThreads, 0, as_stream(stream)>>>(a);
+  } else if (batch <= kPlanCached) {
     prefix_plan_kernel<256, true><<<1, 256, smem, as_stream(stream)>>>(a);
   } else {
     rc = set_max_smem(prefix_plan_kernel<1024, false>, size_t(kPrefixMaxBatch + 1) * sizeof(int32_t),
