@@ -100,7 +100,7 @@ SIGNATURES = {
     "dsr_tree_mla_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "dsr_tree_mla_decode": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, _P, _P, _P, c_int64, _P, c_float, _P, c_int,
                                     _P, _P, c_size_t, _P, c_int64, c_int64, c_int64, _P]),
-    "dsr_prefix_mla_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int64]),
+    "dsr_prefix_mla_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64]),
     "dsr_prefix_mla_decode": (c_int, [_P, c_int, _P, c_int64, _P, c_int64, c_int64, _P, _P, _P, c_int64, _P, _P, _P,
                                       c_float, _P, c_int, _P, _P, c_size_t, _P, c_int64, c_int64, c_int64, _P]),
     "dsr_sample": (c_int, [_P, c_int, c_int64, c_int64, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P]),

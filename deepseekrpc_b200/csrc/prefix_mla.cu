@@ -5,13 +5,15 @@
 //   request b attends over positions p < S_b = 64 floor(prefix_b / 64) through table row
 //   holder_b and over S_b <= p through its own; requests in a row with the same holder and
 //   S form a run, whose (node, head) pairs R are one matrix:
-//     S^T = K Q^T,  P = e^{s - m},  O = P V  over the S shared rows, for all R at once,
+//     S = Q K^T,  P = e^{s - m},  O = P V  over the S shared rows, for all R at once,
 //   and each request's own rows as there.  Every part leaves (m, l, O) in FP32; a row's
 //   parts are joined with its sink:
 //     out = sum_p 2^{m_p - M} O_p / (2^{sink - M} + sum_p 2^{m_p - M} l_p).
 //
-// Three launches without a host read: the plan of the jobs (one CTA), the attention over
-// them, the join.
+// Three launches without a host read: the plan (one CTA), the attention, the join.  More than
+// 64 query rows, or 32 requests: by pairs of CTAs in groups of 128 rows, the runs' and the
+// requests' own rows alike.  Fewer: one group has all rows of a run, and the tree attention's
+// kernel takes the jobs from a list.
 #include "common.cuh"
 #include "host_common.h"
 #include "tree_jobs.cuh"
@@ -20,35 +22,40 @@ namespace dsr {
 namespace {
 
 constexpr int kPrefixMaxBatch = 16384;
-constexpr int kPrefixTileBlocks = 2;  // 128-key tiles of 64-row blocks
+constexpr int kFewBatch = 32, kFewRows = 64;  // what the tree attention's kernel takes
 constexpr int kPlanWaves = 4, kPlanTried = kPlanWaves + 1;
 // A job's cost beside its tiles, in tiles: first copies, output, its part of the join.
 constexpr float kPlanJobTiles = 4.f;
+constexpr int kPairRows = 128;
+// The same of a piece, added to a group's tiles where the pairs share out the work.
+constexpr int kPairLead = 2;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // What the join has to know of a request: its query rows, where its own parts are, and
-// where those of its run.
+// where those of its run: part + segment * rows, or (segments < 0) item -1 - segments.
 struct alignas(16) PrefixRequest {
   int32_t node0, nodes;
-  int32_t own_part, own_segments;              // its rows' parts: own_part + segment * rows
-  int32_t run_part, run_rows, run_segments;    // its run's: run_part + segment * run_rows, or -1 - its pair run
+  int32_t own_part, own_segments;
+  int32_t run_part, run_rows, run_segments;
   int32_t run_node0;
 };
 static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
 
-// A run whose rows, in groups of 128, the pairs of CTAs take.  Its units (group x tile) are
-// numbered from unit0 on, tile by tile of one group after another; pair c has the units
-// [c share, (c + 1) share) of all runs, in one piece per group.  Piece (group g, pair c)
-// leaves its partials at part + 128 (g + c), since g or c rises from piece to piece.
-struct alignas(16) PairRun {
+// What the pairs of CTAs take: a run's shared rows, or a request's own ones.  Its query rows
+// are cut into groups of 128, whose tiles are numbered from unit0 on, kPairLead before each
+// group's first; pair c has the units [c share, (c + 1) share) of all runs, then those of all
+// requests, in one piece per group.  Piece (group g, pair c) leaves its partials at
+// part + 128 (g + c), since g or c rises from piece to piece.
+struct alignas(16) PairItem {
   int64_t unit0;
-  int32_t groups, blocks;
-  int32_t row0, rows;  // query rows
+  int32_t groups, tiles;
+  int32_t row0, rows;            // query rows
   int32_t table, part;
-  __device__ __forceinline__ int32_t tiles() const { return (blocks + kPrefixTileBlocks - 1) / kPrefixTileBlocks; }
+  int32_t block0;                // tile i: positions 64 block0 + 128 i and up
+  int32_t context, drafts, own;  // positions from `context` on are drafted, seen as the masks say
+  __device__ __forceinline__ int32_t span() const { return tiles + kPairLead; }
 };
-static_assert(sizeof(PairRun) == 32, "two 16-byte words");
-constexpr int kPairRows = 128;
+static_assert(sizeof(PairItem) == 48, "three 16-byte words");
 
 struct PrefixArgs {
   const int32_t* table;
@@ -62,17 +69,17 @@ struct PrefixArgs {
   bool out_wide, zero_unused;
   float* lse;
   int32_t* err;
-  int32_t* head;  // {jobs, 1 when no request was refused, pair runs, units of a pair}
+  int32_t* head;  // {jobs, 1 when no request was refused, 0, 0, items of runs, share, items of requests, share}
   PrefixRequest* requests;
-  PairRun* pair_runs;
-  int32_t* places;  // the plan's own: [batch] a run's pair run, [2 batch] an item's partials
+  int32_t* places;   // the plan's own: [batch] a run's item
+  PairItem* items;   // [batch] of runs, [batch] of requests
   TreeJob* jobs;
   float *part_o, *part_m, *part_l;
   int64_t nodes;
   int batch, heads, max_nodes, ctas;
-  int rows;   // of a job's group
-  int pairs;  // of CTAs that take the runs of more rows than that (0: none does)
-  int32_t pair_part;  // where their partials begin
+  int rows;              // of a job's group
+  int pairs;             // of CTAs (0: the jobs are the tree attention's)
+  int32_t own_part;      // where the partials of the requests' own items begin
 };
 
 // ---- request b: what it has to itself, and the blocks that it reads through `holder`
@@ -95,32 +102,34 @@ __device__ __forceinline__ bool prefix_continues(const PrefixSeq& before, const 
   return s.ok && before.ok && s.shared == before.shared && s.holder == before.holder;
 }
 
-// ---- an item of the plan: a run's shared rows (items 0 .. runs - 1), then a request's own
-struct PrefixItem {
-  int32_t table, block0, node0, rows, drafts, context;
-  int32_t tiles, groups;
-};
-__device__ __forceinline__ PrefixItem own_item(const PrefixArgs& a, int b, const PrefixSeq& s) {
-  PrefixItem it{b, s.shared, s.node0, s.nodes * a.heads, s.nodes, s.context, 0, 0};
+// ---- what is to do for a run, or a request's own rows, in groups of `rows` query rows
+__device__ __forceinline__ PairItem own_item(const PrefixArgs& a, int b, const PrefixSeq& s, int rows) {
+  PairItem it{};
   const int32_t keys = s.context + s.nodes - s.shared * DSR_BLOCK_TOKENS;
-  if (s.nodes > 0 && keys > 0) {
-    it.tiles = (keys + 127) / 128;
-    it.groups = (it.rows + a.rows - 1) / a.rows;
-  }
+  if (s.nodes == 0 || keys <= 0) return it;
+  it.row0 = s.node0 * a.heads, it.rows = s.nodes * a.heads;
+  it.groups = (it.rows + rows - 1) / rows;
+  it.tiles = (keys + 127) / 128;
+  it.table = b, it.block0 = s.shared;
+  it.context = s.context, it.drafts = s.nodes, it.own = 1;
   return it;
 }
-// Of a run's first and last request.  (`paired`: what the pairs take, in groups of their own
-// size, else what they do not.)
-__device__ __forceinline__ PrefixItem run_item(const PrefixArgs& a, const PrefixSeq& s, const PrefixSeq& last,
-                                               bool paired) {
-  PrefixItem it{s.holder, 0, s.node0, 0, 0, s.shared * DSR_BLOCK_TOKENS, 0, 0};
-  if (!s.ok || s.shared == 0) return it;
-  const int32_t rows = (last.node0 + last.nodes - s.node0) * a.heads;
-  if (rows == 0 || (a.pairs > 0 && rows > a.rows) != paired) return it;
-  it.rows = rows;
-  it.tiles = (s.shared + kPrefixTileBlocks - 1) / kPrefixTileBlocks;
-  it.groups = (rows + (paired ? kPairRows : a.rows) - 1) / (paired ? kPairRows : a.rows);
+// (Of a run's first and last request.)
+__device__ __forceinline__ PairItem run_item(const PrefixArgs& a, const PrefixSeq& s, const PrefixSeq& last, int rows) {
+  PairItem it{};
+  if (!s.ok || s.shared == 0 || last.node0 + last.nodes == s.node0) return it;
+  it.row0 = s.node0 * a.heads, it.rows = (last.node0 + last.nodes - s.node0) * a.heads;
+  it.groups = (it.rows + rows - 1) / rows;
+  it.tiles = (s.shared + 1) / 2;
+  it.table = s.holder;
+  it.context = s.shared * DSR_BLOCK_TOKENS;
   return it;
+}
+__device__ __forceinline__ int64_t pair_units(const PairItem& it) { return int64_t(it.groups) * it.span(); }
+__device__ __forceinline__ PairItem load_item(const PairItem* item) {
+  const int4* words = reinterpret_cast<const int4*>(item);
+  const int4 x = __ldcg(words), y = __ldcg(words + 1), z = __ldcg(words + 2);
+  return PairItem{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w, y.x, y.y, y.z, y.w, z.x, z.y, z.z, z.w};
 }
 
 // Exclusive sums over the CTA's threads, and their total.  `part` is not used by the scan
@@ -143,41 +152,55 @@ __device__ __forceinline__ T plan_scan(T mine, T& all, T* part) {
   all = __shfl_sync(~0u, upto, 31);
   return sum - mine + __shfl_sync(~0u, upto - one, warp);
 }
+// Rows and (low) items in one sum.
+constexpr int kItemBits = 16;
+static_assert(kPrefixMaxBatch < 1 << kItemBits, "items of a call");
+__device__ __forceinline__ int64_t rows_and_items(const PairItem& it) {
+  return (int64_t(it.rows) << kItemBits) + (it.groups > 0);
+}
 
-// Lays the jobs out.  An item's tiles are cut into segments of at most `length` tiles: one
-// tile each when all units (group x tile) fit the grid, else the best of a few lengths by the
-// time that the busiest CTA takes.  Jobs with long segments come first in the list, so that a
-// CTA with a long one gets a short one next; within that their order does not matter.
-// Threads: 256 for up to 1024 requests, whose sequences are then kept in shared memory.
-constexpr int kPlanCached = 1024, kPlanBuckets = 64;
+// What the pairs share: false, with nothing to do, when sums in disorder give rows to several
+// requests, more than there are partials for.
+__device__ __forceinline__ bool write_pair_head(const PrefixArgs& a, bool writes, bool fine, int64_t run_units,
+                                                int64_t run_all, int64_t own_units, int64_t own_all) {
+  const int64_t run_share = (run_units + a.pairs - 1) / a.pairs, own_share = (own_units + a.pairs - 1) / a.pairs;
+  const int64_t most = a.nodes * a.heads;
+  const bool fits = run_all >> kItemBits <= most && own_all >> kItemBits <= most && run_share <= INT32_MAX &&
+                    own_share <= INT32_MAX;
+  if (writes) {
+    constexpr int64_t kItems = (1 << kItemBits) - 1;
+    int4* head = reinterpret_cast<int4*>(a.head);
+    head[0] = make_int4(0, fits ? int(fine) : 1, 0, 0);
+    head[1] = fits ? make_int4(int(run_all & kItems), int(run_share), int(own_all & kItems), int(own_share))
+                   : make_int4(0, 0, 0, 0);
+  }
+  return fits;
+}
+
+// The plan of the pairs' work.  Threads: 256 for up to 1024 requests, whose sequences are then
+// kept in shared memory.
+constexpr int kPlanCached = 1024;
 template <int Threads, bool Cached>
 __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
-  extern __shared__ int32_t plan_smem[];     // [batch + 1] first request of each run
-  int32_t* starts = plan_smem;
-  __shared__ int32_t kept[Cached ? 3 * kPlanCached : 1];
-  int32_t* places = Cached ? kept : a.places;  // [batch] a run's pair run, or -1
-  int32_t* parts = places + (Cached ? kPlanCached : a.batch);  // [2 batch] where an item's partials are
+  extern __shared__ int32_t starts[];  // [batch + 1] first request of each run
+  __shared__ int32_t kept[Cached ? kPlanCached : 1];
+  int32_t* places = Cached ? kept : a.places;  // [batch] a run's item, or -1
   __shared__ PrefixSeq cache[Cached ? kPlanCached : 1];
-  __shared__ int64_t sums[3][32];
+  __shared__ int64_t sums[4][32];
   __shared__ int32_t start_sums[32];
-  __shared__ unsigned long long totals[2];   // units, rows
-  __shared__ int counted[kPlanTried], longest, bucket[kPlanBuckets];
-  const int tid = threadIdx.x, lane = tid & 31;
+  const int tid = threadIdx.x;
   pdl_launch_dependents();
   const int per = (a.batch + Threads - 1) / Threads;
   const int b0 = min(tid * per, a.batch), b1 = min(b0 + per, a.batch);
-  if (tid < kPlanTried) counted[tid] = 0;
-  if (tid < kPlanBuckets) bucket[tid] = 0;
-  if (tid == 0) longest = 0, totals[0] = totals[1] = 0;
   auto seq = [&](int b) {
     if constexpr (Cached) return cache[b];
     else return prefix_seq(a, b);
   };
-  // ---- the runs
   if constexpr (Cached) {
     for (int b = tid; b < a.batch; b += Threads) cache[b] = prefix_seq(a, b);
     __syncthreads();
   }
+  // ---- the runs
   auto starts_run = [&](int b) { return b == 0 || !prefix_continues(seq(b - 1), seq(b)); };
   int32_t first = 0, runs;
   bool fine = true;
@@ -193,190 +216,58 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
     if (starts_run(b)) starts[r++] = b;
   if (tid == 0) starts[runs] = a.batch;
   fine = __syncthreads_and(fine);
-  // ---- what the pairs take: units, records, rows; and the units and rows of all items
-  const int items = runs + a.batch;
-  auto run = [&](int r, bool paired) { return run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), paired); };
-  auto item = [&](int i) { return i < runs ? run(i, false) : own_item(a, i - runs, seq(i - runs)); };
-  const int per_item = (items + Threads - 1) / Threads, per_run = (runs + Threads - 1) / Threads;
-  const int i0 = min(tid * per_item, items), i1 = min(i0 + per_item, items);
+  // ---- units, rows and items before each
+  auto run = [&](int r) { return run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), kPairRows); };
+  const int per_run = (runs + Threads - 1) / Threads;
   const int r0 = min(tid * per_run, runs), r1 = min(r0 + per_run, runs);
-  {
-    int most = 0;
-    int64_t units = 0, rows = 0;
-    for (int i = i0; i < i1; ++i) {
-      const PrefixItem it = item(i);
-      units += int64_t(it.groups) * it.tiles;
-      rows += it.groups > 0 ? it.rows : 0;
-      most = max(most, it.tiles);
-    }
-    most = __reduce_max_sync(~0u, most);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) units += __shfl_xor_sync(~0u, units, d), rows += __shfl_xor_sync(~0u, rows, d);
-    if (lane == 0 && most > 0) {
-      atomicMax(&longest, most);
-      atomicAdd(totals, (unsigned long long)units);
-      atomicAdd(totals + 1, (unsigned long long)rows);
-    }
+  int64_t unit = 0, at = 0, own_unit = 0, own_at = 0, units, all, own_units, own_all;
+  for (int r = r0; r < r1; ++r) {
+    const PairItem it = run(r);
+    unit += pair_units(it), at += rows_and_items(it);
   }
-  int64_t pair_unit = 0, pair_at = 0, pair_units = 0, pair_all = 0;  // units; rows and (low) records
-  constexpr int kRowsShift = 16;
-  static_assert(kPrefixMaxBatch < 1 << kRowsShift, "records of a call");
-  if (a.pairs > 0) {
-    for (int r = r0; r < r1; ++r) {
-      const PrefixItem it = run(r, true);
-      pair_unit += int64_t(it.groups) * it.tiles;
-      pair_at += (int64_t(it.rows) << kRowsShift) + (it.groups > 0);
-    }
-    pair_unit = plan_scan<Threads>(pair_unit, pair_units, sums[0]);
-    pair_at = plan_scan<Threads>(pair_at, pair_all, sums[1]);
-  } else {
-    __syncthreads();
+  for (int b = b0; b < b1; ++b) {
+    const PairItem it = own_item(a, b, seq(b), kPairRows);
+    own_unit += pair_units(it), own_at += rows_and_items(it);
   }
-  const int64_t share = a.pairs > 0 ? (pair_units + a.pairs - 1) / a.pairs : 0, units = int64_t(totals[0]);
-  const int32_t pair_runs = int32_t(pair_all & ((1 << kRowsShift) - 1));
-  if (int64_t(totals[1]) > 2 * a.nodes * a.heads || pair_all >> kRowsShift > a.nodes * a.heads || share > INT32_MAX) {
-    // sums in disorder that give rows to several requests, more than there are partials for
-    if (tid == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
-    for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
-    return;
-  }
-  if (a.pairs > 0)
-    for (int r = r0; r < r1; ++r) {
-      const PrefixItem it = run(r, true);
-      const int32_t record = int32_t(pair_at & ((1 << kRowsShift) - 1));
-      places[r] = it.groups > 0 ? record : -1;
-      if (it.groups == 0) continue;
-      a.pair_runs[record] = PairRun{pair_unit, it.groups, it.context / DSR_BLOCK_TOKENS, it.node0 * a.heads, it.rows,
-                                    it.table, a.pair_part + int32_t(pair_at >> kRowsShift)};
-      pair_unit += int64_t(it.groups) * it.tiles;
-      pair_at += (int64_t(it.rows) << kRowsShift) + 1;
-    }
-  // ---- the segments' length
-  auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
-  int32_t length = 1;
-  if (units > a.ctas) {
-    int32_t tried[kPlanTried], jobs[kPlanTried] = {};  // at most kPlanWaves * ctas more than groups
-#pragma unroll
-    for (int w = 0; w < kPlanTried; ++w) {
-      const int64_t room = int64_t(w + 1) * a.ctas;
-      // the even share of so many jobs a CTA, or no cut at all
-      tried[w] = w < kPlanWaves ? int32_t(min((units + room - 1) / room, int64_t(longest))) : longest;
-    }
-    for (int i = i0; i < i1; ++i) {
-      const PrefixItem it = item(i);
-#pragma unroll
-      for (int w = 0; w < kPlanTried; ++w) jobs[w] += it.groups * segments(it.tiles, tried[w]);
-    }
-#pragma unroll
-    for (int w = 0; w < kPlanTried; ++w) {
-      jobs[w] = __reduce_add_sync(~0u, jobs[w]);
-      if (lane == 0) atomicAdd(counted + w, jobs[w]);
-    }
-    __syncthreads();
-    float best = CUDART_INF_F;
-#pragma unroll
-    for (int w = 0; w < kPlanTried; ++w) {
-      // the longest job, or a CTA's share of all
-      const float time = fmaxf(float(tried[w]) + kPlanJobTiles,
-                               (float(units) + kPlanJobTiles * float(counted[w])) / float(a.ctas));
-      if (time < best) best = time, length = tried[w];
-    }
-  }
-  // ---- jobs and partials (low) before each item
-  int64_t at = 0, at_all;
-  for (int i = i0; i < i1; ++i) {
-    const PrefixItem it = item(i);
-    const int32_t n = segments(it.tiles, length);
-    at += (int64_t(it.groups * n) << 32) + int64_t(it.rows) * n;
-  }
-  at = plan_scan<Threads>(at, at_all, sums[2]);
-  for (int i = i0; i < i1; ++i) {
-    const PrefixItem it = item(i);
-    const int32_t n = segments(it.tiles, length);
-    parts[i] = int32_t(at & 0xffffffff);
-    at += (int64_t(it.groups * n) << 32) + int64_t(it.rows) * n;
-  }
-  const int32_t jobs_all = int32_t(at_all >> 32);
-  if (tid == 0) a.head[0] = jobs_all, a.head[1] = fine, a.head[2] = pair_runs, a.head[3] = int32_t(share);
-  // ---- more jobs than CTAs: by the length of their segments
-  const bool sorted = jobs_all > a.ctas;
-  auto bucket_of = [&](const PrefixItem& it, int32_t n) {
-    // a segment's share of the longest
-    const int share = int(float(it.tiles) * float(kPlanBuckets - 1) / (float(n) * float(length)));
-    return kPlanBuckets - 1 - min(share, kPlanBuckets - 1);
-  };
-  if (sorted) {
-    for (int i = i0; i < i1; ++i) {
-      const PrefixItem it = item(i);
-      const int32_t n = segments(it.tiles, length);
-      if (n > 0) atomicAdd(bucket + bucket_of(it, n), it.groups * n);
-    }
-    __syncthreads();
-    if (tid < 32) {  // jobs before each bucket
-      static_assert(kPlanBuckets == 64, "two a lane");
-      const int x = bucket[2 * tid], y = bucket[2 * tid + 1];
-      int sum = x + y;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const int up = __shfl_up_sync(~0u, sum, d);
-        if (tid >= d) sum += up;
-      }
-      bucket[2 * tid] = sum - x - y;
-      bucket[2 * tid + 1] = sum - y;
-    }
-  } else if (tid == 0) {
-    bucket[0] = 0;  // in no order: one counter for all
+  unit = plan_scan<Threads>(unit, units, sums[0]);
+  at = plan_scan<Threads>(at, all, sums[1]);
+  own_unit = plan_scan<Threads>(own_unit, own_units, sums[2]);
+  own_at = plan_scan<Threads>(own_at, own_all, sums[3]);
+  const bool fits = write_pair_head(a, tid == 0, fine, units, all, own_units, own_all);
+  for (int r = r0; fits && r < r1; ++r) {
+    PairItem it = run(r);
+    const int32_t index = int32_t(at & ((1 << kItemBits) - 1));
+    places[r] = it.groups > 0 ? index : -1;
+    if (it.groups == 0) continue;
+    it.unit0 = unit, it.part = int32_t(at >> kItemBits);
+    a.items[index] = it;
+    unit += pair_units(it), at += rows_and_items(it);
   }
   __syncthreads();
-  // ---- the jobs: a warp takes 32 items at a time.  An item's segments come one after another,
-  // the groups of one side by side
-  for (int base = (tid - lane); base < items; base += Threads) {
-    PrefixItem it{};
-    int32_t n = 0, place = 0;
-    if (base + lane < items) {
-      it = item(base + lane);
-      n = segments(it.tiles, length);
-      if (n > 0) place = atomicAdd(bucket + (sorted ? bucket_of(it, n) : 0), it.groups * n);
-    }
-    int upto = it.groups * n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int up = __shfl_up_sync(~0u, upto, d);
-      if (lane >= d) upto += up;
-    }
-    const int jobs = __shfl_sync(~0u, upto, 31), before = upto - it.groups * n;
-    for (int j0 = 0; j0 < jobs; j0 += 32) {
-      const int j = j0 + lane;
-      int lo = 0;  // the first item whose jobs end behind j
-#pragma unroll
-      for (int d = 16; d; d >>= 1)
-        if (__shfl_sync(~0u, upto, lo + d - 1) <= j) lo += d;
-      lo = min(lo, 31);
-      const int32_t in = j - __shfl_sync(~0u, before, lo), to = __shfl_sync(~0u, place, lo) + in;
-      const int32_t count = __shfl_sync(~0u, n, lo);
-      if (j >= jobs) continue;
-      const PrefixItem own = item(base + lo);
-      const int32_t segment = in / own.groups, group = in - segment * own.groups;
-      const int32_t whole = own.tiles / count, longer = own.tiles - whole * count, row0 = group * a.rows;
-      a.jobs[to] = TreeJob{own.table, own.block0, own.node0, row0, min(a.rows, own.rows - row0), own.drafts, own.context,
-                           segment * whole + min(segment, longer), whole + (segment < longer),
-                           parts[base + lo] + segment * own.rows + row0, {}};
-    }
-  }
-  // ---- the requests' records
   for (int b = b0, r = run0 - 1; b < b1; ++b) {
     if (r + 1 < runs && starts[r + 1] == b) ++r;
     const PrefixSeq s = seq(b);
-    const PrefixItem it = own_item(a, b, s), shared = run(r, false);
-    const int paired = a.pairs > 0 ? places[r] : -1;
-    a.requests[b] = PrefixRequest{s.node0, s.nodes, parts[runs + b], segments(it.tiles, length), parts[r], shared.rows,
-                                  paired >= 0 ? -1 - paired : segments(shared.tiles, length), shared.node0};
+    PairItem it = own_item(a, b, s, kPairRows);
+    const int32_t index = int32_t(own_at & ((1 << kItemBits) - 1));
+    if (fits && it.groups > 0) {
+      it.unit0 = own_unit, it.part = a.own_part + int32_t(own_at >> kItemBits);
+      a.items[a.batch + index] = it;
+      own_unit += pair_units(it), own_at += rows_and_items(it);
+    }
+    a.requests[b] = !fits ? PrefixRequest{}
+                          : PrefixRequest{s.node0, s.nodes, 0, it.groups > 0 ? -1 - (a.batch + index) : 0, 0, 0,
+                                          places[r] >= 0 ? -1 - places[r] : 0, 0};
   }
 }
 
-// The same for up to 32 requests, without a barrier: lane b of every warp has request b and, if
-// one starts there, its run; each warp finds the whole plan and writes its share of the jobs
-// (7 us of the general kernel's scans become 3).
+// Up to 32 requests, without a barrier: lane b of every warp has request b and, if one starts
+// there, its run; each warp finds the whole plan and writes its share of the jobs (3 us; the
+// scans of the other kernel take 7).
+//
+// The tree attention's jobs (a.pairs == 0): a run's or a request's tiles are cut into segments
+// of at most `length` tiles: one tile each when all units (group x tile) fit the grid, else the
+// best of a few lengths by the time that the busiest CTA takes.  Jobs with long segments come
+// first in the list, so that a CTA with a long one gets a short one next.
 constexpr int kFewThreads = 256;
 __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const __grid_constant__ PrefixArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -394,54 +285,58 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
   const int last = later != 0 ? lane + __ffs(later) - 1 : a.batch - 1;
   const int start = 31 - __clz(all_starts & (~0u >> (31 - lane)));
   const PrefixSeq end{__shfl_sync(~0u, s.node0, last & 31), __shfl_sync(~0u, s.nodes, last & 31), 0, 0, 0, true};
-  const PrefixItem own = here ? own_item(a, lane, s) : PrefixItem{};
-  const PrefixItem run = starts ? run_item(a, s, end, false) : PrefixItem{};
-  const PrefixItem paired = starts && a.pairs > 0 ? run_item(a, s, end, true) : PrefixItem{};
-  auto sum64 = [](int64_t x) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(~0u, x, d);
-    return x;
-  };
-  auto before64 = [&](int64_t x) {  // exclusive sums
+  PairItem own = own_item(a, lane, s, a.rows), run = starts ? run_item(a, s, end, a.rows) : PairItem{};
+  auto before64 = [&](int64_t x, int64_t& all) {  // exclusive sums
     int64_t upto = x;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int64_t up = __shfl_up_sync(~0u, upto, d);
       if (lane >= d) upto += up;
     }
+    all = __shfl_sync(~0u, upto, 31);
     return upto - x;
   };
-  const int64_t units = sum64(int64_t(own.groups) * own.tiles + int64_t(run.groups) * run.tiles);
-  const int32_t rows = __reduce_add_sync(~0u, (own.groups > 0 ? own.rows : 0) + (run.groups > 0 ? run.rows : 0));
-  const int32_t pair_rows = __reduce_add_sync(~0u, paired.rows);
-  const int64_t pair_units = int64_t(paired.groups) * paired.tiles, pair_all = a.pairs > 0 ? sum64(pair_units) : 0;
-  const int64_t share = a.pairs > 0 ? (pair_all + a.pairs - 1) / a.pairs : 0;
-  const unsigned pair_runs = __ballot_sync(~0u, paired.groups > 0);
-  if (rows > 2 * a.nodes * a.heads || pair_rows > a.nodes * a.heads || share > INT32_MAX) {
-    // sums in disorder that give rows to several requests, more than there are partials for
-    if (threadIdx.x == 0) a.head[0] = 0, a.head[1] = 1, a.head[2] = 0, a.head[3] = 0;
-    if (warp == 0 && here) a.requests[lane] = PrefixRequest{0, 0, 0, 0, 0, 0, 0, 0};
+  int64_t run_all, own_all;
+  const int64_t run_at = before64(rows_and_items(run), run_all), own_at = before64(rows_and_items(own), own_all);
+  if (a.pairs > 0) {
+    if (warp > 0) return;
+    int64_t run_units, own_units;
+    run.unit0 = before64(pair_units(run), run_units);
+    own.unit0 = before64(pair_units(own), own_units);
+    const bool fits = write_pair_head(a, lane == 0, fine, run_units, run_all, own_units, own_all);
+    const int32_t run_index = int32_t(run_at & ((1 << kItemBits) - 1)), own_index = int32_t(own_at & ((1 << kItemBits) - 1));
+    run.part = int32_t(run_at >> kItemBits), own.part = a.own_part + int32_t(own_at >> kItemBits);
+    if (fits && run.groups > 0) a.items[run_index] = run;
+    if (fits && own.groups > 0) a.items[a.batch + own_index] = own;
+    const int32_t of = __shfl_sync(~0u, run.groups > 0 ? run_index : -1, start & 31);
+    if (here)
+      a.requests[lane] = !fits ? PrefixRequest{}
+                               : PrefixRequest{s.node0, s.nodes, 0, own.groups > 0 ? -1 - (a.batch + own_index) : 0, 0, 0,
+                                               of >= 0 ? -1 - of : 0, 0};
     return;
   }
-  const int record = paired.groups > 0 ? __popc(pair_runs & ((1u << lane) - 1u)) : -1;
-  if (a.pairs > 0 && warp == 0) {
-    const int64_t unit0 = before64(pair_units), row0 = before64(paired.rows);
-    if (record >= 0)
-      a.pair_runs[record] = PairRun{unit0, paired.groups, paired.context / DSR_BLOCK_TOKENS, paired.node0 * a.heads,
-                                    paired.rows, paired.table, a.pair_part + int32_t(row0)};
+  const int64_t most = a.nodes * a.heads;
+  if (run_all >> kItemBits > most || own_all >> kItemBits > most) {  // as in write_pair_head
+    if (threadIdx.x == 0) a.head[0] = 0, a.head[1] = 1;
+    if (warp == 0 && here) a.requests[lane] = PrefixRequest{};
+    return;
   }
-  // ---- the segments' length, as in the general kernel
+  // ---- the segments' length
   auto segments = [](int32_t tiles, int32_t length) { return (tiles + length - 1) / length; };
+  int64_t units;
+  before64(int64_t(own.groups) * own.tiles + int64_t(run.groups) * run.tiles, units);
   int32_t length = 1;
   if (units > a.ctas) {
     const int32_t longest = __reduce_max_sync(~0u, max(own.tiles, run.tiles));
     float best = CUDART_INF_F;
 #pragma unroll
     for (int w = 0; w < kPlanTried; ++w) {
+      // the even share of so many jobs a CTA, or no cut at all
       const int64_t room = int64_t(w + 1) * a.ctas;
       const int32_t tried = w < kPlanWaves ? int32_t(min((units + room - 1) / room, int64_t(longest))) : longest;
       const int32_t jobs =
           __reduce_add_sync(~0u, own.groups * segments(own.tiles, tried) + run.groups * segments(run.tiles, tried));
+      // the longest job, or a CTA's share of all
       const float time = fmaxf(float(tried) + kPlanJobTiles,
                                (float(units) + kPlanJobTiles * float(jobs)) / float(a.ctas));
       if (time < best) best = time, length = tried;
@@ -450,9 +345,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
   // ---- jobs and partials before each lane's run and request
   const int32_t run_n = segments(run.tiles, length), own_n = segments(own.tiles, length);
   const int32_t run_jobs = run.groups * run_n, own_jobs = own.groups * own_n;
-  const int64_t at = before64((int64_t(run_jobs + own_jobs) << 32) + int64_t(run.rows) * run_n + int64_t(own.rows) * own_n);
+  int64_t at_all;  // jobs, and (low) rows of partials
+  const int64_t at = before64(
+      (int64_t(run_jobs + own_jobs) << 32) + int64_t(run.rows) * run_n + int64_t(own.rows) * own_n, at_all);
   const int32_t first = int32_t(at >> 32), run_part = int32_t(at & 0xffffffff), own_part = run_part + run.rows * run_n;
-  const int32_t jobs = __reduce_add_sync(~0u, run_jobs + own_jobs);
+  const int32_t jobs = int32_t(at_all >> 32);
   // and their places in the list, where CTAs take several: long segments first
   int32_t run_place = first, own_place = first + run_jobs;
   if (jobs > a.ctas) {
@@ -466,14 +363,11 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
       own_place += (r >= own_mine ? rn : 0) + (o > own_mine || (o == own_mine && b < lane) ? on : 0);
     }
   }
-  if (threadIdx.x == 0) a.head[0] = jobs, a.head[1] = fine, a.head[2] = __popc(pair_runs), a.head[3] = int32_t(share);
+  if (threadIdx.x == 0) a.head[0] = jobs, a.head[1] = fine;
   // ---- the requests' records
   const int32_t of_part = __shfl_sync(~0u, run_part, start & 31), of_rows = __shfl_sync(~0u, run.rows, start & 31);
   const int32_t of_n = __shfl_sync(~0u, run_n, start & 31), of_node0 = __shfl_sync(~0u, s.node0, start & 31);
-  const int32_t of_record = __shfl_sync(~0u, record, start & 31);
-  if (warp == 0 && here)
-    a.requests[lane] = PrefixRequest{s.node0, s.nodes, own_part, own_n, of_part, of_rows,
-                                     of_record >= 0 ? -1 - of_record : of_n, of_node0};
+  if (warp == 0 && here) a.requests[lane] = PrefixRequest{s.node0, s.nodes, own_part, own_n, of_part, of_rows, of_n, of_node0};
   // ---- the jobs: an item's segments one after another, the groups of one side by side
   for (int32_t j0 = warp * 32; j0 < jobs; j0 += kFewThreads) {
     const int32_t j = min(j0 + lane, jobs - 1);
@@ -491,27 +385,21 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
     const int32_t in = shared ? in_lane : in_lane - of_run;
     const int32_t groups = pick(run.groups, own.groups), tiles = pick(run.tiles, own.tiles), n = pick(run_n, own_n);
     const int32_t all_rows = pick(run.rows, own.rows), part = pick(run_part, own_part), place = pick(run_place, own_place);
-    const int32_t table = pick(run.table, lane), block0 = pick(0, own.block0), node0 = pick(run.node0, own.node0);
+    const int32_t table = pick(run.table, own.table), block0 = pick(0, own.block0), first_row = pick(run.row0, own.row0);
     const int32_t drafts = pick(0, own.drafts), context = pick(run.context, own.context);
     if (j0 + lane >= jobs) continue;
     const int32_t segment = in / groups, group = in - segment * groups, row0 = group * a.rows;
     const int32_t whole = tiles / n, longer = tiles - whole * n;
-    a.jobs[place + in] = TreeJob{table, block0, node0, row0, min(a.rows, all_rows - row0), drafts, context,
+    a.jobs[place + in] = TreeJob{table, block0, first_row / a.heads, row0, min(a.rows, all_rows - row0), drafts, context,
                                  segment * whole + min(segment, longer), whole + (segment < longer),
                                  part + segment * all_rows + row0, {}};
   }
 }
 
-__device__ __forceinline__ PairRun load_pair_run(const PairRun* run) {
-  const int4* words = reinterpret_cast<const int4*>(run);
-  const int4 x = __ldcg(words), y = __ldcg(words + 1);
-  return PairRun{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w, y.x, y.y, y.z, y.w};
-}
-
 // ---------------------------------------------------------------------------
-// The shared rows of a run, by pairs of CTAs (clusters of two).  A unit is one group of 128
-// query rows x one 128-key tile, 64 rows of it in either CTA; the MMAs are the pair's
-// (cta_group::2, M = 128), issued by CTA 0:
+// The attention by pairs of CTAs (clusters of two).  A unit is one group of 128 query rows x
+// one 128-key tile, 64 rows of it in either CTA; the MMAs are the pair's (cta_group::2,
+// M = 128), issued by CTA 0:
 //   S[row, key]   = Q[row, :576] K[key, :576]      (N = 128 keys, 64 from either CTA)
 //   O[row, dim]  += P[row, key] V[key, dim]        (N = 256 dims x 2, 128 from either CTA)
 // so that an SM reads of every operand its own half only: 4 KB of shared memory for an MMA
@@ -526,7 +414,9 @@ __device__ __forceinline__ PairRun load_pair_run(const PairRun* run) {
 //   warp 4      tensor memory; in CTA 0 the MMAs: S of the next tile, then O of this one, so
 //               that they run through the softmax between
 //   warp 5      query, keys and values by TMA; what arrives in either CTA is counted by CTA
-//               0's barriers
+//               0's barriers.  Values of a request's last tiles come to a barrier of the CTA's
+//               own first: rows that no query sees may hold anything and are cleared, since
+//               0 x NaN would reach the output
 // ---------------------------------------------------------------------------
 constexpr int kPairSoftmax = 128, kPairThreads = kPairSoftmax + 64;
 constexpr int kPairKeys = 128;
@@ -541,7 +431,7 @@ struct PairLayout {
   static constexpr int kVOff = kKOff + 9 * kBlock;           // 2 passes x 2 pages x 2 blocks
   static constexpr int kPOff = kVOff + 8 * kBlock;           // 2 blocks of 64 rows x 64 keys
   static constexpr int kBarOff = kPOff + 2 * kBlock;
-  static constexpr int kBars = 2 * kKStages + 2 * 2 + 2 + 5;
+  static constexpr int kBars = 2 * kKStages + 2 * 2 + 2 + 6;
   static constexpr int kRedOff = kBarOff + (kBars * 8 + 15) / 16 * 16;  // f32[2][64]
   static constexpr int kMiscOff = kRedOff + 2 * 64 * 4;
   static constexpr int kBytes = kMiscOff + 16;
@@ -555,52 +445,63 @@ struct PairArgs {
   bool q_wide;  // fp32 (else bf16)
   const int32_t* table;
   int64_t stride, pool_rows;
+  const int64_t* masks;
   float scale_log2;
   float *part_o, *part_m, *part_l;
   const int32_t* head;
-  const PairRun* runs;
+  const PairItem* items;
   int32_t* err;
+  int batch, heads, pairs;
 };
 
-// A pair's pieces, one after another (every warp walks them for itself).
+// A pair's pieces, one after another (every warp walks them for itself): of the runs, then of
+// the requests.
 struct PairWalk {
-  const PairRun* runs;
+  const PairArgs& a;
   int64_t unit, end;
-  int32_t at, pair;
-  PairRun run;
+  int32_t at, pair, phase;  // phase: 0 runs, 1 requests
+  PairItem item;
   int32_t row0, rows, tile0, count, part;  // of the piece at hand
-  __device__ __forceinline__ PairWalk(const PairArgs& a, int pair_) : runs(a.runs), at(0), pair(pair_) {
-    const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head));
-    const int64_t share = head.w;
-    unit = share * pair;
-    end = unit;
-    if (head.z == 0) return;
-    const PairRun last = load_pair_run(runs + head.z - 1);
-    end = min(unit + share, last.unit0 + int64_t(last.groups) * last.tiles());
-    if (unit >= end) return;
-    // the last run that starts at or before the unit, 32 ways a step
-    for (int n = head.z; n > 1;) {
-      const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
-      const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&runs[at + i].unit0) <= unit);
-      const int lead = (31 - __clz(below)) * stride;
-      at += lead;
-      n = min(stride, n - lead);
-    }
-    run = load_pair_run(runs + at);
-  }
+  __device__ __forceinline__ PairWalk(const PairArgs& a_, int pair_) : a(a_), unit(0), end(0), at(0), pair(pair_), phase(-1) {}
   __device__ __forceinline__ bool next() {
-    if (unit >= end) return false;
-    if (unit >= run.unit0 + int64_t(run.groups) * run.tiles()) run = load_pair_run(runs + ++at);
-    const int64_t in = unit - run.unit0;
-    const int32_t tiles = run.tiles(), group = int32_t(in / tiles);
-    tile0 = int32_t(in - int64_t(group) * tiles);
-    count = int32_t(min(int64_t(tiles - tile0), end - unit));
-    row0 = run.row0 + group * kPairRows;
-    rows = min(kPairRows, run.rows - group * kPairRows);
-    part = run.part + (group + pair) * kPairRows;
-    unit += count;
-    return true;
+    for (;;) {
+      while (unit >= end) {  // the next phase's range, and the item that it starts in
+        if (++phase > 1) return false;
+        const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head) + 1);
+        const PairItem* items = a.items + (phase ? a.batch : 0);
+        const int32_t n_items = phase ? head.z : head.x;
+        const int64_t share = phase ? head.w : head.y;
+        unit = end = share * pair;
+        if (n_items == 0) continue;
+        const PairItem last = load_item(items + n_items - 1);
+        end = min(unit + share, last.unit0 + int64_t(last.groups) * last.span());
+        if (unit >= end) continue;
+        at = 0;  // the last item that starts at or before the unit, 32 ways a step
+        for (int n = n_items; n > 1;) {
+          const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
+          const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&items[at + i].unit0) <= unit);
+          const int lead = (31 - __clz(below)) * stride;
+          at += lead;
+          n = min(stride, n - lead);
+        }
+        item = load_item(items + at);
+      }
+      if (unit >= item.unit0 + int64_t(item.groups) * item.span()) item = load_item(a.items + (phase ? a.batch : 0) + ++at);
+      const int64_t in = unit - item.unit0;
+      const int32_t span = item.span(), group = int32_t(in / span), from = int32_t(in - int64_t(group) * span);
+      const int32_t to = int32_t(min(int64_t(span), from + (end - unit)));
+      unit += to - from;
+      tile0 = max(from - kPairLead, 0);
+      count = max(to - kPairLead, 0) - tile0;
+      row0 = item.row0 + group * kPairRows;
+      rows = min(kPairRows, item.rows - group * kPairRows);
+      part = item.part + (group + pair) * kPairRows;
+      if (count > 0) return true;
+    }
   }
+  // First position of tile i, and whether some of its positions are drafted ones or past the end.
+  __device__ __forceinline__ int32_t position(int32_t i) const { return item.block0 * DSR_BLOCK_TOKENS + i * 128; }
+  __device__ __forceinline__ bool ragged(int32_t i) const { return position(i) + 128 > item.context; }
 };
 
 // ---- barriers of a pair
@@ -718,7 +619,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
   // CTA 0's are waited for
   uint64_t* full_k = bars;                  // [kKStages] in both CTAs (TMA bytes + 1)
-  uint64_t* full_v = full_k + kKStages;     // [2]
+  uint64_t* full_v = full_k + kKStages;     // [2] (TMA bytes + 1 of either CTA)
   uint64_t* bar_p = full_v + 2;             // P written in both CTAs (a warp arrives)
   uint64_t* bar_q = bar_p + 1;              // query in place (TMA bytes + 1; FP32: a warp arrives)
   uint64_t* bar_free = bar_p + 2;           // O read by the output (a warp arrives)
@@ -728,7 +629,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   uint64_t* empty_v = empty_k + kKStages;   // [2] read by the O MMAs (commit)
   uint64_t* bar_s = empty_v + 2;            // [2] S complete (commit)
   uint64_t* bar_o = bar_s + 2;              // the tile's O MMAs complete (commit)
-  static_assert(2 * kKStages + 2 * 2 + 2 + 5 == L::kBars, "");
+  uint64_t* bar_own = bar_o + 1;            // values of a ragged tile here (TMA bytes + 1)
+  static_assert(2 * kKStages + 2 * 2 + 2 + 6 == L::kBars, "");
   float* red = reinterpret_cast<float*>(smem + L::kRedOff);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMiscOff);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::kMiscOff + 4);
@@ -740,12 +642,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     tma_prefetch_desc(&v_map);
     if (!a.q_wide) tma_prefetch_desc(&q_map);
     for (int i = 0; i < kKStages; ++i) mbar_init(full_k + i, 1), mbar_init(empty_k + i, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(full_v + i, 1), mbar_init(empty_v + i, 1), mbar_init(bar_s + i, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(full_v + i, 2), mbar_init(empty_v + i, 1), mbar_init(bar_s + i, 1);
     mbar_init(bar_p, 8);
     mbar_init(bar_q, a.q_wide ? 8 : 1);
     mbar_init(bar_free, 8);
     mbar_init(bar_end, 1);
     mbar_init(bar_o, 1);
+    mbar_init(bar_own, 1);
     *abort = 0;
     fence_barrier_init();
   }
@@ -792,7 +695,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) pair_arrive(to_q);
       }
-      const int32_t blocks = walk.run.blocks;
+      // of the drafted positions, those that this thread's row sees
+      const uint64_t word = walk.item.drafts > 0 && mine < walk.rows ? uint64_t(a.masks[(walk.row0 + mine) / a.heads]) : 0ull;
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
         ok = ok && pair_wait_warp(bar_s + (n & 1), (n >> 1) & 1, abort, a.err);
@@ -806,9 +710,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]), v[32 + c] = __uint_as_float(t1[c]);
-          if (half == 1 && kPrefixTileBlocks * (walk.tile0 + i) + 1 >= blocks) {  // the last tile has one page
+          if (walk.ragged(walk.tile0 + i)) {
+            const int32_t first = walk.position(walk.tile0 + i) + 64 * half - walk.item.context;
 #pragma unroll
-            for (int c = 0; c < 64; ++c) v[c] = -CUDART_INF_F;
+            for (int c = 0; c < 64; ++c) {
+              const int32_t d = first + c;
+              if (d >= 0 && (d >= walk.item.drafts || !(word >> d & 1))) v[c] = -CUDART_INF_F;
+            }
           }
 #pragma unroll
           for (int c = 0; c < 64; ++c) top = fmaxf(top, v[c]);
@@ -993,16 +901,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t to_k = __shfl_sync(~0u, pair_address(full_k, 0), 0);
     const uint32_t to_v = __shfl_sync(~0u, pair_address(full_v, 0), 0);
     const uint32_t to_q = __shfl_sync(~0u, pair_address(bar_q, 0), 0);
+    const uint32_t to_own = __shfl_sync(~0u, pair_address(bar_own, rank), 0);
     const bool leader = elect_lane();
-    int n = 0;
+    int n = 0, cleared = 0;
     bool ok = true;
     while (ok && walk.next()) {
-      const int32_t* table = a.table + int64_t(walk.run.table) * a.stride;
-      const int32_t blocks = walk.run.blocks;
+      const int32_t* table = a.table + int64_t(walk.item.table) * a.stride;
+      const int32_t blocks = int32_t((int64_t(walk.item.context) + walk.item.drafts + DSR_BLOCK_TOKENS - 1) /
+                                     DSR_BLOCK_TOKENS);
       const int32_t none = int32_t(a.pool_rows);  // past the pool: reads zeros
       // the tile's two pages; what a block id means is seen when they are used
       auto pages = [&](int32_t tile) {
-        const int32_t j = kPrefixTileBlocks * tile;
+        const int32_t j = walk.item.block0 + 2 * tile;
         return make_int2(j < blocks ? table[j] : INT32_MIN, j + 1 < blocks ? table[j + 1] : INT32_MIN);
       };
       auto row_of = [&](int32_t blk) {
@@ -1016,6 +926,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // The whole warp runs the loop and one lane issues, as the MMAs are: a copy from a
       // one-lane branch takes some 200 cycles to be on its way
       auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
+      // what any of the group's rows sees of the drafted positions (8 nodes at most)
+      uint64_t seen = 0;
+      if (walk.item.drafts > 0) {
+        const int32_t node = walk.row0 / a.heads + lane;
+        const uint64_t word = node <= (walk.row0 + walk.rows - 1) / a.heads ? uint64_t(a.masks[node]) : 0ull;
+        seen = uint64_t(__reduce_or_sync(~0u, uint32_t(word >> 32))) << 32 | __reduce_or_sync(~0u, uint32_t(word));
+      }
       if (!a.q_wide) {
         // the query, once the last S MMA of the piece before has read the one there
         if (n > 0) ok = wait(bar_s + ((n - 1) & 1), ((n - 1) >> 1) & 1);
@@ -1038,18 +955,37 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
         }
       };
-      auto values = [&](int k, int32_t y0, int32_t y1) {
+      auto values = [&](int k, int32_t tile, int32_t y0, int32_t y1) {
+        // a request's rows from its context on: hidden ones are cleared before they count
+        const bool clears = walk.item.own != 0 && walk.ragged(tile);
+        if (clears && leader) mbar_arrive_expect_tx(bar_own, 2 * 4 * L::kBlock);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           ok = ok && wait(empty_v + c, (k & 1) ^ 1);
           if (!ok) return;
           if (leader) {
-            if (rank == 0) mbar_arrive_expect_tx(full_v + c, 2 * 4 * L::kBlock);
+            if (!clears && rank == 0) mbar_arrive_expect_tx(full_v + c, 2 * 4 * L::kBlock);
+            const uint32_t bar = clears ? to_own : to_v + 8 * c;
             const int32_t z = 4 * rank + kVBlocks * c;
-            pair_load(sb + L::kVOff + 4 * c * L::kBlock, &v_map, to_v + 8 * c, y0, z);
-            pair_load(sb + L::kVOff + (4 * c + 2) * L::kBlock, &v_map, to_v + 8 * c, y1, z);
+            pair_load(sb + L::kVOff + 4 * c * L::kBlock, &v_map, bar, y0, z);
+            pair_load(sb + L::kVOff + (4 * c + 2) * L::kBlock, &v_map, bar, y1, z);
+            if (!clears && rank == 1) pair_arrive(to_v + 8 * c);
           }
         }
+        if (!clears) return;
+        ok = wait(bar_own, cleared++ & 1);
+        if (!ok) return;
+        // a lane has 16 bytes of a row: its four blocks' parts are 512 bytes
+        const int32_t first = walk.position(tile) - walk.item.context;
+        uint8_t* mine = smem + L::kVOff + (4 * (lane >> 4) + (lane >> 3 & 1)) * L::kBlock + (lane & 7) * 16;
+        for (int x = max(-first, 0); x < kPairKeys; ++x) {
+          const int32_t d = first + x;
+          if (d < walk.item.drafts && (seen >> d & 1)) continue;
+          *reinterpret_cast<uint4*>(mine + 2 * (x >> 6) * L::kBlock + (x & 63) * 128) = make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (leader) pair_arrive(to_v), pair_arrive(to_v + 8);
       };
       const int count = __shfl_sync(~0u, walk.count, 0);
       int2 now = pages(walk.tile0), next = count > 1 ? pages(walk.tile0 + 1) : now;
@@ -1062,7 +998,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (i + 2 < count) next = pages(walk.tile0 + i + 2);  // a tile ahead
           keys(n + 1, rank == 0 ? y0 : y1);
         }
-        if (ok) values(n, x0, x1);
+        if (ok) values(n, walk.tile0 + i, x0, x1);
         x0 = y0, x1 = y1;
       }
     }
@@ -1143,19 +1079,23 @@ __global__ void __launch_bounds__(kJoinThreads * Split) prefix_join_kernel(const
     }
     s = record(lo);
   }
-  const int32_t own_rows = s.nodes * a.heads;
-  const int64_t own0 = s.own_part + row - int64_t(s.node0) * a.heads;
+  int64_t own0 = s.own_part + row - int64_t(s.node0) * a.heads;
   int64_t run0 = s.run_part + row - int64_t(s.run_node0) * a.heads;
-  if (s.run_segments < 0) {
-    const PairRun run = load_pair_run(a.pair_runs - 1 - s.run_segments);
-    const int64_t share = __ldcg(a.head + 3);
-    const int32_t in = int32_t(row - run.row0);
-    const int64_t unit = run.unit0 + int64_t(in / kPairRows) * run.tiles();
-    const int32_t first = int32_t(unit / share), last = int32_t((unit + run.tiles() - 1) / share);
-    run0 = run.part + in + int64_t(kPairRows) * first;
-    s.run_rows = kPairRows;
-    s.run_segments = last - first + 1;
-  }
+  int32_t own_rows = s.nodes * a.heads;
+  // an item's parts: those of the pairs that have a tile of the row's group
+  auto resolve = [&](int32_t& segments, int32_t& stride, int64_t& first_row, int share_at) {
+    if (segments >= 0) return;
+    const PairItem item = load_item(a.items - 1 - segments);
+    const int64_t share = __ldcg(a.head + share_at);
+    const int32_t in = int32_t(row - item.row0);
+    const int64_t unit = item.unit0 + int64_t(in / kPairRows) * item.span();
+    const int32_t first = int32_t((unit + kPairLead) / share), last = int32_t((unit + item.span() - 1) / share);
+    first_row = item.part + in + int64_t(kPairRows) * first;
+    stride = kPairRows;
+    segments = last - first + 1;
+  };
+  resolve(s.own_segments, own_rows, own0, 7);
+  resolve(s.run_segments, s.run_rows, run0, 5);
   const int own = s.own_segments, parts = own + s.run_segments;
   auto place = [&](int p) { return p < own ? own0 + int64_t(p) * own_rows : run0 + int64_t(p - own) * s.run_rows; };
   float4 v[kBatch][Columns];
@@ -1264,7 +1204,7 @@ int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaS
     if (rc != DSR_OK) return rc;
   }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(2 * (tree_ctas() / 2)), 1, 1);
+  cfg.gridDim = dim3(unsigned(2 * a.pairs), 1, 1);
   cfg.blockDim = dim3(kPairThreads, 1, 1);
   cfg.dynamicSmemBytes = PairLayout::kAlloc;
   cfg.stream = stream;
@@ -1281,41 +1221,45 @@ int launch_pairs(const PairArgs& a, const uint16_t* kv_pool, int64_t rows, cudaS
   return DSR_OK;
 }
 
-// ---- scratch: the head, the requests' records, the plan's own, the pair runs, the jobs, the
-// partials
+// ---- scratch: the head, the requests' records, the plan's own, the pairs' items or the jobs,
+// the partials
 size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
-
-int pair_count() { return tree_ctas() / 2; }
 
 struct PrefixSizes {
   int rows;
-  size_t requests, places, pair_runs, jobs;  // bytes
-  size_t parts, pair_part;                   // rows of partials, and where the pairs' begin
+  int pairs;
+  size_t requests, places, items, jobs;  // bytes
+  size_t parts, own_part;                // rows of partials, and where those of the requests' items begin
 };
-PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads, int64_t max_nodes) {
-  PrefixSizes s;
-  // rows of a group: a request's, as in the tree attention; all of them where that is one group
-  s.rows = tree_rows(heads, nodes * heads <= 64 ? nodes : max_nodes);
-  // a segment or more per group: a cut adds at most kPlanWaves jobs a CTA, and an item's
-  // last group may be short of rows
-  const size_t groups = 2 * (size_t(nodes) * heads / s.rows + size_t(batch)), cut = size_t(kPlanWaves) * tree_ctas();
+PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads) {
+  PrefixSizes s = {};
+  const size_t rows = size_t(nodes) * heads;
   s.requests = rounded(size_t(batch) * sizeof(PrefixRequest));
-  s.places = rounded(size_t(batch) * 3 * sizeof(int32_t));
-  s.pair_runs = size_t(batch) * sizeof(PairRun);
-  s.jobs = rounded((groups + cut) * sizeof(TreeJob));
-  s.pair_part = 2 * size_t(nodes) * heads + cut * s.rows;
-  s.parts = s.pair_part + size_t(nodes) * heads + size_t(kPairRows) * pair_count();
+  if (nodes * heads <= kFewRows && batch <= kFewBatch) {
+    s.rows = tree_rows(heads, nodes);  // all rows in one group
+    // a job per run and request; a cut adds at most kPlanWaves jobs a CTA
+    const size_t cut = size_t(kPlanWaves) * tree_ctas();
+    s.jobs = rounded((2 * size_t(batch) + cut) * sizeof(TreeJob));
+    s.parts = 2 * rows + cut * s.rows;
+  } else {
+    s.rows = kPairRows;
+    s.pairs = tree_ctas() / 2;
+    s.places = rounded(size_t(batch) * sizeof(int32_t));
+    s.items = rounded(2 * size_t(batch) * sizeof(PairItem));
+    s.own_part = rows + size_t(kPairRows) * s.pairs;
+    s.parts = 2 * s.own_part;
+  }
   return s;
 }
 
 }  // namespace
 }  // namespace dsr
 
-extern "C" size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads, int64_t max_nodes) {
+extern "C" size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads) {
   using namespace dsr;
-  if (batch <= 0 || nodes <= 0 || heads <= 0 || max_nodes <= 0) return 0;
-  const PrefixSizes s = prefix_sizes(batch, nodes, heads, max_nodes);
-  return 256 + s.requests + s.places + rounded(s.pair_runs) + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
+  if (batch <= 0 || nodes <= 0 || heads <= 0) return 0;
+  const PrefixSizes s = prefix_sizes(batch, nodes, heads);
+  return 256 + s.requests + s.places + s.items + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
 }
 
 extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
@@ -1351,9 +1295,9 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
               "prefix_mla_decode: q, kv_pool and out must be 16-byte aligned");
   DSR_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255u) == 0,
               "prefix_mla_decode: workspace must be 256-byte aligned");
-  const size_t need = dsr_prefix_mla_workspace_bytes(batch, nodes, heads, max_nodes);
+  const size_t need = dsr_prefix_mla_workspace_bytes(batch, nodes, heads);
   DSR_REQUIRE(workspace_bytes >= need, "prefix_mla_decode: workspace %zu < %zu bytes", workspace_bytes, need);
-  const PrefixSizes sizes = prefix_sizes(batch, nodes, heads, max_nodes);
+  const PrefixSizes sizes = prefix_sizes(batch, nodes, heads);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   PrefixArgs a = {};
   a.table = block_table;
@@ -1373,8 +1317,8 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.requests = reinterpret_cast<PrefixRequest*>(ws + 256);
   a.places = reinterpret_cast<int32_t*>(ws + 256 + sizes.requests);
   uint8_t* at = ws + 256 + sizes.requests + sizes.places;
-  a.pair_runs = reinterpret_cast<PairRun*>(at);
-  at += rounded(sizes.pair_runs);
+  a.items = reinterpret_cast<PairItem*>(at);
+  at += sizes.items;
   a.jobs = reinterpret_cast<TreeJob*>(at);
   a.part_o = reinterpret_cast<float*>(at + sizes.jobs);
   a.part_m = a.part_o + sizes.parts * DSR_V_DIM;
@@ -1385,11 +1329,10 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.max_nodes = int(max_nodes);
   a.ctas = tree_ctas();
   a.rows = sizes.rows;
-  a.pairs = nodes * heads > sizes.rows ? pair_count() : 0;  // else no run has rows enough
-  a.pair_part = int32_t(sizes.pair_part);
-  // few requests: scans over few warps
+  a.pairs = sizes.pairs;
+  a.own_part = int32_t(sizes.own_part);
   const size_t smem = size_t(batch + 1) * sizeof(int32_t);
-  if (batch <= 32) {
+  if (batch <= kFewBatch) {
     prefix_plan_few_kernel<<<1, kFewThreads, 0, as_stream(stream)>>>(a);
   } else if (batch <= kPlanCached) {
     prefix_plan_kernel<256, true><<<1, 256, smem, as_stream(stream)>>>(a);
@@ -1401,30 +1344,17 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   }
   rc = launch_status("prefix_mla_decode launch");
   if (rc != DSR_OK) return rc;
+  const float scale_log2 = scale * kTreeLog2e;
   if (a.pairs > 0) {
-    rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, scale * kTreeLog2e, a.part_o,
-                               a.part_m, a.part_l, a.head, a.pair_runs, err},
+    rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2, a.part_o,
+                               a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs},
                       kv_pool, nodes * heads, as_stream(stream));
-    if (rc != DSR_OK) return rc;
+  } else {
+    rc = launch_tree_listed(TreeListedCall{q, q_dtype, kv_pool, pa.rows, block_table, table_stride, tree_mask, scale_log2,
+                                           nodes, a.heads, a.rows, TreeListed{a.jobs, a.head}, a.part_o, a.part_m,
+                                           a.part_l, err},
+                            as_stream(stream));
   }
-  TreeListedCall call = {};
-  call.q = q;
-  call.q_dtype = q_dtype;
-  call.kv_pool = kv_pool;
-  call.pool_rows = pa.rows;
-  call.table = block_table;
-  call.stride = table_stride;
-  call.masks = tree_mask;
-  call.scale_log2 = scale * kTreeLog2e;
-  call.nodes = nodes;
-  call.heads = int(heads);
-  call.rows = sizes.rows;
-  call.list = TreeListed{a.jobs, a.head, a.pairs == 0};
-  call.part_o = a.part_o;
-  call.part_m = a.part_m;
-  call.part_l = a.part_l;
-  call.err = err;
-  rc = launch_tree_listed(call, as_stream(stream));
   if (rc != DSR_OK) return rc;
   // a CTA has all columns of its rows where there are rows enough to fill the SMs with those;
   // with up to eight a SM it is bound by latency, and more parts at once pay (2576 rows: 14 to

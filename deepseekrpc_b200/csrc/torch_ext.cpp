@@ -807,7 +807,7 @@ std::vector<at::Tensor> ds_prefix_mla_decode(at::Tensor q, at::Tensor kv_pool, a
   at::Tensor lse;
   if (return_lse && out) lse = at::full({nodes, heads}, -INFINITY, q.options().dtype(at::kFloat));
   else if (return_lse) lse = fresh({nodes, heads}, at::kFloat, q);
-  const size_t ws_bytes = dsr_prefix_mla_workspace_bytes(batch, nodes, heads, max_nodes);
+  const size_t ws_bytes = dsr_prefix_mla_workspace_bytes(batch, nodes, heads);
   auto ws = fresh({int64_t(ws_bytes)}, at::kByte, q);
   ok(dsr_prefix_mla_decode(q.data_ptr(), dtype, bf16(kv_pool), kv_pool.size(0) / DSR_BLOCK_TOKENS,
                            block_table.data_ptr<int32_t>(), block_table.size(0), block_table.size(1),

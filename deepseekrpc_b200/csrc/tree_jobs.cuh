@@ -29,7 +29,6 @@ static_assert(sizeof(TreeJob) == 48, "three 16-byte words");
 struct TreeListed {
   const TreeJob* jobs;
   const int32_t* count;
-  bool after_plan;  // the kernel before this one wrote the jobs (else one before that)
 };
 
 __device__ __forceinline__ float ex2(float x) {

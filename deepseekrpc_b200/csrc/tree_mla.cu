@@ -439,8 +439,7 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
   }
 
   // ---- the work of all requests
-  if constexpr (Listed)
-    if (a.list.after_plan) pdl_wait();
+  if constexpr (Listed) pdl_wait();
   TreeEntry* entries = reinterpret_cast<TreeEntry*>(smem + L::kChunkOff);  // in the chunks' place
   static_assert(32 * sizeof(TreeEntry) <= 2 * kTreeThreads * 4, "");
   auto walk = [&] {
@@ -998,8 +997,6 @@ __global__ void __launch_bounds__(kTreeThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem_o, L::kTmemCols);
   }
-  if constexpr (Listed)
-    if (!a.list.after_plan) pdl_wait();  // so that what waits for this kernel waits for the one before it
 }
 
 // ---------------------------------------------------------------------------

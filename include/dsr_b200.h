@@ -601,8 +601,7 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
  * all may count as unused).  batch <= 16384, nodes * heads <= 2^24.
  * Scratch: dsr_prefix_mla_workspace_bytes() on the current device, 256-byte aligned,
  * need not be cleared; calls sharing it must not overlap. */
-size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads,
-                                      int64_t max_nodes);
+size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads);
 int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool,
                           int64_t pool_blocks, const int32_t* block_table, int64_t table_rows,
                           int64_t table_stride, const int32_t* context, const int32_t* cu_nodes,
