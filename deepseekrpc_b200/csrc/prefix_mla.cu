@@ -780,7 +780,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) pair_arrive(to_p);
       }
-      if (!ok) break;
 
       // ---- the piece's partials
       ok = ok && pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err);

@@ -146,6 +146,30 @@ def test_the_tree_attention_agrees(cuda):
     assert torch.allclose(lse, same[2], rtol=0, atol=2 ** -10)
 
 
+def test_many_places_for_few_requests(cuda):
+    """Most of a batch is finished or not there: few rows, more than 32 requests."""
+    for n in (31, 32, 33, 1025):
+        requests = [(3, 0)] * n
+        requests[n // 2] = requests[n - 1] = (70, 2)
+        verify(*problem(n, [(500, requests)], 16), requests=[n // 2, n - 1])
+
+
+@pytest.mark.parametrize("heads", [16, 64, 128])
+def test_edges_of_tiles_and_groups(cuda, heads):
+    """Own rows that end at, before and behind tiles of 128 that start at any block; drafts
+    across them; groups of 128 rows that are nearly empty."""
+    prompts = [(tokens, [(mine, drafts) for mine in (0, 1, 63, 64, 65, 127, 128, 129, 200) for drafts in (1, 5)])
+               for tokens in (64, 128, 191, 320)]
+    verify(*problem(heads, prompts, heads, tree="any"))
+
+
+def test_padding_queries_may_hold_anything(cuda):
+    d, rows, masks = problem(17, [(700, [(3, 1)] * 10)], 32, gap=30)
+    d["q"][10:] = float("nan")
+    d["q"][20:] = float("inf")
+    verify(d, rows, masks)
+
+
 def test_scores_that_keep_growing(cuda):
     """Later keys score far higher: the running maximum moves and the output is rescaled."""
     d, rows, masks = problem(10, [(1400, [(20, 1)] * 5)], 32)

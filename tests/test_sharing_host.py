@@ -1,8 +1,10 @@
-"""Blocks that several requests map, without a GPU: refusals of the C ABI, and the
-definitions that the GPU tests rest on."""
+"""Blocks that several requests map, and the attention over common prompts, without a GPU:
+refusals of the C ABI, the definitions that the GPU tests rest on, and rules of the source."""
 from __future__ import annotations
 
 import ctypes
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -36,7 +38,22 @@ def copy(n, pools=(P, 512), row_bytes=(1152, 256), gens=(P,), rows=64, moves=P, 
     return n.dsr_paged_copy(data, widths, len(pools), bumps, len(gens), rows, moves, count, room, err, None)
 
 
+def prefix(n, q=P, dtype=0, pool=P, blocks=8, table=P, rows=3, stride=4, context=P, cu=P, mask=P, most=4, prefix=P,
+           holder=P, scale=1.0, out=P, out_dtype=0, ws=P, ws_bytes=1 << 40, err=P, batch=2, nodes=4, heads=16):
+    return n.dsr_prefix_mla_decode(q, dtype, pool, blocks, table, rows, stride, context, cu, mask, most, prefix, holder, None,
+                                   scale, out, out_dtype, None, ws, ws_bytes, err, batch, nodes, heads, None)
+
+
 @pytest.mark.parametrize("call", [
+    *(lambda n, k=k: prefix(n, **{k: None}) for k in ("q", "pool", "table", "context", "cu", "mask", "prefix", "holder",
+                                                      "out", "ws", "err")),
+    lambda n: prefix(n, dtype=2), lambda n: prefix(n, out_dtype=5), lambda n: prefix(n, blocks=0),
+    lambda n: prefix(n, rows=1), lambda n: prefix(n, rows=1 << 31), lambda n: prefix(n, stride=0),
+    lambda n: prefix(n, most=0), lambda n: prefix(n, most=65), lambda n: prefix(n, scale=0.0),
+    lambda n: prefix(n, scale=float("nan")), lambda n: prefix(n, out=264), lambda n: prefix(n, q=264),
+    lambda n: prefix(n, ws=128), lambda n: prefix(n, ws_bytes=1000), lambda n: prefix(n, batch=0),
+    lambda n: prefix(n, batch=16385, rows=20000), lambda n: prefix(n, nodes=0), lambda n: prefix(n, nodes=(1 << 20) + 1),
+    lambda n: prefix(n, heads=24), lambda n: prefix(n, heads=0),
     *(lambda n, k=k: fork(n, **{k: None}) for k in ("parent", "lengths", "held", "table", "ring", "state", "shares",
                                                     "moves", "count", "err")),
     lambda n: fork(n, stride=0), lambda n: fork(n, stride=1 << 25), lambda n: fork(n, blocks=0),
@@ -70,6 +87,26 @@ def test_workspaces_are_pure_host_functions():
     assert lib.dsr_paged_release_workspace_bytes(0, 8) == lib.dsr_paged_compact_workspace_bytes(0) == 0
     assert lib.dsr_paged_release_workspace_bytes(16384, 1000) >= 16385 * 4 + 1000 // 8
     assert lib.dsr_paged_compact_workspace_bytes(1000) >= 1000 // 8
+    assert lib.dsr_prefix_mla_workspace_bytes(0, 1, 16) == lib.dsr_prefix_mla_workspace_bytes(1, 0, 16) == 0
+    # partials of all rows, of the prompts' and the requests' own parts
+    assert lib.dsr_prefix_mla_workspace_bytes(64, 64, 128) >= 2 * 64 * 128 * 514 * 4
+
+
+def test_rules_of_the_pairs_waits():
+    """What no run can show.  A warp has one answer to a wait: outside the helper that asks all
+    lanes nothing waits for a pair's barrier.  Softmax warps meet in named barriers, which know
+    no limit: one whose wait gives up says so in the next vote and does not leave by itself."""
+    source = Path(__file__).resolve().parent.parent / "deepseekrpc_b200" / "csrc" / "prefix_mla.cu"
+    text = re.sub(r"//[^\n]*", "", source.read_text())
+    helper = re.search(r"bool pair_wait_warp\([^{]*\{(.*?)\n\}", text, re.S)
+    assert helper and "__all_sync(~0u, pair_wait(" in helper.group(1)
+    assert len(re.findall(r"\bpair_wait\(", text)) == 2  # its definition, and there
+    softmax = text[text.index("if (warp < 4) {"):text.index("} else if (warp == 4) {")]
+    leaves = [m.start() for m in re.finditer(r"if \(!ok\) break;", softmax)]
+    assert len(leaves) == 3
+    for at in leaves:  # behind a vote of the rows' two warps
+        assert "rows_sync(pack," in softmax[:at].rstrip().rsplit("\n", 1)[-1], softmax[at - 120:at]
+    assert "multicast" not in re.sub(r"tcgen05\.commit[^;]*;", "", text)  # no copy to several CTAs
 
 
 def consistent(held, table, ring, state, shares):
