@@ -462,29 +462,39 @@ struct PairWalk {
   int32_t at, pair, phase;  // phase: 0 runs, 1 requests
   PairItem item;
   int32_t row0, rows, tile0, count, part;  // of the piece at hand
-  __device__ __forceinline__ PairWalk(const PairArgs& a_, int pair_) : a(a_), unit(0), end(0), at(0), pair(pair_), phase(-1) {}
+  // the requests' range and first item, found with the runs'
+  int64_t own_unit, own_end;
+  int32_t own_at;
+  PairItem own_item;
+  __device__ __forceinline__ PairWalk(const PairArgs& a_, int pair_) : a(a_), pair(pair_), phase(0) {
+    const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head) + 1);
+    find(a.items, head.x, head.y, unit, end, at, item);
+    find(a.items + a.batch, head.z, head.w, own_unit, own_end, own_at, own_item);
+  }
+  // The pair's range of a list's units, and the item that it starts in.
+  __device__ __forceinline__ void find(const PairItem* items, int32_t n_items, int64_t share, int64_t& from, int64_t& to,
+                                       int32_t& first, PairItem& it) {
+    from = to = share * pair;
+    first = 0;
+    if (n_items == 0) return;
+    const PairItem last = load_item(items + n_items - 1);
+    to = min(from + share, last.unit0 + int64_t(last.groups) * last.span());
+    // the last item that starts at or before the unit, 32 ways a step
+    for (int n = n_items; n > 1;) {
+      const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
+      const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&items[first + i].unit0) <= from);
+      const int lead = (31 - __clz(below)) * stride;
+      first += lead;
+      n = min(stride, n - lead);
+    }
+    it = load_item(items + first);
+  }
   __device__ __forceinline__ bool next() {
     for (;;) {
-      while (unit >= end) {  // the next phase's range, and the item that it starts in
-        if (++phase > 1) return false;
-        const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head) + 1);
-        const PairItem* items = a.items + (phase ? a.batch : 0);
-        const int32_t n_items = phase ? head.z : head.x;
-        const int64_t share = phase ? head.w : head.y;
-        unit = end = share * pair;
-        if (n_items == 0) continue;
-        const PairItem last = load_item(items + n_items - 1);
-        end = min(unit + share, last.unit0 + int64_t(last.groups) * last.span());
-        if (unit >= end) continue;
-        at = 0;  // the last item that starts at or before the unit, 32 ways a step
-        for (int n = n_items; n > 1;) {
-          const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
-          const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&items[at + i].unit0) <= unit);
-          const int lead = (31 - __clz(below)) * stride;
-          at += lead;
-          n = min(stride, n - lead);
-        }
-        item = load_item(items + at);
+      if (unit >= end) {
+        if (phase == 1 || own_unit >= own_end) return false;
+        phase = 1;
+        unit = own_unit, end = own_end, at = own_at, item = own_item;
       }
       if (unit >= item.unit0 + int64_t(item.groups) * item.span()) item = load_item(a.items + (phase ? a.batch : 0) + ++at);
       const int64_t in = unit - item.unit0;
@@ -798,11 +808,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // one column of its four rows
       const int q = lane & 3;
       float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(walk.part) + (mine & ~3)) * DSR_V_DIM);
+      uint32_t next[32];
+      tmem_ld32(tmem_o + lanes, next);
 #pragma unroll 1
       for (int c0 = 0; c0 < 256; c0 += 32) {
         uint32_t o[32];
-        tmem_ld32(tmem_o + c0 + lanes, o);
         tmem_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = next[c];
+        if (c0 < 224) tmem_ld32(tmem_o + c0 + 32 + lanes, next);
         const int d0 = half * 256 + c0;  // a pass has 128 columns of either CTA's 256
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -977,11 +991,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         // a lane has 16 bytes of a row: its four blocks' parts are 512 bytes
         const int32_t first = walk.position(tile) - walk.item.context;
         uint8_t* mine = smem + L::kVOff + (4 * (lane >> 4) + (lane >> 3 & 1)) * L::kBlock + (lane & 7) * 16;
-        for (int x = max(-first, 0); x < kPairKeys; ++x) {
-          const int32_t d = first + x;
-          if (d < walk.item.drafts && (seen >> d & 1)) continue;
+        auto clear = [&](int x) {
           *reinterpret_cast<uint4*>(mine + 2 * (x >> 6) * L::kBlock + (x & 63) * 128) = make_uint4(0, 0, 0, 0);
-        }
+        };
+        const int past = min(max(walk.item.drafts - first, 0), kPairKeys);
+        for (int x = max(-first, 0); x < past; ++x)
+          if (!(seen >> (first + x) & 1)) clear(x);
+#pragma unroll 4
+        for (int x = past; x < kPairKeys; ++x) clear(x);
         fence_proxy_async_smem();
         __syncwarp();
         if (leader) pair_arrive(to_v), pair_arrive(to_v + 8);
@@ -1345,8 +1362,8 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   if (rc != DSR_OK) return rc;
   const float scale_log2 = scale * kTreeLog2e;
   if (a.pairs > 0) {
-    rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2, a.part_o,
-                               a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs},
+    rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2,
+                               a.part_o, a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs},
                       kv_pool, nodes * heads, as_stream(stream));
   } else {
     rc = launch_tree_listed(TreeListedCall{q, q_dtype, kv_pool, pa.rows, block_table, table_stride, tree_mask, scale_log2,
