@@ -13,7 +13,16 @@
 // Three launches without a host read: the plan (one CTA), the attention, the join.  More than
 // 64 query rows, or 32 requests: by pairs of CTAs in groups of 128 rows, the runs' and the
 // requests' own rows alike.  Fewer: one group has all rows of a run, and the tree attention's
-// kernel takes the jobs from a list.
+// kernel takes the jobs from a list (two requests of 16 heads over 4096 rows: 22 us; by pairs
+// in an earlier form 38, for 27 by the list).
+//
+// Bound by the tensor cores, and by the power that they may take.  Measured alone, with cold
+// inputs: 64 requests of 128 heads that share 32768 rows and have up to 1500 of their own 399
+// us (598 GFLOP, 1.50 PFLOP/s, 90% of a measured BF16 GEMM); 256 of 64 heads over 65472 rows
+// 1626 us (1.44 PFLOP/s, 86%), one call after another 1930 us (1.21 PFLOP/s, 88% of the
+// measured sustained rate); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 78 us (55%:
+// 7 us until the first tile is there, 8 us of outputs, 11 us of the join).  The same by the
+// tree attention's groups of 64 rows: 831, 3133 and 122 us.
 #include "common.cuh"
 #include "host_common.h"
 #include "tree_jobs.cuh"
@@ -405,7 +414,12 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
 // so that an SM reads of every operand its own half only: 4 KB of shared memory for an MMA
 // of 32 cycles, 6 KB for one of 64 (a CTA alone, with 64 rows: 6 KB for 32).  For S a CTA has
 // its 64 keys of the tile with all columns, for O all 128 keys with its half of the value
-// columns, which are fetched once more, from L2.
+// columns, which are fetched once more, from L2.  A tile takes 2360 cycles, its 52 MMAs 2209
+// (measured by themselves: 32.6 and 64.7 cycles); 139 KB arrive in either SM meanwhile, 12 TB/s
+// in all.  What got it there, for the 64 requests above: copies of three and two column blocks
+// issued by a converged warp (a lane by itself takes some 200 cycles a copy), page ids a tile
+// ahead, and arrivals at the pair's barriers without a release to the cluster (1000 cycles).
+// Not kept: pages prefetched into L2 a tile ahead (402 to 438 us).
 // An accumulator of 64 rows takes tensor memory's lanes twice: lanes 0..63 have the rows and
 // the first half of the columns, lanes 64..127 the same rows and the second half.
 //   warps 0..3  (FP32 query -> shared memory,) softmax: warp w has rows 32 (w % 2) .. of

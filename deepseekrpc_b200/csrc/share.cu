@@ -11,7 +11,8 @@
 //
 // Small calls are bound by their launches: all kernels here are launched while the one
 // before them runs (programmatic dependent launch) and wait for its end before their first
-// access, and small tables are released and compacted by one CTA in one launch.
+// access, and small tables are released and compacted by one CTA in one launch.  A fork of one
+// child, its copy and its release: 12.4 us from a graph, 16 us as three calls of the extension.
 #include "common.cuh"
 #include "host_common.h"
 
@@ -87,7 +88,8 @@ __device__ __forceinline__ int share_owner(const int32_t* cu, int n, int32_t i) 
 // Fork.  Every CTA scans all requests itself, as the plan does; an entry of a child is
 // read from its parent's row, which no child's is.  held and the ring's state are written
 // by the CTA that is the last to have read them (a ticket in the ring state, drawn when a
-// CTA has its sums: it runs beside the entries).
+// CTA has its sums: it runs beside the entries).  Bound by latency: 64 children of 513 blocks
+// 8 us with cold inputs, one child 6 us.
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 512;
 
@@ -187,7 +189,9 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
 // go to the ring, in the order of their ids, so that the order in which the counts were
 // lowered does not matter.  Tables of up to kWholeEntries entries: by the same CTA, with
 // its bit per freed block in shared memory; larger ones by two more launches.
-// Scratch of two launches: {ok, taken, dropped} and cu_drop[batch + 1], then the bits.
+// Scratch of three launches: {ok, taken, dropped} and cu_drop[batch + 1], then the bits.
+// Bound by latency: 448 requests cut somewhere, 65000 entries dropped, 22 us with cold inputs
+// (7.5, 7.5 and 6.7; the freed blocks by the last CTA of the second launch took 16 instead).
 // ---------------------------------------------------------------------------
 constexpr int kScanThreads = 1024, kDropThreads = 512;
 constexpr int kScanPer = kShareMaxBatch / kScanThreads;
@@ -529,8 +533,10 @@ __global__ void __launch_bounds__(kCompactThreads) compact_apply_kernel(const Sh
 }
 
 // ---------------------------------------------------------------------------
-// Copies.  A work item is a piece of one move's rows in one pool; the generations of the
-// written rows are a pool's last items.
+// Copies.  A work item is a piece of one move's rows in one pool, four 16-byte units a thread
+// on their way at once; the generations of the written rows are a move's last item.  Bound by
+// memory: 3900 blocks of 90 KB 117 us (6.3 TB/s read and written, 97% of a plain copy), 495
+// copies of up to 63 rows in four layers 30 us (5.9 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kCopyThreads = 256, kCopyPiece = 16384;  // bytes of an item
 constexpr int kCopyMax = 64;                           // pools, and generations, of a call

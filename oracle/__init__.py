@@ -29,4 +29,4 @@ from .ops import (  # noqa: F401
 )
 from .append import append_kv_index, append_kv_index_ring, paged_rows, ring_rows  # noqa: F401
 from .pool import PoolOracle, ReferenceRowPool  # noqa: F401
-from . import serving  # noqa: F401
+from . import serving, sharing  # noqa: F401
