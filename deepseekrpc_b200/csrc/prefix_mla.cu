@@ -114,11 +114,11 @@ __device__ __forceinline__ bool prefix_continues(const PrefixSeq& before, const 
 // ---- what is to do for a run, or a request's own rows, in groups of `rows` query rows
 __device__ __forceinline__ PairItem own_item(const PrefixArgs& a, int b, const PrefixSeq& s, int rows) {
   PairItem it{};
-  const int32_t keys = s.context + s.nodes - s.shared * DSR_BLOCK_TOKENS;
+  const int64_t keys = int64_t(s.context) + s.nodes - s.shared * DSR_BLOCK_TOKENS;
   if (s.nodes == 0 || keys <= 0) return it;
   it.row0 = s.node0 * a.heads, it.rows = s.nodes * a.heads;
   it.groups = (it.rows + rows - 1) / rows;
-  it.tiles = (keys + 127) / 128;
+  it.tiles = int32_t((keys + 127) / 128);
   it.table = b, it.block0 = s.shared;
   it.context = s.context, it.drafts = s.nodes, it.own = 1;
   return it;
@@ -525,7 +525,7 @@ struct PairWalk {
   }
   // First position of tile i, and whether some of its positions are drafted ones or past the end.
   __device__ __forceinline__ int32_t position(int32_t i) const { return item.block0 * DSR_BLOCK_TOKENS + i * 128; }
-  __device__ __forceinline__ bool ragged(int32_t i) const { return position(i) + 128 > item.context; }
+  __device__ __forceinline__ bool ragged(int32_t i) const { return item.context - position(i) < 128; }
 };
 
 // ---- barriers of a pair

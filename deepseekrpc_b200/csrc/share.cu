@@ -518,7 +518,10 @@ __global__ void __launch_bounds__(kCompactThreads) compact_apply_kernel(const Sh
   }
   for (int64_t i = first; i < a.blocks; i += step) a.ring[i] = i < a.blocks - used ? int32_t(i) + used : -1;
   for (int64_t i = used + first; i < a.blocks; i += step) {
-    if (!((Whole ? live[i >> 5] : __ldcg(s.live + (i >> 5))) >> (i & 31) & 1)) continue;
+    if (!((Whole ? live[i >> 5] : __ldcg(s.live + (i >> 5))) >> (i & 31) & 1)) {
+      a.shares[i] = 0;  // free, whatever it was
+      continue;
+    }
     const int32_t n = rank(int32_t(i)) - kept, to = hole(n);
     a.moves[n] = make_int4(int32_t(i) * DSR_BLOCK_TOKENS, to * DSR_BLOCK_TOKENS, DSR_BLOCK_TOKENS, 0);
     a.shares[to] = a.shares[i];

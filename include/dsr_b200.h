@@ -511,7 +511,7 @@ int dsr_paged_release(const int32_t* lengths, int32_t* held, int32_t* block_tabl
  * held (of all `batch` rows of the table), the i-th mapped id from L on becomes the i-th
  * id below L that is not mapped; entries and shares follow, the ring is rebuilt as
  * L .. pool_blocks-1 (state {0, pool_blocks-L}, -1 behind them).  A block that no entry
- * maps is free afterwards, whether the ring had it or not.  moves is
+ * maps is free afterwards, whether the ring had it or not, with no shares.  moves is
  * i32[max(1, pool_blocks/2)][4]: whole blocks, by ascending source.  pool_blocks <= 8388608.  Scratch as above. */
 size_t dsr_paged_compact_workspace_bytes(int64_t pool_blocks);
 int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t table_stride,

@@ -122,6 +122,7 @@ def paged_compact(held, table, ring, state, shares):
         table[at] = target.get(int(table[at]), table[at])
     for source, to in target.items():
         shares[to], shares[source] = shares[source], 0
+    shares[used:] = 0
     ring[:] = -1
     ring[:blocks - used] = np.arange(used, blocks)
     state[0], state[1] = 0, blocks - used

@@ -189,6 +189,17 @@ def test_refused_release_changes_nothing(cuda, fault):
     release(lengths, tables)
 
 
+def test_blocks_that_were_lost_are_free_after_compaction(cuda):
+    """Blocks that neither the ring nor an entry has, with counts left behind."""
+    for spare in (9, 70000):
+        tables = problem(15, 5, 4, 700, spare=spare)[2]
+        held, table, _, state, shares = tables
+        state[1] = 0
+        mapped = np.unique(table[table >= 0])
+        shares[np.setdiff1d(np.arange(len(shares)), mapped)[::2]] = 3
+        compact(tables)
+
+
 def test_refused_compaction_changes_nothing(cuda):
     tables = problem(9, 3, 3, 500)[2]
     tables[0][4] = tables[1].shape[1] + 1
