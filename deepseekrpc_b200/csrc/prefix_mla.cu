@@ -720,7 +720,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (lane == 0) pair_arrive(to_q);
       }
       // of the drafted positions, those that this thread's row sees
-      const uint64_t word = walk.item.drafts > 0 && mine < walk.rows ? uint64_t(a.masks[(walk.row0 + mine) / a.heads]) : 0ull;
+      uint64_t word = 0;
+      if (walk.item.drafts > 0 && mine < walk.rows) {
+        word = uint64_t(a.masks[(walk.row0 + mine) / a.heads]);
+        if (walk.item.drafts < 64) word &= (1ull << walk.item.drafts) - 1ull;
+      }
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
         ok = ok && pair_wait_warp(bar_s + (n & 1), (n >> 1) & 1, abort, a.err);
@@ -735,11 +739,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]), v[32 + c] = __uint_as_float(t1[c]);
           if (walk.ragged(walk.tile0 + i)) {
+            // bit c: this thread's key c is seen; key c is drafted position `first` + c
             const int32_t first = walk.position(walk.tile0 + i) + 64 * half - walk.item.context;
+            const uint64_t shown = first >= 64    ? 0ull
+                                   : first >= 0   ? word >> first
+                                   : first <= -64 ? ~0ull
+                                                  : word << -first | ((1ull << -first) - 1ull);
+            const uint32_t low = uint32_t(shown), high = uint32_t(shown >> 32);
 #pragma unroll
-            for (int c = 0; c < 64; ++c) {
-              const int32_t d = first + c;
-              if (d >= 0 && (d >= walk.item.drafts || !(word >> d & 1))) v[c] = -CUDART_INF_F;
+            for (int c = 0; c < 32; ++c) {
+              if (!(low >> c & 1u)) v[c] = -CUDART_INF_F;
+              if (!(high >> c & 1u)) v[32 + c] = -CUDART_INF_F;
             }
           }
 #pragma unroll
@@ -822,15 +832,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // one column of its four rows
       const int q = lane & 3;
       float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(walk.part) + (mine & ~3)) * DSR_V_DIM);
-      uint32_t next[32];
-      tmem_ld32(tmem_o + lanes, next);
-#pragma unroll 1
+      uint32_t ahead[2][32];
+      tmem_ld32(tmem_o + lanes, ahead[0]);
+      tmem_ld32(tmem_o + 32 + lanes, ahead[1]);
+#pragma unroll 2
       for (int c0 = 0; c0 < 256; c0 += 32) {
         uint32_t o[32];
         tmem_wait_ld();
+        const int at = c0 / 32 % 2;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = next[c];
-        if (c0 < 224) tmem_ld32(tmem_o + c0 + 32 + lanes, next);
+        for (int c = 0; c < 32; ++c) o[c] = ahead[at][c];
+        if (c0 < 192) tmem_ld32(tmem_o + c0 + 64 + lanes, ahead[at]);
         const int d0 = half * 256 + c0;  // a pass has 128 columns of either CTA's 256
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
