@@ -134,6 +134,14 @@ __device__ __forceinline__ PairItem run_item(const PrefixArgs& a, const PrefixSe
   it.context = s.shared * DSR_BLOCK_TOKENS;
   return it;
 }
+// The pair that has a unit: a quotient below 256, for which a 64-bit division would take a
+// hundred instructions.
+__device__ __forceinline__ int32_t pair_of(int64_t unit, int64_t share) {
+  int32_t c = int32_t(float(unit) / float(share));  // off by one at most
+  if (c * share > unit) --c;
+  if ((c + 1) * share <= unit) ++c;
+  return c;
+}
 __device__ __forceinline__ int64_t pair_units(const PairItem& it) { return int64_t(it.groups) * it.span(); }
 __device__ __forceinline__ PairItem load_item(const PairItem* item) {
   const int4* words = reinterpret_cast<const int4*>(item);
@@ -1131,7 +1139,7 @@ __global__ void __launch_bounds__(kJoinThreads * Split) prefix_join_kernel(const
     const int64_t share = __ldcg(a.head + share_at);
     const int32_t in = int32_t(row - item.row0);
     const int64_t unit = item.unit0 + int64_t(in / kPairRows) * item.span();
-    const int32_t first = int32_t((unit + kPairLead) / share), last = int32_t((unit + item.span() - 1) / share);
+    const int32_t first = pair_of(unit + kPairLead, share), last = pair_of(unit + item.span() - 1, share);
     first_row = item.part + in + int64_t(kPairRows) * first;
     stride = kPairRows;
     segments = last - first + 1;
@@ -1398,11 +1406,12 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
                             as_stream(stream));
   }
   if (rc != DSR_OK) return rc;
-  // a CTA has all columns of its rows where there are rows enough to fill the SMs with those;
-  // with up to eight a SM it is bound by latency, and more parts at once pay (2576 rows: 14 to
-  // 11 us), with more it is not (8192 rows: 17 and 22 us)
+  // The pairs' parts: a CTA has all columns of its rows.  With up to eight CTAs a SM it is bound
+  // by latency, and more parts at once pay (2576 rows: 14 to 11 us), with more it is not (8192
+  // rows: 17 and 22 us).  The list's few rows and many parts: a column and every fourth part a
+  // thread (384 rows of the pairs' few parts took 15 us so, for 4)
   const int64_t quads = nodes * heads / 4;
-  const bool whole = quads >= 4 * sm_count();
+  const bool whole = a.pairs > 0;
   const auto join = !whole ? prefix_join_kernel<1, 4, 8>
                            : quads <= 8 * sm_count() ? prefix_join_kernel<4, 1, 4> : prefix_join_kernel<4, 1, 2>;
   cudaLaunchConfig_t cfg = {};
