@@ -430,17 +430,17 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
 // Not kept: pages prefetched into L2 a tile ahead (402 to 438 us).
 // An accumulator of 64 rows takes tensor memory's lanes twice: lanes 0..63 have the rows and
 // the first half of the columns, lanes 64..127 the same rows and the second half.
-//   warps 0..3  (FP32 query -> shared memory,) softmax: warp w has rows 32 (w % 2) .. of
-//               this CTA and the keys, value columns of half w / 2; the running maximum of a
-//               row is followed only when it grows by more than 2^8
-//   warp 4      tensor memory; in CTA 0 the MMAs: S of the next tile, then O of this one, so
+//   warps 0..7  (FP32 query -> shared memory,) softmax: warp w has rows 32 (w % 2) .. of
+//               this CTA and of the keys, value columns in half w / 2 % 2 those in half w / 4;
+//               the running maximum of a row is followed only when it grows by more than 2^8
+//   warp 8      tensor memory; in CTA 0 the MMAs: S of the next tile, then O of this one, so
 //               that they run through the softmax between
-//   warp 5      query, keys and values by TMA; what arrives in either CTA is counted by CTA
+//   warp 9      query, keys and values by TMA; what arrives in either CTA is counted by CTA
 //               0's barriers.  Values of a request's last tiles come to a barrier of the CTA's
 //               own first: rows that no query sees may hold anything and are cleared, since
 //               0 x NaN would reach the output
 // ---------------------------------------------------------------------------
-constexpr int kPairSoftmax = 128, kPairThreads = kPairSoftmax + 64;
+constexpr int kPairSoftmax = 256, kPairThreads = kPairSoftmax + 64;
 constexpr int kPairKeys = 128;
 constexpr int kKStages = 3, kKBlocks = 3;  // 64-column blocks of a copy: the nine of a key,
 constexpr int kVBlocks = 2;                // and a CTA's of a pass over 256 value columns
@@ -454,8 +454,8 @@ struct PairLayout {
   static constexpr int kPOff = kVOff + 8 * kBlock;           // 2 blocks of 64 rows x 64 keys
   static constexpr int kBarOff = kPOff + 2 * kBlock;
   static constexpr int kBars = 2 * kKStages + 2 * 2 + 2 + 6;
-  static constexpr int kRedOff = kBarOff + (kBars * 8 + 15) / 16 * 16;  // f32[2][64]
-  static constexpr int kMiscOff = kRedOff + 2 * 64 * 4;
+  static constexpr int kRedOff = kBarOff + (kBars * 8 + 15) / 16 * 16;  // f32[4][64]
+  static constexpr int kMiscOff = kRedOff + 4 * 64 * 4;
   static constexpr int kBytes = kMiscOff + 16;
   static constexpr int kAlloc = kBytes + 1024;
   static constexpr uint32_t kTmemCols = 512;  // O: 256 columns, S: two of 64
@@ -487,15 +487,15 @@ struct PairWalk {
   // the requests' range and first item, found with the runs'
   int64_t own_unit, own_end;
   int32_t own_at;
-  PairItem own_item;
   __device__ __forceinline__ PairWalk(const PairArgs& a_, int pair_) : a(a_), pair(pair_), phase(0) {
     const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head) + 1);
-    find(a.items, head.x, head.y, unit, end, at, item);
-    find(a.items + a.batch, head.z, head.w, own_unit, own_end, own_at, own_item);
+    find(a.items, head.x, head.y, unit, end, at);
+    find(a.items + a.batch, head.z, head.w, own_unit, own_end, own_at);
+    if (unit < end) item = load_item(a.items + at);
   }
   // The pair's range of a list's units, and the item that it starts in.
   __device__ __forceinline__ void find(const PairItem* items, int32_t n_items, int64_t share, int64_t& from, int64_t& to,
-                                       int32_t& first, PairItem& it) {
+                                       int32_t& first) {
     from = to = share * pair;
     first = 0;
     if (n_items == 0) return;
@@ -509,14 +509,14 @@ struct PairWalk {
       first += lead;
       n = min(stride, n - lead);
     }
-    it = load_item(items + first);
   }
   __device__ __forceinline__ bool next() {
     for (;;) {
       if (unit >= end) {
         if (phase == 1 || own_unit >= own_end) return false;
         phase = 1;
-        unit = own_unit, end = own_end, at = own_at, item = own_item;
+        unit = own_unit, end = own_end, at = own_at;
+        item = load_item(a.items + a.batch + at);
       }
       if (unit >= item.unit0 + int64_t(item.groups) * item.span()) item = load_item(a.items + (phase ? a.batch : 0) + ++at);
       const int64_t in = unit - item.unit0;
@@ -613,12 +613,13 @@ __device__ __forceinline__ bool elect_lane() {
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
   return r != 0;
 }
-// The 64 softmax threads of one half of a CTA's rows: a barrier, and whether every one is fine.
+// The softmax threads of one half of a CTA's rows, four a row: a barrier, and whether every one
+// is fine.
 __device__ __forceinline__ bool rows_sync(int half, bool ok) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-      "barrier.cta.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      "barrier.cta.red.and.pred q, %2, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"(uint32_t(ok)), "r"(1 + half)
       : "memory");
@@ -675,16 +676,17 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (!a.q_wide) tma_prefetch_desc(&q_map);
     for (int i = 0; i < kKStages; ++i) mbar_init(full_k + i, 1), mbar_init(empty_k + i, 1);
     for (int i = 0; i < 2; ++i) mbar_init(full_v + i, 2), mbar_init(empty_v + i, 1), mbar_init(bar_s + i, 1);
-    mbar_init(bar_p, 8);
-    mbar_init(bar_q, a.q_wide ? 8 : 1);
-    mbar_init(bar_free, 8);
+    constexpr int kWarps = 2 * kPairSoftmax / 32;  // of both CTAs
+    mbar_init(bar_p, kWarps);
+    mbar_init(bar_q, a.q_wide ? kWarps : 1);
+    mbar_init(bar_free, kWarps);
     mbar_init(bar_end, 1);
     mbar_init(bar_o, 1);
     mbar_init(bar_own, 1);
     *abort = 0;
     fence_barrier_init();
   }
-  if (warp == 4) {
+  if (warp == 8) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(L::kTmemCols)
                  : "memory");
@@ -699,10 +701,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   pdl_launch_dependents();
   PairWalk walk(a, pair);
 
-  if (warp < 4) {
+  if (warp < 8) {
     // ------------------------------------------------------------ softmax
-    const int half = warp >> 1, pack = warp & 1, r = 32 * pack + lane;  // this thread's row of the CTA's
-    const uint32_t lanes = uint32_t(warp) * 32 << 16;                  // this warp's TMEM lanes
+    const int pack = warp & 1, r = 32 * pack + lane;            // this thread's row of the CTA's
+    const int half = warp >> 1 & 1, side = warp >> 2;           // of the columns, and of that half
+    const uint32_t lanes = uint32_t(warp & 3) * 32 << 16;       // this warp's TMEM lanes
     const uint32_t to_p = pair_address(bar_p, 0), to_q = pair_address(bar_q, 0), to_free = pair_address(bar_free, 0);
     int n = 0;
     bool ok = true;
@@ -736,43 +739,39 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
         ok = ok && pair_wait_warp(bar_s + (n & 1), (n >> 1) & 1, abort, a.err);
-        float v[64];
+        float v[32];
         float top = -CUDART_INF_F;
         if (ok) {
           tc_fence_after();
-          uint32_t t0[32], t1[32];
-          tmem_ld32(tmem_s + (n & 1) * 64 + lanes, t0);
-          tmem_ld32(tmem_s + (n & 1) * 64 + 32 + lanes, t1);
+          uint32_t t0[32];
+          tmem_ld32(tmem_s + (n & 1) * 64 + 32 * side + lanes, t0);
           tmem_wait_ld();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]), v[32 + c] = __uint_as_float(t1[c]);
+          for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]);
           if (walk.ragged(walk.tile0 + i)) {
             // bit c: this thread's key c is seen; key c is drafted position `first` + c
-            const int32_t first = walk.position(walk.tile0 + i) + 64 * half - walk.item.context;
-            const uint64_t shown = first >= 64    ? 0ull
-                                   : first >= 0   ? word >> first
-                                   : first <= -64 ? ~0ull
-                                                  : word << -first | ((1ull << -first) - 1ull);
-            const uint32_t low = uint32_t(shown), high = uint32_t(shown >> 32);
+            const int32_t first = walk.position(walk.tile0 + i) + 64 * half + 32 * side - walk.item.context;
+            const uint32_t shown = first >= 64    ? 0u
+                                   : first >= 0   ? uint32_t(word >> first)
+                                   : first <= -32 ? ~0u
+                                                  : uint32_t(word) << -first | ((1u << -first) - 1u);
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              if (!(low >> c & 1u)) v[c] = -CUDART_INF_F;
-              if (!(high >> c & 1u)) v[32 + c] = -CUDART_INF_F;
-            }
+            for (int c = 0; c < 32; ++c)
+              if (!(shown >> c & 1u)) v[c] = -CUDART_INF_F;
           }
 #pragma unroll
-          for (int c = 0; c < 64; ++c) top = fmaxf(top, v[c]);
+          for (int c = 0; c < 32; ++c) top = fmaxf(top, v[c]);
           top *= a.scale_log2;
         }
         // weights against the running maximum as it stands; their sums are of the weights as
         // formed, for the product with V they are rounded to BF16 (as in the tree attention)
-        uint32_t packed[32];
+        uint32_t packed[16];
         float sum = 0.f;
         auto weigh = [&] {
           const float base = m == -CUDART_INF_F ? 0.f : m;
           float s0 = 0.f, s1 = 0.f;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
+          for (int c = 0; c < 16; ++c) {
             const float x = ex2(fmaf(v[2 * c], a.scale_log2, -base)), y = ex2(fmaf(v[2 * c + 1], a.scale_log2, -base));
             s0 += x;
             s1 += y;
@@ -786,9 +785,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (!rows_sync(pack, fits)) {
           ok = rows_sync(pack, ok);
           if (!ok) break;
-          red[64 * half + r] = top;
+          red[64 * (2 * half + side) + r] = top;
           rows_sync(pack, true);
-          top = fmaxf(top, red[64 * (half ^ 1) + r]);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) top = fmaxf(top, red[64 * x + r]);
           float f = 1.f;
           if (top > m + kPairSlack) f = ex2(m - top), l *= f, m = top;  // f: 0 when the row had seen nothing
           if (i > 0) {
@@ -796,7 +796,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (!ok) break;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < 256; c += 32) {
+            for (int c = 128 * side; c < 128 * side + 128; c += 32) {
               uint32_t o[32];
               tmem_ld32(tmem_o + c + lanes, o);
               tmem_wait_ld();
@@ -814,8 +814,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (n > 0) ok = pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
         if (!ok) continue;
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
-          *reinterpret_cast<uint4*>(smem + L::kPOff + half * L::kBlock + sw128_offset(r, 8 * c)) =
+        for (int c = 0; c < 4; ++c)
+          *reinterpret_cast<uint4*>(smem + L::kPOff + half * L::kBlock + sw128_offset(r, 32 * side + 8 * c)) =
               make_uint4(packed[4 * c], packed[4 * c + 1], packed[4 * c + 2], packed[4 * c + 3]);
         fence_proxy_async_smem();
         tc_fence_before();
@@ -825,12 +825,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
       // ---- the piece's partials
       ok = ok && pair_wait_warp(bar_o, (n - 1) & 1, abort, a.err);
-      if (half == 1) red[64 + r] = l;
+      red[64 * (2 * half + side) + r] = l;
       ok = rows_sync(pack, ok);
       if (!ok) break;
       const bool valid = mine < walk.rows;
-      if (half == 0 && valid) {
-        const float total = l + red[64 + r];
+      if (half == 0 && side == 0 && valid) {
+        const float total = (red[r] + red[64 + r]) + (red[128 + r] + red[192 + r]);
         if (!(total < CUDART_INF_F)) flag(a.err, DSR_ERR_NONFINITE);
         a.part_m[int64_t(walk.part) + mine] = m;
         a.part_l[int64_t(walk.part) + mine] = total;
@@ -840,17 +840,16 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // one column of its four rows
       const int q = lane & 3;
       float4* dst = reinterpret_cast<float4*>(a.part_o + (int64_t(walk.part) + (mine & ~3)) * DSR_V_DIM);
-      uint32_t ahead[2][32];
-      tmem_ld32(tmem_o + lanes, ahead[0]);
-      tmem_ld32(tmem_o + 32 + lanes, ahead[1]);
-#pragma unroll 2
-      for (int c0 = 0; c0 < 256; c0 += 32) {
+      const int first = 128 * side;  // of its 256 columns, this thread's
+      uint32_t next[32];
+      tmem_ld32(tmem_o + first + lanes, next);
+#pragma unroll 1
+      for (int c0 = first; c0 < first + 128; c0 += 32) {
         uint32_t o[32];
         tmem_wait_ld();
-        const int at = c0 / 32 % 2;
 #pragma unroll
-        for (int c = 0; c < 32; ++c) o[c] = ahead[at][c];
-        if (c0 < 192) tmem_ld32(tmem_o + c0 + 64 + lanes, ahead[at]);
+        for (int c = 0; c < 32; ++c) o[c] = next[c];
+        if (c0 < first + 96) tmem_ld32(tmem_o + c0 + 32 + lanes, next);
         const int d0 = half * 256 + c0;  // a pass has 128 columns of either CTA's 256
 #pragma unroll
         for (int c = 0; c < 32; c += 4) {
@@ -871,7 +870,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       __syncwarp();
       if (lane == 0) pair_arrive(to_free);
     }
-  } else if (warp == 4) {
+  } else if (warp == 8) {
     if (rank == 0) {
       // ------------------------------------------------------------ MMA issuer
       // The whole warp runs the loop and one lane issues, on values that are the same in all
@@ -887,6 +886,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
       int n = 0, piece = 0;
       bool ok = true;
+      // A descriptor that the compiler takes for a new value, so that it adds the steps below
+      // each time and does not keep all 52 sums in registers
+      auto anew = [](uint64_t x) {
+        asm volatile("" : "+l"(x));
+        return x;
+      };
       // S of tile k: a step of 16 columns moves both operands by 32 bytes
       auto scores = [&](int k) {
 #pragma unroll
@@ -895,10 +900,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           if (!ok) return;
           tc_fence_after();
           if (leader) {
+            const uint64_t q = anew(desc_q), key = anew(desc_k);
 #pragma unroll
             for (int x = 0; x < 4 * kKBlocks; ++x)
-              pair_umma(ts + (k & 1) * 64, desc_q + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3),
-                        desc_k + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3), idesc_s,
+              pair_umma(ts + (k & 1) * 64, q + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3),
+                        key + (kKBlocks * c + (x >> 2)) * (L::kBlock / 16) + 2 * (x & 3), idesc_s,
                         (c | x) != 0 ? 1u : 0u);
             pair_commit(empty_k + c);
           }
@@ -923,10 +929,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
             if (!ok) break;
             tc_fence_after();
             if (leader) {
+              const uint64_t weights = anew(desc_p), value = anew(desc_v);
 #pragma unroll
               for (int ks = 0; ks < kPairKeys / 16; ++ks)
-                pair_umma(to + c * 128, desc_p + (ks >> 2) * (L::kBlock / 16) + 2 * (ks & 3),
-                          desc_v + (4 * c + 2 * (ks >> 2)) * (L::kBlock / 16) + (ks & 3) * (2048 / 16), idesc_o,
+                pair_umma(to + c * 128, weights + (ks >> 2) * (L::kBlock / 16) + 2 * (ks & 3),
+                          value + (4 * c + 2 * (ks >> 2)) * (L::kBlock / 16) + (ks & 3) * (2048 / 16), idesc_o,
                           ks > 0 ? 1u : accumulate);
               pair_commit(empty_v + c);
             }
@@ -1062,7 +1069,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   }
   __syncthreads();
   pair_sync();  // neither CTA leaves while the other's copies, commits or MMAs may reach it
-  if (warp == 4) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_o), "r"(L::kTmemCols) : "memory");
   }

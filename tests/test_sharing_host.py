@@ -101,10 +101,10 @@ def test_rules_of_the_pairs_waits():
     helper = re.search(r"bool pair_wait_warp\([^{]*\{(.*?)\n\}", text, re.S)
     assert helper and "__all_sync(~0u, pair_wait(" in helper.group(1)
     assert len(re.findall(r"\bpair_wait\(", text)) == 2  # its definition, and there
-    softmax = text[text.index("if (warp < 4) {"):text.index("} else if (warp == 4) {")]
+    softmax = text[text.index("if (warp < 8) {"):text.index("} else if (warp == 8) {")]
     leaves = [m.start() for m in re.finditer(r"if \(!ok\) break;", softmax)]
     assert len(leaves) == 3
-    for at in leaves:  # behind a vote of the rows' two warps
+    for at in leaves:  # behind a vote of the rows' warps
         assert "rows_sync(pack," in softmax[:at].rstrip().rsplit("\n", 1)[-1], softmax[at - 120:at]
     assert "multicast" not in re.sub(r"tcgen05\.commit[^;]*;", "", text)  # no copy to several CTAs
 
