@@ -66,6 +66,13 @@ struct alignas(16) PairItem {
 };
 static_assert(sizeof(PairItem) == 48, "three 16-byte words");
 
+// Where the parts of a node's rows are: of its request's own rows, then of its run.  The pairs'
+// idle warp finds it, so that a CTA of the join has one load to wait for and not four.
+struct alignas(16) PairNode {
+  int32_t own_part, own_parts;  // of the node's first row; -1: a row of no request
+  int32_t run_part, run_parts;
+};
+
 struct PrefixArgs {
   const int32_t* table;
   int64_t stride, table_rows;
@@ -82,6 +89,7 @@ struct PrefixArgs {
   PrefixRequest* requests;
   int32_t* places;   // the plan's own: [batch] a run's item
   PairItem* items;   // [batch] of runs, [batch] of requests
+  PairNode* records; // [nodes]
   TreeJob* jobs;
   float *part_o, *part_m, *part_l;
   int64_t nodes;
@@ -474,7 +482,53 @@ struct PairArgs {
   const PairItem* items;
   int32_t* err;
   int batch, heads, pairs;
+  const int32_t* cu_nodes;
+  const PrefixRequest* requests;
+  PairNode* records;
+  int32_t nodes;
 };
+
+__device__ __forceinline__ PrefixRequest load_request(const PrefixRequest* request) {
+  const int4* words = reinterpret_cast<const int4*>(request);
+  const int4 x = __ldcg(words), y = __ldcg(words + 1);
+  return PrefixRequest{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+__device__ __forceinline__ PairNode find_node(const PairArgs& a, int32_t node) {
+  int lo = 0;  // the largest b with cu_nodes[b] <= node
+  for (int hi = a.batch; hi - lo > 1;) {
+    const int mid = (lo + hi) >> 1;
+    if (a.cu_nodes[mid] <= node) lo = mid;
+    else hi = mid;
+  }
+  PrefixRequest s = load_request(a.requests + lo);
+  if (node < s.node0 || node >= s.node0 + s.nodes) {
+    // a padding row.  Where a request was refused the sums may be in disorder and the search
+    // may have missed the request that has the row: every one is asked
+    lo = -1;
+    if (!__ldcg(a.head + 1))
+      for (int b = 0; b < a.batch; ++b) {
+        s = load_request(a.requests + b);
+        if (node >= s.node0 && node < s.node0 + s.nodes) lo = b;
+      }
+    if (lo < 0) return PairNode{0, -1, 0, 0};
+    s = load_request(a.requests + lo);
+  }
+  // an item's parts: those of the pairs that have a tile of the node's group
+  auto parts = [&](int32_t index, int share_at, int32_t& part, int32_t& count) {
+    if (index >= 0) return;
+    const PairItem item = load_item(a.items - 1 - index);
+    const int64_t share = __ldcg(a.head + share_at);
+    const int32_t in = node * a.heads - item.row0;
+    const int64_t unit = item.unit0 + int64_t(in / kPairRows) * item.span();
+    const int32_t first = pair_of(unit + kPairLead, share), last = pair_of(unit + item.span() - 1, share);
+    part = item.part + in + kPairRows * first;
+    count = last - first + 1;
+  };
+  PairNode found{0, 0, 0, 0};
+  parts(s.own_segments, 7, found.own_part, found.own_parts);
+  parts(s.run_segments, 5, found.run_part, found.run_parts);
+  return found;
+}
 
 // A pair's pieces, one after another (every warp walks them for itself): of the runs, then of
 // the requests.
@@ -948,6 +1002,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
                          smem_u32(bar_end))
                      : "memory");
       mbar_drain(bar_end, 0);
+    } else {
+      // ------------------------------------------------------------ what the join asks for
+      for (int32_t node = pair * 32 + lane; node < a.nodes; node += a.pairs * 32) a.records[node] = find_node(a, node);
     }
   } else {
     // ------------------------------------------------------------ copies
@@ -1084,77 +1141,61 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 constexpr int kJoinThreads = 128;
 constexpr int kJoinMaxParts = kPlanWaves * kTreeMaxCtas + 16;
 
-template <int Columns, int Split, int kBatch>  // kBatch: parts requested together
+template <bool kPairs, int Columns, int Split, int kBatch>  // kBatch: parts requested together
 __global__ void __launch_bounds__(kJoinThreads * Split) prefix_join_kernel(const __grid_constant__ PrefixArgs a) {
-  __shared__ float weight[4][kJoinMaxParts];
+  __shared__ float weight[4][kPairs ? kTreeMaxCtas + 2 : kJoinMaxParts];
   __shared__ float inverse[4], tops[4][Split], sums[4][Split];
   __shared__ float4 others[Split > 1 ? Split - 1 : 1][Columns][kJoinThreads];
-  __shared__ int owner;
   const int64_t row = int64_t(blockIdx.x) * 4;
   const int32_t node = int32_t(row / a.heads);
   const int tid = threadIdx.x, thread = tid % kJoinThreads, turn = tid / kJoinThreads;
   const int d = blockIdx.y * Columns * kJoinThreads + thread;  // the first column
-  // the request of the node: the largest b with cu_nodes[b] <= node, 32 ways a step
-  int lo = 0;
-  for (int n = a.batch; n > 1;) {
-    const int stride = (n + 31) / 32, at = (tid & 31) * stride;
-    const unsigned below = __ballot_sync(~0u, at < n && a.cu_nodes[lo + at] <= node);
-    const int last = below == 0 ? 0 : (31 - __clz(below)) * stride;
-    lo += last;
-    n = min(stride, n - last);
-  }
-  pdl_wait();  // before any CTA leaves: the join must not end ahead of the attention
-  auto record = [&](int b) {
-    const int4* words = reinterpret_cast<const int4*>(a.requests + b);
-    const int4 x = __ldcg(words), y = __ldcg(words + 1);
-    return PrefixRequest{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-  };
-  PrefixRequest s = record(lo);
-  if (node < s.node0 || node >= s.node0 + s.nodes) {
-    // a padding row.  Where a request was refused the sums may be in disorder and the search
-    // may have missed the request that has the row: every one is asked
-    lo = -1;
-    if (!__ldcg(a.head + 1)) {
-      if (tid == 0) owner = -1;
-      __syncthreads();
-      for (int b = tid; b < a.batch; b += kJoinThreads * Split) {
-        const PrefixRequest other = record(b);
-        if (node >= other.node0 && node < other.node0 + other.nodes) atomicMax(&owner, b);
-      }
-      __syncthreads();
-      lo = owner;
+  // ---- where the row's parts are: part p at own0 + p own_rows, then run0 + p run_rows
+  int64_t own0, run0;
+  int32_t own_rows = kPairRows, run_rows = kPairRows;
+  int own = -1, parts = 0;
+  if constexpr (kPairs) {
+    pdl_wait();  // before any CTA leaves: the join must not end ahead of the attention
+    const int4 found = __ldcg(reinterpret_cast<const int4*>(a.records + node));
+    const int64_t in = row - int64_t(node) * a.heads;
+    own0 = found.x + in, own = found.y;
+    run0 = found.z + in, parts = own + found.w;
+  } else {
+    // the request (of up to 32) that has the node: the last whose first node is not behind it
+    const int lane = tid & 31;
+    const unsigned below = __ballot_sync(~0u, lane < a.batch && a.cu_nodes[lane] <= node);
+    const int last = below == 0 ? 0 : 31 - __clz(below);
+    pdl_wait();
+    PrefixRequest s = load_request(a.requests + last);
+    auto has_node = [&] { return node >= s.node0 && node < s.node0 + s.nodes; };
+    bool found = has_node();
+    if (!found) {
+      // a padding row.  Where a request was refused the sums may be in disorder: all are asked
+      s = lane < a.batch ? load_request(a.requests + lane) : PrefixRequest{};
+      const unsigned has = __ballot_sync(~0u, has_node());
+      found = has != 0;
+      if (found) s = load_request(a.requests + 31 - __clz(has));
     }
-    if (lo < 0) {
-      if (!a.zero_unused || turn > 0) return;
-      for (int x = 0; x < 4 * Columns; ++x) {
-        const int64_t at = (row + x % 4) * DSR_V_DIM + d + x / 4 * kJoinThreads;
-        if (a.out_wide) static_cast<float*>(a.out)[at] = 0.f;
-        else static_cast<uint16_t*>(a.out)[at] = 0;
-      }
-      if (a.lse != nullptr && blockIdx.y == 0 && tid < 4) a.lse[row + tid] = -CUDART_INF_F;
-      return;
+    if (found) {
+      own0 = s.own_part + row - int64_t(s.node0) * a.heads;
+      run0 = s.run_part + row - int64_t(s.run_node0) * a.heads;
+      own_rows = s.nodes * a.heads;
+      run_rows = s.run_rows;
+      own = s.own_segments;
+      parts = own + s.run_segments;
     }
-    s = record(lo);
   }
-  int64_t own0 = s.own_part + row - int64_t(s.node0) * a.heads;
-  int64_t run0 = s.run_part + row - int64_t(s.run_node0) * a.heads;
-  int32_t own_rows = s.nodes * a.heads;
-  // an item's parts: those of the pairs that have a tile of the row's group
-  auto resolve = [&](int32_t& segments, int32_t& stride, int64_t& first_row, int share_at) {
-    if (segments >= 0) return;
-    const PairItem item = load_item(a.items - 1 - segments);
-    const int64_t share = __ldcg(a.head + share_at);
-    const int32_t in = int32_t(row - item.row0);
-    const int64_t unit = item.unit0 + int64_t(in / kPairRows) * item.span();
-    const int32_t first = pair_of(unit + kPairLead, share), last = pair_of(unit + item.span() - 1, share);
-    first_row = item.part + in + int64_t(kPairRows) * first;
-    stride = kPairRows;
-    segments = last - first + 1;
-  };
-  resolve(s.own_segments, own_rows, own0, 7);
-  resolve(s.run_segments, s.run_rows, run0, 5);
-  const int own = s.own_segments, parts = own + s.run_segments;
-  auto place = [&](int p) { return p < own ? own0 + int64_t(p) * own_rows : run0 + int64_t(p - own) * s.run_rows; };
+  if (own < 0) {  // a padding row
+    if (!a.zero_unused || turn > 0) return;
+    for (int x = 0; x < 4 * Columns; ++x) {
+      const int64_t at = (row + x % 4) * DSR_V_DIM + d + x / 4 * kJoinThreads;
+      if (a.out_wide) static_cast<float*>(a.out)[at] = 0.f;
+      else static_cast<uint16_t*>(a.out)[at] = 0;
+    }
+    if (a.lse != nullptr && blockIdx.y == 0 && tid < 4) a.lse[row + tid] = -CUDART_INF_F;
+    return;
+  }
+  auto place = [&](int p) { return p < own ? own0 + int64_t(p) * own_rows : run0 + int64_t(p - own) * run_rows; };
   float4 v[kBatch][Columns];
   auto request = [&](int p0) {
 #pragma unroll
@@ -1285,7 +1326,7 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 struct PrefixSizes {
   int rows;
   int pairs;
-  size_t requests, places, items, jobs;  // bytes
+  size_t requests, places, items, records, jobs;  // bytes
   size_t parts, own_part;                // rows of partials, and where those of the requests' items begin
 };
 PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads) {
@@ -1303,6 +1344,7 @@ PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads) {
     s.pairs = tree_ctas() / 2;
     s.places = rounded(size_t(batch) * sizeof(int32_t));
     s.items = rounded(2 * size_t(batch) * sizeof(PairItem));
+    s.records = rounded(size_t(nodes) * sizeof(PairNode));
     s.own_part = rows + size_t(kPairRows) * s.pairs;
     s.parts = 2 * s.own_part;
   }
@@ -1316,7 +1358,7 @@ extern "C" size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, i
   using namespace dsr;
   if (batch <= 0 || nodes <= 0 || heads <= 0) return 0;
   const PrefixSizes s = prefix_sizes(batch, nodes, heads);
-  return 256 + s.requests + s.places + s.items + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
+  return 256 + s.requests + s.places + s.items + s.records + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
 }
 
 extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
@@ -1376,6 +1418,8 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   uint8_t* at = ws + 256 + sizes.requests + sizes.places;
   a.items = reinterpret_cast<PairItem*>(at);
   at += sizes.items;
+  a.records = reinterpret_cast<PairNode*>(at);
+  at += sizes.records;
   a.jobs = reinterpret_cast<TreeJob*>(at);
   a.part_o = reinterpret_cast<float*>(at + sizes.jobs);
   a.part_m = a.part_o + sizes.parts * DSR_V_DIM;
@@ -1404,7 +1448,8 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   const float scale_log2 = scale * kTreeLog2e;
   if (a.pairs > 0) {
     rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2,
-                               a.part_o, a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs},
+                               a.part_o, a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs, cu_nodes,
+                               a.requests, a.records, int32_t(nodes)},
                       kv_pool, nodes * heads, as_stream(stream));
   } else {
     rc = launch_tree_listed(TreeListedCall{q, q_dtype, kv_pool, pa.rows, block_table, table_stride, tree_mask, scale_log2,
@@ -1419,8 +1464,9 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   // thread (384 rows of the pairs' few parts took 15 us so, for 4)
   const int64_t quads = nodes * heads / 4;
   const bool whole = a.pairs > 0;
-  const auto join = !whole ? prefix_join_kernel<1, 4, 8>
-                           : quads <= 8 * sm_count() ? prefix_join_kernel<4, 1, 4> : prefix_join_kernel<4, 1, 2>;
+  const auto join = !whole                      ? prefix_join_kernel<false, 1, 4, 8>
+                    : quads <= 8 * sm_count() ? prefix_join_kernel<true, 4, 1, 4>
+                                              : prefix_join_kernel<true, 4, 1, 2>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(quads), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
   cfg.blockDim = dim3(kJoinThreads * (whole ? 1 : 4), 1, 1);
