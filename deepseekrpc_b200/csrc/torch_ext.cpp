@@ -649,11 +649,20 @@ at::Tensor ds_paged_copy(std::vector<at::Tensor> pools, std::vector<at::Tensor> 
   for (const at::Tensor& p : pools) {
     check(p, p.scalar_type(), moves);
     TORCH_CHECK(p.dim() == 2 && p.size(0) == rows, "paged_copy: pools [rows, width] of as many rows expected");
+    const int64_t bytes = p.size(1) * p.element_size();  // before the first of several launches
+    TORCH_CHECK(bytes > 0 && bytes <= 65536 && bytes % 16 == 0 && reinterpret_cast<uintptr_t>(p.data_ptr()) % 16 == 0,
+                "paged_copy: 16-byte aligned rows of 16 to 65536 bytes expected");
   }
   for (const at::Tensor& g : generations)
     check_vector(g, at::kLong, rows, moves, "paged_copy: generations [rows] of the pools' rows expected");
   for (const at::Tensor& p : pools) overwrite(p, "paged_copy");
   constexpr size_t most = 64;  // of a launch
+  if (generations.size() > most) {  // (the launch's own check is of its 64)
+    std::vector<const void*> all;
+    for (const at::Tensor& g : generations) all.push_back(g.data_ptr());
+    std::sort(all.begin(), all.end());
+    TORCH_CHECK(std::adjacent_find(all.begin(), all.end()) == all.end(), "paged_copy: the same generations twice");
+  }
   for (size_t i = 0; i < std::max(pools.size(), generations.size()); i += most) {
     std::vector<void*> data;
     std::vector<int64_t> bytes;

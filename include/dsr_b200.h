@@ -512,7 +512,8 @@ int dsr_paged_release(const int32_t* lengths, int32_t* held, int32_t* block_tabl
  * id below L that is not mapped; entries and shares follow, the ring is rebuilt as
  * L .. pool_blocks-1 (state {0, pool_blocks-L}, -1 behind them).  A block that no entry
  * maps is free afterwards, whether the ring had it or not, with no shares.  moves is
- * i32[max(1, pool_blocks/2)][4]: whole blocks, by ascending source.  pool_blocks <= 8388608.  Scratch as above. */
+ * i32[max(1, pool_blocks/2)][4]: whole blocks, by ascending source.  pool_blocks <=
+ * 8388608.  Scratch as above. */
 size_t dsr_paged_compact_workspace_bytes(int64_t pool_blocks);
 int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t table_stride,
                       int32_t* free_ring, int32_t* ring_state, int32_t* shares,
@@ -521,10 +522,10 @@ int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t table_stride,
 
 /* Copies the rows of the first *count moves in each of up to 64 pools of pool_rows rows
  * (row_bytes[i] a multiple of 16, at most 65536; 16-byte aligned) and adds 1 to the
- * written rows' entries of up to 64 generations i64[pool_rows] (an append's bump).  The
- * three host arrays are read by the call.  A move of more than 64 rows, or with rows
- * outside the pool, and a count outside [0, max_moves] give status 1 and are skipped.
- * No destination may be another move's source or destination. */
+ * written rows' entries of up to 64 generations i64[pool_rows] (an append's bump; the same
+ * one twice is refused).  The three host arrays are read by the call.  A move of more than
+ * 64 rows, or with rows outside the pool, and a count outside [0, max_moves] give status 1
+ * and are skipped.  No destination may be another move's source or destination. */
 int dsr_paged_copy(void* const* pools, const int64_t* row_bytes, int64_t pool_count,
                    int64_t* const* generations, int64_t generation_count, int64_t pool_rows,
                    const int32_t* moves, const int32_t* count, int64_t max_moves, int32_t* err,

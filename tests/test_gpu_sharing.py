@@ -351,3 +351,21 @@ def test_checked_calls_and_refusals(cuda):
                 ([pool.float().requires_grad_()], [gens], moves, count)):
         with pytest.raises(RuntimeError):
             ext.paged_copy(*bad)
+
+
+def test_copies_in_several_launches_are_refused_as_a_whole(cuda):
+    """More pools and generations than a launch takes: a bad one at the end, or one given twice."""
+    pools = [torch.arange(128 * 8, device="cuda", dtype=torch.int16).view(128, 8) for _ in range(70)]
+    gens = [torch.zeros(128, dtype=torch.int64, device="cuda") for _ in range(70)]
+    moves = gpu([np.array([(0, 64, 5, 0)], np.int32), np.array([1], np.int32)])
+    before = pools[0].clone()
+    narrow = torch.zeros((128, 4), device="cuda", dtype=torch.int16)
+    misplaced = torch.zeros(128 * 8 + 1, device="cuda", dtype=torch.int16)[1:].view(128, 8)
+    for bad in ((pools + [narrow], gens), (pools + [misplaced], gens), (pools, gens + gens[:1]), (pools, gens[:1] * 2)):
+        with pytest.raises(RuntimeError):
+            cuda_ops.extension().paged_copy(*bad, *moves)
+        assert torch.equal(pools[0], before) and not gens[0].any()
+    assert int(cuda_ops.extension().paged_copy(pools, gens, *moves)) == 0
+    before[64:69] = before[:5]
+    for p, g in zip(pools, gens):
+        assert torch.equal(p, before) and int(g.sum()) == int(g[64:69].sum()) == 5

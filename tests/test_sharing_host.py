@@ -69,6 +69,7 @@ def prefix(n, q=P, dtype=0, pool=P, blocks=8, table=P, rows=3, stride=4, context
     lambda n: copy(n, row_bytes=(0, 256)), lambda n: copy(n, row_bytes=(1152, 65552)), lambda n: copy(n, gens=(None,)),
     lambda n: copy(n, rows=0), lambda n: copy(n, rows=1 << 31), lambda n: copy(n, room=-1),
     lambda n: copy(n, pools=(P,) * 65, row_bytes=(16,) * 65), lambda n: copy(n, gens=(P,) * 65),
+    lambda n: copy(n, gens=(P, 512, P)),
 ])
 def test_host_side_validation_refuses_without_touching_a_device(call):
     lib = _native.library()
