@@ -40,8 +40,8 @@ constexpr int kPairRows = 128;
 constexpr int kPairLead = 2;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
-// What the join has to know of a request: its query rows, where its own parts are, and
-// where those of its run: part + segment * rows, or (segments < 0) item -1 - segments.
+// A request: its query rows, where its own parts are, and where those of its run: part +
+// segment * rows, or (segments < 0, the pairs') item -1 - segments.
 struct alignas(16) PrefixRequest {
   int32_t node0, nodes;
   int32_t own_part, own_segments;
@@ -505,11 +505,13 @@ __device__ __forceinline__ PairNode find_node(const PairArgs& a, int32_t node) {
     // a padding row.  Where a request was refused the sums may be in disorder and the search
     // may have missed the request that has the row: every one is asked
     lo = -1;
-    if (!__ldcg(a.head + 1))
+    if (!__ldcg(a.head + 1)) {
+#pragma unroll 8
       for (int b = 0; b < a.batch; ++b) {
-        s = load_request(a.requests + b);
-        if (node >= s.node0 && node < s.node0 + s.nodes) lo = b;
+        const int2 rows = __ldcg(reinterpret_cast<const int2*>(a.requests + b));  // node0, nodes
+        if (node >= rows.x && node < rows.x + rows.y) lo = b;
       }
+    }
     if (lo < 0) return PairNode{0, -1, 0, 0};
     s = load_request(a.requests + lo);
   }

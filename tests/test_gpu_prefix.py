@@ -298,3 +298,33 @@ def test_refusals(cuda):
         ext.prefix_mla_decode(*args, SCALE, sink=d["sink"][:3])
     with pytest.raises(RuntimeError):
         ext.prefix_mla_decode(*args, SCALE, out=torch.empty(2, 16, 576, device="cuda"))
+
+
+def test_bad_requests_of_a_few_rows(cuda):
+    """Up to 64 query rows: a refused request and the rows behind the last one stay as they are."""
+    base, rows, masks = problem(18, [(200, [(5, 1), (0, 1)]), (64, ONE)], 16, gap=1)
+    for change in (dict(context=[205, -1, 64]), dict(prefix=[200, 300, 64]), dict(holder=[3, 5, 4]), dict(cu=[0, 1, 0, 3])):
+        d = dict(base)
+        for key, value in change.items():
+            d[key] = torch.tensor(value, dtype=torch.int32).cuda()
+        out = torch.full((4, 16, 512), 5.0, device="cuda")
+        _, status = call(d, out=out)
+        assert int(status.item()) == 1
+        check(base, rows, masks, out, requests=[0] if "cu" in change else [0, 2])
+        if "cu" not in change:
+            assert torch.all(out[1] == 5.0)
+        assert torch.all(out[3] == 5.0)
+    fresh, _, lse = call(base, return_lse=True)
+    assert torch.all(fresh[3] == 0) and torch.all(torch.isneginf(lse[3]))
+
+
+def test_a_bad_request_of_a_large_batch(cuda):
+    """Its rows and those behind the last request stay as they are, the others are right."""
+    d, rows, masks = problem(19, [(300, [(2, 1)] * 700), (0, [(9, 2)] * 500)], 16, gap=40)
+    d["prefix"][700] = 10
+    d["holder"][3] = -7
+    out = torch.full((1740, 16, 512), 5.0, device="cuda")
+    _, status = call(d, out=out)
+    assert int(status.item()) == 1
+    check(d, rows, masks, out, requests=[0, 2, 4, 699, 701, 1199])
+    assert torch.all(out[3] == 5.0) and torch.all(out[700:702] == 5.0) and torch.all(out[1700:] == 5.0)
