@@ -23,6 +23,8 @@
 // measured sustained rate); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 78 us (55%:
 // 7 us until the first tile is there, 8 us of outputs, 11 us of the join).  The same by the
 // tree attention's groups of 64 rows: 831, 3133 and 122 us.
+#include <type_traits>
+
 #include "common.cuh"
 #include "host_common.h"
 #include "tree_jobs.cuh"
@@ -38,6 +40,9 @@ constexpr float kPlanJobTiles = 4.f;
 constexpr int kPairRows = 128;
 // The same of a piece, added to a group's tiles where the pairs share out the work.
 constexpr int kPairLead = 2;
+// Tiles that a request may add to be taken with its run's groups (below): an output of a piece
+// and its part of the join take as long as some five.
+constexpr int kPairStraddle = 4;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // A request: its query rows, where its own parts are, and where those of its run: part +
@@ -50,21 +55,41 @@ struct alignas(16) PrefixRequest {
 };
 static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
 
-// What the pairs of CTAs take: a run's shared rows, or a request's own ones.  Its query rows
-// are cut into groups of 128, whose tiles are numbered from unit0 on, kPairLead before each
-// group's first; pair c has the units [c share, (c + 1) share) of all runs, then those of all
-// requests, in one piece per group.  Piece (group g, pair c) leaves its partials at
-// part + 128 (g + c), since g or c rises from piece to piece.
+// What the pairs of CTAs take.  A run's query rows are cut into groups of 128.  A group has the
+// tiles of the shared rows, then those of the own rows of the requests that have rows in it: the
+// rows of other requests see nothing there, but O stays where it is.  (A request that lies across
+// one group more than its rows need would have its own rows multiplied once more.  Where that
+// makes more than kPairStraddle tiles, or without a run, its own rows are an item by themselves,
+// in groups of its own rows.)
+// Units are tiles, and kPairLead before each group's first; pair c has the units [c share,
+// (c + 1) share) of all runs, then those of all items by themselves, in one piece per group.
+// Piece (group g, pair c) leaves its partials at part + 128 (g + c), since g or c rises from
+// piece to piece.
 struct alignas(16) PairItem {
-  int64_t unit0;
-  int32_t groups, tiles;
+  int64_t unit0;                 // (of a run: its first group)
+  int32_t groups, tiles;         // tiles: of a run's shared rows
   int32_t row0, rows;            // query rows
   int32_t table, part;
   int32_t block0;                // tile i: positions 64 block0 + 128 i and up
-  int32_t context, drafts, own;  // positions from `context` on are drafted, seen as the masks say
+  int32_t context, drafts;       // positions from `context` on are drafted, seen as the masks say
+  int32_t unused;
   __device__ __forceinline__ int32_t span() const { return tiles + kPairLead; }
 };
 static_assert(sizeof(PairItem) == 48, "three 16-byte words");
+// A run's group; behind the last one its end.
+struct alignas(16) PairGroup {
+  int64_t unit0;
+  int32_t item, unused;
+};
+// A request's own rows that are taken with its run.  Its tiles in group g begin at unit
+// base + (g + 1) span + (g - first group of the request) tiles, with the run's span.
+struct alignas(16) PairSegment {
+  int64_t base;
+  int32_t row0, rows, tiles;  // tiles: 0 when they are an item by themselves
+  int32_t block0, context, drafts;
+  int32_t unused[2];
+};
+static_assert(sizeof(PairSegment) == 48, "three 16-byte words");
 
 // Where the parts of a node's rows are: of its request's own rows, then of its run.  The pairs'
 // idle warp finds it, so that a CTA of the join has one load to wait for and not four.
@@ -85,11 +110,13 @@ struct PrefixArgs {
   bool out_wide, zero_unused;
   float* lse;
   int32_t* err;
-  int32_t* head;  // {jobs, 1 when no request was refused, 0, 0, items of runs, share, items of requests, share}
+  int32_t* head;  // {jobs, 1 when no request was refused, 0, 0, groups of runs, share, items of requests, share}
   PrefixRequest* requests;
-  int32_t* places;   // the plan's own: [batch] a run's item
-  PairItem* items;   // [batch] of runs, [batch] of requests
-  PairNode* records; // [nodes]
+  PairItem* items;        // [batch] of runs, [batch] of requests
+  PairGroup* groups;      // [groups of runs + 1]
+  PairSegment* segments;  // [batch]
+  int32_t* owner;         // [nodes] the request, where it has a run
+  PairNode* records;      // [nodes]
   TreeJob* jobs;
   float *part_o, *part_m, *part_l;
   int64_t nodes;
@@ -128,7 +155,7 @@ __device__ __forceinline__ PairItem own_item(const PrefixArgs& a, int b, const P
   it.groups = (it.rows + rows - 1) / rows;
   it.tiles = int32_t((keys + 127) / 128);
   it.table = b, it.block0 = s.shared;
-  it.context = s.context, it.drafts = s.nodes, it.own = 1;
+  it.context = s.context, it.drafts = s.nodes;
   return it;
 }
 // (Of a run's first and last request.)
@@ -177,11 +204,19 @@ __device__ __forceinline__ T plan_scan(T mine, T& all, T* part) {
   all = __shfl_sync(~0u, upto, 31);
   return sum - mine + __shfl_sync(~0u, upto - one, warp);
 }
-// Rows and (low) items in one sum.
-constexpr int kItemBits = 16;
-static_assert(kPrefixMaxBatch < 1 << kItemBits, "items of a call");
-__device__ __forceinline__ int64_t rows_and_items(const PairItem& it) {
-  return (int64_t(it.rows) << kItemBits) + (it.groups > 0);
+// Groups (which overflow only in sums that are refused for their rows), rows (64 nodes of 128
+// heads each at most) and items in one sum.
+constexpr int kItemBits = 16, kRowBits = 28;
+static_assert(kPrefixMaxBatch < 1 << kItemBits && int64_t(kPrefixMaxBatch) * 64 * 128 < 1 << kRowBits, "of a call");
+__device__ __forceinline__ int64_t pair_counts(const PairItem& it) {
+  return int64_t(uint64_t(it.groups) << (kItemBits + kRowBits)) + (int64_t(it.rows) << kItemBits) + (it.groups > 0);
+}
+__device__ __forceinline__ int32_t items_of(int64_t counts) { return int32_t(counts & ((1 << kItemBits) - 1)); }
+__device__ __forceinline__ int32_t rows_of(int64_t counts) {
+  return int32_t(counts >> kItemBits & ((1 << kRowBits) - 1));
+}
+__device__ __forceinline__ int32_t groups_of(int64_t counts) {
+  return int32_t(uint64_t(counts) >> (kItemBits + kRowBits));
 }
 
 // What the pairs share: false, with nothing to do, when sums in disorder give rows to several
@@ -190,16 +225,46 @@ __device__ __forceinline__ bool write_pair_head(const PrefixArgs& a, bool writes
                                                 int64_t run_all, int64_t own_units, int64_t own_all) {
   const int64_t run_share = (run_units + a.pairs - 1) / a.pairs, own_share = (own_units + a.pairs - 1) / a.pairs;
   const int64_t most = a.nodes * a.heads;
-  const bool fits = run_all >> kItemBits <= most && own_all >> kItemBits <= most && run_share <= INT32_MAX &&
+  const bool fits = rows_of(run_all) <= most && rows_of(own_all) <= most && run_share <= INT32_MAX &&
                     own_share <= INT32_MAX;
   if (writes) {
-    constexpr int64_t kItems = (1 << kItemBits) - 1;
     int4* head = reinterpret_cast<int4*>(a.head);
     head[0] = make_int4(0, fits ? int(fine) : 1, 0, 0);
-    head[1] = fits ? make_int4(int(run_all & kItems), int(run_share), int(own_all & kItems), int(own_share))
+    head[1] = fits ? make_int4(groups_of(run_all), int(run_share), items_of(own_all), int(own_share))
                    : make_int4(0, 0, 0, 0);
+    if (fits) a.groups[groups_of(run_all)] = PairGroup{run_units, -1, 0};
   }
   return fits;
+}
+// The groups that a request lies across, and whether its own rows are taken with them.
+struct PairShare {
+  int32_t first, n, tiles;  // tiles: its own ones, or 0
+};
+__device__ __forceinline__ PairShare pair_share(int32_t run_groups, int32_t run_row0, const PairItem& own) {
+  if (run_groups == 0 || own.groups == 0) return PairShare{0, 0, 0};
+  const int32_t in = own.row0 - run_row0, first = in / kPairRows, n = (in + own.rows - 1) / kPairRows - first + 1;
+  return PairShare{first, n, int64_t(own.tiles) * (n - own.groups) <= kPairStraddle ? own.tiles : 0};
+}
+// What the pairs have to know of a request of a run: its segment, the groups that begin in its
+// rows, and whose its nodes are.
+__device__ __forceinline__ void write_share(const PrefixArgs& a, int b, const PrefixSeq& s, const PairItem& own,
+                                            const PairShare& share, int64_t base, int32_t run_item, int32_t run_row0,
+                                            int32_t run_group0, int32_t span) {
+  a.segments[b] = PairSegment{base, own.row0, own.rows, share.tiles, own.block0, own.context, own.drafts, {}};
+  const int32_t from = share.first + (own.row0 - run_row0 > share.first * kPairRows);
+  for (int32_t g = from; g < share.first + share.n; ++g)
+    a.groups[run_group0 + g] = PairGroup{base + int64_t(g) * span + int64_t(g - share.first) * share.tiles, run_item, 0};
+  for (int32_t x = 0; x < s.nodes; ++x) a.owner[s.node0 + x] = b;
+}
+// Sums in disorder may give a node to two runs, whose groups would not be whole then.
+__device__ __forceinline__ bool owns_all(const PrefixArgs& a, int b, const PrefixSeq& s) {
+  bool all = true;
+  for (int32_t x = 0; x < s.nodes; ++x) all &= __ldcg(a.owner + s.node0 + x) == b;
+  return all;
+}
+__device__ __forceinline__ void write_nothing(const PrefixArgs& a) {
+  int4* head = reinterpret_cast<int4*>(a.head);
+  head[0] = make_int4(0, 1, 0, 0), head[1] = make_int4(0, 0, 0, 0);
 }
 
 // The plan of the pairs' work.  Threads: 256 for up to 1024 requests, whose sequences are then
@@ -208,8 +273,6 @@ constexpr int kPlanCached = 1024;
 template <int Threads, bool Cached>
 __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_constant__ PrefixArgs a) {
   extern __shared__ int32_t starts[];  // [batch + 1] first request of each run
-  __shared__ int32_t kept[Cached ? kPlanCached : 1];
-  int32_t* places = Cached ? kept : a.places;  // [batch] a run's item, or -1
   __shared__ PrefixSeq cache[Cached ? kPlanCached : 1];
   __shared__ int64_t sums[4][32];
   __shared__ int32_t start_sums[32];
@@ -241,48 +304,67 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
     if (starts_run(b)) starts[r++] = b;
   if (tid == 0) starts[runs] = a.batch;
   fine = __syncthreads_and(fine);
-  // ---- units, rows and items before each
-  auto run = [&](int r) { return run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), kPairRows); };
-  const int per_run = (runs + Threads - 1) / Threads;
-  const int r0 = min(tid * per_run, runs), r1 = min(r0 + per_run, runs);
+  // ---- this thread's requests with their runs: f(b, its sequence, the run, whether it begins
+  // there, its own rows, what is taken with the run)
+  auto each = [&](auto&& f) {
+    PairItem run{};
+    for (int b = b0, r = run0 - 1; b < b1; ++b) {
+      const bool begins = r + 1 < runs && starts[r + 1] == b;
+      if (begins) ++r;
+      if (begins || b == b0) run = run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), kPairRows);
+      const PrefixSeq s = seq(b);
+      const PairItem own = own_item(a, b, s, kPairRows);
+      f(b, s, run, begins, own, pair_share(run.groups, run.row0, own));
+    }
+  };
+  // ---- units and counts before each
   int64_t unit = 0, at = 0, own_unit = 0, own_at = 0, units, all, own_units, own_all;
-  for (int r = r0; r < r1; ++r) {
-    const PairItem it = run(r);
-    unit += pair_units(it), at += rows_and_items(it);
-  }
-  for (int b = b0; b < b1; ++b) {
-    const PairItem it = own_item(a, b, seq(b), kPairRows);
-    own_unit += pair_units(it), own_at += rows_and_items(it);
-  }
+  auto add = [&](const PairItem& run, bool begins, const PairItem& own, const PairShare& share) {
+    if (begins) unit += pair_units(run), at += pair_counts(run);
+    unit += int64_t(share.n) * share.tiles;
+    if (share.tiles == 0) own_unit += pair_units(own), own_at += pair_counts(own);
+  };
+  each([&](int, const PrefixSeq&, const PairItem& run, bool begins, const PairItem& own, const PairShare& share) {
+    add(run, begins, own, share);
+  });
   unit = plan_scan<Threads>(unit, units, sums[0]);
   at = plan_scan<Threads>(at, all, sums[1]);
   own_unit = plan_scan<Threads>(own_unit, own_units, sums[2]);
   own_at = plan_scan<Threads>(own_at, own_all, sums[3]);
   const bool fits = write_pair_head(a, tid == 0, fine, units, all, own_units, own_all);
-  for (int r = r0; fits && r < r1; ++r) {
-    PairItem it = run(r);
-    const int32_t index = int32_t(at & ((1 << kItemBits) - 1));
-    places[r] = it.groups > 0 ? index : -1;
-    if (it.groups == 0) continue;
-    it.unit0 = unit, it.part = int32_t(at >> kItemBits);
-    a.items[index] = it;
-    unit += pair_units(it), at += rows_and_items(it);
-  }
-  __syncthreads();
-  for (int b = b0, r = run0 - 1; b < b1; ++b) {
-    if (r + 1 < runs && starts[r + 1] == b) ++r;
-    const PrefixSeq s = seq(b);
-    PairItem it = own_item(a, b, s, kPairRows);
-    const int32_t index = int32_t(own_at & ((1 << kItemBits) - 1));
-    if (fits && it.groups > 0) {
-      it.unit0 = own_unit, it.part = a.own_part + int32_t(own_at >> kItemBits);
-      a.items[a.batch + index] = it;
-      own_unit += pair_units(it), own_at += rows_and_items(it);
+  each([&](int b, const PrefixSeq& s, PairItem run, bool begins, PairItem own, const PairShare& share) {
+    if (!fits) {
+      a.requests[b] = PrefixRequest{};
+      return;
     }
-    a.requests[b] = !fits ? PrefixRequest{}
-                          : PrefixRequest{s.node0, s.nodes, 0, it.groups > 0 ? -1 - (a.batch + index) : 0, 0, 0,
-                                          places[r] >= 0 ? -1 - places[r] : 0, 0};
-  }
+    // (behind its first request the sums have the run in them)
+    const int64_t base = begins ? unit : unit - pair_units(run), before = begins ? at : at - pair_counts(run);
+    const int32_t index = items_of(before), own_index = items_of(own_at);
+    const PairItem whole_run = run, whole_own = own;
+    if (begins && run.groups > 0) {
+      run.unit0 = groups_of(before), run.part = rows_of(before);
+      a.items[index] = run;
+    }
+    if (run.groups > 0 && own.groups > 0)
+      write_share(a, b, s, own, share, base, index, run.row0, groups_of(before), run.span());
+    const bool alone = own.groups > 0 && share.tiles == 0;
+    if (alone) {
+      own.unit0 = own_unit, own.part = a.own_part + rows_of(own_at);
+      a.items[a.batch + own_index] = own;
+    }
+    a.requests[b] = PrefixRequest{s.node0, s.nodes, 0, alone ? -1 - (a.batch + own_index) : 0, 0, 0,
+                                  run.groups > 0 ? -1 - index : 0, 0};
+    add(whole_run, begins, whole_own, share);
+  });
+  if (fine || !fits) return;
+  __syncthreads();
+  bool mine = true;
+  each([&](int b, const PrefixSeq& s, const PairItem& run, bool, const PairItem&, const PairShare&) {
+    if (run.groups > 0) mine &= owns_all(a, b, s);
+  });
+  if (__syncthreads_and(mine)) return;
+  if (tid == 0) write_nothing(a);
+  for (int b = b0; b < b1; ++b) a.requests[b] = PrefixRequest{};
 }
 
 // Up to 32 requests, without a barrier: lane b of every warp has request b and, if one starts
@@ -321,27 +403,48 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
     all = __shfl_sync(~0u, upto, 31);
     return upto - x;
   };
-  int64_t run_all, own_all;
-  const int64_t run_at = before64(rows_and_items(run), run_all), own_at = before64(rows_and_items(own), own_all);
   if (a.pairs > 0) {
     if (warp > 0) return;
-    int64_t run_units, own_units;
-    run.unit0 = before64(pair_units(run), run_units);
-    own.unit0 = before64(pair_units(own), own_units);
-    const bool fits = write_pair_head(a, lane == 0, fine, run_units, run_all, own_units, own_all);
-    const int32_t run_index = int32_t(run_at & ((1 << kItemBits) - 1)), own_index = int32_t(own_at & ((1 << kItemBits) - 1));
-    run.part = int32_t(run_at >> kItemBits), own.part = a.own_part + int32_t(own_at >> kItemBits);
-    if (fits && run.groups > 0) a.items[run_index] = run;
-    if (fits && own.groups > 0) a.items[a.batch + own_index] = own;
-    const int32_t of = __shfl_sync(~0u, run.groups > 0 ? run_index : -1, start & 31);
+    const int32_t groups = __shfl_sync(~0u, run.groups, start & 31), row0 = __shfl_sync(~0u, run.row0, start & 31);
+    const int32_t span = __shfl_sync(~0u, run.span(), start & 31);
+    const PairShare share = pair_share(groups, row0, own);
+    const PairItem alone = share.tiles > 0 ? PairItem{} : own;
+    int64_t units, run_all, own_units, own_all;
+    const int64_t unit = before64(pair_units(run) + int64_t(share.n) * share.tiles, units);
+    const int64_t at = before64(pair_counts(run), run_all), own_unit = before64(pair_units(alone), own_units);
+    const int64_t own_at = before64(pair_counts(alone), own_all);
+    const bool fits = write_pair_head(a, lane == 0, fine, units, run_all, own_units, own_all);
+    const int32_t index = __shfl_sync(~0u, items_of(at), start & 31), own_index = items_of(own_at);
+    const int32_t group0 = __shfl_sync(~0u, groups_of(at), start & 31);
+    if (fits && run.groups > 0) {
+      PairItem it = run;
+      it.unit0 = group0, it.part = rows_of(at);
+      a.items[index] = it;
+    }
+    // (behind its first request the sums have the run in them)
+    if (fits && groups > 0 && own.groups > 0)
+      write_share(a, lane, s, own, share, starts ? unit : unit - int64_t(groups) * span, index, row0, group0, span);
+    if (fits && alone.groups > 0) {
+      PairItem it = alone;
+      it.unit0 = own_unit, it.part = a.own_part + rows_of(own_at);
+      a.items[a.batch + own_index] = it;
+    }
+    bool whole = fits;
+    if (!fine) {
+      __syncwarp();
+      whole = __all_sync(~0u, fits && (groups == 0 || owns_all(a, lane, s)));
+      if (!whole && lane == 0) write_nothing(a);
+    }
     if (here)
-      a.requests[lane] = !fits ? PrefixRequest{}
-                               : PrefixRequest{s.node0, s.nodes, 0, own.groups > 0 ? -1 - (a.batch + own_index) : 0, 0, 0,
-                                               of >= 0 ? -1 - of : 0, 0};
+      a.requests[lane] = !whole ? PrefixRequest{}
+                                : PrefixRequest{s.node0, s.nodes, 0, alone.groups > 0 ? -1 - (a.batch + own_index) : 0, 0, 0,
+                                                groups > 0 ? -1 - index : 0, 0};
     return;
   }
+  int64_t run_all, own_all;
+  before64(pair_counts(run), run_all), before64(pair_counts(own), own_all);
   const int64_t most = a.nodes * a.heads;
-  if (run_all >> kItemBits > most || own_all >> kItemBits > most) {  // as in write_pair_head
+  if (rows_of(run_all) > most || rows_of(own_all) > most) {  // as in write_pair_head
     if (threadIdx.x == 0) a.head[0] = 0, a.head[1] = 1;
     if (warp == 0 && here) a.requests[lane] = PrefixRequest{};
     return;
@@ -480,6 +583,9 @@ struct PairArgs {
   float *part_o, *part_m, *part_l;
   const int32_t* head;
   const PairItem* items;
+  const PairGroup* groups;
+  const PairSegment* segments;
+  const int32_t* owner;
   int32_t* err;
   int batch, heads, pairs;
   const int32_t* cu_nodes;
@@ -492,6 +598,15 @@ __device__ __forceinline__ PrefixRequest load_request(const PrefixRequest* reque
   const int4* words = reinterpret_cast<const int4*>(request);
   const int4 x = __ldcg(words), y = __ldcg(words + 1);
   return PrefixRequest{x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+}
+__device__ __forceinline__ PairGroup load_group(const PairGroup* group) {
+  const int4 x = __ldcg(reinterpret_cast<const int4*>(group));
+  return PairGroup{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w};
+}
+__device__ __forceinline__ PairSegment load_segment(const PairSegment* segment) {
+  const int4* words = reinterpret_cast<const int4*>(segment);
+  const int4 x = __ldcg(words), y = __ldcg(words + 1);
+  return PairSegment{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w, y.x, y.y, y.z, y.w, {}};
 }
 __device__ __forceinline__ PairNode find_node(const PairArgs& a, int32_t node) {
   int lo = 0;  // the largest b with cu_nodes[b] <= node
@@ -515,56 +630,74 @@ __device__ __forceinline__ PairNode find_node(const PairArgs& a, int32_t node) {
     if (lo < 0) return PairNode{0, -1, 0, 0};
     s = load_request(a.requests + lo);
   }
-  // an item's parts: those of the pairs that have a tile of the node's group
-  auto parts = [&](int32_t index, int share_at, int32_t& part, int32_t& count) {
-    if (index >= 0) return;
-    const PairItem item = load_item(a.items - 1 - index);
+  // the parts: those of the pairs that have a tile of the node's group
+  auto parts = [&](const PairItem& item, int64_t unit, int64_t end, int share_at, int32_t& part, int32_t& count) {
     const int64_t share = __ldcg(a.head + share_at);
-    const int32_t in = node * a.heads - item.row0;
-    const int64_t unit = item.unit0 + int64_t(in / kPairRows) * item.span();
-    const int32_t first = pair_of(unit + kPairLead, share), last = pair_of(unit + item.span() - 1, share);
-    part = item.part + in + kPairRows * first;
+    const int32_t first = pair_of(unit + kPairLead, share), last = pair_of(end - 1, share);
+    part = item.part + node * a.heads - item.row0 + kPairRows * first;
     count = last - first + 1;
   };
   PairNode found{0, 0, 0, 0};
-  parts(s.own_segments, 7, found.own_part, found.own_parts);
-  parts(s.run_segments, 5, found.run_part, found.run_parts);
+  if (s.own_segments < 0) {
+    const PairItem item = load_item(a.items - 1 - s.own_segments);
+    const int64_t unit = item.unit0 + int64_t((node * a.heads - item.row0) / kPairRows) * item.span();
+    parts(item, unit, unit + item.span(), 7, found.own_part, found.own_parts);
+  }
+  if (s.run_segments < 0) {
+    const PairItem item = load_item(a.items - 1 - s.run_segments);
+    const PairGroup* group = a.groups + item.unit0 + (node * a.heads - item.row0) / kPairRows;
+    parts(item, load_group(group).unit0, load_group(group + 1).unit0, 5, found.run_part, found.run_parts);
+  }
   return found;
 }
 
 // A pair's pieces, one after another (every warp walks them for itself): of the runs, then of
-// the requests.
+// the requests by themselves.
 struct PairWalk {
   const PairArgs& a;
   int64_t unit, end;
-  int32_t at, pair, phase;  // phase: 0 runs, 1 requests
+  int32_t at, pair, phase;  // phase: 0 runs (`at` a group), 1 requests (an item)
   PairItem item;
+  int64_t group_unit, next_unit;  // of a run's group, and the one behind it
+  int32_t item_at, next_item, group;
   int32_t row0, rows, tile0, count, part;  // of the piece at hand
   // the requests' range and first item, found with the runs'
   int64_t own_unit, own_end;
   int32_t own_at;
   __device__ __forceinline__ PairWalk(const PairArgs& a_, int pair_) : a(a_), pair(pair_), phase(0) {
     const int4 head = __ldcg(reinterpret_cast<const int4*>(a.head) + 1);
-    find(a.items, head.x, head.y, unit, end, at);
-    find(a.items + a.batch, head.z, head.w, own_unit, own_end, own_at);
-    if (unit < end) item = load_item(a.items + at);
-  }
-  // The pair's range of a list's units, and the item that it starts in.
-  __device__ __forceinline__ void find(const PairItem* items, int32_t n_items, int64_t share, int64_t& from, int64_t& to,
-                                       int32_t& first) {
-    from = to = share * pair;
-    first = 0;
-    if (n_items == 0) return;
-    const PairItem last = load_item(items + n_items - 1);
-    to = min(from + share, last.unit0 + int64_t(last.groups) * last.span());
-    // the last item that starts at or before the unit, 32 ways a step
-    for (int n = n_items; n > 1;) {
-      const int stride = (n + 31) / 32, i = int(threadIdx.x & 31) * stride;
-      const unsigned below = __ballot_sync(~0u, i < n && __ldcg(&items[first + i].unit0) <= from);
-      const int lead = (31 - __clz(below)) * stride;
-      first += lead;
-      n = min(stride, n - lead);
+    unit = end = int64_t(head.y) * pair;
+    own_unit = own_end = int64_t(head.w) * pair;
+    at = own_at = 0;
+    if (head.x > 0) {
+      end = min(unit + head.y, load_group(a.groups + head.x).unit0);
+      at = find(&a.groups->unit0, sizeof(PairGroup), head.x, unit);
     }
+    if (head.z > 0) {
+      const PairItem last = load_item(a.items + a.batch + head.z - 1);
+      own_end = min(own_unit + head.w, last.unit0 + int64_t(last.groups) * last.span());
+      own_at = find(&a.items[a.batch].unit0, sizeof(PairItem), head.z, own_unit);
+    }
+    if (unit >= end) return;
+    const PairGroup here = load_group(a.groups + at), next = load_group(a.groups + at + 1);
+    group_unit = here.unit0, item_at = here.item;
+    next_unit = next.unit0, next_item = next.item;
+    item = load_item(a.items + item_at);
+  }
+  // The last of n records, their first units `stride` bytes apart, that starts at or before the
+  // unit, 32 ways a step.
+  __device__ __forceinline__ int32_t find(const int64_t* units, int64_t stride, int32_t n_all, int64_t from) {
+    int32_t first = 0;
+    const char* base = reinterpret_cast<const char*>(units);
+    for (int n = n_all; n > 1;) {
+      const int step = (n + 31) / 32, i = int(threadIdx.x & 31) * step;
+      const unsigned below =
+          __ballot_sync(~0u, i < n && __ldcg(reinterpret_cast<const int64_t*>(base + (first + i) * stride)) <= from);
+      const int lead = (31 - __clz(below)) * step;
+      first += lead;
+      n = min(step, n - lead);
+    }
+    return first;
   }
   __device__ __forceinline__ bool next() {
     for (;;) {
@@ -574,10 +707,22 @@ struct PairWalk {
         unit = own_unit, end = own_end, at = own_at;
         item = load_item(a.items + a.batch + at);
       }
-      if (unit >= item.unit0 + int64_t(item.groups) * item.span()) item = load_item(a.items + (phase ? a.batch : 0) + ++at);
-      const int64_t in = unit - item.unit0;
-      const int32_t span = item.span(), group = int32_t(in / span), from = int32_t(in - int64_t(group) * span);
-      const int32_t to = int32_t(min(int64_t(span), from + (end - unit)));
+      int64_t start, stop;  // the group's units
+      if (phase == 0) {
+        if (unit >= next_unit) {
+          group_unit = next_unit;
+          if (next_item != item_at) item_at = next_item, item = load_item(a.items + item_at);
+          const PairGroup next = load_group(a.groups + ++at + 1);
+          next_unit = next.unit0, next_item = next.item;
+        }
+        group = at - int32_t(item.unit0);
+        start = group_unit, stop = next_unit;
+      } else {
+        if (unit >= item.unit0 + int64_t(item.groups) * item.span()) item = load_item(a.items + a.batch + ++at);
+        group = int32_t((unit - item.unit0) / item.span());
+        start = item.unit0 + int64_t(group) * item.span(), stop = start + item.span();
+      }
+      const int32_t from = int32_t(unit - start), to = int32_t(min(stop, end) - start);
       unit += to - from;
       tile0 = max(from - kPairLead, 0);
       count = max(to - kPairLead, 0) - tile0;
@@ -587,9 +732,24 @@ struct PairWalk {
       if (count > 0) return true;
     }
   }
-  // First position of tile i, and whether some of its positions are drafted ones or past the end.
-  __device__ __forceinline__ int32_t position(int32_t i) const { return item.block0 * DSR_BLOCK_TOKENS + i * 128; }
-  __device__ __forceinline__ bool ragged(int32_t i) const { return item.context - position(i) < 128; }
+  // The group's first tiles, of rows that all of it shares.
+  __device__ __forceinline__ int32_t shared() const { return phase == 0 ? item.tiles : 0; }
+  // A request's own tiles in the group: [first, first + tiles), of positions from `position` on.
+  struct Own {
+    int32_t request, first, tiles, position, context, drafts;
+  };
+  __device__ __forceinline__ Own own(int32_t node) const {
+    if (phase == 1) return Own{item.table, 0, item.tiles, item.block0 * DSR_BLOCK_TOKENS, item.context, item.drafts};
+    const int32_t request = __ldcg(a.owner + node);
+    const PairSegment s = load_segment(a.segments + request);
+    const int64_t start = s.base + int64_t(group + 1) * item.span() +
+                          int64_t(group - (s.row0 - item.row0) / kPairRows) * s.tiles;
+    return Own{request, int32_t(start - group_unit) - kPairLead, s.tiles, s.block0 * DSR_BLOCK_TOKENS, s.context, s.drafts};
+  }
+  // Whether some query rows of the group do not see all of a tile.
+  __device__ __forceinline__ bool masked(int32_t tile) const {
+    return item.block0 * DSR_BLOCK_TOKENS - item.context + int64_t(tile) * 128 > -128;  // (of a run: past its shared rows too)
+  }
 };
 
 // ---- barriers of a pair
@@ -786,11 +946,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) pair_arrive(to_q);
       }
-      // of the drafted positions, those that this thread's row sees
+      // the tiles that this thread's row sees by itself, and of the drafted positions those
       uint64_t word = 0;
-      if (walk.item.drafts > 0 && mine < walk.rows) {
-        word = uint64_t(a.masks[(walk.row0 + mine) / a.heads]);
-        if (walk.item.drafts < 64) word &= (1ull << walk.item.drafts) - 1ull;
+      int32_t own_first = 0, own_tiles = 0, own_left = 0;  // left: where its context is behind the first tile's start
+      if (mine < walk.rows) {
+        const int32_t node = (walk.row0 + mine) / a.heads;
+        const PairWalk::Own own = walk.own(node);
+        own_first = own.first, own_tiles = own.tiles, own_left = own.context - own.position;
+        word = uint64_t(a.masks[node]);
+        if (own.drafts < 64) word &= (1ull << own.drafts) - 1ull;
       }
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
@@ -804,13 +968,19 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           tmem_wait_ld();
 #pragma unroll
           for (int c = 0; c < 32; ++c) v[c] = __uint_as_float(t0[c]);
-          if (walk.ragged(walk.tile0 + i)) {
-            // bit c: this thread's key c is seen; key c is drafted position `first` + c
-            const int32_t first = walk.position(walk.tile0 + i) + 64 * half + 32 * side - walk.item.context;
+          const int32_t tile = walk.tile0 + i;
+          if (walk.masked(tile)) {
+            // bit c: this thread's key c is seen; key c is drafted position `first` + c.  (None
+            // of a run's are drafted; another request's are all past everything)
+            const bool common = tile < walk.shared(), its = uint32_t(tile - own_first) < uint32_t(own_tiles);
+            const int32_t first = 64 * half + 32 * side + (common ? int32_t(128u * tile - walk.item.context)
+                                                           : its  ? int32_t(128u * (tile - own_first) - own_left)
+                                                                  : 64);
+            const uint64_t drafted = common ? 0ull : word;
             const uint32_t shown = first >= 64    ? 0u
-                                   : first >= 0   ? uint32_t(word >> first)
+                                   : first >= 0   ? uint32_t(drafted >> first)
                                    : first <= -32 ? ~0u
-                                                  : uint32_t(word) << -first | ((1u << -first) - 1u);
+                                                  : uint32_t(drafted) << -first | ((1u << -first) - 1u);
 #pragma unroll
             for (int c = 0; c < 32; ++c)
               if (!(shown >> c & 1u)) v[c] = -CUDART_INF_F;
@@ -1019,13 +1189,33 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int n = 0, cleared = 0;
     bool ok = true;
     while (ok && walk.next()) {
-      const int32_t* table = a.table + int64_t(walk.item.table) * a.stride;
-      const int32_t blocks = int32_t((int64_t(walk.item.context) + walk.item.drafts + DSR_BLOCK_TOKENS - 1) /
-                                     DSR_BLOCK_TOKENS);
+      // Lane k: the own tiles of the group's node k, and what any of the group's rows of that
+      // request sees of its drafted positions (8 nodes at most)
+      const int32_t shared = walk.shared(), node = walk.row0 / a.heads + lane;
+      const bool has_node = lane * a.heads < walk.rows;
+      const PairWalk::Own own = has_node ? walk.own(node) : PairWalk::Own{-1, 0, 0, 0, 0, 0};
+      const uint64_t word = has_node ? uint64_t(a.masks[node]) : 0ull;
+      uint64_t seen = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint64_t other = __shfl_sync(~0u, word, k);
+        if (__shfl_sync(~0u, own.request, k) == own.request) seen |= other;
+      }
+      // the lane of a tile that is not of the shared ones
+      auto lane_of = [&](int32_t tile) {
+        return (__ffs(__ballot_sync(~0u, uint32_t(tile - own.first) < uint32_t(own.tiles))) - 1) & 31;
+      };
       const int32_t none = int32_t(a.pool_rows);  // past the pool: reads zeros
       // the tile's two pages; what a block id means is seen when they are used
       auto pages = [&](int32_t tile) {
-        const int32_t j = walk.item.block0 + 2 * tile;
+        int32_t row = walk.item.table, j = 2 * tile, blocks = walk.item.context / DSR_BLOCK_TOKENS;
+        if (tile >= shared) {
+          const int k = lane_of(tile);
+          row = __shfl_sync(~0u, own.request, k);
+          j = __shfl_sync(~0u, own.position / DSR_BLOCK_TOKENS - 2 * own.first, k) + 2 * tile;
+          blocks = __shfl_sync(~0u, int32_t((int64_t(own.context) + own.drafts + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS), k);
+        }
+        const int32_t* table = a.table + int64_t(row) * a.stride;
         return make_int2(j < blocks ? table[j] : INT32_MIN, j + 1 < blocks ? table[j + 1] : INT32_MIN);
       };
       auto row_of = [&](int32_t blk) {
@@ -1039,13 +1229,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // The whole warp runs the loop and one lane issues, as the MMAs are: a copy from a
       // one-lane branch takes some 200 cycles to be on its way
       auto wait = [&](uint64_t* bar, uint32_t parity) { return pair_wait_warp(bar, parity, abort, a.err); };
-      // what any of the group's rows sees of the drafted positions (8 nodes at most)
-      uint64_t seen = 0;
-      if (walk.item.drafts > 0) {
-        const int32_t node = walk.row0 / a.heads + lane;
-        const uint64_t word = node <= (walk.row0 + walk.rows - 1) / a.heads ? uint64_t(a.masks[node]) : 0ull;
-        seen = uint64_t(__reduce_or_sync(~0u, uint32_t(word >> 32))) << 32 | __reduce_or_sync(~0u, uint32_t(word));
-      }
       if (!a.q_wide) {
         // the query, once the last S MMA of the piece before has read the one there
         if (n > 0) ok = wait(bar_s + ((n - 1) & 1), ((n - 1) >> 1) & 1);
@@ -1070,7 +1253,14 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       };
       auto values = [&](int k, int32_t tile, int32_t y0, int32_t y1) {
         // a request's rows from its context on: hidden ones are cleared before they count
-        const bool clears = walk.item.own != 0 && walk.ragged(tile);
+        int32_t first = -kPairKeys, drafts = 0;  // of its drafted positions, where the tile starts
+        uint64_t visible = 0;
+        if (tile >= shared) {
+          const int k = lane_of(tile);
+          first = int32_t(__shfl_sync(~0u, uint32_t(own.position) - own.context - 128u * own.first, k) + 128u * tile);
+          drafts = __shfl_sync(~0u, own.drafts, k), visible = __shfl_sync(~0u, seen, k);
+        }
+        const bool clears = first > -kPairKeys;
         if (clears && leader) mbar_arrive_expect_tx(bar_own, 2 * 4 * L::kBlock);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
@@ -1089,14 +1279,13 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         ok = wait(bar_own, cleared++ & 1);
         if (!ok) return;
         // a lane has 16 bytes of a row: its four blocks' parts are 512 bytes
-        const int32_t first = walk.position(tile) - walk.item.context;
         uint8_t* mine = smem + L::kVOff + (4 * (lane >> 4) + (lane >> 3 & 1)) * L::kBlock + (lane & 7) * 16;
         auto clear = [&](int x) {
           *reinterpret_cast<uint4*>(mine + 2 * (x >> 6) * L::kBlock + (x & 63) * 128) = make_uint4(0, 0, 0, 0);
         };
-        const int past = min(max(walk.item.drafts - first, 0), kPairKeys);
+        const int past = min(max(drafts - first, 0), kPairKeys);
         for (int x = max(-first, 0); x < past; ++x)
-          if (!(seen >> (first + x) & 1)) clear(x);
+          if (!(visible >> (first + x) & 1)) clear(x);
 #pragma unroll 4
         for (int x = past; x < kPairKeys; ++x) clear(x);
         fence_proxy_async_smem();
@@ -1328,7 +1517,7 @@ size_t rounded(size_t bytes) { return (bytes + 255) / 256 * 256; }
 struct PrefixSizes {
   int rows;
   int pairs;
-  size_t requests, places, items, records, jobs;  // bytes
+  size_t requests, items, groups, segments, owner, records, jobs;  // bytes
   size_t parts, own_part;                // rows of partials, and where those of the requests' items begin
 };
 PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads) {
@@ -1344,8 +1533,10 @@ PrefixSizes prefix_sizes(int64_t batch, int64_t nodes, int64_t heads) {
   } else {
     s.rows = kPairRows;
     s.pairs = tree_ctas() / 2;
-    s.places = rounded(size_t(batch) * sizeof(int32_t));
     s.items = rounded(2 * size_t(batch) * sizeof(PairItem));
+    s.groups = rounded((rows / kPairRows + size_t(batch) + 1) * sizeof(PairGroup));
+    s.segments = rounded(size_t(batch) * sizeof(PairSegment));
+    s.owner = rounded(size_t(nodes) * sizeof(int32_t));
     s.records = rounded(size_t(nodes) * sizeof(PairNode));
     s.own_part = rows + size_t(kPairRows) * s.pairs;
     s.parts = 2 * s.own_part;
@@ -1360,7 +1551,8 @@ extern "C" size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, i
   using namespace dsr;
   if (batch <= 0 || nodes <= 0 || heads <= 0) return 0;
   const PrefixSizes s = prefix_sizes(batch, nodes, heads);
-  return 256 + s.requests + s.places + s.items + s.records + s.jobs + s.parts * (DSR_V_DIM + 2) * 4;
+  return 256 + s.requests + s.items + s.groups + s.segments + s.owner + s.records + s.jobs +
+         s.parts * (DSR_V_DIM + 2) * 4;
 }
 
 extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int64_t pool_blocks,
@@ -1416,12 +1608,16 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   a.err = err;
   a.head = reinterpret_cast<int32_t*>(ws);
   a.requests = reinterpret_cast<PrefixRequest*>(ws + 256);
-  a.places = reinterpret_cast<int32_t*>(ws + 256 + sizes.requests);
-  uint8_t* at = ws + 256 + sizes.requests + sizes.places;
-  a.items = reinterpret_cast<PairItem*>(at);
-  at += sizes.items;
-  a.records = reinterpret_cast<PairNode*>(at);
-  at += sizes.records;
+  uint8_t* at = ws + 256 + sizes.requests;
+  auto take = [&](auto*& p, size_t bytes) {
+    p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(at);
+    at += bytes;
+  };
+  take(a.items, sizes.items);
+  take(a.groups, sizes.groups);
+  take(a.segments, sizes.segments);
+  take(a.owner, sizes.owner);
+  take(a.records, sizes.records);
   a.jobs = reinterpret_cast<TreeJob*>(at);
   a.part_o = reinterpret_cast<float*>(at + sizes.jobs);
   a.part_m = a.part_o + sizes.parts * DSR_V_DIM;
@@ -1450,7 +1646,8 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   const float scale_log2 = scale * kTreeLog2e;
   if (a.pairs > 0) {
     rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2,
-                               a.part_o, a.part_m, a.part_l, a.head, a.items, err, a.batch, a.heads, a.pairs, cu_nodes,
+                               a.part_o, a.part_m, a.part_l, a.head, a.items, a.groups, a.segments, a.owner, err,
+                               a.batch, a.heads, a.pairs, cu_nodes,
                                a.requests, a.records, int32_t(nodes)},
                       kv_pool, nodes * heads, as_stream(stream));
   } else {
