@@ -1657,25 +1657,29 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
                             as_stream(stream));
   }
   if (rc != DSR_OK) return rc;
-  // The pairs' parts: a CTA has all columns of its rows.  With up to eight CTAs a SM it is bound
-  // by latency, and more parts at once pay (2576 rows: 14 to 11 us), with more it is not (8192
-  // rows: 17 and 22 us).  The list's few rows and many parts: a column and every fourth part a
-  // thread (384 rows of the pairs' few parts took 15 us so, for 4)
+  // The list's few rows and many parts: a column and every fourth part a thread.  The pairs':
+  // with a CTA a SM at most, a part is a large share of a row's too, two columns and every fourth
+  // part a thread (128 rows of 75 parts: 66 to 42 us in all, 448 rows 75 to 62, 384 rows of three
+  // parts 24 to 25.5).  Else a CTA has all columns of its rows (2048 rows: 105 us, 113 the other
+  // way); with up to eight CTAs a SM it is bound by latency, and more parts at once pay (2576
+  // rows: 14 to 11 us), with more it is not (8192 rows: 17 and 22 us)
   const int64_t quads = nodes * heads / 4;
-  const bool whole = a.pairs > 0;
-  const auto join = !whole                      ? prefix_join_kernel<false, 1, 4, 8>
-                    : quads <= 8 * sm_count() ? prefix_join_kernel<true, 4, 1, 4>
-                                              : prefix_join_kernel<true, 4, 1, 2>;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(quads), whole ? 1 : DSR_V_DIM / kJoinThreads, 1);
-  cfg.blockDim = dim3(kJoinThreads * (whole ? 1 : 4), 1, 1);
-  cfg.stream = as_stream(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join, a);
+  auto launch_join = [&](auto* join, int columns, int split) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(unsigned(quads), DSR_V_DIM / (kJoinThreads * columns), 1);
+    cfg.blockDim = dim3(kJoinThreads * split, 1, 1);
+    cfg.stream = as_stream(stream);
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join, a);
+  };
+  const cudaError_t e = a.pairs == 0                ? launch_join(prefix_join_kernel<false, 1, 4, 8>, 1, 4)
+                        : quads <= sm_count()     ? launch_join(prefix_join_kernel<true, 2, 4, 4>, 2, 4)
+                        : quads <= 8 * sm_count() ? launch_join(prefix_join_kernel<true, 4, 1, 4>, 4, 1)
+                                                  : launch_join(prefix_join_kernel<true, 4, 1, 2>, 4, 1);
   if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode join launch: %s", cudaGetErrorString(e));
   return DSR_OK;
 }
