@@ -163,6 +163,15 @@ def test_edges_of_tiles_and_groups(cuda, heads):
     verify(*problem(heads, prompts, heads, tree="any"))
 
 
+@pytest.mark.parametrize("heads,nodes", [(16, 3), (16, 5), (32, 3), (64, 3), (128, 2)])
+def test_requests_across_groups_of_rows(cuda, heads, nodes):
+    """Own rows, short and long, of requests whose rows lie in one group of 128 or across several."""
+    mine = (1000, 10, 2000, 0, 5000, 513, 511, 127, 640, 641, 1, 4000)
+    requests = [(m, (nodes, 1, 0, nodes + 4)[i % 4]) for i, m in enumerate(mine)]
+    for prompts in ([(700, requests)], [(64, requests[:5]), (30, requests[5:]), (64, requests[::-1])]):
+        verify(*problem(heads + nodes, prompts, heads, tree="any", kept=False))
+
+
 def test_padding_queries_may_hold_anything(cuda):
     d, rows, masks = problem(17, [(700, [(3, 1)] * 10)], 32, gap=30)
     d["q"][10:] = float("nan")
