@@ -841,6 +841,35 @@ __device__ __forceinline__ bool rows_sync(int half, bool ok) {
       : "memory");
   return r != 0;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two FP32 values an instruction, each rounded as by itself.
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -986,7 +1015,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               if (!(shown >> c & 1u)) v[c] = -CUDART_INF_F;
           }
 #pragma unroll
-          for (int c = 0; c < 32; ++c) top = fmaxf(top, v[c]);
+          for (int c = 0; c < 32; c += 2) top = max3(top, v[c], v[c + 1]);
           top *= a.scale_log2;
         }
         // weights against the running maximum as it stands; their sums are of the weights as
@@ -995,14 +1024,18 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         float sum = 0.f;
         auto weigh = [&] {
           const float base = m == -CUDART_INF_F ? 0.f : m;
-          float s0 = 0.f, s1 = 0.f;
+          const uint64_t scales = pack2(a.scale_log2, a.scale_log2), bases = pack2(-base, -base);
+          uint64_t both = 0;
 #pragma unroll
           for (int c = 0; c < 16; ++c) {
-            const float x = ex2(fmaf(v[2 * c], a.scale_log2, -base)), y = ex2(fmaf(v[2 * c + 1], a.scale_log2, -base));
-            s0 += x;
-            s1 += y;
+            float x, y;
+            unpack2(fma2(pack2(v[2 * c], v[2 * c + 1]), scales, bases), x, y);
+            x = ex2(x), y = ex2(y);
+            both = add2(both, pack2(x, y));
             packed[c] = pack_bf16(x, y);
           }
+          float s0, s1;
+          unpack2(both, s0, s1);
           sum = s0 + s1;
         };
         bool fits = ok && i > 0 && !(top > m + kPairSlack);
@@ -1027,7 +1060,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
               tmem_ld32(tmem_o + c + lanes, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              for (int x = 0; x < 32; x += 2) {
+                float lo, hi;
+                unpack2(mul2(pack2(__uint_as_float(o[x]), __uint_as_float(o[x + 1])), pack2(f, f)), lo, hi);
+                o[x] = __float_as_uint(lo), o[x + 1] = __float_as_uint(hi);
+              }
               tmem_st32(tmem_o + c + lanes, o);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
