@@ -13,16 +13,16 @@
 // Three launches without a host read: the plan (one CTA), the attention, the join.  More than
 // 64 query rows, or 32 requests: by pairs of CTAs in groups of 128 rows, the runs' and the
 // requests' own rows alike.  Fewer: one group has all rows of a run, and the tree attention's
-// kernel takes the jobs from a list (two requests of 16 heads over 4096 rows: 22 us; by pairs
+// kernel takes the jobs from a list (two requests of 16 heads over 4096 rows: 21 us; by pairs
 // in an earlier form 38, for 27 by the list).
 //
 // Bound by the tensor cores, and by the power that they may take.  Measured alone, with cold
-// inputs: 64 requests of 128 heads that share 32768 rows and have up to 1500 of their own 399
-// us (598 GFLOP, 1.50 PFLOP/s, 90% of a measured BF16 GEMM); 256 of 64 heads over 65472 rows
-// 1626 us (1.44 PFLOP/s, 86%), one call after another 1930 us (1.21 PFLOP/s, 88% of the
-// measured sustained rate); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 78 us (55%:
-// 7 us until the first tile is there, 8 us of outputs, 11 us of the join).  The same by the
-// tree attention's groups of 64 rows: 831, 3133 and 122 us.
+// inputs: 64 requests of 128 heads that share 32768 rows and have up to 1500 of their own 389
+// us (598 GFLOP, 1.54 PFLOP/s, 92% of a measured BF16 GEMM); 256 of 64 heads over 65472 rows
+// 1640 us (1.43 PFLOP/s, 86%), one call after another 1930 us (1.22 PFLOP/s, 88% of the
+// measured sustained rate); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 68 us (63%:
+// the plan 3.5 us, 7 until the first tile is there, outputs of 3.5, the join 7.5).  The same by
+// the tree attention's groups of 64 rows: 831, 3133 and 122 us.
 #include <type_traits>
 
 #include "common.cuh"
@@ -40,9 +40,10 @@ constexpr float kPlanJobTiles = 4.f;
 constexpr int kPairRows = 128;
 // The same of a piece, added to a group's tiles where the pairs share out the work.
 constexpr int kPairLead = 2;
-// Tiles that a request may add to be taken with its run's groups (below): an output of a piece
-// and its part of the join take as long as some five.
-constexpr int kPairStraddle = 4;
+// Tiles that a request may add to be taken with its run's groups (below): what an output of a
+// piece and its part of the join take.  (100 requests of 3 nodes and 32 heads over 4096 rows: with
+// 5 tiles of their own 108 us, 114 by themselves; with 16 151 and 144, with 32 218 and 189.)
+constexpr int kPairStraddle = 12;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // A request: its query rows, where its own parts are, and where those of its run: part +
@@ -57,7 +58,9 @@ static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
 
 // What the pairs of CTAs take.  A run's query rows are cut into groups of 128.  A group has the
 // tiles of the shared rows, then those of the own rows of the requests that have rows in it: the
-// rows of other requests see nothing there, but O stays where it is.  (A request that lies across
+// rows of other requests see nothing there, but O stays where it is (137 requests of 128 heads
+// over 752 shared rows: 92 us with every request's own rows by themselves, 72 so; the 64 requests
+// above 412 and 393, 190 of 16 heads, most without a run, 44 and 46).  (A request that lies across
 // one group more than its rows need would have its own rows multiplied once more.  Where that
 // makes more than kPairStraddle tiles, or without a run, its own rows are an item by themselves,
 // in groups of its own rows.)
@@ -533,17 +536,19 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
 // so that an SM reads of every operand its own half only: 4 KB of shared memory for an MMA
 // of 32 cycles, 6 KB for one of 64 (a CTA alone, with 64 rows: 6 KB for 32).  For S a CTA has
 // its 64 keys of the tile with all columns, for O all 128 keys with its half of the value
-// columns, which are fetched once more, from L2.  A tile takes 2360 cycles, its 52 MMAs 2209
-// (measured by themselves: 32.6 and 64.7 cycles); 139 KB arrive in either SM meanwhile, 12 TB/s
-// in all.  What got it there, for the 64 requests above: copies of three and two column blocks
-// issued by a converged warp (a lane by itself takes some 200 cycles a copy), page ids a tile
-// ahead, and arrivals at the pair's barriers without a release to the cluster (1000 cycles).
+// columns, which are fetched once more, from L2.  A tile takes some 2450 cycles, its 52 MMAs
+// 2209 (measured by themselves: 32.6 and 64.7 cycles); 139 KB arrive in either SM meanwhile, 12
+// TB/s in all.  A change of the group takes 9000: output, query, first tile.  What got it there,
+// for the 64 requests above: copies of three and two column blocks issued by a converged warp (a
+// lane by itself takes some 200 cycles a copy), page ids a tile ahead, and arrivals at the pair's
+// barriers without a release to the cluster (1000 cycles).
 // Not kept: pages prefetched into L2 a tile ahead (402 to 438 us).
 // An accumulator of 64 rows takes tensor memory's lanes twice: lanes 0..63 have the rows and
 // the first half of the columns, lanes 64..127 the same rows and the second half.
 //   warps 0..7  (FP32 query -> shared memory,) softmax: warp w has rows 32 (w % 2) .. of
 //               this CTA and of the keys, value columns in half w / 2 % 2 those in half w / 4;
 //               the running maximum of a row is followed only when it grows by more than 2^8
+//               (four warps: 2 to 8% slower where pieces are short, 1% faster in the largest)
 //   warp 8      tensor memory; in CTA 0 the MMAs: S of the next tile, then O of this one, so
 //               that they run through the softmax between
 //   warp 9      query, keys and values by TMA; what arrives in either CTA is counted by CTA
@@ -1364,7 +1369,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 // Joins the parts of a row: one CTA per four query rows (of one node, since heads come in
 // sixteens) and 128 Columns value columns, a thread Columns of them of all four and every
 // Split-th part.  Few rows of many parts are bound by the latency of one part after another
-// (32 rows of 34 parts: 10 us by one thread a column, each after eight others).
+// (32 rows of 34 parts: 10 us by one thread a column, each after eight others), many rows by
+// the partials that come from L2 (17536 rows, 54 MB: 15 us).
 // ---------------------------------------------------------------------------
 constexpr int kJoinThreads = 128;
 constexpr int kJoinMaxParts = kPlanWaves * kTreeMaxCtas + 16;
