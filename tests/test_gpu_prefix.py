@@ -135,6 +135,15 @@ def test_many_requests(cuda):
     verify(d, rows, masks, requests=[0, 1, 2, 700, 1500, len(rows) - 600, len(rows) - 300, len(rows) - 1])
 
 
+def test_the_largest_batch(cuda):
+    d, rows, masks = problem(20, [(64, [(1, 1)] * 16384)], 16)
+    verify(d, rows, masks, requests=[0, 1, 7, 8, 8191, 16383])
+    d["context"][77] = -1
+    out, status = call(d, out=torch.full((16384, 16, 512), 5.0, device="cuda"))
+    assert int(status.item()) == 1 and torch.all(out[77] == 5.0)
+    check(d, rows, masks, out, requests=[0, 76, 78, 16383])
+
+
 def test_the_tree_attention_agrees(cuda):
     d, rows, masks = problem(9, [(1000, [(30, 2), (40, 3)] * 8), (64, ONE)], 32)
     out, status, lse = call(d, return_lse=True)
