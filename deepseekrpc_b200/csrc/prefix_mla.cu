@@ -40,10 +40,6 @@ constexpr float kPlanJobTiles = 4.f;
 constexpr int kPairRows = 128;
 // The same of a piece, added to a group's tiles where the pairs share out the work.
 constexpr int kPairLead = 2;
-// Tiles that a request may add to be taken with its run's groups (below): what an output of a
-// piece and its part of the join take.  (100 requests of 3 nodes and 32 heads over 4096 rows: with
-// 5 tiles of their own 108 us, 114 by themselves; with 16 151 and 144, with 32 218 and 189.)
-constexpr int kPairStraddle = 12;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // A request: its query rows, where its own parts are, and where those of its run: part +
@@ -57,13 +53,13 @@ struct alignas(16) PrefixRequest {
 static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
 
 // What the pairs of CTAs take.  A run's query rows are cut into groups of 128.  A group has the
-// tiles of the shared rows, then those of the own rows of the requests that have rows in it: the
-// rows of other requests see nothing there, but O stays where it is (137 requests of 128 heads
-// over 752 shared rows: 92 us with every request's own rows by themselves, 72 so; the 64 requests
-// above 412 and 393, 190 of 16 heads, most without a run, 44 and 46).  (A request that lies across
-// one group more than its rows need would have its own rows multiplied once more.  Where that
-// makes more than kPairStraddle tiles, or without a run, its own rows are an item by themselves,
-// in groups of its own rows.)
+// tiles of the shared rows, then, where all of its rows are one request's, those of the request's
+// own rows: O stays where it is (137 requests of 128 heads over 752 shared rows: 92 us with every
+// request's own rows by themselves, 72 so; the 64 requests above 412 and 393).  The own rows of a
+// request whose groups have other requests' rows too, or that has no run, are an item by
+// themselves, in groups of its own rows: with weights of zero another request's values would
+// still reach a row where they are not finite.  (Taken all the same: 23 requests of 5 prompts 68 us
+// for 74, 52 of 32 heads 35 for 39, 256 of 64 heads over 65472 rows 1642 for 1659.)
 // Units are tiles, and kPairLead before each group's first; pair c has the units [c share,
 // (c + 1) share) of all runs, then those of all items by themselves, in one piece per group.
 // Piece (group g, pair c) leaves its partials at part + 128 (g + c), since g or c rises from
@@ -79,20 +75,17 @@ struct alignas(16) PairItem {
   __device__ __forceinline__ int32_t span() const { return tiles + kPairLead; }
 };
 static_assert(sizeof(PairItem) == 48, "three 16-byte words");
-// A run's group; behind the last one its end.
+// A run's group, with the request that has its first row; behind the last one its end.
 struct alignas(16) PairGroup {
   int64_t unit0;
-  int32_t item, unused;
+  int32_t item, request;
 };
-// A request's own rows that are taken with its run.  Its tiles in group g begin at unit
-// base + (g + 1) span + (g - first group of the request) tiles, with the run's span.
+// A request's own rows, where they are taken with its run: as in an item.
 struct alignas(16) PairSegment {
-  int64_t base;
-  int32_t row0, rows, tiles;  // tiles: 0 when they are an item by themselves
   int32_t block0, context, drafts;
-  int32_t unused[2];
+  int32_t unused;
 };
-static_assert(sizeof(PairSegment) == 48, "three 16-byte words");
+static_assert(sizeof(PairSegment) == 16, "a 16-byte word");
 
 // Where the parts of a node's rows are: of its request's own rows, then of its run.  The pairs'
 // idle warp finds it, so that a CTA of the join has one load to wait for and not four.
@@ -118,7 +111,7 @@ struct PrefixArgs {
   PairItem* items;        // [batch] of runs, [batch] of requests
   PairGroup* groups;      // [groups of runs + 1]
   PairSegment* segments;  // [batch]
-  int32_t* owner;         // [nodes] the request, where it has a run
+  int32_t* owner;         // [nodes] the request, where it has a run (see owns_all)
   PairNode* records;      // [nodes]
   TreeJob* jobs;
   float *part_o, *part_m, *part_l;
@@ -235,28 +228,31 @@ __device__ __forceinline__ bool write_pair_head(const PrefixArgs& a, bool writes
     head[0] = make_int4(0, fits ? int(fine) : 1, 0, 0);
     head[1] = fits ? make_int4(groups_of(run_all), int(run_share), items_of(own_all), int(own_share))
                    : make_int4(0, 0, 0, 0);
-    if (fits) a.groups[groups_of(run_all)] = PairGroup{run_units, -1, 0};
+    if (fits) a.groups[groups_of(run_all)] = PairGroup{run_units, -1, -1};
   }
   return fits;
 }
-// The groups that a request lies across, and whether its own rows are taken with them.
+// The groups of its run that a request lies across, and its own tiles in each of them: none where
+// they have other requests' rows too.
 struct PairShare {
-  int32_t first, n, tiles;  // tiles: its own ones, or 0
+  int32_t first, n, tiles;
 };
-__device__ __forceinline__ PairShare pair_share(int32_t run_groups, int32_t run_row0, const PairItem& own) {
+__device__ __forceinline__ PairShare pair_share(const PairItem& own, int32_t run_groups, int32_t run_row0,
+                                                int32_t run_rows) {
   if (run_groups == 0 || own.groups == 0) return PairShare{0, 0, 0};
-  const int32_t in = own.row0 - run_row0, first = in / kPairRows, n = (in + own.rows - 1) / kPairRows - first + 1;
-  return PairShare{first, n, int64_t(own.tiles) * (n - own.groups) <= kPairStraddle ? own.tiles : 0};
+  const int32_t in = own.row0 - run_row0, end = in + own.rows, first = in / kPairRows;
+  const bool whole = in % kPairRows == 0 && (end % kPairRows == 0 || end == run_rows);
+  return PairShare{first, (end - 1) / kPairRows - first + 1, whole ? own.tiles : 0};
 }
 // What the pairs have to know of a request of a run: its segment, the groups that begin in its
-// rows, and whose its nodes are.
+// rows, and whose its nodes are.  base: the run's first unit, and the own tiles before the request's.
 __device__ __forceinline__ void write_share(const PrefixArgs& a, int b, const PrefixSeq& s, const PairItem& own,
                                             const PairShare& share, int64_t base, int32_t run_item, int32_t run_row0,
                                             int32_t run_group0, int32_t span) {
-  a.segments[b] = PairSegment{base, own.row0, own.rows, share.tiles, own.block0, own.context, own.drafts, {}};
+  a.segments[b] = PairSegment{own.block0, own.context, own.drafts, 0};
   const int32_t from = share.first + (own.row0 - run_row0 > share.first * kPairRows);
   for (int32_t g = from; g < share.first + share.n; ++g)
-    a.groups[run_group0 + g] = PairGroup{base + int64_t(g) * span + int64_t(g - share.first) * share.tiles, run_item, 0};
+    a.groups[run_group0 + g] = PairGroup{base + int64_t(g) * span + int64_t(g - share.first) * share.tiles, run_item, b};
   for (int32_t x = 0; x < s.nodes; ++x) a.owner[s.node0 + x] = b;
 }
 // Sums in disorder may give a node to two runs, whose groups would not be whole then.
@@ -317,7 +313,7 @@ __global__ void __launch_bounds__(Threads, 1) prefix_plan_kernel(const __grid_co
       if (begins || b == b0) run = run_item(a, seq(starts[r]), seq(starts[r + 1] - 1), kPairRows);
       const PrefixSeq s = seq(b);
       const PairItem own = own_item(a, b, s, kPairRows);
-      f(b, s, run, begins, own, pair_share(run.groups, run.row0, own));
+      f(b, s, run, begins, own, pair_share(own, run.groups, run.row0, run.rows));
     }
   };
   // ---- units and counts before each
@@ -410,7 +406,7 @@ __global__ void __launch_bounds__(kFewThreads, 1) prefix_plan_few_kernel(const _
     if (warp > 0) return;
     const int32_t groups = __shfl_sync(~0u, run.groups, start & 31), row0 = __shfl_sync(~0u, run.row0, start & 31);
     const int32_t span = __shfl_sync(~0u, run.span(), start & 31);
-    const PairShare share = pair_share(groups, row0, own);
+    const PairShare share = pair_share(own, groups, row0, __shfl_sync(~0u, run.rows, start & 31));
     const PairItem alone = share.tiles > 0 ? PairItem{} : own;
     int64_t units, run_all, own_units, own_all;
     const int64_t unit = before64(pair_units(run) + int64_t(share.n) * share.tiles, units);
@@ -590,7 +586,6 @@ struct PairArgs {
   const PairItem* items;
   const PairGroup* groups;
   const PairSegment* segments;
-  const int32_t* owner;
   int32_t* err;
   int batch, heads, pairs;
   const int32_t* cu_nodes;
@@ -609,9 +604,8 @@ __device__ __forceinline__ PairGroup load_group(const PairGroup* group) {
   return PairGroup{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w};
 }
 __device__ __forceinline__ PairSegment load_segment(const PairSegment* segment) {
-  const int4* words = reinterpret_cast<const int4*>(segment);
-  const int4 x = __ldcg(words), y = __ldcg(words + 1);
-  return PairSegment{int64_t(uint32_t(x.x)) | int64_t(x.y) << 32, x.z, x.w, y.x, y.y, y.z, y.w, {}};
+  const int4 x = __ldcg(reinterpret_cast<const int4*>(segment));
+  return PairSegment{x.x, x.y, x.z, 0};
 }
 __device__ __forceinline__ PairNode find_node(const PairArgs& a, int32_t node) {
   int lo = 0;  // the largest b with cu_nodes[b] <= node
@@ -665,6 +659,7 @@ struct PairWalk {
   PairItem item;
   int64_t group_unit, next_unit;  // of a run's group, and the one behind it
   int32_t item_at, next_item, group;
+  int32_t request, next_request;  // of their first rows
   int32_t row0, rows, tile0, count, part;  // of the piece at hand
   // the requests' range and first item, found with the runs'
   int64_t own_unit, own_end;
@@ -685,8 +680,8 @@ struct PairWalk {
     }
     if (unit >= end) return;
     const PairGroup here = load_group(a.groups + at), next = load_group(a.groups + at + 1);
-    group_unit = here.unit0, item_at = here.item;
-    next_unit = next.unit0, next_item = next.item;
+    group_unit = here.unit0, item_at = here.item, request = here.request;
+    next_unit = next.unit0, next_item = next.item, next_request = next.request;
     item = load_item(a.items + item_at);
   }
   // The last of n records, their first units `stride` bytes apart, that starts at or before the
@@ -715,10 +710,10 @@ struct PairWalk {
       int64_t start, stop;  // the group's units
       if (phase == 0) {
         if (unit >= next_unit) {
-          group_unit = next_unit;
+          group_unit = next_unit, request = next_request;
           if (next_item != item_at) item_at = next_item, item = load_item(a.items + item_at);
           const PairGroup next = load_group(a.groups + ++at + 1);
-          next_unit = next.unit0, next_item = next.item;
+          next_unit = next.unit0, next_item = next.item, next_request = next.request;
         }
         group = at - int32_t(item.unit0);
         start = group_unit, stop = next_unit;
@@ -739,17 +734,14 @@ struct PairWalk {
   }
   // The group's first tiles, of rows that all of it shares.
   __device__ __forceinline__ int32_t shared() const { return phase == 0 ? item.tiles : 0; }
-  // A request's own tiles in the group: [first, first + tiles), of positions from `position` on.
+  // What the tiles behind those are of: a request's own rows, from `position` on.
   struct Own {
-    int32_t request, first, tiles, position, context, drafts;
+    int32_t request, position, context, drafts;
   };
-  __device__ __forceinline__ Own own(int32_t node) const {
-    if (phase == 1) return Own{item.table, 0, item.tiles, item.block0 * DSR_BLOCK_TOKENS, item.context, item.drafts};
-    const int32_t request = __ldcg(a.owner + node);
+  __device__ __forceinline__ Own own() const {
+    if (phase == 1) return Own{item.table, item.block0 * DSR_BLOCK_TOKENS, item.context, item.drafts};
     const PairSegment s = load_segment(a.segments + request);
-    const int64_t start = s.base + int64_t(group + 1) * item.span() +
-                          int64_t(group - (s.row0 - item.row0) / kPairRows) * s.tiles;
-    return Own{request, int32_t(start - group_unit) - kPairLead, s.tiles, s.block0 * DSR_BLOCK_TOKENS, s.context, s.drafts};
+    return Own{request, s.block0 * DSR_BLOCK_TOKENS, s.context, s.drafts};
   }
   // Whether some query rows of the group do not see all of a tile.
   __device__ __forceinline__ bool masked(int32_t tile) const {
@@ -980,16 +972,12 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) pair_arrive(to_q);
       }
-      // the tiles that this thread's row sees by itself, and of the drafted positions those
-      uint64_t word = 0;
-      int32_t own_first = 0, own_tiles = 0, own_left = 0;  // left: where its context is behind the first tile's start
-      if (mine < walk.rows) {
-        const int32_t node = (walk.row0 + mine) / a.heads;
-        const PairWalk::Own own = walk.own(node);
-        own_first = own.first, own_tiles = own.tiles, own_left = own.context - own.position;
-        word = uint64_t(a.masks[node]);
-        if (own.drafts < 64) word &= (1ull << own.drafts) - 1ull;
-      }
+      // the drafted positions that this thread's row sees, and where they are behind the first own
+      // tile's start
+      const PairWalk::Own own = walk.own();
+      const int32_t shared = walk.shared(), own_left = own.context - own.position;
+      uint64_t word = mine < walk.rows ? uint64_t(a.masks[(walk.row0 + mine) / a.heads]) : 0ull;
+      if (own.drafts < 64) word &= (1ull << own.drafts) - 1ull;
       float m = -CUDART_INF_F, l = 0.f;
       for (int i = 0; i < count; ++i, ++n) {
         ok = ok && pair_wait_warp(bar_s + (n & 1), (n >> 1) & 1, abort, a.err);
@@ -1005,11 +993,10 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           const int32_t tile = walk.tile0 + i;
           if (walk.masked(tile)) {
             // bit c: this thread's key c is seen; key c is drafted position `first` + c.  (None
-            // of a run's are drafted; another request's are all past everything)
-            const bool common = tile < walk.shared(), its = uint32_t(tile - own_first) < uint32_t(own_tiles);
+            // of a run's are drafted)
+            const bool common = tile < shared;
             const int32_t first = 64 * half + 32 * side + (common ? int32_t(128u * tile - walk.item.context)
-                                                           : its  ? int32_t(128u * (tile - own_first) - own_left)
-                                                                  : 64);
+                                                                  : int32_t(128u * (tile - shared) - own_left));
             const uint64_t drafted = common ? 0ull : word;
             const uint32_t shown = first >= 64    ? 0u
                                    : first >= 0   ? uint32_t(drafted >> first)
@@ -1231,31 +1218,20 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     int n = 0, cleared = 0;
     bool ok = true;
     while (ok && walk.next()) {
-      // Lane k: the own tiles of the group's node k, and what any of the group's rows of that
-      // request sees of its drafted positions (8 nodes at most)
-      const int32_t shared = walk.shared(), node = walk.row0 / a.heads + lane;
-      const bool has_node = lane * a.heads < walk.rows;
-      const PairWalk::Own own = has_node ? walk.own(node) : PairWalk::Own{-1, 0, 0, 0, 0, 0};
-      const uint64_t word = has_node ? uint64_t(a.masks[node]) : 0ull;
-      uint64_t seen = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint64_t other = __shfl_sync(~0u, word, k);
-        if (__shfl_sync(~0u, own.request, k) == own.request) seen |= other;
-      }
-      // the lane of a tile that is not of the shared ones
-      auto lane_of = [&](int32_t tile) {
-        return (__ffs(__ballot_sync(~0u, uint32_t(tile - own.first) < uint32_t(own.tiles))) - 1) & 31;
-      };
+      // of the own rows, the drafted positions that any of the group's rows sees (8 nodes at most)
+      const int32_t shared = walk.shared();
+      const PairWalk::Own own = walk.own();
+      const uint64_t word = lane * a.heads < walk.rows ? uint64_t(a.masks[walk.row0 / a.heads + lane]) : 0ull;
+      const uint64_t seen = uint64_t(__reduce_or_sync(~0u, uint32_t(word))) |
+                            uint64_t(__reduce_or_sync(~0u, uint32_t(word >> 32))) << 32;
       const int32_t none = int32_t(a.pool_rows);  // past the pool: reads zeros
       // the tile's two pages; what a block id means is seen when they are used
       auto pages = [&](int32_t tile) {
         int32_t row = walk.item.table, j = 2 * tile, blocks = walk.item.context / DSR_BLOCK_TOKENS;
         if (tile >= shared) {
-          const int k = lane_of(tile);
-          row = __shfl_sync(~0u, own.request, k);
-          j = __shfl_sync(~0u, own.position / DSR_BLOCK_TOKENS - 2 * own.first, k) + 2 * tile;
-          blocks = __shfl_sync(~0u, int32_t((int64_t(own.context) + own.drafts + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS), k);
+          row = own.request;
+          j = own.position / DSR_BLOCK_TOKENS + 2 * (tile - shared);
+          blocks = int32_t((int64_t(own.context) + own.drafts + DSR_BLOCK_TOKENS - 1) / DSR_BLOCK_TOKENS);
         }
         const int32_t* table = a.table + int64_t(row) * a.stride;
         return make_int2(j < blocks ? table[j] : INT32_MIN, j + 1 < blocks ? table[j + 1] : INT32_MIN);
@@ -1295,13 +1271,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       };
       auto values = [&](int k, int32_t tile, int32_t y0, int32_t y1) {
         // a request's rows from its context on: hidden ones are cleared before they count
-        int32_t first = -kPairKeys, drafts = 0;  // of its drafted positions, where the tile starts
-        uint64_t visible = 0;
-        if (tile >= shared) {
-          const int k = lane_of(tile);
-          first = int32_t(__shfl_sync(~0u, uint32_t(own.position) - own.context - 128u * own.first, k) + 128u * tile);
-          drafts = __shfl_sync(~0u, own.drafts, k), visible = __shfl_sync(~0u, seen, k);
-        }
+        int32_t first = -kPairKeys;  // of its drafted positions, where the tile starts
+        if (tile >= shared) first = int32_t(128u * (tile - shared) + own.position - own.context);
         const bool clears = first > -kPairKeys;
         if (clears && leader) mbar_arrive_expect_tx(bar_own, 2 * 4 * L::kBlock);
 #pragma unroll
@@ -1325,9 +1296,9 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         auto clear = [&](int x) {
           *reinterpret_cast<uint4*>(mine + 2 * (x >> 6) * L::kBlock + (x & 63) * 128) = make_uint4(0, 0, 0, 0);
         };
-        const int past = min(max(drafts - first, 0), kPairKeys);
+        const int past = min(max(own.drafts - first, 0), kPairKeys);
         for (int x = max(-first, 0); x < past; ++x)
-          if (!(visible >> (first + x) & 1)) clear(x);
+          if (!(seen >> (first + x) & 1)) clear(x);
 #pragma unroll 4
         for (int x = past; x < kPairKeys; ++x) clear(x);
         fence_proxy_async_smem();
@@ -1689,7 +1660,7 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   const float scale_log2 = scale * kTreeLog2e;
   if (a.pairs > 0) {
     rc = launch_pairs(PairArgs{q, q_dtype == DSR_F32, block_table, table_stride, pa.rows, tree_mask, scale_log2,
-                               a.part_o, a.part_m, a.part_l, a.head, a.items, a.groups, a.segments, a.owner, err,
+                               a.part_o, a.part_m, a.part_l, a.head, a.items, a.groups, a.segments, err,
                                a.batch, a.heads, a.pairs, cu_nodes,
                                a.requests, a.records, int32_t(nodes)},
                       kv_pool, nodes * heads, as_stream(stream));

@@ -599,8 +599,8 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
  * beyond the order of FP32 sums; all else, and the status, as in dsr_tree_mla_decode.
  * Status 1 also for a prefix or holder out of range (that request's rows count as
  * unused), and where disordered sums of cu_nodes give rows to several requests (then
- * all may count as unused).  With status 2 rows of a request that has only finite values
- * may be non-finite, where another one in its run has not.  batch <= 16384, nodes * heads <= 2^24.
+ * all may count as unused).  A non-finite row of a request's own reaches that request's
+ * output alone.  batch <= 16384, nodes * heads <= 2^24.
  * Scratch: dsr_prefix_mla_workspace_bytes() on the current device, 256-byte aligned,
  * need not be cleared; calls sharing it must not overlap. */
 size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads);
