@@ -19,6 +19,20 @@ class ValidationError(ValueError):
     """An input or device state the operation refused (the reference's ValidationError)."""
 
 
+class BlockError(ValidationError):
+    """A change of block tables that was done all the same, around a bad block.
+
+    A block id outside the pool (or a count of shares that is too low) was met on the way: it
+    has -1 or nothing in its place, and every other request is as asked.  `value` is what the
+    call returns; its moves are to be copied as ever (paged_copy), or blocks that the other
+    requests hold now miss their rows.  Where nothing has changed, plain ValidationError is raised.
+    """
+
+    def __init__(self, message, value):
+        super().__init__(message)
+        self.value = value
+
+
 @lru_cache(maxsize=1)
 def extension():
     import torch
@@ -116,33 +130,50 @@ def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, to
     return tuple(value)
 
 
+def _moves(result, changed):
+    """(moves, count) of a call that reports; changed(count): whether it has changed any table."""
+    moves, count, status = result
+    code = int(status.item())
+    if code and changed(int(count.item())):
+        raise BlockError(f"native CUDA operation met a bad block (code {code}); its moves are still to be copied",
+                         (moves, count))
+    _status(status)
+    return moves, count
+
+
 def paged_fork(parent, lengths, held, block_table, free_ring, ring_state, shares):
     """Requests with a parent become its first `lengths` tokens, on the parent's whole blocks.
 
     Updates the five tables in place; returns (moves, count), the rows of partial last
-    blocks that paged_copy has to copy in every pool.  A refused batch changes nothing.
+    blocks that paged_copy has to copy in every pool.  A refused batch changes nothing; one
+    that is done around a bad block raises BlockError, which has the moves.
     """
-    *value, status = extension().paged_fork(parent, lengths, held, block_table, free_ring, ring_state, shares)
-    _status(status)
-    return tuple(value)
+    before = held.clone()
+    return _moves(extension().paged_fork(parent, lengths, held, block_table, free_ring, ring_state, shares),
+                  lambda count: count > 0 or not before.equal(held))
 
 
 def paged_release(lengths, held, block_table, free_ring, ring_state, shares):
     """Cuts every request to `lengths` tokens; blocks that nobody maps any more are free again.
 
     Returns (moves, count): a partial last block that others map too is exchanged for a
-    fresh one, whose rows paged_copy has to copy.  A refused batch changes nothing.
+    fresh one, whose rows paged_copy has to copy.  A refused batch (too few free blocks for
+    those among its reasons, whatever else the batch gives back) changes nothing; one that is
+    done around a bad block raises BlockError, which has the moves.
     """
-    *value, status = extension().paged_release(lengths, held, block_table, free_ring, ring_state, shares)
-    _status(status)
-    return tuple(value)
+    before = held.clone()
+    return _moves(extension().paged_release(lengths, held, block_table, free_ring, ring_state, shares),
+                  lambda count: count > 0 or not before.equal(held))
 
 
 def paged_compact(held, block_table, free_ring, ring_state, shares):
-    """The blocks in use get the lowest ids; returns (moves, count) of the blocks to copy."""
-    *value, status = extension().paged_compact(held, block_table, free_ring, ring_state, shares)
-    _status(status)
-    return tuple(value)
+    """The blocks in use get the lowest ids; returns (moves, count) of the blocks to copy.
+
+    A `held` out of range is refused, with nothing changed; a bad block id raises BlockError,
+    which has the moves of the others.
+    """
+    return _moves(extension().paged_compact(held, block_table, free_ring, ring_state, shares),
+                  lambda _: not bool(((held < 0) | (held > block_table.shape[1])).any()))
 
 
 def paged_copy(pools, generations, moves, count):

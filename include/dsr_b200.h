@@ -478,8 +478,9 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
  * The caller copies them (dsr_paged_copy) in every pool that the table maps, before
  * anything is appended.  batch <= 16384.  Refused with status 1, the tables unchanged
  * and count 0: what each call says, too few free blocks for the copies, a held or a
- * ring state out of range.  A block id outside the pool met on the way gives status 1,
- * -1 in the new entries and no move. */
+ * ring state out of range.  A block id outside the pool met on the way gives status 1 too,
+ * -1 in the new entries and no move; all else is done, so that the other moves have to be
+ * copied (of a refused call there are none). */
 
 /* Forks requests: request b with parent[b] = p >= 0 becomes the first lengths[b] tokens
  * of request p.  Its whole blocks are p's (shares + 1), the rows of a last, partial one
