@@ -90,6 +90,8 @@ SIGNATURES = {
                                          _P, _P, _P, c_int64, _P]),
     "dsr_paged_plan": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64,
                                _P]),
+    "dsr_paged_plan_shared": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P,
+                                      c_int64, _P]),
     "dsr_paged_fork": (c_int, [_P, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_int64, _P]),
     "dsr_paged_release_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "dsr_paged_release": (c_int, [_P, _P, _P, c_int64, _P, _P, _P, c_int64, _P, _P, _P, c_size_t, _P, c_int64, _P]),

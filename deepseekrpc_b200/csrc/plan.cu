@@ -19,6 +19,13 @@
 // dependent read of the block id, one store.  Measured: 7 us a call for 1 request as for
 // 256 with 8 tokens each (launch and the extension's allocation); 1M tokens of 256
 // requests 15.6 us, 12 MB written (0.8 TB/s).
+//
+// With `shares` every CTA first looks at the held blocks that the call would write to or give
+// back.  A CTA that is ahead may have set a given back entry to -1 already: only one that has
+// found no shared block does, so that all CTAs come to the same answer.  (1 request 5.1 us for
+// 3.9 from a graph, 256 with 8 tokens each 7.8 for 5.8; 16000 blocks given back 25 more.  The
+// counts are a parameter of a kernel by itself: as a member of the arguments of all they cost
+// the plan without them 0.5 us.)
 #include "common.cuh"
 #include "host_common.h"
 
@@ -75,6 +82,17 @@ __device__ __forceinline__ bool plan_request(const PlanArgs& a, int b, int32_t& 
   return true;
 }
 
+// A request's held blocks that the call writes to (it has new tokens) or gives back: from `first` on.
+struct Touched {
+  int32_t first, n;
+};
+__device__ __forceinline__ Touched plan_touched(const PlanArgs& a, int b) {
+  int32_t len, fresh, have, need;
+  plan_request(a, b, len, fresh, have, need);
+  const int32_t first = fresh > 0 ? len >> kBlockShift : need;
+  return Touched{first, max(have - first, 0)};
+}
+
 // The largest b with cu[b] <= i (cu[0] = 0, cu increasing weakly, i < cu[n]).
 __device__ __forceinline__ int plan_owner(const int32_t* cu, int n, int32_t i) {
   int lo = 0, hi = n;  // cu[lo] <= i < cu[hi]
@@ -86,7 +104,46 @@ __device__ __forceinline__ int plan_owner(const int32_t* cu, int n, int32_t i) {
   return lo;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
+// Whether others map a block that the call writes to or gives back, alike for the CTA.
+// cu [batch + 1]: the blocks to look at before each request.
+__device__ __forceinline__ bool plan_meets_shared(const PlanArgs& a, int b0, int b1, int32_t* cu,
+                                                  const int32_t* shares) {
+  __shared__ int64_t warp_blocks[kPlanThreads / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += plan_touched(a, b).n;
+  int64_t at = mine, all = 0;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t up = __shfl_up_sync(~0u, at, d);
+    if (lane >= d) at += up;
+  }
+  if (lane == 31) warp_blocks[warp] = at;
+  __syncthreads();
+  at -= mine;
+  for (int w = 0; w < kPlanThreads / 32; ++w) {
+    if (w < warp) at += warp_blocks[w];
+    all += warp_blocks[w];
+  }
+  if (all > INT32_MAX) return true;
+  for (int b = b0; b < b1; ++b) {
+    cu[b] = int32_t(at);
+    at += plan_touched(a, b).n;
+  }
+  if (tid == 0) cu[a.batch] = int32_t(all);
+  __syncthreads();
+  bool meets = false;
+  for (int64_t i = tid; i < all; i += kPlanThreads) {
+    const int b = plan_owner(cu, a.batch, int32_t(i));
+    const int32_t blk = a.table[int64_t(b) * a.stride + plan_touched(a, b).first + (int32_t(i) - cu[b])];
+    meets |= blk >= 0 && blk < a.blocks && shares[blk] > 0;
+  }
+  return __syncthreads_or(meets);
+}
+
+// Shares: the counts of shared blocks, or nothing.
+template <typename... Shares>
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a, Shares... shares) {
   extern __shared__ int32_t plan_smem[];
   int32_t* cu_tokens = plan_smem;                  // [batch + 1]
   int32_t* cu_take = cu_tokens + a.batch + 1;      // [batch + 1]
@@ -121,7 +178,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   }
   const int64_t head = a.state[0], count = a.state[1];
   const bool ok = bad == 0 && all.tokens <= a.tokens && all.take <= count && head >= 0 && head < a.blocks &&
-                  count >= 0 && count + all.give <= a.blocks;
+                  count >= 0 && count + all.give <= a.blocks &&
+                  !(... || plan_meets_shared(a, b0, b1, cu_give, shares));
   Sums at = before + run;
   at = Sums{at.tokens - mine.tokens, at.take - mine.take, at.give - mine.give};
   if (ok) {
@@ -275,15 +333,10 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs a) {
   if (tid == 0) a.state[2] = 0;
 }
 
-}  // namespace
-}  // namespace dsr
-
-extern "C" int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* held, int32_t* block_table,
-                              int64_t table_stride, int32_t* free_ring, int32_t* ring_state, int64_t pool_blocks,
-                              int32_t* seq, int32_t* positions, int32_t* slots, int64_t tokens, int32_t* cu_tokens,
-                              int32_t* visible, int32_t* err, int64_t batch, void* stream) {
-  using namespace dsr;
-  clear_error();
+int launch_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* held, int32_t* block_table,
+                int64_t table_stride, int32_t* free_ring, int32_t* ring_state, const int32_t* shares,
+                int64_t pool_blocks, int32_t* seq, int32_t* positions, int32_t* slots, int64_t tokens,
+                int32_t* cu_tokens, int32_t* visible, int32_t* err, int64_t batch, void* stream) {
   PoolAddr pa;  // the range checks of every paged entry point
   const int rc = paged_addr(&pa, block_table, table_stride, pool_blocks, "paged_plan");
   if (rc != DSR_OK) return rc;
@@ -295,8 +348,6 @@ extern "C" int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens,
               (long long)tokens);
   DSR_REQUIRE(tokens == 0 || (seq && positions && slots), "paged_plan: null token map");
   const size_t smem = 3 * size_t(batch + 1) * sizeof(int32_t);
-  const int set = set_max_smem(plan_kernel, 3 * size_t(kPlanMaxBatch + 1) * sizeof(int32_t), "paged_plan");
-  if (set != DSR_OK) return set;
   const PlanArgs a{lengths, new_tokens, held,  block_table, table_stride, free_ring, ring_state,  pool_blocks, seq,
                    positions, slots,    cu_tokens, visible, err,          tokens,    int(batch)};
   // a CTA for every four tokens a thread, and for the moves of blocks, whose number is not
@@ -305,6 +356,35 @@ extern "C" int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens,
   const int64_t by_table = (batch * table_stride + kPlanThreads * 32 - 1) / (kPlanThreads * 32);
   int64_t grid = by_tokens > by_table ? by_tokens : by_table;
   if (grid > sm_count()) grid = sm_count();
-  plan_kernel<<<unsigned(grid), kPlanThreads, smem, as_stream(stream)>>>(a);
-  return launch_status("paged_plan launch");
+  const auto launch = [&](auto* kernel, auto... more) {
+    const int set = set_max_smem(kernel, 3 * size_t(kPlanMaxBatch + 1) * sizeof(int32_t), "paged_plan");
+    if (set != DSR_OK) return set;
+    kernel<<<unsigned(grid), kPlanThreads, smem, as_stream(stream)>>>(a, more...);
+    return launch_status("paged_plan launch");
+  };
+  return shares != nullptr ? launch(plan_kernel<const int32_t*>, shares) : launch(plan_kernel<>);
+}
+
+}  // namespace
+}  // namespace dsr
+
+extern "C" int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* held, int32_t* block_table,
+                              int64_t table_stride, int32_t* free_ring, int32_t* ring_state, int64_t pool_blocks,
+                              int32_t* seq, int32_t* positions, int32_t* slots, int64_t tokens, int32_t* cu_tokens,
+                              int32_t* visible, int32_t* err, int64_t batch, void* stream) {
+  dsr::clear_error();
+  return dsr::launch_plan(lengths, new_tokens, held, block_table, table_stride, free_ring, ring_state, nullptr,
+                          pool_blocks, seq, positions, slots, tokens, cu_tokens, visible, err, batch, stream);
+}
+
+extern "C" int dsr_paged_plan_shared(const int32_t* lengths, const int32_t* new_tokens, int32_t* held,
+                                     int32_t* block_table, int64_t table_stride, int32_t* free_ring,
+                                     int32_t* ring_state, const int32_t* shares, int64_t pool_blocks, int32_t* seq,
+                                     int32_t* positions, int32_t* slots, int64_t tokens, int32_t* cu_tokens,
+                                     int32_t* visible, int32_t* err, int64_t batch, void* stream) {
+  using namespace dsr;
+  clear_error();
+  DSR_REQUIRE(shares, "paged_plan: null pointer");
+  return launch_plan(lengths, new_tokens, held, block_table, table_stride, free_ring, ring_state, shares, pool_blocks,
+                     seq, positions, slots, tokens, cu_tokens, visible, err, batch, stream);
 }

@@ -516,7 +516,8 @@ void check_vector(const at::Tensor& t, at::ScalarType dtype, int64_t n, const at
 
 std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens, at::Tensor held,
                                       at::Tensor block_table, at::Tensor free_ring, at::Tensor ring_state,
-                                      int64_t tokens, c10::optional<at::Tensor> status) {
+                                      int64_t tokens, c10::optional<at::Tensor> status,
+                                      c10::optional<at::Tensor> shares) {
   check(lengths, at::kInt, lengths);
   const int64_t batch = lengths.numel();
   const char* shapes =
@@ -529,6 +530,7 @@ std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens,
   TORCH_CHECK(block_table.dim() == 2 && block_table.size(0) == batch, shapes);
   check_vector(free_ring, at::kInt, free_ring.numel(), lengths, shapes);
   check_vector(ring_state, at::kInt, 4, lengths, shapes);
+  if (shares) check_vector(*shares, at::kInt, free_ring.numel(), lengths, "paged_plan: shares [pool blocks] expected");
   TORCH_CHECK(tokens >= 0 && tokens < (int64_t(1) << 31), "paged_plan: invalid token count");
   const c10::cuda::CUDAGuard guard(lengths.device());
   auto error = status_or(status, lengths);
@@ -544,11 +546,14 @@ std::vector<at::Tensor> ds_paged_plan(at::Tensor lengths, at::Tensor new_tokens,
     return t;
   };
   auto seq = part(tokens), positions = part(tokens), slots = part(tokens), cu = part(batch + 1), visible = part(batch);
-  ok(dsr_paged_plan(lengths.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
-                    block_table.data_ptr<int32_t>(), block_table.size(1), free_ring.data_ptr<int32_t>(),
-                    ring_state.data_ptr<int32_t>(), free_ring.size(0), seq.data_ptr<int32_t>(),
-                    positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), tokens, cu.data_ptr<int32_t>(),
-                    visible.data_ptr<int32_t>(), error.data_ptr<int32_t>(), batch, current_stream()));
+  const auto call = [&](auto plan, auto... extra) {
+    return plan(lengths.data_ptr<int32_t>(), new_tokens.data_ptr<int32_t>(), held.data_ptr<int32_t>(),
+                block_table.data_ptr<int32_t>(), block_table.size(1), free_ring.data_ptr<int32_t>(),
+                ring_state.data_ptr<int32_t>(), extra..., free_ring.size(0), seq.data_ptr<int32_t>(),
+                positions.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), tokens, cu.data_ptr<int32_t>(),
+                visible.data_ptr<int32_t>(), error.data_ptr<int32_t>(), batch, current_stream());
+  };
+  ok(shares ? call(dsr_paged_plan_shared, shares->data_ptr<int32_t>()) : call(dsr_paged_plan));
   return {seq, positions, slots, cu, visible, error};
 }
 
@@ -889,7 +894,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("kv_values"), py::arg("index_values"));
   m.def("paged_plan", &ds_paged_plan, py::arg("lengths"), py::arg("new_tokens"), py::arg("held"),
         py::arg("block_table"), py::arg("free_ring"), py::arg("ring_state"), py::arg("tokens"),
-        py::arg("status") = py::none());
+        py::arg("status") = py::none(), py::arg("shares") = py::none());
   m.def("paged_fork", &ds_paged_fork, py::arg("parent"), py::arg("lengths"), py::arg("held"),
         py::arg("block_table"), py::arg("free_ring"), py::arg("ring_state"), py::arg("shares"),
         py::arg("status") = py::none());

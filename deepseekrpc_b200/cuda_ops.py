@@ -118,14 +118,19 @@ def append_kv_index(kv_pool, index_pool, generations, block_table, seq, position
 
 
 # -------------------------------------------------- around the decode path
-def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens: int):
+def paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens: int, *, shares=None):
     """Blocks for every request's new tokens and the map of those tokens to pool rows.
 
     Updates held, block_table, free_ring and ring_state in place; returns
     (seq, positions, slots, cu_tokens, visible).  A batch whose counts are refused changes
     nothing; one that met a block id outside the pool raises too, and has -1 in its place.
+
+    Where requests share blocks (paged_fork), one that became shorter goes through paged_release
+    first: the plan would give its surplus blocks to the ring, and map its new tokens to the
+    others, whoever else has them.  With `shares` such a batch is refused.
     """
-    *value, status = extension().paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens)
+    *value, status = extension().paged_plan(lengths, new_tokens, held, block_table, free_ring, ring_state, tokens,
+                                            shares=shares)
     _status(status)
     return tuple(value)
 

@@ -465,6 +465,15 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
                    int32_t* ring_state, int64_t pool_blocks, int32_t* seq, int32_t* positions,
                    int32_t* slots, int64_t tokens, int32_t* cu_tokens, int32_t* visible,
                    int32_t* err, int64_t batch, void* stream);
+/* The same where several requests may map a block: shares i32[pool_blocks] as below, which
+ * stays as it is.  A batch that would map a new token to a block with shares, or give one
+ * back, is refused too (a request became shorter without dsr_paged_release). */
+int dsr_paged_plan_shared(const int32_t* lengths, const int32_t* new_tokens, int32_t* held,
+                          int32_t* block_table, int64_t table_stride, int32_t* free_ring,
+                          int32_t* ring_state, const int32_t* shares, int64_t pool_blocks,
+                          int32_t* seq, int32_t* positions, int32_t* slots, int64_t tokens,
+                          int32_t* cu_tokens, int32_t* visible, int32_t* err, int64_t batch,
+                          void* stream);
 
 /* Blocks that several requests map.  shares i32[pool_blocks] holds, for every block,
  * the number of table entries that map it beyond the first (all zeros without shared
@@ -472,7 +481,8 @@ int dsr_paged_plan(const int32_t* lengths, const int32_t* new_tokens, int32_t* h
  * block_table, free_ring, ring_state as in dsr_paged_plan; all five are updated in
  * place, and calls on them must not overlap on the GPU.  Where blocks are shared,
  * dsr_paged_release gives blocks back; a request that dsr_paged_plan finds holding
- * more than it needs would put a block that others map into the ring.
+ * more than it needs would put a block that others map into the ring, which
+ * dsr_paged_plan_shared refuses.
  * moves i32[batch][4], 16-byte aligned: (source row, destination row, rows, 0) of the
  * rows to copy, in request order, (-1,-1,0,0) behind the last; count i32[1] how many.
  * The caller copies them (dsr_paged_copy) in every pool that the table maps, before

@@ -11,8 +11,10 @@ import numpy as np
 BLOCK, V_DIM = 64, 512
 
 
-def paged_plan(lengths, new_tokens, held, table, ring, state, tokens):
-    """New (held, table, ring, state), the token map and the status of one plan."""
+def paged_plan(lengths, new_tokens, held, table, ring, state, tokens, shares=None):
+    """New (held, table, ring, state), the token map and the status of one plan.
+
+    With shares: a plan that maps a new token to a block with shares, or gives one back, is refused."""
     held, table, ring, state = (np.array(a) for a in (held, table, ring, state))
     batch, blocks = len(lengths), len(ring)
     head, count = int(state[0]), int(state[1])
@@ -23,7 +25,8 @@ def paged_plan(lengths, new_tokens, held, table, ring, state, tokens):
     maps = [np.full(tokens, -1, np.int32) for _ in range(3)]
     if ((lengths < 0) | (new_tokens < 0) | (total > table.shape[1] * BLOCK) | (held < 0) |
             (held > table.shape[1])).any() or int(new_tokens.sum()) > tokens or takes > count or \
-            not 0 <= head < blocks or count < 0 or count + gives > blocks:
+            not 0 <= head < blocks or count < 0 or count + gives > blocks or \
+            shares is not None and meets_shared(lengths, new_tokens, need, held, table, shares):
         return held, table, ring, state, maps, np.zeros(batch + 1, np.int32), lengths.copy(), 1
     status, i = 0, 0
     tail = head + count
@@ -52,6 +55,16 @@ def paged_plan(lengths, new_tokens, held, table, ring, state, tokens):
     state[0], state[1] = head % blocks, count - takes + gives
     cu = np.concatenate([[0], np.cumsum(new_tokens)]).astype(np.int32)
     return need.astype(np.int32), table, ring, state, maps, cu, total.astype(np.int32), status
+
+
+def meets_shared(lengths, new_tokens, need, held, table, shares):
+    """Whether a held block that new tokens go to, or that is given back, has shares."""
+    for b, n in enumerate(lengths):
+        touched = {p // BLOCK for p in range(n, n + new_tokens[b])} | set(range(need[b], held[b]))
+        blocks = [table[b, j] for j in touched if j < held[b]]
+        if any(shares[i] > 0 for i in blocks if 0 <= i < len(shares)):
+            return True
+    return False
 
 
 def rope(x, positions, frequencies, offset, interleaved, mscale=1.0, inverse=False):
