@@ -215,8 +215,9 @@ __device__ __forceinline__ int32_t groups_of(int64_t counts) {
   return int32_t(uint64_t(counts) >> (kItemBits + kRowBits));
 }
 
-// What the pairs share: false, with nothing to do, when sums in disorder give rows to several
-// requests, more than there are partials for.
+// What the pairs share: false, with nothing to do and a status, when sums in disorder give rows to
+// several requests, more than there are partials for, or a pair's share is above 2^31 units (in
+// all 2.6e15 pairs of a query row and a key).
 __device__ __forceinline__ bool write_pair_head(const PrefixArgs& a, bool writes, bool fine, int64_t run_units,
                                                 int64_t run_all, int64_t own_units, int64_t own_all) {
   const int64_t run_share = (run_units + a.pairs - 1) / a.pairs, own_share = (own_units + a.pairs - 1) / a.pairs;
@@ -224,6 +225,7 @@ __device__ __forceinline__ bool write_pair_head(const PrefixArgs& a, bool writes
   const bool fits = rows_of(run_all) <= most && rows_of(own_all) <= most && run_share <= INT32_MAX &&
                     own_share <= INT32_MAX;
   if (writes) {
+    if (!fits) flag(a.err, DSR_ERR_ID);
     int4* head = reinterpret_cast<int4*>(a.head);
     head[0] = make_int4(0, fits ? int(fine) : 1, 0, 0);
     head[1] = fits ? make_int4(groups_of(run_all), int(run_share), items_of(own_all), int(own_share))

@@ -609,9 +609,10 @@ int dsr_tree_mla_decode(const void* q, int q_dtype, const uint16_t* kv_pool, int
  * is best in the order of its prompts.  The result does not depend on the grouping
  * beyond the order of FP32 sums; all else, and the status, as in dsr_tree_mla_decode.
  * Status 1 also for a prefix or holder out of range (that request's rows count as
- * unused), and where disordered sums of cu_nodes give rows to several requests (then
- * all may count as unused).  A non-finite row of a request's own reaches that request's
- * output alone.  batch <= 16384, nodes * heads <= 2^24.
+ * unused), where disordered sums of cu_nodes give rows to several requests (then all
+ * may count as unused), and for a batch of more than 2^31 tiles of 128 query rows and
+ * 128 keys for every two SMs (then all do).  A non-finite row of a request's own reaches
+ * that request's output alone.  batch <= 16384, nodes * heads <= 2^24.
  * Scratch: dsr_prefix_mla_workspace_bytes() on the current device, 256-byte aligned,
  * need not be cleared; calls sharing it must not overlap. */
 size_t dsr_prefix_mla_workspace_bytes(int64_t batch, int64_t nodes, int64_t heads);

@@ -66,3 +66,24 @@ def test_a_drafted_row_that_one_group_sees(cuda):
     out, status, lse = call(d, return_lse=True)
     assert int(status.item()) == 0
     check(d, rows, masks, out, lse)
+
+
+def test_more_work_than_can_be_shared_out_is_reported(cuda):
+    """150 requests of 64 nodes and 128 heads whose contexts fill the longest table: more than
+    2^31 units a pair of SMs.  Nothing is computed, and nothing of the 20 GB of entries is read."""
+    batch, nodes, heads, stride = 150, 64, 128, (1 << 25) - 1
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table = torch.empty((batch, stride), **i32)
+    d = dict(q=torch.zeros((batch * nodes, heads, 576), device="cuda", dtype=torch.bfloat16), sink=None, most=nodes,
+             pool=torch.zeros((64, 576), device="cuda", dtype=torch.bfloat16), table=table,
+             context=torch.full((batch,), stride * 64 - nodes, **i32), cu=torch.arange(0, batch * nodes + 1, nodes, **i32),
+             mask=torch.ones(batch * nodes, device="cuda", dtype=torch.int64),
+             prefix=torch.zeros(batch, **i32), holder=torch.full((batch,), -1, **i32))
+    try:
+        out, status, lse = call(d, return_lse=True)
+        assert int(status.item()) == 1
+        assert not out.any() and torch.all(torch.isneginf(lse))
+    finally:
+        d.clear()
+        del table
+        torch.cuda.empty_cache()
