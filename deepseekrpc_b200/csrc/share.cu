@@ -784,8 +784,11 @@ extern "C" int dsr_paged_copy(void* const* pools, const int64_t* row_bytes, int6
   }
   for (int64_t i = 0; i < generation_count; ++i) {
     DSR_REQUIRE(generations[i], "paged_copy: null pointer");
-    for (int64_t j = 0; j < i; ++j)  // two threads would add to one entry
-      DSR_REQUIRE(generations[i] != generations[j], "paged_copy: the same generations twice");
+    for (int64_t j = 0; j < i; ++j) {  // two threads would add to one entry
+      const int64_t apart = reinterpret_cast<intptr_t>(generations[i]) - reinterpret_cast<intptr_t>(generations[j]);
+      DSR_REQUIRE((apart < 0 ? -apart : apart) >= pool_rows * int64_t(sizeof(int64_t)),
+                  "paged_copy: the same generations twice");
+    }
     a.generations[i] = generations[i];
   }
   if (max_moves == 0 || pool_count + generation_count == 0) return DSR_OK;

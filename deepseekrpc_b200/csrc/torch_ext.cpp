@@ -660,14 +660,13 @@ at::Tensor ds_paged_copy(std::vector<at::Tensor> pools, std::vector<at::Tensor> 
   }
   for (const at::Tensor& g : generations)
     check_vector(g, at::kLong, rows, moves, "paged_copy: generations [rows] of the pools' rows expected");
+  constexpr size_t most = 64;  // of a launch, whose own check is of its generations
+  std::vector<const int64_t*> all;
+  for (const at::Tensor& g : generations) all.push_back(g.data_ptr<int64_t>());
+  std::sort(all.begin(), all.end());
+  TORCH_CHECK(std::adjacent_find(all.begin(), all.end(), [&](auto a, auto b) { return b - a < rows; }) == all.end(),
+              "paged_copy: the same generations twice");
   for (const at::Tensor& p : pools) overwrite(p, "paged_copy");
-  constexpr size_t most = 64;  // of a launch
-  if (generations.size() > most) {  // (the launch's own check is of its 64)
-    std::vector<const void*> all;
-    for (const at::Tensor& g : generations) all.push_back(g.data_ptr());
-    std::sort(all.begin(), all.end());
-    TORCH_CHECK(std::adjacent_find(all.begin(), all.end()) == all.end(), "paged_copy: the same generations twice");
-  }
   for (size_t i = 0; i < std::max(pools.size(), generations.size()); i += most) {
     std::vector<void*> data;
     std::vector<int64_t> bytes;

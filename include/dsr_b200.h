@@ -534,7 +534,7 @@ int dsr_paged_compact(int32_t* held, int32_t* block_table, int64_t table_stride,
 /* Copies the rows of the first *count moves in each of up to 64 pools of pool_rows rows
  * (row_bytes[i] a multiple of 16, at most 65536; 16-byte aligned) and adds 1 to the
  * written rows' entries of up to 64 generations i64[pool_rows] (an append's bump; the same
- * one twice is refused).  The three host arrays are read by the call.  A move of more than
+ * entries twice are refused).  The three host arrays are read by the call.  A move of more than
  * 64 rows, or with rows outside the pool, and a count outside [0, max_moves] give status 1
  * and are skipped.  No destination may be another move's source or destination. */
 int dsr_paged_copy(void* const* pools, const int64_t* row_bytes, int64_t pool_count,
