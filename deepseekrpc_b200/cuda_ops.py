@@ -162,9 +162,10 @@ def paged_release(lengths, held, block_table, free_ring, ring_state, shares):
     """Cuts every request to `lengths` tokens; blocks that nobody maps any more are free again.
 
     Returns (moves, count): a partial last block that others map too is exchanged for a
-    fresh one, whose rows paged_copy has to copy.  A refused batch (too few free blocks for
-    those among its reasons, whatever else the batch gives back) changes nothing; one that is
-    done around a bad block raises BlockError, which has the moves.
+    fresh one, whose rows paged_copy has to copy.  A refused batch changes nothing; one that is
+    done around a bad block raises BlockError, which has the moves.  Too few free blocks for the
+    exchanges is a refusal, whatever else the batch gives back: a call with the lengths rounded
+    up to 64 needs none, and frees them for the one with the lengths.
     """
     before = held.clone()
     return _moves(extension().paged_release(lengths, held, block_table, free_ring, ring_state, shares),

@@ -508,7 +508,10 @@ int dsr_paged_fork(const int32_t* parent, const int32_t* lengths, int32_t* held,
  * and those that nobody maps any more go behind the ring's tail, in the order of their
  * ids, free from the next call on.  A partial last block that others map too is
  * exchanged for one from the ring's head, its rows to be copied, so that what is
- * appended next is seen by this request alone.  A block whose count is too low for its
+ * appended next is seen by this request alone.  Others count as they were before the call,
+ * those that it cuts or ends among them, and what it frees serves no exchange of its own:
+ * where the ring is short, a call with the lengths rounded up to 64 takes no block and
+ * gives all others back, and the one with the lengths themselves follows.  A block whose count is too low for its
  * entries gives status 1.  Scratch: 256-byte aligned, need not be cleared; calls
  * sharing it must not overlap. */
 size_t dsr_paged_release_workspace_bytes(int64_t batch, int64_t pool_blocks);
