@@ -360,6 +360,24 @@ __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;"
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+// Launches a kernel that may start while the one before it in the stream runs.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const char* what,
+                 const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+  if (e != cudaSuccess) return fail(DSR_ECUDA, "%s launch: %s", what, cudaGetErrorString(e));
+  return DSR_OK;
+}
 
 // The MLA query of the same decode step, FP32 [batch, heads, 576] -> BF16 in the
 // shared-memory image the sparse MLA kernel contracts against: per (sequence,

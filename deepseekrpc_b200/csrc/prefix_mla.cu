@@ -95,7 +95,6 @@ struct alignas(16) PairNode {
 };
 
 struct PrefixArgs {
-  const int32_t* table;
   int64_t stride, table_rows;
   const int32_t* context;
   const int32_t* cu_nodes;
@@ -822,12 +821,6 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
       "h"(uint16_t(3))
       : "memory");
 }
-// True in one lane of a converged warp.
-__device__ __forceinline__ bool elect_lane() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
 // The softmax threads of one half of a CTA's rows, four a row: a barrier, and whether every one
 // is fine.
 __device__ __forceinline__ bool rows_sync(int half, bool ok) {
@@ -1136,7 +1129,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       constexpr uint32_t idesc_o = umma_idesc_bf16(kPairRows, 256, false, true);
       const uint32_t sb = __shfl_sync(~0u, sbase, 0);
       const uint32_t ts = __shfl_sync(~0u, tmem_s, 0), to = __shfl_sync(~0u, tmem_o, 0);
-      const bool leader = elect_lane();
+      const bool leader = elect_one();
       const uint64_t desc_q = umma_desc_sw128(sb + L::kQOff, 16, 1024), desc_k = umma_desc_sw128(sb + L::kKOff, 16, 1024);
       const uint64_t desc_p = umma_desc_sw128(sb + L::kPOff, 16, 1024);
       const uint64_t desc_v = umma_desc_sw128(sb + L::kVOff, L::kBlock, 1024);
@@ -1216,7 +1209,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     const uint32_t to_v = __shfl_sync(~0u, pair_address(full_v, 0), 0);
     const uint32_t to_q = __shfl_sync(~0u, pair_address(bar_q, 0), 0);
     const uint32_t to_own = __shfl_sync(~0u, pair_address(bar_own, rank), 0);
-    const bool leader = elect_lane();
+    const bool leader = elect_one();
     int n = 0, cleared = 0;
     bool ok = true;
     while (ok && walk.next()) {
@@ -1609,7 +1602,6 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   const PrefixSizes sizes = prefix_sizes(batch, nodes, heads);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   PrefixArgs a = {};
-  a.table = block_table;
   a.stride = table_stride;
   a.table_rows = table_rows;
   a.context = context;
@@ -1681,21 +1673,11 @@ extern "C" int dsr_prefix_mla_decode(const void* q, int q_dtype, const uint16_t*
   // rows: 14 to 11 us), with more it is not (8192 rows: 17 and 22 us)
   const int64_t quads = nodes * heads / 4;
   auto launch_join = [&](auto* join, int columns, int split) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(unsigned(quads), DSR_V_DIM / (kJoinThreads * columns), 1);
-    cfg.blockDim = dim3(kJoinThreads * split, 1, 1);
-    cfg.stream = as_stream(stream);
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join, a);
+    return launch_after(join, dim3(unsigned(quads), DSR_V_DIM / (kJoinThreads * columns)), kJoinThreads * split, 0,
+                        as_stream(stream), "prefix_mla_decode join", a);
   };
-  const cudaError_t e = a.pairs == 0                ? launch_join(prefix_join_kernel<false, 1, 4, 8>, 1, 4)
-                        : quads <= sm_count()     ? launch_join(prefix_join_kernel<true, 2, 4, 4>, 2, 4)
-                        : quads <= 8 * sm_count() ? launch_join(prefix_join_kernel<true, 4, 1, 4>, 4, 1)
-                                                  : launch_join(prefix_join_kernel<true, 4, 1, 2>, 4, 1);
-  if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode join launch: %s", cudaGetErrorString(e));
-  return DSR_OK;
+  return a.pairs == 0              ? launch_join(prefix_join_kernel<false, 1, 4, 8>, 1, 4)
+         : quads <= sm_count()     ? launch_join(prefix_join_kernel<true, 2, 4, 4>, 2, 4)
+         : quads <= 8 * sm_count() ? launch_join(prefix_join_kernel<true, 4, 1, 4>, 4, 1)
+                                   : launch_join(prefix_join_kernel<true, 4, 1, 2>, 4, 1);
 }

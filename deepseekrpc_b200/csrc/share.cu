@@ -635,24 +635,6 @@ unsigned share_grid(int64_t items, int64_t per) {
   return unsigned(grid < 1 ? 1 : grid < sm_count() ? grid : sm_count());
 }
 
-template <typename... P, typename... A>
-int launch_after(void (*kernel)(P...), unsigned grid, int threads, size_t smem, cudaStream_t stream, const char* what,
-                 const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, 1, 1);
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-  if (e != cudaSuccess) return fail(DSR_ECUDA, "%s launch: %s", what, cudaGetErrorString(e));
-  return DSR_OK;
-}
-
 }  // namespace
 }  // namespace dsr
 

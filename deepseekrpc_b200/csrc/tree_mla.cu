@@ -299,13 +299,6 @@ __device__ __forceinline__ bool tree_wait_warp(uint64_t* bar, uint32_t parity, v
   return __all_sync(~0u, tree_wait(bar, parity, abort, err));
 }
 
-// True in one lane of a converged warp.
-__device__ __forceinline__ bool elect_one() {
-  uint32_t r;
-  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
-  return r != 0;
-}
-
 // 16 TMEM lanes x 8 C columns: thread i holds lanes i/4 and i/4 + 8 (of the 16),
 // columns 8c + 2(i%4) and the next: r[4c + 2h + e] is lane i/4 + 8h, column + e.
 template <int C>
@@ -1172,19 +1165,8 @@ int launch_listed(const TreeArgs& a, const uint16_t* kv_pool, cudaStream_t strea
   CUtensorMap map, q_map;
   rc = tree_maps<N>(a, kv_pool, map, q_map);
   if (rc != DSR_OK) return rc;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(a.ctas), 1, 1);
-  cfg.blockDim = dim3(kTreeThreads, 1, 1);
-  cfg.dynamicSmemBytes = L::kAlloc;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_mla_kernel<N, true>, map, q_map, a);
-  if (e != cudaSuccess) return fail(DSR_ECUDA, "prefix_mla_decode launch: %s", cudaGetErrorString(e));
-  return DSR_OK;
+  return launch_after(tree_mla_kernel<N, true>, dim3(unsigned(a.ctas)), kTreeThreads, L::kAlloc, stream,
+                      "prefix_mla_decode", map, q_map, a);
 }
 
 }  // namespace
