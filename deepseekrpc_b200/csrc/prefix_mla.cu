@@ -38,8 +38,12 @@ constexpr int kPlanWaves = 4, kPlanTried = kPlanWaves + 1;
 // A job's cost beside its tiles, in tiles: first copies, output, its part of the join.
 constexpr float kPlanJobTiles = 4.f;
 constexpr int kPairRows = 128;
-// The same of a piece, added to a group's tiles where the pairs share out the work.
-constexpr int kPairLead = 2;
+// The same of a piece, added to a group's tiles where the pairs share out the work.  (A change of
+// the group takes 9000 cycles, 3.7 tiles, but a pair's last output is not one.  With 2, 3 and 4:
+// 256 requests of 64 heads over 65472 rows 1670, 1646 and 1663 us, 64 of 128 heads over 32768 385,
+// 385 and 387, 23 of 5 prompts 73.8, 71.8 and 73.7, 9 of 128 heads over 5184 38.9, 35.8 and 35.8;
+// 100 of 3 nodes and 32 heads with 4000 rows of their own 195 with 2, 197 with 3.)
+constexpr int kPairLead = 3;
 static_assert(DSR_BLOCK_TOKENS == 64, "64-row blocks");
 
 // A request: its query rows, where its own parts are, and where those of its run: part +
@@ -59,7 +63,8 @@ static_assert(sizeof(PrefixRequest) == 32, "two 16-byte words");
 // request whose groups have other requests' rows too, or that has no run, are an item by
 // themselves, in groups of its own rows: with weights of zero another request's values would
 // still reach a row where they are not finite.  (Taken all the same: 23 requests of 5 prompts 68 us
-// for 74, 52 of 32 heads 35 for 39, 256 of 64 heads over 65472 rows 1642 for 1659.)
+// for 74, 52 of 32 heads 35 for 39, 100 of 3 nodes and 32 heads with 640 rows of their own 111 for
+// 124, 256 of 64 heads over 65472 rows 1642 for 1659.)
 // Units are tiles, and kPairLead before each group's first; pair c has the units [c share,
 // (c + 1) share) of all runs, then those of all items by themselves, in one piece per group.
 // Piece (group g, pair c) leaves its partials at part + 128 (g + c), since g or c rises from
