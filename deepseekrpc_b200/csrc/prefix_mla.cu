@@ -16,13 +16,14 @@
 // kernel takes the jobs from a list (two requests of 16 heads over 4096 rows: 21 us; by pairs
 // in an earlier form 38, for 27 by the list).
 //
-// Bound by the tensor cores, and by the power that they may take.  Measured alone, with cold
-// inputs: 64 requests of 128 heads that share 32768 rows and have up to 1500 of their own 389
-// us (598 GFLOP, 1.54 PFLOP/s, 92% of a measured BF16 GEMM); 256 of 64 heads over 65472 rows
-// 1640 us (1.43 PFLOP/s, 86%), one call after another 1930 us (1.22 PFLOP/s, 88% of the
-// measured sustained rate); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 68 us (63%:
-// the plan 3.5 us, 7 until the first tile is there, outputs of 3.5, the join 7.5).  The same by
-// the tree attention's groups of 64 rows: 831, 3133 and 122 us.
+// Bound by the tensor cores, and by the power that they may take.  Measured with cold inputs,
+// alone and one call after another: 64 requests of 128 heads that share 32768 rows and have up to
+// 1500 of their own 385 and 471 us (598 GFLOP: 1.55 PFLOP/s, 93% of a measured BF16 GEMM, and 1.27,
+// 91% of a sustained one); 256 of 64 heads over 65472 rows 1640 and 1930 us (1.43 PFLOP/s, 86%, and
+// 1.22, 88%); 23 requests of 1 to 6 nodes and 32 heads over 5 prompts 72 and 71 us (60%: the plan
+// 3.5 us, 7 until the first tile is there, outputs of 3.5, the join 7.5).  The same by the tree
+// attention's groups of 64 rows, alone: 831, 3133 and 122 us.  FP32 queries: 390, 1668 and 82 us
+// alone, since the softmax warps convert them before a piece's first product.
 #include <type_traits>
 
 #include "common.cuh"

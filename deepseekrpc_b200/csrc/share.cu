@@ -3,7 +3,7 @@
 //
 //   shares[blk] = table entries that map block blk beyond the first (0: one request's
 //   own, or free), so that a program without shared blocks has zeros there for good and
-//   dsr_paged_plan, which only ever maps free blocks, need not know of it.
+//   dsr_paged_plan, which only ever maps free blocks, leaves it alone.
 //
 // A move (source row, destination row, rows, 0) names up to one block of rows to copy.
 // The tables are changed once for all layers; dsr_paged_copy then runs per cache, or for
@@ -190,8 +190,8 @@ __global__ void __launch_bounds__(kForkThreads) fork_kernel(const ShareArgs a) {
 // lowered does not matter.  Tables of up to kWholeEntries entries: by the same CTA, with
 // its bit per freed block in shared memory; larger ones by two more launches.
 // Scratch of three launches: {ok, taken, dropped} and cu_drop[batch + 1], then the bits.
-// Bound by latency: 448 requests cut somewhere, 65000 entries dropped, 22 us with cold inputs
-// (7.5, 7.5 and 6.7; the freed blocks by the last CTA of the second launch took 16 instead).
+// Bound by latency: 512 requests cut somewhere, 41000 entries dropped, 22 us with cold inputs
+// (7.5, 7.6 and 6.7; the freed blocks by the last CTA of the second launch took 16 instead).
 // ---------------------------------------------------------------------------
 constexpr int kScanThreads = 1024, kDropThreads = 512;
 constexpr int kScanPer = kShareMaxBatch / kScanThreads;
@@ -538,8 +538,9 @@ __global__ void __launch_bounds__(kCompactThreads) compact_apply_kernel(const Sh
 // ---------------------------------------------------------------------------
 // Copies.  A work item is a piece of one move's rows in one pool, four 16-byte units a thread
 // on their way at once; the generations of the written rows are a move's last item.  Bound by
-// memory: 3900 blocks of 90 KB 117 us (6.3 TB/s read and written, 97% of a plain copy), 495
-// copies of up to 63 rows in four layers 30 us (5.9 TB/s).
+// memory: 4039 blocks of 90 KB with their generations, 732 MB read and written, 118 us (6.2 TB/s,
+// 95% of the rate of a 2 GB copy and 99% of one of this size); 489 copies of up to 63 rows in four
+// layers, 178 MB, 30.5 us (5.8 TB/s).
 // ---------------------------------------------------------------------------
 constexpr int kCopyThreads = 256, kCopyPiece = 16384;  // bytes of an item
 constexpr int kCopyMax = 64;                           // pools, and generations, of a call
