@@ -40,8 +40,8 @@ constexpr int kPlanWaves = 4, kPlanTried = kPlanWaves + 1;
 constexpr float kPlanJobTiles = 4.f;
 constexpr int kPairRows = 128;
 // The same of a piece, added to a group's tiles where the pairs share out the work.  (A change of
-// the group takes 9000 cycles, 3.7 tiles, but a pair's last output is not one.  With 2, 3 and 4:
-// 256 requests of 64 heads over 65472 rows 1670, 1646 and 1663 us, 64 of 128 heads over 32768 385,
+// the group takes 9000 cycles, 3.7 tiles, but a pair's last output holds up no other group.  With
+// 2, 3 and 4: 256 requests of 64 heads over 65472 rows 1670, 1646 and 1663 us, 64 of 128 heads over 32768 385,
 // 385 and 387, 23 of 5 prompts 73.8, 71.8 and 73.7, 9 of 128 heads over 5184 38.9, 35.8 and 35.8;
 // 100 of 3 nodes and 32 heads with 4000 rows of their own 195 with 2, 197 with 3.)
 constexpr int kPairLead = 3;
